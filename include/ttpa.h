@@ -598,6 +598,110 @@ int ttpa_paged_fill_latent(void *cache, const void *latent, int64_t latent_user_
                            int32_t table_rows, int32_t seq_len, int32_t block_size, int32_t latent_size,
                            int32_t rope_size, int32_t table_width, int32_t num_blocks, void *stream);
 
+/*
+ * ---- the 8-bit cache with a scale for each block of tokens and head ----
+ *
+ * Caches of one byte per element for layers whose context is long; no counterpart in the reference.
+ *   k_cache, v_cache    e4m3 (OCP) [num_blocks, kv_heads, block_size, head_size], contiguous
+ *   k_scales, v_scales  float [num_blocks, kv_heads]: an element stands for itself times its block's scale of that head, a power
+ *                       of two in [2^-110, 2^119]
+ *   key_bounds          bfloat16 [num_blocks, kv_heads, 2, head_size] or NULL: the least and the largest key of every block,
+ *                       feature by feature, for the sparse decode
+ * The scale of a block is the smallest power of two with which its largest finite magnitude is at most 448.  Elements are rounded once, to
+ * nearest even; beyond 448 * 2^119 they are that; NaN and infinities become NaN and have no part in scales, NaN none in bounds.
+ * Rows of a block behind its last token hold anything.  head_size 64, 128 or 256, block_size a multiple of 16 up to 4096.  Keys, values and
+ * queries are bfloat16, addressed by strides in multiples of 8 elements, 16-byte aligned.
+ */
+
+/*
+ * RMS norm of every head of the queries and of the keys, and the position rotation, in one pass:
+ *   y = x / sqrt(mean(x^2) + eps) * weight   (q_weight / k_weight of head_size, bfloat16 or, weights_are_f32, float; NULL: y = x)
+ *   out_i = y_i c_j - y_k s_j,  out_k = y_k c_j + y_i s_j   for j < rotary / 2 and (i, k) = (j, j + rotary / 2), or, interleaved, (2 j, 2 j + 1);
+ * features from `rotary` (a multiple of 16) on are not rotated.  cos_sin is [max_positions, rotary], row p holding c and then s of position p,
+ * bfloat16 or (cos_sin_is_f32) float.  A token whose position is outside the table is not rotated.  q [tokens, q_heads, head_size] and
+ * k [tokens, k_heads, head_size] by strides; the outputs may be the operands.
+ */
+int ttpa_qk_norm_rope(void *q_out, int64_t q_out_token_stride, int64_t q_out_head_stride, void *k_out, int64_t k_out_token_stride,
+                      int64_t k_out_head_stride, const void *q, int64_t q_token_stride, int64_t q_head_stride, const void *k, int64_t k_token_stride,
+                      int64_t k_head_stride, const void *cos_sin, int cos_sin_is_f32, int64_t cos_sin_row_stride, int64_t max_positions,
+                      const void *positions, int positions_is_i64, const void *q_weight, const void *k_weight, int weights_are_f32, float eps,
+                      int32_t tokens, int32_t q_heads, int32_t k_heads, int32_t head_size, int32_t rotary, int interleaved, void *stream);
+
+/*
+ * A step's write: the token of user u goes to position update_indices[u] of page-table row u.  Row 0 of a block begins it: its scale and
+ * bounds are the row's own, what the block held before is void.  A later row may make the scale grow; the rows before it are then rounded
+ * again for the new one.  Users at negative positions, at positions outside the table and with blocks outside the cache write nothing.  Users
+ * whose tokens go to the same block write in turn, as in calls of one user each.
+ */
+int ttpa_paged_update_fp8_cache(void *k_cache, void *v_cache, float *k_scales, float *v_scales, void *key_bounds, const void *k_fill,
+                                int64_t k_user_stride, int64_t k_head_stride, const void *v_fill, int64_t v_user_stride, int64_t v_head_stride,
+                                const void *update_indices, int indices_is_i64, const int32_t *page_table, int64_t page_table_row_stride,
+                                int32_t users, int32_t kv_heads, int32_t block_size, int32_t head_size, int32_t table_width, int32_t num_blocks,
+                                void *stream);
+
+/*
+ * ttpa_qk_norm_rope on a step's tokens (token u of user u at position positions[u]) and ttpa_paged_update_fp8_cache of the result and of
+ * v, in one launch; the keys go to the cache alone.  Results are those of the two calls.
+ */
+int ttpa_qk_norm_rope_update_fp8(void *q_out, int64_t q_out_token_stride, int64_t q_out_head_stride, const void *q, int64_t q_token_stride,
+                                 int64_t q_head_stride, const void *k, int64_t k_token_stride, int64_t k_head_stride, const void *v,
+                                 int64_t v_token_stride, int64_t v_head_stride, const void *cos_sin, int cos_sin_is_f32, int64_t cos_sin_row_stride,
+                                 int64_t max_positions, const void *positions, int positions_is_i64, const void *q_weight, const void *k_weight,
+                                 int weights_are_f32, float eps, void *k_cache, void *v_cache, float *k_scales, float *v_scales, void *key_bounds,
+                                 const int32_t *page_table, int64_t page_table_row_stride, int32_t users, int32_t q_heads, int32_t kv_heads,
+                                 int32_t head_size, int32_t rotary, int interleaved, int32_t block_size, int32_t table_width, int32_t num_blocks,
+                                 void *stream);
+
+/*
+ * Prompts: ttpa_paged_fill_cache for both 8-bit caches.  Token t of fill row i goes to block t / block_size of page-table row batch_idx[i]
+ * (NULL: row 0, of one fill row); every block's scale and bounds are those of the rows written.  Rows behind seq_len keep their bytes.  No block
+ * may be named twice among the columns written: which of the writers its scale then belongs to is not defined.
+ */
+int ttpa_paged_fill_fp8_cache(void *k_cache, void *v_cache, float *k_scales, float *v_scales, void *key_bounds, const void *k_fill,
+                              int64_t k_user_stride, int64_t k_head_stride, int64_t k_token_stride, const void *v_fill, int64_t v_user_stride,
+                              int64_t v_head_stride, int64_t v_token_stride, const int32_t *page_table, int64_t page_table_row_stride,
+                              const void *batch_idx, int batch_idx_is_i64, int32_t fill_users, int32_t table_rows, int32_t kv_heads,
+                              int32_t seq_len, int32_t block_size, int32_t head_size, int32_t table_width, int32_t num_blocks, void *stream);
+
+/*
+ * ttpa_paged_sdpa_decode_windowed over the 8-bit cache, up to 16 query heads per KV head and 2048 users.  The workspace is
+ * ttpa_paged_decode_workspace_bytes(users, q_heads, kv_heads, head_size) bytes.
+ */
+int ttpa_paged_fp8_decode(void *out, int64_t out_user_stride, int64_t out_head_stride, const void *q, int64_t q_user_stride, int64_t q_head_stride,
+                          const void *k_cache, const void *v_cache, const float *k_scales, const float *v_scales, const int32_t *page_table,
+                          int64_t page_table_row_stride, const void *cur_pos, int cur_pos_is_i64, int32_t users, int32_t q_heads,
+                          int32_t kv_heads, int32_t head_size, int32_t block_size, int32_t table_width, int32_t num_blocks, float scale,
+                          int32_t sliding_window, const float *attention_sink, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * The decode over `kept_blocks` (at least 2) of each user's blocks, chosen for each KV head: the first, the one that holds cur_pos, and of the others
+ * those with the largest
+ *   score = max over the KV head's query heads of  sum_d  max(q_d, 0) * high_d + min(q_d, 0) * low_d
+ * (a bound of q . k over the block), in 64 bits; of equal scores the lower column; a score that is no finite number counts as the
+ * largest.  columns [users, kv_heads, kept_blocks] receives the page-table columns in order, then -1.  A context of no more blocks is attended whole.
+ * q and out are [users, q_heads, head_size] with users q_heads * head stride apart.
+ */
+size_t ttpa_paged_fp8_sparse_decode_workspace_bytes(int32_t users, int32_t q_heads, int32_t kv_heads, int32_t head_size, int32_t table_width,
+                                                    int32_t kept_blocks);
+int ttpa_paged_fp8_sparse_decode(void *out, int64_t out_head_stride, int32_t *columns, const void *q, int64_t q_head_stride, const void *k_cache,
+                                 const void *v_cache, const float *k_scales, const float *v_scales, const void *key_bounds,
+                                 const int32_t *page_table, int64_t page_table_row_stride, const void *cur_pos, int cur_pos_is_i64,
+                                 int32_t users, int32_t q_heads, int32_t kv_heads, int32_t head_size, int32_t block_size, int32_t table_width,
+                                 int32_t num_blocks, int32_t kept_blocks, float scale, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * The paged causal form of ttpa_sdpa_prefill (a prompt's continuation chunk) over the 8-bit cache; block_size a multiple of 32.  most_keys > 0: a
+ * bound of chunk_start + q_len that the caller knows; keys from there on are not read, and the workspace has room for no more.
+ */
+int64_t ttpa_chunked_fp8_attention_workspace_bytes(int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t q_len, int32_t head_size,
+                                                   int32_t block_size, int32_t table_width, int64_t most_keys);
+int ttpa_chunked_fp8_attention(void *out, int64_t out_batch_stride, int64_t out_head_stride, int64_t out_token_stride, const void *q,
+                               int64_t q_batch_stride, int64_t q_head_stride, int64_t q_token_stride, const void *k_cache, const void *v_cache,
+                               const float *k_scales, const float *v_scales, const int32_t *page_table, int64_t page_table_row_stride,
+                               const int32_t *chunk_start, int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t q_len, int32_t head_size,
+                               int32_t block_size, int32_t table_width, int32_t num_blocks, float scale, int64_t most_keys, void *workspace,
+                               int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

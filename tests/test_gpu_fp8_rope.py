@@ -1,0 +1,135 @@
+"""Norms of queries and keys with the position rotation (``tt::qk_norm_rope``, ``tt::qk_norm_rope_``) against the same in
+64 bits.
+
+Tolerance: the result is rounded to bfloat16 once, 2^-8 of it; before that a feature is a sum of two products of float32
+values, each of which carries the rounding of x * (inv * weight) (two products), of inv (a division, a root and a mean over up to
+256 squares in a tree of at most 16 additions in a row) and of the cosine: less than 32 half units, 32 * 2^-24 of the two products' size.  The row's
+largest result bounds neither, so the bound is 2^-19 of |y_i| + |y_j| <= 2 max |y| of the normed row, and of the result."""
+
+import pytest
+import torch
+
+import __graft_entry__ as entry
+import fp8_reference as R
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _pkg():
+    entry.ensure_built()
+    import tt_xla_amd  # noqa: F401
+
+
+def _table(positions, rotary, dtype=torch.float32):
+    from tt_xla_amd.fp8_ops import rope_table
+
+    return rope_table(positions, rotary, 10000.0, "cpu", dtype)
+
+
+def _inputs(tokens, hq, hk, d, seed, gain=1.0):
+    g = torch.Generator().manual_seed(seed)
+    qkv = (torch.randn(tokens, (hq + 2 * hk) * d, generator=g) * gain).to(torch.bfloat16)
+    return qkv, g
+
+
+def _check(got, x, weight, table, pos, eps, interleaved):
+    want = R.turn(x, weight, table, pos, eps, interleaved)
+    size = 2 * want.abs().amax(-1, keepdim=True)
+    err = (got.cpu().double() - want).abs()
+    assert bool((err <= 2.0**-8 * want.abs() + 2.0**-19 * size + 2.0**-126).all()), float((err - 2.0**-8 * want.abs()).max())
+
+
+@pytest.mark.parametrize("tokens", [1, 2, 37, 700])
+@pytest.mark.parametrize("hq, hk, d, rotary", [(8, 2, 64, 64), (32, 8, 128, 128), (5, 1, 128, 64), (16, 8, 256, 256), (3, 3, 256, 96), (7, 2, 64, 16)])
+def test_rows(tokens, hq, hk, d, rotary):
+    qkv, g = _inputs(tokens, hq, hk, d, tokens * 1000 + hq)
+    table = _table(300, rotary)
+    pos = torch.randint(0, 300, (tokens,), generator=g, dtype=torch.int32)
+    qw, kw = (1 + 0.3 * torch.randn(d, generator=g)).to(torch.bfloat16), (1 + 0.3 * torch.randn(d, generator=g)).to(torch.bfloat16)
+    dev = qkv.cuda()
+    q, k, _ = dev.split([hq * d, hk * d, hk * d], 1)  # views of a projection's output
+    q, k = q.unflatten(1, (hq, d)), k.unflatten(1, (hk, d))
+    for interleaved in (False, True):
+        for weights in ((qw, kw), (None, None), (qw.float(), None)):
+            on = [None if w is None else w.cuda() for w in weights]
+            a, b = torch.ops.tt.qk_norm_rope(q, k, table.cuda(), pos.cuda(), *on, 1e-5, interleaved)
+            _check(a, q.cpu(), weights[0], table, pos, 1e-5, interleaved)
+            _check(b, k.cpu(), weights[1], table, pos, 1e-5, interleaved)
+            # in place on the views: the same bits, and the values between them untouched
+            own = dev.clone()
+            q2, k2, v2 = own.split([hq * d, hk * d, hk * d], 1)
+            torch.ops.tt.qk_norm_rope_(q2.unflatten(1, (hq, d)), k2.unflatten(1, (hk, d)), table.cuda(), pos.cuda(), *on, 1e-5, interleaved)
+            assert torch.equal(q2.unflatten(1, (hq, d)), a) and torch.equal(k2.unflatten(1, (hk, d)), b)
+            assert torch.equal(v2, dev[:, (hq + hk) * d :])
+
+
+def test_table_in_bfloat16_long_positions_and_positions_outside():
+    tokens, hq, hk, d = 6, 4, 2, 128
+    qkv, _ = _inputs(tokens, hq, hk, d, 3)
+    q, k = qkv[:, : hq * d].view(tokens, hq, d), qkv[:, hq * d : (hq + hk) * d].reshape(tokens, hk, d)
+    for dtype in (torch.float32, torch.bfloat16):
+        table = _table(70000, 128, dtype)
+        pos = torch.tensor([-1, 0, 1, 69999, 70000, 1 << 40])
+        a, b = torch.ops.tt.qk_norm_rope(q.cuda(), k.cuda(), table.cuda(), pos.cuda())
+        _check(a, q, None, table, pos, 1e-6, False)
+        _check(b, k, None, table, pos, 1e-6, False)
+        assert torch.equal(a[0].cpu(), q[0]) and torch.equal(a[4].cpu(), q[4])  # no norm, not turned: a copy
+
+
+@pytest.mark.parametrize("gain", [0.0, 1e-18, 1e18])
+def test_rows_of_zeros_and_of_extreme_size(gain):
+    """Squares of 10^18 add up to 10^38 below the largest float; eps keeps rows of zeros finite."""
+    qkv, g = _inputs(9, 4, 2, 64, 11, gain)
+    q, k = qkv[:, :256].view(9, 4, 64), qkv[:, 256:384].reshape(9, 2, 64)
+    w = torch.ones(64, dtype=torch.bfloat16)
+    table, pos = _table(16, 64), torch.arange(9)
+    a, b = torch.ops.tt.qk_norm_rope(q.cuda(), k.cuda(), table.cuda(), pos.cuda(), w.cuda(), w.cuda(), 1e-30)
+    _check(a, q, w, table, pos, 1e-30, False)
+    _check(b, k, w, table, pos, 1e-30, False)
+
+
+def test_rows_that_vector_loads_cannot_take():
+    """Odd strides and bases: copies inside the call, the same result in place."""
+    g = torch.Generator().manual_seed(5)
+    base = torch.randn(3 * (5 * 64 + 3) + 1, generator=g).to(torch.bfloat16).cuda()
+    q = base[1:].as_strided((3, 3, 64), (5 * 64 + 3, 64, 1), 1)
+    k = base[1:].as_strided((3, 2, 64), (5 * 64 + 3, 64, 1), 1 + 3 * 64)
+    table, pos = _table(8, 64), torch.tensor([7, 0, 3])
+    want = torch.ops.tt.qk_norm_rope(q.contiguous(), k.contiguous(), table.cuda(), pos.cuda())
+    got = torch.ops.tt.qk_norm_rope(q, k, table.cuda(), pos.cuda())
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    torch.ops.tt.qk_norm_rope_(q, k, table.cuda(), pos.cuda())
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+
+
+def test_no_tokens():
+    q, k = torch.empty(0, 4, 64, dtype=torch.bfloat16, device="cuda"), torch.empty(0, 2, 64, dtype=torch.bfloat16, device="cuda")
+    a, b = torch.ops.tt.qk_norm_rope(q, k, _table(4, 64).cuda(), torch.empty(0, dtype=torch.int32, device="cuda"))
+    assert a.shape == q.shape and b.shape == k.shape
+
+
+def test_refusals():
+    z = dict(device="cuda")
+    q, k = torch.zeros(2, 4, 64, dtype=torch.bfloat16, **z), torch.zeros(2, 2, 64, dtype=torch.bfloat16, **z)
+    table, pos = _table(4, 64).cuda(), torch.zeros(2, dtype=torch.int32, **z)
+    op = torch.ops.tt.qk_norm_rope
+    bad = [
+        (q.float(), k, table, pos), (q, k.half(), table, pos), (q[0], k, table, pos), (q, k[:1], table, pos),
+        (q, k, table.half(), pos), (q, k, table[0], pos), (q, k, table[:, :24], pos), (q, k, torch.zeros(4, 80, **z), pos),
+        (q, k, table, pos[:1]), (q, k, table, pos.float()), (q, k, table, pos, torch.ones(32, **z)),
+        (q, k, table, pos, torch.ones(64, dtype=torch.float64, **z)),
+    ]
+    for args in bad:
+        with pytest.raises(ValueError):
+            op(*args)
+    with pytest.raises(RuntimeError):  # a head size without a kernel
+        op(torch.zeros(2, 4, 96, dtype=torch.bfloat16, **z), torch.zeros(2, 2, 96, dtype=torch.bfloat16, **z), table, pos)
+    with pytest.raises(RuntimeError):
+        op(q, k, table, pos, None, None, -1.0)
+    with pytest.raises(NotImplementedError):
+        op(q, k, table.cpu(), pos)
+    with pytest.raises(NotImplementedError):
+        op(q.clone().requires_grad_(), k, table, pos)
+    with torch.no_grad():
+        op(q.clone().requires_grad_(), k, table, pos)

@@ -1,0 +1,141 @@
+// Attention of a prompt's chunk over the 8-bit cache: the blocks that the pass reads become bfloat16 copies in the caller's scratch
+// (exactly: an element times its block's power of two is a bfloat16 value), and the bfloat16 prefill kernels run over the copies.
+//
+// A chunk is bound by its matrix products, 4 D q_heads operations per (row, key) pair, and every workgroup of 128 rows reads every key, so keys
+// are expanded once here and not once per workgroup; the copies cost 1 byte read and 2 written per element.  Memory bound: a
+// wavefront asks for four pieces of 512 elements before it writes the first.
+//
+// The prefill kernels take keys by tiles of 64 and give what is behind the last row's own position weight zero, whatever it is, so it has to be
+// numbers: rows behind the chunk are copied as zeros, up to the end of the tile, and block 0 of the copies, which stands in for
+// whatever the table does not hold, is zeros.
+#include "fp8.h"
+
+#include <algorithm>
+
+namespace ttpa {
+namespace fp8 {
+int check_cache(const void *k_cache, const void *v_cache, const float *k_scales, const float *v_scales, const int32_t *page_table, int kv_heads,
+                int head_size, int block_size, int table_width, int num_blocks);
+
+namespace {
+
+struct ExpandArgs {
+  const uint8_t *k, *v;
+  const float *k_scales, *v_scales;
+  uint16_t *k_copy, *v_copy;  // [1 + batch * width][kv_heads][block_size][head_size]
+  int32_t *table;             // [batch][width]: the copies' page table
+  const int32_t *pt;
+  int64_t pt_rs;
+  const int32_t *chunk_start;
+  int batch, w, hkv, bs, nb, q_len, d;
+};
+
+constexpr int kExpandWorkgroups = 2048, kPieces = 4;
+
+__global__ __launch_bounds__(256) void fp8_expand_kernel(ExpandArgs e) {
+  // keys 0 .. chunk_start + q_len - 1 are read, in tiles of 64
+  const int64_t end = (int64_t)(e.chunk_start ? max(*e.chunk_start, 0) : 0) + e.q_len;
+  const int cols = (int)min((int64_t)e.w, ((end + 63) / 64 * 64 + e.bs - 1) / e.bs);
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)e.batch * e.w; i += (int64_t)gridDim.x * 256)
+    e.table[i] = (int)(i % e.w) < cols ? (int)i + 1 : 0;
+  const int per_slab = e.bs * e.d / 512;  // pieces of 64 lanes x 8 elements
+  const uint32_t slabs = 2u * e.hkv, per_block = slabs * per_slab;
+  const int64_t pieces = ((int64_t)e.batch * cols + 1) * per_block;
+  const int lane = threadIdx.x & 63;
+  const int64_t step = (int64_t)gridDim.x * 4 * kPieces;
+  for (int64_t at = ((int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6)) * kPieces; at < pieces; at += step) {
+    u32x2 raw[kPieces];
+    float scale[kPieces];
+    bool zero[kPieces];
+    uint16_t *dst[kPieces];
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j) {
+      const int64_t p = min(at + j, pieces - 1);
+      const uint32_t r = (uint32_t)(p / per_block), in_block = (uint32_t)(p - (int64_t)r * per_block);
+      const uint32_t slab = in_block / per_slab, element = 512 * (in_block - slab * per_slab) + 8 * lane;
+      // r = 0: the block of zeros; then the users' columns
+      const int b = r ? (int)((r - 1) / (uint32_t)cols) : 0, col = r ? (int)(r - 1 - (uint32_t)b * cols) : 0;
+      const int64_t x = r ? (int64_t)b * e.w + col + 1 : 0;
+      const bool is_v = slab >= (uint32_t)e.hkv;
+      const int h = (int)slab - (is_v ? e.hkv : 0);
+      int phys = e.pt[(int64_t)b * e.pt_rs + col];
+      if ((unsigned)phys >= (unsigned)e.nb) phys = 0;
+      const int64_t from = (int64_t)phys * e.hkv + h, elements = (int64_t)e.bs * e.d;
+      raw[j] = *reinterpret_cast<const u32x2 *>((is_v ? e.v : e.k) + from * elements + element);
+      scale[j] = (is_v ? e.v_scales : e.k_scales)[from];
+      zero[j] = r == 0 || (int64_t)col * e.bs + (int)(element / (uint32_t)e.d) >= end;
+      dst[j] = (is_v ? e.v_copy : e.k_copy) + (x * e.hkv + h) * elements + element;
+    }
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j)
+      if (at + j < pieces) *reinterpret_cast<u32x4 *>(dst[j]) = zero[j] ? u32x4{0, 0, 0, 0} : decode8(raw[j].x, raw[j].y, scale[j]);
+  }
+}
+
+struct ChunkLayout {
+  int width;       // columns of the copies
+  int64_t copy, table, parts;
+};
+ChunkLayout chunk_layout(int batch, int q_heads, int kv_heads, int q_len, int head_size, int block_size, int table_width, int64_t most_keys) {
+  ChunkLayout l;
+  const int64_t keys = most_keys > 0 ? std::min<int64_t>(most_keys, (int64_t)table_width * block_size) : (int64_t)table_width * block_size;
+  l.width = (int)((keys + block_size - 1) / block_size);
+  l.copy = ((int64_t)batch * l.width + 1) * kv_heads * block_size * head_size * 2;
+  l.table = ((int64_t)batch * l.width * 4 + 255) / 256 * 256;
+  l.parts = ttpa_sdpa_prefill_bounded_scratch_bytes(batch, q_heads, kv_heads, q_len, head_size, block_size, l.width, TTPA_KV_BF16, most_keys);
+  return l;
+}
+
+}  // namespace
+}  // namespace fp8
+}  // namespace ttpa
+
+using namespace ttpa;
+
+extern "C" int64_t ttpa_chunked_fp8_attention_workspace_bytes(int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t q_len, int32_t head_size,
+                                                              int32_t block_size, int32_t table_width, int64_t most_keys) {
+  if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || q_len <= 0 || head_size <= 0 || block_size <= 0 || table_width <= 0)
+    return 0;
+  const fp8::ChunkLayout l = fp8::chunk_layout(batch, q_heads, kv_heads, q_len, head_size, block_size, table_width, most_keys);
+  return 2 * l.copy + l.table + l.parts;
+}
+
+extern "C" int ttpa_chunked_fp8_attention(void *out, int64_t out_batch_stride, int64_t out_head_stride, int64_t out_token_stride, const void *q,
+                                          int64_t q_batch_stride, int64_t q_head_stride, int64_t q_token_stride, const void *k_cache,
+                                          const void *v_cache, const float *k_scales, const float *v_scales, const int32_t *page_table,
+                                          int64_t page_table_row_stride, const int32_t *chunk_start, int32_t batch, int32_t q_heads,
+                                          int32_t kv_heads, int32_t q_len, int32_t head_size, int32_t block_size, int32_t table_width,
+                                          int32_t num_blocks, float scale, int64_t most_keys, void *workspace, int64_t workspace_bytes,
+                                          void *stream) {
+  if (int rc = fp8::check_cache(k_cache, v_cache, k_scales, v_scales, page_table, kv_heads, head_size, block_size, table_width, num_blocks)) return rc;
+  TTPA_REQUIRE(out && q, "fp8 chunk: null pointer argument");
+  TTPA_REQUIRE(batch > 0 && q_heads > 0 && q_len > 0 && most_keys >= 0, "fp8 chunk: non-positive dimension");
+  TTPA_REQUIRE(q_heads % kv_heads == 0, "fp8 chunk: q_heads %d not divisible by kv_heads %d", q_heads, kv_heads);
+  if (block_size % 32) return fail(TTPA_ERR_UNSUPPORTED, "fp8 chunk: block_size %d must be a multiple of 32", block_size);
+  const fp8::ChunkLayout l = fp8::chunk_layout(batch, q_heads, kv_heads, q_len, head_size, block_size, table_width, most_keys);
+  const int64_t need = 2 * l.copy + l.table + l.parts;
+  if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u))
+    return fail(TTPA_ERR_WORKSPACE, "fp8 chunk: workspace of %lld bytes (256-byte aligned) required, got %lld", (long long)need,
+                (long long)workspace_bytes);
+  TTPA_REQUIRE((int64_t)batch * l.width < (1ll << 31) - 2, "fp8 chunk: too many blocks");
+  uint8_t *ws = static_cast<uint8_t *>(workspace);
+  fp8::ExpandArgs e = {static_cast<const uint8_t *>(k_cache), static_cast<const uint8_t *>(v_cache), k_scales, v_scales,
+                       reinterpret_cast<uint16_t *>(ws), reinterpret_cast<uint16_t *>(ws + l.copy), reinterpret_cast<int32_t *>(ws + 2 * l.copy),
+                       page_table, page_table_row_stride, chunk_start, batch, l.width, kv_heads, block_size, num_blocks, q_len, head_size};
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const int64_t pieces = ((int64_t)batch * l.width + 1) * 2 * kv_heads * (block_size * head_size / 512);
+  // armed events: the pair brackets both launches
+  hipEvent_t before, after;
+  take_profile_events(before, after);
+  const dim3 grid((unsigned)std::min<int64_t>((pieces + 4 * fp8::kPieces - 1) / (4 * fp8::kPieces), fp8::kExpandWorkgroups));
+  if (before)
+    hipExtLaunchKernelGGL(fp8::fp8_expand_kernel, grid, dim3(256), 0u, st, before, nullptr, 0u, e);
+  else
+    fp8::fp8_expand_kernel<<<grid, dim3(256), 0, st>>>(e);
+  if (const int rc = check_launch("fp8 chunk (expansion)")) return rc;
+  if (after) arm_profile_events(nullptr, after);
+  return ttpa_sdpa_prefill_bounded(out, out_batch_stride, out_head_stride, out_token_stride, q, q_batch_stride, q_head_stride, q_token_stride,
+                                   e.k_copy, e.v_copy, 0, 0, 0, e.table, l.width, chunk_start, nullptr, 0, 0, batch, q_heads, kv_heads, q_len,
+                                   l.width * block_size, head_size, block_size, l.width, batch * l.width + 1, 1, scale, 0, TTPA_KV_BF16, most_keys,
+                                   l.parts ? ws + 2 * l.copy + l.table : nullptr, l.parts, stream);
+}

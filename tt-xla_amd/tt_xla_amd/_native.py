@@ -149,6 +149,42 @@ SIGNATURES = {
          _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32,
          _p, _p, _p, _i64, _p, _int, _i32, _i32, _i32, _i32, _p],
     ),
+    "ttpa_qk_norm_rope": (
+        _int,
+        [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _int, _i64, _i64, _p, _int, _p, _p, _int, _f32,
+         _i32, _i32, _i32, _i32, _i32, _int, _p],
+    ),
+    "ttpa_qk_norm_rope_update_fp8": (
+        _int,
+        [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _int, _i64, _i64, _p, _int, _p, _p, _int, _f32,
+         _p, _p, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _i32, _int, _i32, _i32, _i32, _p],
+    ),
+    "ttpa_paged_update_fp8_cache": (
+        _int,
+        [_p, _p, _p, _p, _p, _p, _i64, _i64, _p, _i64, _i64, _p, _int, _p, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _p],
+    ),
+    "ttpa_paged_fill_fp8_cache": (
+        _int,
+        [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _p, _int, _i32, _i32, _i32, _i32, _i32,
+         _i32, _i32, _i32, _p],
+    ),
+    "ttpa_paged_fp8_decode": (
+        _int,
+        [_p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _p, _p, _i64, _p, _int, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32,
+         _i32, _p, _p, _sz, _p],
+    ),
+    "ttpa_paged_fp8_sparse_decode_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32]),
+    "ttpa_paged_fp8_sparse_decode": (
+        _int,
+        [_p, _i64, _p, _p, _i64, _p, _p, _p, _p, _p, _p, _i64, _p, _int, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32,
+         _p, _sz, _p],
+    ),
+    "ttpa_chunked_fp8_attention_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i64]),
+    "ttpa_chunked_fp8_attention": (
+        _int,
+        [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _p, _p, _p, _i64, _p, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
+         _i32, _f32, _i64, _p, _i64, _p],
+    ),
     "ttpa_bfp8_quantize": (_int, [_p, _p, _p, _i64, _p]),
     "ttpa_bfp8_dequantize": (_int, [_p, _p, _p, _i64, _p]),
 }
