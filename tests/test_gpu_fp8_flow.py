@@ -1,0 +1,239 @@
+"""The operators around the 8-bit cache together, as a serving program runs them: prompts, chunks and steps through the attention
+backend; steps with norm, rotation and write in one launch, sparse steps, captured steps, several streams.  The caches are compared with
+their definition (equal), attention with softmax in 64 bits over what the caches stand for (tolerance as in the operators' own tests)."""
+
+import pytest
+import torch
+
+import __graft_entry__ as entry
+import fp8_reference as R
+from test_gpu_fp8_chunk import _check as check_chunk
+from test_gpu_fp8_decode import _bounds, _check, _check_sparse, _setup
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _pkg():
+    entry.ensure_built()
+    import tt_xla_amd  # noqa: F401
+
+
+def _layer(nb, hkv, bs, d, bounds=True):
+    from tt_xla_amd import TTAttentionBackend as B, fp8_ops
+
+    k, ks = fp8_ops.fp8_empty_cache(nb, hkv, bs, d, "cuda")
+    v, vs = fp8_ops.fp8_empty_cache(nb, hkv, bs, d, "cuda")
+    b = fp8_ops.fp8_empty_key_bounds(nb, hkv, d, "cuda")
+    assert tuple(k.shape) == B.get_kv_cache_storage_shape(nb, bs, hkv, d, "fp8_e4m3")
+    assert tuple(ks.shape) == B.get_kv_cache_scale_shape(nb, hkv) and tuple(b.shape) == B.get_kv_cache_bounds_shape(nb, hkv, d)
+    return [k, v, ks, vs, b] if bounds else [k, v, ks, vs]
+
+
+@pytest.mark.parametrize("hq, hkv, d, bs", [(8, 2, 64, 32), (32, 8, 128, 64), (4, 4, 256, 32)])
+@pytest.mark.parametrize("sparse", [None, 3])
+@pytest.mark.parametrize("aligned", [True, False])
+def test_backend_prompt_chunk_and_steps(hq, hkv, d, bs, sparse, aligned):
+    from tt_xla_amd import TTAttentionBackendImpl, TTMetadata
+
+    users, first, chunk, steps = 2, 2 * bs, bs, bs + 3
+    g = torch.Generator().manual_seed(d)
+    width = 6
+    kv = _layer(users * width + 1, hkv, bs, d)
+    want = R.Cache(*kv)
+    table = (torch.randperm(users * width, generator=g) + 1).view(users, width).int()
+    impl = TTAttentionBackendImpl(hq, d, d**-0.5, hkv, kv_cache_dtype="fp8_e4m3", sparse_kept_blocks=sparse)
+    assert impl.kv_cache_quantized_dtype == torch.float8_e4m3fn
+    batch_idx = torch.arange(users, dtype=torch.int32).cuda()
+
+    def tokens(n):
+        return [torch.randn(users, n, h, d, generator=g).to(torch.bfloat16) for h in (hq, hkv, hkv)]
+
+    def forward(q, k, v, meta):
+        n = q.shape[0] * q.shape[1] * hq * d
+        out = torch.empty(n, dtype=torch.bfloat16, device="cuda") if aligned else torch.empty(n + 1, dtype=torch.bfloat16, device="cuda")[1:]
+        impl.forward(None, *(t.flatten(0, 1).flatten(1).cuda() for t in (q, k, v)), kv, meta, output=out.view(-1, hq * d))
+        return out.cpu().view(q.shape)
+
+    want.b = torch.zeros(users * width + 1, hkv, 2, d, dtype=torch.float64)
+    # a first chunk attends its own keys and values as they are
+    q, k, v = tokens(first)
+    out = forward(q, k, v, TTMetadata(page_table=table.cuda(), batch_idx=batch_idx, num_users=users))
+    want.fill(k.transpose(1, 2), v.transpose(1, 2), table, range(users))
+    assert want.differences(*kv) == {}
+    allowed = torch.arange(first)[None, :] <= torch.arange(first)[:, None]
+    for h in range(0, hq, 3):
+        one, size = R.softmax_rows(q[1, :, h], k[1, :, h * hkv // hq].double(), v[1, :, h * hkv // hq].double(), allowed, d**-0.5)
+        assert bool(((out[1, :, h].double() - one).abs() <= 2.0**-8 * one.abs() + 0.0085 * size).all())
+    # a continuation chunk attends the cache
+    q, k, v = tokens(chunk)
+    rolled = torch.roll(table, -(first // bs), 1)
+    out = forward(q, k, v, TTMetadata(page_table=table.cuda(), fill_page_table=rolled.contiguous().cuda(), batch_idx=batch_idx, num_users=users,
+                                      chunk_start_idx=torch.tensor([first], dtype=torch.int32).cuda(), chunk_end=first + chunk))
+    want.fill(k.transpose(1, 2), v.transpose(1, 2), rolled, range(users))
+    assert want.differences(*kv) == {}
+    cache = [t.cpu() for t in kv[:4]]
+    check_chunk(out.transpose(1, 2), q.transpose(1, 2), cache, table, first, d**-0.5)
+    # steps; a padded row among them
+    pad = torch.zeros(1, width, dtype=torch.int32)
+    for s in range(steps):
+        q, k, v = (torch.cat([t, t[:1]]) for t in tokens(1))
+        pos = torch.tensor([first + chunk + s] * users + [-1], dtype=torch.int32)
+        tables = torch.cat([table, pad])
+        out = forward(q, k, v, TTMetadata(cache_position=pos.cuda(), page_table=tables.cuda(), num_users=users + 1))
+        want.update(k[:, 0], v[:, 0], pos, tables)
+        if s % 8 == 0 or s == steps - 1:
+            assert want.differences(*kv) == {}
+            cache = [t.cpu() for t in kv[:4]]
+            chosen = None
+            if sparse:
+                chosen = [[R.choose(q[u, 0, h * hq // hkv : (h + 1) * hq // hkv], kv[4].cpu(), tables[u].tolist(), h, int(pos[u]) // bs + 1, sparse)
+                           for h in range(hkv)] for u in range(users)] + [None]
+            _check(out[:, 0], q[:, 0], cache, tables, pos, d**-0.5, columns=chosen)
+
+
+def test_backend_windows_sinks_and_a_shared_cache():
+    from tt_xla_amd import TTAttentionBackendImpl, TTMetadata
+
+    hq, hkv, d, bs, users = 8, 2, 64, 32, 3
+    cache, table, cur, q, g = _setup(users, hkv, hq // hkv, d, bs, [100, 5, 64], 3)
+    kv = [t.cuda() for t in cache]
+    sink = torch.randn(hq, generator=g)
+    impl = TTAttentionBackendImpl(hq, d, 0.2, hkv, sliding_window=40, sinks=sink.cuda(), kv_cache_dtype="fp8", kv_sharing_target_layer_name="other")
+    out = torch.empty(users, hq * d, dtype=torch.bfloat16, device="cuda")
+    new = torch.randn(users, hkv * d, generator=g).to(torch.bfloat16).cuda()
+    before = [t.clone() for t in kv]
+    impl.forward(None, q.flatten(1).cuda(), new, new, kv, TTMetadata(cache_position=cur.cuda(), page_table=table.cuda(), num_users=users), output=out)
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(kv, before))
+    _check(out.cpu().view(users, hq, d), q, cache, table, cur, 0.2, 40, sink)
+    # a prompt over keys and values that another layer has written
+    impl = TTAttentionBackendImpl(hq, d, 0.2, hkv, kv_cache_dtype="fp8", kv_sharing_target_layer_name="other")
+    q = torch.randn(32, hq * d, generator=g).to(torch.bfloat16)
+    out = torch.empty(32, hq * d, dtype=torch.bfloat16, device="cuda")
+    impl.forward(None, q.cuda(), new[:1].repeat(32, 1), new[:1].repeat(32, 1), kv,
+                 TTMetadata(page_table=table[:1].cuda(), num_users=1, batch_idx=torch.zeros(1, dtype=torch.int32).cuda()), output=out)
+    check_chunk(out.cpu().view(1, 32, hq, d).transpose(1, 2), q.view(1, 32, hq, d).transpose(1, 2), cache, table[:1], 0, 0.2)
+    for bad in (dict(is_causal=False), dict(attn_mask=torch.zeros(1, device="cuda"))):
+        with pytest.raises(NotImplementedError):
+            impl.forward(None, q.cuda(), new, new, kv, TTMetadata(page_table=table.cuda(), num_users=1, **bad), output=out)
+    with pytest.raises(ValueError):
+        impl.forward(None, q.cuda(), new, new, kv[:2], TTMetadata(page_table=table.cuda(), num_users=1), output=out)
+
+
+def _step(state, sparse):
+    """Norm, rotation, write and attention of one step, as a layer runs them."""
+    tt = torch.ops.tt
+    q = tt.qk_norm_rope_update_fp8_(state["q"], state["k"], state["v"], state["angles"], state["pos"], *state["kv"][:4], state["table"],
+                                    state["qw"], state["kw"], state["kv"][4])
+    if sparse:
+        return tt.paged_fp8_sparse_attention_decode(q[None], *state["kv"], state["table"], state["pos"], 4)[0]
+    return tt.paged_fp8_attention_decode(q[None], *state["kv"][:4], state["table"], state["pos"])
+
+
+def _state(seed, users=9, hq=16, hkv=4, d=128, bs=32):
+    from tt_xla_amd.fp8_ops import rope_table
+
+    lengths = [1 + (37 * u * u) % 400 for u in range(users)]
+    cache, table, cur, q, g = _setup(users, hkv, hq // hkv, d, bs, lengths, seed)
+    kv = [*cache, _bounds(cache)]
+    s = {"q": q, "k": torch.randn(users, hkv, d, generator=g).to(torch.bfloat16), "v": torch.randn(users, hkv, d, generator=g).to(torch.bfloat16),
+         "qw": 1 + torch.rand(d, generator=g), "kw": 1 + torch.rand(d, generator=g), "angles": rope_table(512, d), "pos": cur, "table": table}
+    on = {n: t.cuda() for n, t in s.items()}
+    on["kv"] = [t.cuda() for t in kv]
+    return on
+
+
+@pytest.mark.parametrize("sparse", [False, True])
+def test_a_step_of_a_layer(sparse):
+    s = _state(1)
+    want = R.Cache(*s["kv"])
+    turned = R.turn(s["k"].cpu(), s["kw"].cpu(), s["angles"].cpu(), s["pos"].cpu(), 1e-6, False)
+    got_k = torch.ops.tt.qk_norm_rope(s["q"], s["k"], s["angles"], s["pos"], s["qw"], s["kw"])
+    assert float((got_k[1].cpu().double() - turned).abs().max()) <= 2.0**-7 * float(turned.abs().max())
+    want.update(got_k[1], s["v"], s["pos"].cpu(), s["table"].cpu())
+    out = _step(s, sparse)
+    assert want.differences(*s["kv"]) == {}
+    cache, q = [t.cpu() for t in s["kv"][:4]], got_k[0].cpu()
+    if sparse:
+        _, cols = torch.ops.tt.paged_fp8_sparse_attention_decode(got_k[0][None], *s["kv"], s["table"], s["pos"], 4)
+        _check_sparse(out[0].cpu(), cols.cpu(), q, cache, s["kv"][4].cpu(), s["table"].cpu(), s["pos"].cpu(), 4, 128**-0.5)
+    else:
+        _check(out[0].cpu(), q, cache, s["table"].cpu(), s["pos"].cpu(), 128**-0.5)
+
+
+@pytest.mark.parametrize("sparse", [False, True])
+def test_captured_steps(sparse):
+    """Two graphs in one process, replayed between eager steps on other tensors; every replay against an eager step on a copy."""
+    states = [_state(2), _state(3, users=5, hq=8, hkv=8)]
+    graphs, outs = [], []
+    for s in states:
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        start = [t.clone() for t in s["kv"]]
+        with torch.cuda.stream(side):
+            _step(s, sparse)
+        torch.cuda.current_stream().wait_stream(side)
+        for t, b in zip(s["kv"], start):
+            t.view(torch.uint8).copy_(b.view(torch.uint8))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(_step(s, sparse))
+        graphs.append(graph)
+    g = torch.Generator().manual_seed(7)
+    for n in range(6):
+        for s, graph, out in zip(states, graphs, outs):
+            s["pos"] += 1
+            for t in ("q", "k", "v"):
+                s[t].copy_(torch.randn(s[t].shape, generator=g).to(torch.bfloat16))
+            s["table"][:, :] = torch.where(s["table"] < 0, 0, s["table"])
+            copy = dict(s, kv=[t.clone() for t in s["kv"]])
+            graph.replay()
+            want = _step(copy, sparse)
+            if n % 2:
+                torch.cuda.synchronize()
+            assert torch.equal(out, want)
+            assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(s["kv"], copy["kv"]))
+
+
+def test_calls_on_other_streams():
+    """Steps of two layers at once on streams of their own, without waits between them."""
+    states = [_state(4), _state(5)]
+    want = []
+    for s in states:
+        copy = dict(s, kv=[t.clone() for t in s["kv"]])
+        want.append([_step(copy, True).clone() for _ in range(3)] + [_step(copy, False).clone() for _ in range(3)])
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in states]
+    got = [[], []]
+    for n in range(6):
+        for i, (s, st) in enumerate(zip(states, streams)):
+            with torch.cuda.stream(st):
+                got[i].append(_step(s, n < 3))
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_equal_calls_give_equal_results():
+    s = _state(6)
+    first = _step(s, False).clone(), _step(s, True).clone()
+    for _ in range(5):
+        assert torch.equal(_step(s, False), first[0]) and torch.equal(_step(s, True), first[1])
+
+
+def test_tracing_sees_shapes():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    s = _state(8)
+    q = s["q"][None]
+    with FakeTensorMode() as mode:
+        f = {n: mode.from_tensor(t) for n, t in s.items() if n != "kv"}
+        kv = [mode.from_tensor(t) for t in s["kv"]]
+        fq = mode.from_tensor(q)
+        tt = torch.ops.tt
+        assert tt.paged_fp8_attention_decode(fq, *kv[:4], f["table"], f["pos"]).shape == q.shape
+        out, cols = tt.paged_fp8_sparse_attention_decode(fq, *kv, f["table"], f["pos"], 4)
+        assert out.shape == q.shape and cols.shape == (9, 4, 4) and cols.dtype == torch.int32
+        assert tt.qk_norm_rope_update_fp8_(f["q"], f["k"], f["v"], f["angles"], f["pos"], *kv[:4], f["table"]).shape == f["q"].shape
+        a, b = tt.qk_norm_rope(f["q"], f["k"], f["angles"], f["pos"])
+        assert a.shape == f["q"].shape and b.shape == f["k"].shape

@@ -29,6 +29,7 @@ import torch
 
 from . import _native
 from . import custom_ops  # noqa: F401  (registers torch.ops.tt.*)
+from . import fp8_ops
 
 try:  # pragma: no cover - vLLM is not part of the test image
     from vllm.v1.attention.backend import AttentionBackend as _BackendBase
@@ -171,6 +172,18 @@ class TTAttentionBackend(_BackendBase):
         return (num_blocks, num_kv_heads, block_size, head_size)
 
     @staticmethod
+    def get_kv_cache_scale_shape(num_blocks: int, num_kv_heads: int) -> tuple:
+        """Shape of the float32 scales that go with one 8-bit cache (``kv_cache_dtype="fp8_e4m3"``: elements of
+        ``torch.float8_e4m3fn`` in ``get_kv_cache_shape``, one power of two per block and head).  A layer's kv_cache is then
+        [k, v, k_scales, v_scales], or with ``get_kv_cache_bounds_shape``'s tensor behind them."""
+        return (num_blocks, num_kv_heads)
+
+    @staticmethod
+    def get_kv_cache_bounds_shape(num_blocks: int, num_kv_heads: int, head_size: int) -> tuple:
+        """Shape of the bfloat16 bounds of every block's keys, which sparse decode over an 8-bit cache reads."""
+        return (num_blocks, num_kv_heads, 2, head_size)
+
+    @staticmethod
     def swap_blocks(src_kv_cache, dst_kv_cache, src_to_dst) -> None:
         raise RuntimeError("swap_blocks is not used for the TPU backend.")
 
@@ -221,7 +234,10 @@ class TTAttentionBackendImpl(_ImplBase):
         kv_sharing_target_layer_name: Optional[str] = None,
         sinks: Optional[torch.Tensor] = None,
         functional_cache_ops: bool = False,
+        sparse_kept_blocks: Optional[int] = None,
     ) -> None:
+        """sparse_kept_blocks: decode passes over an 8-bit cache with key bounds attend that many blocks of each context, chosen
+        per KV head, instead of all of them."""
         self.num_heads = num_heads
         self.head_size = head_size
         self.scale = float(scale)
@@ -231,6 +247,7 @@ class TTAttentionBackendImpl(_ImplBase):
         self.kv_sharing_target_layer_name = kv_sharing_target_layer_name
         self.num_queries_per_kv = num_heads // num_kv_heads
         self.functional_cache_ops = functional_cache_ops
+        self.sparse_kept_blocks = sparse_kept_blocks
         if alibi_slopes is not None:
             raise NotImplementedError("Alibi slopes is not supported.")
         if attn_type not in (_DECODER, _ENCODER, _ENCODER_ONLY):
@@ -266,6 +283,9 @@ class TTAttentionBackendImpl(_ImplBase):
         the result is written into ``output`` [tokens, Hq*D]."""
         assert attn_metadata is not None, "TT attention requires metadata."
         assert output is not None, "TT attention requires an output buffer."
+        if isinstance(kv_cache, (list, tuple)) and kv_cache[0].dtype == torch.float8_e4m3fn:
+            self._fp8_pass(query, key, value, kv_cache, attn_metadata, output)
+            return
         if self._native_pass(query, key, value, kv_cache, attn_metadata, output):
             return
         inputs = self._prepare_inputs(query, key, value, attn_metadata)
@@ -354,6 +374,57 @@ class TTAttentionBackendImpl(_ImplBase):
         if status != 0:
             _native.check(*status)
         return True
+
+    def _fp8_pass(self, query, key, value, kv_cache, attn_metadata: TTMetadata, output) -> None:
+        """A causal pass over an 8-bit cache, kv_cache = [k, v, k_scales, v_scales] or with key bounds behind them: the cache write and
+        the attention, as operators that write into ``output`` where it can be viewed that way."""
+        if not attn_metadata.is_causal or attn_metadata.attn_mask is not None:
+            raise NotImplementedError("attention over an 8-bit cache is built for causal passes without a mask")
+        if self.functional_cache_ops:
+            raise NotImplementedError("an 8-bit cache is written in place")
+        if len(kv_cache) not in (4, 5):
+            raise ValueError("an 8-bit kv_cache is [k, v, k_scales, v_scales] or with key bounds behind them")
+        ops, cache, bounds = torch.ops.tt, tuple(kv_cache[:4]), kv_cache[4] if len(kv_cache) == 5 else None
+        inputs = self._prepare_inputs(query, key, value, attn_metadata)
+        shared = self.kv_sharing_target_layer_name is not None
+        writes = not shared and cache[0].numel() > 0  # (an empty cache stands in while vLLM profiles memory)
+        out = self._output_view(output, inputs)
+        into = torch.empty(inputs.query.shape, dtype=query.dtype, device=query.device) if out is None else out
+        if not inputs.is_prefill:
+            positions, table = attn_metadata.cache_position, attn_metadata.page_table
+            if writes:
+                ops.paged_update_fp8_cache_(*cache, inputs.key.transpose(0, 1), inputs.value.transpose(0, 1), positions, table, bounds)
+            q, target = inputs.query.transpose(0, 1), into.transpose(0, 1)
+            if self.sparse_kept_blocks is not None:
+                if bounds is None or self.sinks is not None or self.sliding_window is not None:
+                    raise NotImplementedError("sparse decode needs key bounds, and is built without sinks and sliding windows")
+                ops.paged_fp8_sparse_attention_decode_out(q, *cache, bounds, table, positions, target, self.sparse_kept_blocks, scale=self.scale)
+            else:
+                ops.paged_fp8_attention_decode_out(q, *cache, table, positions, target, attention_sink=self.sinks, scale=self.scale,
+                                                   sliding_window_size=self.sliding_window)
+        else:
+            assert self.sinks is None, "Attention sink is unsupported in SDPA prefill"
+            k, v = inputs.key.transpose(1, 2), inputs.value.transpose(1, 2)
+            if writes:
+                batch_idx = attn_metadata.batch_idx
+                assert batch_idx is not None, "batch_idx must be provided for prefill."
+                if attn_metadata.dp_size > 1:
+                    batch_idx = batch_idx % (k.shape[0] // attn_metadata.dp_size)
+                ops.paged_fill_fp8_cache_(*cache, k, v, attn_metadata.fill_page_table, batch_idx, bounds)
+            q, target = inputs.query.transpose(1, 2), into.transpose(1, 2)
+            if attn_metadata.chunk_start_idx is not None and writes:
+                # (what a graph captures is replayed for other chunks: it has to have room for all that the table holds)
+                known = 0 if torch.cuda.is_current_stream_capturing() else attn_metadata.chunk_end or 0
+                ops.chunked_fp8_attention_out(q, *cache, attn_metadata.page_table, attn_metadata.chunk_start_idx, target,
+                                              scale=self.scale, most_keys=known)
+            else:
+                if shared:
+                    k = self._gather_paged_to_dense(cache[0], attn_metadata.page_table, inputs.kv_num_tokens, cache[2])
+                    v = self._gather_paged_to_dense(cache[1], attn_metadata.page_table, inputs.kv_num_tokens, cache[3])
+                ops.scaled_dot_product_attention_out(q, k, v, target, is_causal=True, scale=self.scale,
+                                                     sliding_window_size=self.sliding_window)
+        if out is None:
+            output.copy_(into.reshape(-1, self.num_heads * self.head_size).reshape_as(output))
 
     def _output_view(self, output: torch.Tensor, inputs) -> Optional[torch.Tensor]:
         """``output`` as [users, tokens, heads, head_size] without a copy, or None."""
@@ -488,15 +559,20 @@ class TTAttentionBackendImpl(_ImplBase):
         out = torch.ops.tt.scaled_dot_product_attention(q, k, v, **kwargs)
         return out.transpose(-3, -2)  # [users, tokens, Hq, D]
 
-    def _gather_paged_to_dense(self, cache: torch.Tensor, page_table: torch.Tensor, num_tokens: int):
+    def _gather_paged_to_dense(self, cache: torch.Tensor, page_table: torch.Tensor, num_tokens: int,
+                               scales: Optional[torch.Tensor] = None):
         """[NB, Hkv, bs, D] -> [users, Hkv, num_tokens, D] in page-table order (a block-float-8
-        cache comes out as the bfloat16 values it encodes)."""
+        or 8-bit cache, the latter with its scales, comes out as the bfloat16 values it stands for)."""
         users, width = page_table.shape
         # ids outside the cache (padding -1, stale entries) read block 0, as in the kernels; left
         # alone they would trip a device-side index assert
         ids = page_table.reshape(-1).to(torch.int64)
         ids = torch.where((ids >= 0) & (ids < cache.shape[0]), ids, torch.zeros_like(ids))
-        g = torch.index_select(cache, 0, ids)
+        if scales is not None:
+            g = fp8_ops.fp8_unpack_cache(torch.index_select(cache.view(torch.uint8), 0, ids).view(cache.dtype),
+                                         torch.index_select(scales, 0, ids))
+        else:
+            g = torch.index_select(cache, 0, ids)
         if cache.dtype == torch.uint8:
             g = custom_ops.bfp8_unpack_cache(g)
         _, hkv, bs, d = g.shape
