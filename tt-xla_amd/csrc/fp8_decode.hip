@@ -353,7 +353,10 @@ int attend(DecodeArgs a, const float *k_scales, const float *v_scales, int head_
   if (!segment_units_forced()) a.seg_free_tiles = a.n_waves;
   if (!a.direct && (int64_t)a.users * a.hkv > (int64_t)a.n_waves * kWave)
     return fail(TTPA_ERR_UNSUPPORTED, "fp8 decode: %d x %d segments need a grid of more than %d wavefronts", a.users, a.hkv, a.n_waves);
-  const Fp8Args fa = {a, k_scales, v_scales};
+  const uint32_t runs = (uint32_t)a.bs / (head_size <= 128 ? 16 : 8);
+  const uint32_t negate = a.scale_log2e < 0.f ? 0x80008000u : 0u;
+  a.scale_log2e = fabsf(a.scale_log2e);
+  const Fp8Args fa = {a, k_scales, v_scales, negate, runs, 0xffffffffu / runs};
   const bool ok = head_size == 64 ? launch_fp8_d64(&fa, st) : head_size == 128 ? launch_fp8_d128(&fa, st) : launch_fp8_d256(&fa, st);
   hipEvent_t ev0, ev1;
   take_profile_events(ev0, ev1);  // still armed only if the launch did not happen
