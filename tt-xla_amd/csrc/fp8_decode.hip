@@ -3,15 +3,16 @@
 // Sparse form.  For every (user, KV head) the blocks of the context are scored by what their key bounds allow,
 //   score(block) = max over the group's heads of  sum_d  max(q_d, 0) high_d + min(q_d, 0) low_d,
 // an upper bound of q . k over the block's keys; the block that holds the newest token, the first block and the best of the others are
-// attended, `kept` in all, of equal scores the lower column.  A choice flips with the last bit of a score, so scores
-// are sums in 64 bits: products of bfloat16 values are exact there and a sum of 256 of them keeps 30 bits to spare, so that
-// neither the order of the sum nor its split matters in practice.
-//   block_scores_kernel   a block's bounds are 4 D consecutive bytes, D / 4 lanes of 16 bytes: half of them hold lows and the negative
-//                         parts of the queries, half highs and the positive parts.  Memory bound: each bound is read once for up to
-//                         eight heads, whose parts a lane keeps in registers as doubles.
-//   choose_blocks_kernel  one workgroup per (user, KV head): a histogram over the scores' range finds the bin the last kept block
-//                         lies in, ranks inside that bin (or histograms of it, while it is crowded) find the block; the columns come out in
-//                         order, as a page table of their own.
+// attended, `kept` in all, of equal scores the lower column.  A choice flips with the last bit of a score, so scores are
+// sums in 64 bits: products of bfloat16 values are exact there and a sum of 512 of them keeps 28 bits to spare, so that neither
+// the order of the sum nor its split matters in practice.  But 64-bit sums for all blocks took 13 and 21 us (27 000 blocks with four heads, 46 000
+// with eight), three times what reading the bounds takes, and hardly any of them decides anything.  So:
+//   block_scores_kernel   scores by the matrix pipe, in 32 bits, and with them the sums of the products' magnitudes, which bound their
+//                         error.  Memory bound: a block's bounds are 4 D bytes, read once.
+//   choose_blocks_kernel  one workgroup per (user, KV head): finds the last score that is kept, T (a histogram over the scores' range, ranks inside the bin
+//                         T lies in).  With scores at most e from the true ones, what is more than 2 e above T is kept and what is more
+//                         than 2 e below is not; the few blocks between (about one in practice) are scored again in 64 bits and
+//                         the best of them kept.  The columns come out in order, as a page table of their own.
 // The attention is the decode kernel on that table: each (user, KV head) is a user with one KV head, its blocks the slabs of the cache.
 #include "fp8_decode_kernel.h"
 
@@ -33,6 +34,7 @@ bool launch_fp8_d256(const void *args, hipStream_t st);
 namespace {
 
 // ---- scores ----------------------------------------------------------------------------------------
+using fp8::u32x4;
 struct ScoreArgs {
   const uint16_t *q;
   int64_t q_us, q_hs;
@@ -42,10 +44,12 @@ struct ScoreArgs {
   const void *cur;
   int cur_i64;
   int users, hkv, g, bs, w, nb, kept;
-  uint64_t *keys;  // [users * hkv][w]
+  float2 *scores;  // [users * hkv][w]: score in 32 bits, sum of its products' magnitudes
+  uint64_t *keys;  // [users * hkv][w]: exact scores, where too many are in question for LDS
   int32_t *table;  // [users * hkv][kept]
   int32_t *pos;    // [users * hkv]
   int32_t *columns;  // [users, hkv, kept], the caller's
+  int *arrived;      // [users * hkv], zeroed for the attention
 };
 
 // Blocks of a user's context; 0 for a padded row.
@@ -56,7 +60,7 @@ __device__ __forceinline__ int blocks_of(const ScoreArgs &a, int u, int64_t &pos
   return pos < 0 ? 0 : (int)(pos / a.bs) + 1;
 }
 
-constexpr uint64_t kAlways = ~0ull, kUnbounded = ~0ull - 1;
+constexpr uint64_t kUnbounded = ~0ull;
 // Whole numbers in the order of the scores; what is no number, or no finite one above, comes first.
 __device__ __forceinline__ uint64_t score_key(double s) {
   if (!(s < (double)INFINITY)) return kUnbounded;
@@ -71,109 +75,91 @@ __device__ __forceinline__ double dpp_move_f64(double v) {
   const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, 0xf, 0xf, true);
   return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
-template <int CTRL>
-__device__ __forceinline__ uint64_t dpp_max_u64(uint64_t b) {
-  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, 0xf, 0xf, true);
-  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, 0xf, 0xf, true);
-  const uint64_t o = (uint64_t)hi << 32 | lo;
-  return b > o ? b : o;
+
+// A wavefront scores 16 blocks at a time: A = 16 rows of bounds x 32 features (lane n: block n), B = the heads' queries, positive parts against
+// highs, negative ones against lows.
+template <int D>
+constexpr int score_tiles() {
+  return D == 64 ? 2 : 1;
 }
-constexpr int kDppRor1 = 0x121, kDppRor2 = 0x122, kDppRor4 = 0x124, kDppRor8 = 0x128;
-
-// One level of the exchange that leaves each lane the sums of half of its heads: lanes with `bit` keep the upper half.
-template <int CTRL, int N>
-__device__ __forceinline__ void halve(double (&v)[N], int count, bool bit) {
-#pragma unroll
-  for (int i = 0; i < N / 2; ++i)
-    if (i < count / 2) {
-      const double keep = bit ? v[i + count / 2] : v[i], send = bit ? v[i] : v[i + count / 2];
-      v[i] = keep + dpp_move_f64<CTRL>(send);
-    }
-}
-
-constexpr int kScoreBlocks = 64;  // context blocks per workgroup: enough of them for eight users of 8 heads and 512 blocks to fill the chip
-
-template <int D, int GH>
+template <int D>
 __global__ __launch_bounds__(256) void block_scores_kernel(ScoreArgs a) {
-  constexpr int LPB = D / 4, BPW = 64 / LPB;  // lanes per block, blocks per wavefront and load
-  constexpr int UNROLL = 4;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  constexpr int KSTEPS = D / 32, TILES = score_tiles<D>();
+  const int lane = threadIdx.x & 63, n = lane & 15, quad = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int seg = blockIdx.y, u = seg / a.hkv, h = seg - u * a.hkv;
+  const int c0 = ((int)blockIdx.x * 4 + wave) * 16 * TILES;
+  // (the table row is as wide for every user: a page that the context does not reach is looked up, too, and goes no further)
+  int page[TILES];
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) page[t] = a.pt[u * a.pt_rs + min(c0 + 16 * t + n, a.w - 1)];
+  u32x4 q[KSTEPS];
+  const uint32_t head = n < a.g ? 0xffffffffu : 0u;
+#pragma unroll
+  for (int s = 0; s < KSTEPS; ++s) {
+    q[s] = *reinterpret_cast<const u32x4 *>(a.q + u * a.q_us + (int64_t)(h * a.g + min(n, a.g - 1)) * a.q_hs + 32 * s + 8 * quad);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[s][i] &= head;
+  }
   int64_t pos;
   const int nblk = blocks_of(a, u, pos);
-  if (nblk <= a.kept) return;  // all are attended
-  const int from = blockIdx.x * kScoreBlocks, to = min(nblk, from + kScoreBlocks);
-  const int in_block = lane % LPB, which = lane / LPB;
-  const bool high = in_block >= LPB / 2;
-  const int f = 8 * (in_block % (LPB / 2));
-  const int32_t *pt = a.pt + u * a.pt_rs;
-  for (int g0 = 0; g0 < a.g; g0 += GH) {
-    double q[GH][8];
+  if (nblk <= a.kept || c0 >= nblk) return;  // (up to `kept` blocks: all are attended)
+  u32x4 low[TILES][KSTEPS], high[TILES][KSTEPS];
 #pragma unroll
-    for (int g = 0; g < GH; ++g) {
-      fp8::u32x4 t = {0, 0, 0, 0};
-      if (g0 + g < a.g) t = *reinterpret_cast<const fp8::u32x4 *>(a.q + u * a.q_us + (int64_t)(h * a.g + g0 + g) * a.q_hs + f);
+  for (int t = 0; t < TILES; ++t) {
+    const int64_t slab = (int64_t)((unsigned)page[t] < (unsigned)a.nb ? page[t] : 0) * a.hkv + h;
+    const uint16_t *b = a.bounds + slab * (2 * D) + 8 * quad;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float v0 = bf16_lo(t[i]), v1 = bf16_hi(t[i]);
-        // (a NaN stays one in both parts)
-        q[g][2 * i] = high ? (v0 < 0.f ? 0.f : v0) : (v0 > 0.f ? 0.f : v0);
-        q[g][2 * i + 1] = high ? (v1 < 0.f ? 0.f : v1) : (v1 > 0.f ? 0.f : v1);
-      }
+    for (int s = 0; s < KSTEPS; ++s) low[t][s] = *reinterpret_cast<const u32x4 *>(b + 32 * s);
+#pragma unroll
+    for (int s = 0; s < KSTEPS; ++s) high[t][s] = *reinterpret_cast<const u32x4 *>(b + D + 32 * s);
+  }
+  floatx4 sum[TILES], size[TILES];
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) sum[t] = size[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int s = 0; s < KSTEPS; ++s) {
+    // the parts of the queries; a NaN stays one in both (it counts as positive and as negative)
+    u32x4 plus, minus, less;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w = q[s][i];
+      const uint32_t lo_nan = (w & 0x7fffu) > 0x7f80u ? 0xffffu : 0u, hi_nan = (w & 0x7fff0000u) > 0x7f800000u ? 0xffff0000u : 0u;
+      const uint32_t negative = ((w >> 15) & 0x00010001u) * 0xffffu;
+      plus[i] = w & (~negative | lo_nan | hi_nan), minus[i] = w & (negative | lo_nan | hi_nan), less[i] = minus[i] & 0x7fff7fffu;
     }
-    for (int c0 = from + wave * BPW * UNROLL; c0 < to; c0 += 4 * BPW * UNROLL) {
-      fp8::u32x4 raw[UNROLL];
 #pragma unroll
-      for (int j = 0; j < UNROLL; ++j) {
-        const int c = min(c0 + j * BPW + which, to - 1);
-        const int id = pt[c];
-        const int64_t slab = (int64_t)((unsigned)id < (unsigned)a.nb ? id : 0) * a.hkv + h;
-        raw[j] = __builtin_nontemporal_load(reinterpret_cast<const fp8::u32x4 *>(a.bounds + slab * (2 * D) + (high ? D : 0) + f));
-      }
+    for (int t = 0; t < TILES; ++t) {
+      u32x4 low_size, high_size;
 #pragma unroll
-      for (int j = 0; j < UNROLL; ++j) {
-        double s[GH];
-#pragma unroll
-        for (int g = 0; g < GH; ++g) s[g] = 0.0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const double b0 = bf16_lo(raw[j][i]), b1 = bf16_hi(raw[j][i]);
-#pragma unroll
-          for (int g = 0; g < GH; ++g) s[g] = __builtin_fma(q[g][2 * i], b0, s[g]);
-#pragma unroll
-          for (int g = 0; g < GH; ++g) s[g] = __builtin_fma(q[g][2 * i + 1], b1, s[g]);
-        }
-        int count = GH;
-        if constexpr (GH >= 8) halve<kDppHalfMirror>(s, count, lane & 4), count /= 2;
-        if constexpr (GH >= 4) halve<kDppXor2>(s, count, lane & 2), count /= 2;
-        if constexpr (GH >= 2) halve<kDppXor1>(s, count, lane & 1), count /= 2;
-        double t = s[0];
-        t += dpp_move_f64<kDppRor8>(t);
-        if constexpr (GH < 8) t += dpp_move_f64<kDppRor4>(t);
-        if constexpr (GH < 4) t += dpp_move_f64<kDppRor2>(t);
-        if constexpr (GH < 2) t += dpp_move_f64<kDppRor1>(t);
-        if constexpr (LPB >= 32) t += __shfl_xor(t, 16);
-        if constexpr (LPB >= 64) t += __shfl_xor(t, 32);
-        uint64_t key = g0 + (lane & (GH - 1)) < a.g ? score_key(t) : 0;
-        if constexpr (GH >= 2) key = dpp_max_u64<kDppXor1>(key);
-        if constexpr (GH >= 4) key = dpp_max_u64<kDppXor2>(key);
-        if constexpr (GH >= 8) key = dpp_max_u64<kDppHalfMirror>(key);
-        const int c = c0 + j * BPW + which;
-        if (in_block == 0 && c < to) {
-          uint64_t *dst = a.keys + (int64_t)seg * a.w + c;
-          if (g0 > 0) key = max(key, *dst);
-          if (c == 0 || c == nblk - 1) key = kAlways;
-          *dst = key;
-        }
-      }
+      for (int i = 0; i < 4; ++i) low_size[i] = low[t][s][i] & 0x7fff7fffu, high_size[i] = high[t][s][i] & 0x7fff7fffu;
+      sum[t] = mma16<false>(high[t][s], plus, sum[t]);
+      size[t] = mma16<false>(high_size, plus, size[t]);
+      sum[t] = mma16<false>(low[t][s], minus, sum[t]);
+      size[t] = mma16<false>(low_size, less, size[t]);
     }
+  }
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) {
+    // lane (head n, quad) holds blocks 4 quad + r: the largest over the heads; a sum that is no number is as good as infinite
+    float best[4], most[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      best[r] = row16_max(n < a.g ? (sum[t][r] == sum[t][r] ? sum[t][r] : INFINITY) : -INFINITY);
+      most[r] = row16_max(n < a.g ? (size[t][r] == size[t][r] ? size[t][r] : INFINITY) : 0.f);
+    }
+    const int c = c0 + 16 * t + 4 * quad + n;
+    if (n < 4 && c < nblk)
+      a.scores[(int64_t)seg * a.w + c] = make_float2(n == 0 ? best[0] : n == 1 ? best[1] : n == 2 ? best[2] : best[3],
+                                                     n == 0 ? most[0] : n == 1 ? most[1] : n == 2 ? most[2] : most[3]);
   }
 }
 
 // ---- choice ----------------------------------------------------------------------------------------
-constexpr int kBins = 1024, kHeld = 4096, kRanked = 256;
+constexpr int kBins = 1024, kRanked = 256;
 
-__device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) { return wave_max_u32(v); }
+__device__ __forceinline__ uint64_t wave_max(uint64_t v) {
   for (int m = 1; m < 64; m <<= 1) {
     const uint64_t o = (uint64_t)__shfl_xor((unsigned long long)v, m);
     v = v > o ? v : o;
@@ -181,149 +167,294 @@ __device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
   return v;
 }
 
-__global__ __launch_bounds__(256) void choose_blocks_kernel(ScoreArgs a) {
-  __shared__ uint64_t s_keys[kHeld];
-  __shared__ uint32_t s_bins[kBins];
-  __shared__ uint64_t s_cand[kRanked];
-  __shared__ uint64_t s_red[8];
-  __shared__ int s_int[8];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int seg = blockIdx.x, u = seg / a.hkv, h = seg - u * a.hkv;
-  int64_t pos;
-  const int nblk = blocks_of(a, u, pos);
-  const int32_t *pt = a.pt + u * a.pt_rs;
-  int32_t *table = a.table + (int64_t)seg * a.kept, *columns = a.columns + (int64_t)seg * a.kept;
-  const int chosen = min(nblk, a.kept);
-  const auto emit = [&](int at, int c) {
-    const int id = pt[c];
-    table[at] = ((unsigned)id < (unsigned)a.nb ? id : 0) * a.hkv + h;
-    columns[at] = c;
-  };
-  for (int i = chosen + tid; i < a.kept; i += 256) table[i] = h, columns[i] = -1;
-  if (tid == 0) a.pos[seg] = nblk ? (int)((int64_t)(chosen - 1) * a.bs + (pos - (int64_t)(nblk - 1) * a.bs)) : -1;
-  if (nblk <= a.kept) {
-    for (int c = tid; c < nblk; c += 256) emit(c, c);
-    return;
-  }
-  const uint64_t *keys = a.keys + (int64_t)seg * a.w;
-  const bool held = nblk <= kHeld;
-  const auto key_at = [&](int c) { return held ? s_keys[c] : keys[c]; };
-  // The range of the keys that are not always kept; the first and the last block are.
-  uint64_t hi = 0, lo = ~0ull;
-  for (int c = tid; c < nblk; c += 256) {
-    const uint64_t k = keys[c];
-    if (held) s_keys[c] = k;
-    if (k != kAlways) hi = max(hi, k), lo = min(lo, k);
-  }
-  hi = wave_max_u64(hi), lo = ~wave_max_u64(~lo);
-  if (lane == 0) s_red[wave] = hi, s_red[4 + wave] = lo;
+// Whole numbers in the order of 32-bit scores.
+__device__ __forceinline__ uint32_t float_key(float s) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, s + 0.f);
+  return (b >> 31) ? ~b : b | 0x80000000u;
+}
+
+struct Choice {
+  uint64_t threshold;  // keys above it are kept, and of those equal to it the first `ties`
+  int ties;
+};
+constexpr int kThreads = 512, kWaves = kThreads / 64;
+constexpr int kHeldColumns = 8192;  // contexts of up to so many blocks: scores and pages in LDS
+struct ChoiceLds {
+  uint32_t bins[kBins];
+  uint64_t cand[kRanked], high[kWaves], low[kWaves];
+  int num[2][kWaves], column[kRanked], bin, over, count, next;
+  float size[kWaves];
+  uint8_t kept[kRanked];
+};
+// This thread's places in two running counts over the workgroup, and the counts of all.
+struct Counts {
+  int before[2], all[2];
+};
+__device__ __forceinline__ Counts running_counts(ChoiceLds &s, int x, int y) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int ix = wave_prefix_sum(x), iy = wave_prefix_sum(y);
   __syncthreads();
-  hi = max(max(s_red[0], s_red[1]), max(s_red[2], s_red[3]));
-  lo = min(min(s_red[4], s_red[5]), min(s_red[6], s_red[7]));
-  // `need` blocks with keys in [lo, hi] are kept besides those with larger keys: narrow the range until few are in question.
-  int need = a.kept - 2;
-  uint64_t threshold = 0;  // keys above it are kept, and of those equal to it the first `ties` columns
-  int ties = 0;
+  if (lane == 63) s.num[0][wave] = ix, s.num[1][wave] = iy;
+  __syncthreads();
+  Counts c = {{ix - x, iy - y}, {0, 0}};
+  for (int w = 0; w < kWaves; ++w) {
+    const int nx = s.num[0][w], ny = s.num[1][w];
+    if (w < wave) c.before[0] += nx, c.before[1] += ny;
+    c.all[0] += nx, c.all[1] += ny;
+  }
+  return c;
+}
+
+// Where the `need` largest of the keys key_at(1) .. key_at(n - 2) with `among` end; all threads.  A histogram over the keys' range finds the bin; the keys
+// in it are ranked, or its range is the next histogram's.
+template <typename Key, typename KeyAt, typename Among>
+__device__ __forceinline__ Choice last_kept(ChoiceLds &s, int n, int need, const KeyAt &key_at, const Among &among) {
+  constexpr int OWN = kBins / kThreads;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  Key hi = 0, lo = ~(Key)0;
+#pragma unroll 1
+  for (int c = 1 + tid; c < n - 1; c += kThreads)
+    if (among(c)) {
+      const Key k = key_at(c);
+      hi = max(hi, k), lo = min(lo, k);
+    }
+  hi = wave_max(hi), lo = ~wave_max((Key)~lo);
+  __syncthreads();
+  if (lane == 0) s.high[wave] = hi, s.low[wave] = lo;
+  __syncthreads();
+  for (int w = 0; w < kWaves; ++w) hi = max(hi, (Key)s.high[w]), lo = min(lo, (Key)s.low[w]);
+#pragma unroll 1
   for (;;) {
-    if (need == 0) {
-      threshold = hi;
-      break;
-    }
-    if (lo == hi) {
-      threshold = lo, ties = need;
-      break;
-    }
-    const int shift = max(0, 64 - __builtin_clzll(hi - lo) - 10);  // (hi - lo) >> shift < 1024
-    for (int i = tid; i < kBins; i += 256) s_bins[i] = 0;
-    __syncthreads();
-    for (int c = tid; c < nblk; c += 256) {
-      const uint64_t k = key_at(c);
-      if (k >= lo && k <= hi) atomicAdd(&s_bins[(k - lo) >> shift], 1u);
-    }
-    __syncthreads();
-    // the bin, from the top, where the count reaches `need`: thread t owns bins 4 (255 - t) .. + 3
-    const int base = 4 * (255 - tid);
-    uint32_t mine[4], sum = 0;
+    if (need == 0) return {hi, 0};
+    if (lo == hi) return {lo, need};
+    const int shift = max(0, 64 - __builtin_clzll((uint64_t)(hi - lo)) - 10);  // (hi - lo) >> shift < 1024
 #pragma unroll
-    for (int j = 0; j < 4; ++j) mine[j] = s_bins[base + j], sum += mine[j];
-    const int incl = wave_prefix_sum((int)sum);
-    if (lane == 63) s_int[wave] = incl;
+    for (int j = 0; j < OWN; ++j) s.bins[tid + j * kThreads] = 0;
+    if (tid == 0) s.next = 0;
     __syncthreads();
-    int above = incl - (int)sum;
-    for (int w = 0; w < wave; ++w) above += s_int[w];
-    if (above < need && above + (int)sum >= need) {  // one thread
-      int b = 3;
-      while (above + (int)mine[b] < need) above += mine[b], --b;
-      s_int[4] = base + b, s_int[5] = above, s_int[6] = (int)mine[b];
+#pragma unroll 1
+    for (int c = 1 + tid; c < n - 1; c += kThreads) {
+      const Key k = key_at(c);
+      if (among(c) && k >= lo && k <= hi) atomicAdd(&s.bins[(k - lo) >> shift], 1u);
     }
     __syncthreads();
-    const int bin = s_int[4], over = s_int[5], count = s_int[6];
-    need -= over;
-    const uint64_t span = ((uint64_t)1 << shift) - 1;
-    lo += (uint64_t)bin << shift;
+    // the bin, from the top, where the count reaches `need`: each thread owns neighbouring bins
+    const int base = kBins - OWN * (tid + 1);
+    int mine[OWN], sum = 0;
+#pragma unroll
+    for (int j = 0; j < OWN; ++j) mine[j] = (int)s.bins[base + j], sum += mine[j];
+    int above = running_counts(s, sum, 0).before[0];
+    if (above < need && above + sum >= need) {  // one thread
+      int b = OWN - 1;
+      while (above + mine[b] < need) above += mine[b], --b;
+      s.bin = base + b, s.over = above, s.count = mine[b];
+    }
+    __syncthreads();
+    const int count = s.count;
+    need -= s.over;
+    const Key span = ((Key)1 << shift) - 1;
+    lo += (Key)s.bin << shift;
     hi = hi - lo < span ? hi : lo + span;  // (the last bin may reach past the largest number)
-    if (shift == 0 || count == need) {
-      // all keys of the bin are alike, or all are kept
-      if (count == need) threshold = lo - 1;
-      else threshold = lo, ties = need;
-      break;
-    }
+    if (shift == 0) return {lo, need};     // all of the bin are alike
     if (count <= kRanked) {
-      if (tid == 0) s_int[7] = 0;
-      __syncthreads();
-      for (int c = tid; c < nblk; c += 256) {
-        const uint64_t k = key_at(c);
-        if (k >= lo && k <= hi) s_cand[atomicAdd(&s_int[7], 1)] = k;
+#pragma unroll 1
+      for (int c = 1 + tid; c < n - 1; c += kThreads) {
+        const Key k = key_at(c);
+        if (among(c) && k >= lo && k <= hi) s.cand[atomicAdd(&s.next, 1)] = k;
       }
       __syncthreads();
       if (tid < count) {
         // the need-th largest: fewer than `need` keys are larger, and with its equals there are enough
-        const uint64_t k = s_cand[tid];
+        const uint64_t k = s.cand[tid];
         int larger = 0, equal = 0;
-        for (int i = 0; i < count; ++i) larger += s_cand[i] > k, equal += s_cand[i] == k;
-        if (larger < need && larger + equal >= need) s_red[0] = k, s_int[4] = need - larger;  // (equal keys write the same)
+#pragma unroll 1
+        for (int i = 0; i < count; ++i) larger += s.cand[i] > k, equal += s.cand[i] == k;
+        if (larger < need && larger + equal >= need) s.high[0] = k, s.over = need - larger;  // (equal keys write the same)
       }
       __syncthreads();
-      threshold = s_red[0], ties = s_int[4];
-      break;
+      return {s.high[0], s.over};
     }
     __syncthreads();
-  }
-  // the columns in order: a run of `per` neighbouring columns per thread would serialise; 256 at a time with running counts
-  int at = 0, tied = 0;
-  for (int c0 = 0; c0 < nblk; c0 += 256) {
-    const int c = c0 + tid;
-    const uint64_t k = c < nblk ? key_at(c) : 0;
-    const bool is = c < nblk, tie = is && k == threshold && ties > 0, above = is && k > threshold;
-    const uint64_t tie_lanes = __builtin_amdgcn_ballot_w64(tie);
-    __syncthreads();  // (the counts of the pass before are read)
-    if (lane == 0) s_int[wave] = __builtin_popcountll(tie_lanes);
-    __syncthreads();
-    int rank = tied + __builtin_amdgcn_mbcnt_hi((uint32_t)(tie_lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)tie_lanes, 0));
-    for (int w = 0; w < 4; ++w) {
-      if (w < wave) rank += s_int[w];
-      tied += s_int[w];
-    }
-    const bool take = above || (tie && rank < ties);
-    const uint64_t take_lanes = __builtin_amdgcn_ballot_w64(take);
-    if (lane == 0) s_int[4 + wave] = __builtin_popcountll(take_lanes);
-    __syncthreads();
-    int to = at + __builtin_amdgcn_mbcnt_hi((uint32_t)(take_lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)take_lanes, 0));
-    for (int w = 0; w < 4; ++w) {
-      if (w < wave) to += s_int[4 + w];
-      at += s_int[4 + w];
-    }
-    if (take && to < a.kept) emit(to, c);
   }
 }
 
+// The exact score in 64 bits of one head's query over one page's bounds, as a key: D / 4 lanes, each with a page and a head of their own per such group.
 template <int D>
-void launch_scores(const ScoreArgs &a, hipStream_t st) {
-  const dim3 grid((a.w + kScoreBlocks - 1) / kScoreBlocks, a.users * a.hkv);
-  if (a.g <= 1) block_scores_kernel<D, 1><<<grid, dim3(256), 0, st>>>(a);
-  else if (a.g <= 2) block_scores_kernel<D, 2><<<grid, dim3(256), 0, st>>>(a);
-  else if (a.g <= 4) block_scores_kernel<D, 4><<<grid, dim3(256), 0, st>>>(a);
-  else block_scores_kernel<D, 8><<<grid, dim3(256), 0, st>>>(a);
+__device__ __forceinline__ uint64_t exact_key(const ScoreArgs &a, int u, int h, int g, int page) {
+  constexpr int LPB = D / 4;
+  const int in_block = (int)(threadIdx.x & 63) % LPB;
+  const bool high = in_block >= LPB / 2;
+  const int f = 8 * (in_block % (LPB / 2));
+  const int64_t slab = (int64_t)((unsigned)page < (unsigned)a.nb ? page : 0) * a.hkv + h;
+  const u32x4 raw = *reinterpret_cast<const u32x4 *>(a.bounds + slab * (2 * D) + (high ? D : 0) + f);
+  const u32x4 t = *reinterpret_cast<const u32x4 *>(a.q + u * a.q_us + (int64_t)(h * a.g + g) * a.q_hs + f);
+  double s = 0.0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float v0 = bf16_lo(t[i]), v1 = bf16_hi(t[i]);
+    // (a NaN stays one in both parts)
+    const double q0 = high ? (v0 < 0.f ? 0.f : v0) : (v0 > 0.f ? 0.f : v0), q1 = high ? (v1 < 0.f ? 0.f : v1) : (v1 > 0.f ? 0.f : v1);
+    s = __builtin_fma(q0, (double)bf16_lo(raw[i]), s);
+    s = __builtin_fma(q1, (double)bf16_hi(raw[i]), s);
+  }
+  s += dpp_move_f64<kDppXor1>(s);
+  s += dpp_move_f64<kDppXor2>(s);
+  s += dpp_move_f64<kDppHalfMirror>(s);
+  s += dpp_move_f64<kDppMirror>(s);
+  if constexpr (LPB >= 32) s += __shfl_xor(s, 16);
+  if constexpr (LPB >= 64) s += __shfl_xor(s, 32);
+  return score_key(s);
+}
+
+// One workgroup per (user, KV head); what bounds it is its own chain (four round trips to memory, a dozen barriers) and, as every launch begins with a cold
+// instruction cache, its code: loops are not unrolled, scores and pages lie in LDS.  (Unrolled, in registers, 1024 threads took 21 us over 1500 blocks.)
+template <int D>
+__global__ __launch_bounds__(kThreads) void choose_blocks_kernel(ScoreArgs a) {
+  __shared__ ChoiceLds s;
+  extern __shared__ float s_held[];  // [columns], then the pages
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int seg = blockIdx.x, u = seg / a.hkv, h = seg - u * a.hkv;
+  const int32_t *pt = a.pt + u * a.pt_rs;
+  const float2 *scores = a.scores + (int64_t)seg * a.w;
+  const bool held = a.w <= kHeldColumns;
+  int *const s_page = reinterpret_cast<int *>(s_held) + a.w;
+  float size = 0.f;  // largest sum of magnitudes
+  int64_t pos = load_index(a.cur, a.cur_i64, u);
+  // (the first columns are asked for before it is known how many there are)
+  const int c_first = min(tid, a.w - 1);
+  const float2 first_score = a.w > a.kept ? scores[c_first] : make_float2(0.f, 0.f);
+  const int first_page = pt[c_first];
+  const int nblk = blocks_of(a, u, pos);
+  int32_t *table = a.table + (int64_t)seg * a.kept, *columns = a.columns + (int64_t)seg * a.kept;
+  const int chosen = min(nblk, a.kept);
+  const auto emit = [&](int at, int c, int id) {
+    table[at] = ((unsigned)id < (unsigned)a.nb ? id : 0) * a.hkv + h;
+    columns[at] = c;
+  };
+#pragma unroll 1
+  for (int i = chosen + tid; i < a.kept; i += kThreads) table[i] = h, columns[i] = -1;
+  if (tid == 0) {
+    a.pos[seg] = nblk ? (int)((int64_t)(chosen - 1) * a.bs + (pos - (int64_t)(nblk - 1) * a.bs)) : -1;
+    a.arrived[seg] = 0;
+  }
+  if (nblk <= a.kept) {
+#pragma unroll 1
+    for (int c = tid; c < nblk; c += kThreads) emit(c, c, pt[c]);
+    return;
+  }
+#pragma unroll 1
+  for (int c = tid; c < nblk; c += kThreads) {
+    const float2 v = c == tid ? first_score : scores[c];
+    size = fmaxf(size, v.y);
+    if (held) s_held[c] = v.x, s_page[c] = c == tid ? first_page : pt[c];
+  }
+  // (magnitudes: their order is that of their bits)
+  size = __builtin_bit_cast(float, wave_max_u32(__builtin_bit_cast(uint32_t, size)));
+  if (lane == 0) s.size[wave] = size;
+  __syncthreads();
+  for (int w = 0; w < kWaves; ++w) size = fmaxf(size, s.size[w]);
+  const auto score = [&](int c) { return held ? s_held[c] : scores[c].x; };
+  const auto page = [&](int c) { return held ? s_page[c] : pt[c]; };
+  const int need = a.kept - 2;  // of the blocks but the first and the last
+  const Choice approx = last_kept<uint32_t>(s, nblk, need, [&](int c) { return float_key(score(c)); }, [](int) { return true; });
+  // T, and how far a score may be from the exact one: at most 512 additions, each off by at most a unit in the last place of what the magnitudes
+  // add up to (2^-23), twice that for what the matrix pipe's own order and rounding may be; and what falls below the smallest normal number.
+  const uint32_t tb = (uint32_t)approx.threshold;
+  const float t = __builtin_bit_cast(float, (tb >> 31) ? tb & 0x7fffffffu : ~tb);
+  const float e = size * 0x1p-13f + 0x1p-100f;
+  const bool exact_all = !(size < INFINITY) || !(fabsf(t) < INFINITY);  // infinities among the scores: no bound says anything
+  const float sure = exact_all ? INFINITY : t + 2.f * e, out = exact_all ? -INFINITY : t - 2.f * e;
+  const auto kept_surely = [&](int c) { return !exact_all && need > 0 && score(c) > sure; };
+  const auto in_question = [&](int c) { return exact_all || (need > 0 && score(c) >= out && !(score(c) > sure)); };
+  // Each thread has neighbouring columns from here on, so that the chosen ones come out in order behind running counts.
+  const int per = (nblk + kThreads - 1) / kThreads, from = max(min(tid * per, nblk), 1), to = min(tid * per + per, nblk - 1);
+  int sure_mine = 0, open_mine = 0;
+#pragma unroll 1
+  for (int c = from; c < to; ++c) sure_mine += kept_surely(c), open_mine += in_question(c);
+  const Counts n = running_counts(s, sure_mine, open_mine);
+  const int open = n.all[1], need_open = need - n.all[0];
+  constexpr int GROUPS = 256 / D;  // of lanes with a score of their own, in a wavefront
+  const int group = wave * GROUPS + lane / (D / 4);
+  uint64_t *const keys = a.keys + (int64_t)seg * a.w;
+  int place = 1 + n.before[0];  // of the thread's first kept column (column 0 is in front)
+  if (open <= kRanked) {
+    // few in question: their exact scores and ranks in LDS
+    int at = n.before[1];
+#pragma unroll 1
+    for (int c = from; c < to; ++c)
+      if (in_question(c)) s.column[at] = c, s.cand[at] = 0, ++at;
+    __syncthreads();
+#pragma unroll 1
+    for (int i = group; i - group < open * a.g; i += kWaves * GROUPS) {
+      const int x = min(i, open * a.g - 1), o = x / a.g;
+      const uint64_t k = exact_key<D>(a, u, h, x - o * a.g, page(s.column[o]));
+      if (lane % (D / 4) == 0 && i < open * a.g) atomicMax(reinterpret_cast<unsigned long long *>(&s.cand[o]), (unsigned long long)k);
+    }
+    __syncthreads();
+    if (tid < open) {
+      const uint64_t k = s.cand[tid];
+      int better = 0;  // (columns are in order: of equals the first ones)
+#pragma unroll 1
+      for (int i = 0; i < open; ++i) better += s.cand[i] > k || (s.cand[i] == k && i < tid);
+      s.kept[tid] = better < need_open;
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int i = 0; i < n.before[1]; ++i) place += s.kept[i];
+    at = n.before[1];
+#pragma unroll 1
+    for (int c = from; c < to; ++c) {
+      bool is = kept_surely(c);
+      if (in_question(c)) is = s.kept[at++];
+      if (is) emit(place++, c, page(c));
+    }
+  } else {
+    // many (scores alike, infinities): exact scores of all in memory, and the choice among those in question by them
+#pragma unroll 1
+    for (int i = group; i - group < nblk; i += kWaves * GROUPS) {
+      const int c = min(i, nblk - 1);
+      uint64_t k = 0;
+#pragma unroll 1
+      for (int g = 0; g < a.g; ++g) k = max(k, exact_key<D>(a, u, h, g, page(c)));
+      if (lane % (D / 4) == 0 && i < nblk) keys[i] = k;
+    }
+    __syncthreads();
+    const Choice exact = last_kept<uint64_t>(s, nblk, need_open, [&](int c) { return keys[c]; }, in_question);
+    // of the blocks tied for the last places the first ones win
+    int above = 0, tied = 0;
+#pragma unroll 1
+    for (int c = from; c < to; ++c)
+      if (in_question(c)) above += keys[c] > exact.threshold, tied += keys[c] == exact.threshold;
+    const Counts m = running_counts(s, above, tied);
+    int t_at = m.before[1];
+    place += m.before[0] + min(t_at, exact.ties);
+#pragma unroll 1
+    for (int c = from; c < to; ++c) {
+      bool is = kept_surely(c);
+      if (in_question(c)) {
+        is = keys[c] > exact.threshold || (keys[c] == exact.threshold && t_at < exact.ties);
+        t_at += keys[c] == exact.threshold;
+      }
+      if (is) emit(place++, c, page(c));
+    }
+  }
+  if (tid == 0) emit(0, 0, page(0)), emit(a.kept - 1, nblk - 1, page(nblk - 1));
+}
+
+template <int D>
+int launch_choice(const ScoreArgs &a, hipStream_t st) {
+  const int segments = a.users * a.hkv;
+  if (a.w > a.kept) {
+    constexpr int kBlocks = 4 * 16 * score_tiles<D>();
+    block_scores_kernel<D><<<dim3((a.w + kBlocks - 1) / kBlocks, segments), dim3(256), 0, st>>>(a);
+    if (const int rc = check_launch("fp8 sparse decode (scores)")) return rc;
+  }
+  const size_t lds = a.w <= kHeldColumns ? (size_t)a.w * 8 : 0;
+  static std::atomic<uint64_t> lds_ready{0};
+  if (!ensure_dynamic_lds(reinterpret_cast<const void *>(&choose_blocks_kernel<D>), kHeldColumns * 8, lds_ready))
+    return fail(TTPA_ERR_LAUNCH, "fp8 sparse decode: cannot configure the choice of blocks");
+  choose_blocks_kernel<D><<<dim3(segments), dim3(kThreads), lds, st>>>(a);
+  return check_launch("fp8 sparse decode (choice)");
 }
 
 // ---- the attention's launch ----------------------------------------------------------------------------
@@ -340,7 +471,8 @@ int fp8_direct_waves(int users, int kv_heads, int head_size, int64_t tokens) {
   return head_size > 128 || segments > cus || tokens <= 4 * tile ? 4 : 8;
 }
 
-int attend(DecodeArgs a, const float *k_scales, const float *v_scales, int head_size, hipStream_t st) {
+// arrived: counters of the segments, at zero, with which several workgroups may share a segment of equal ones; or null.
+int attend(DecodeArgs a, const float *k_scales, const float *v_scales, int head_size, int *arrived, hipStream_t st) {
   const int g = a.hq / a.hkv;
   int64_t tokens = (int64_t)a.w * a.bs;
   a.bs_magic = block_magic(tokens, a.bs);
@@ -348,20 +480,31 @@ int attend(DecodeArgs a, const float *k_scales, const float *v_scales, int head_
   a.slot_floats = slot_floats_for(g, head_size);
   a.kv_format = -1;
   a.direct = fp8_direct_waves(a.users, a.hkv, head_size, tokens);
+  const int segments = a.users * a.hkv;
+  int parts = 1;
+  if (arrived) {
+    // Segments of one length, about: as many workgroups each as there are CUs for, and tiles for their wavefronts.  us a pass by wavefronts of a
+    // workgroup and workgroups of a segment, 128 segments of 2048 tokens 4/1 38.7, 4/2 36.2, 4/4 36.4, 8/1 37.2, 8/2 35.7, 8/4 40.6; 32 of 4096
+    // 4/4 37.9, 4/8 35.9, 4/16 38.6, 8/2 42.8, 8/4 36.9, 8/8 35.1.
+    const int tile = head_size <= 128 ? 64 : 32, tiles = (int)((tokens + tile - 1) / tile);
+    const int cus = std::max(device_cus(), 1);
+    a.direct = head_size <= 128 ? 8 : 4;
+    parts = std::max(1, std::min({(cus + segments - 1) / segments, (tiles + a.direct - 1) / a.direct, kMostParts}));
+  }
   a.n_waves = waves_for_device(4.0);
   a.seg_units = segment_units(1);
   if (!segment_units_forced()) a.seg_free_tiles = a.n_waves;
-  if (!a.direct && (int64_t)a.users * a.hkv > (int64_t)a.n_waves * kWave)
-    return fail(TTPA_ERR_UNSUPPORTED, "fp8 decode: %d x %d segments need a grid of more than %d wavefronts", a.users, a.hkv, a.n_waves);
+  if (!a.direct && segments > (int64_t)a.n_waves * kWave)
+    return fail(TTPA_ERR_UNSUPPORTED, "fp8 decode: %d segments need a grid of more than %d wavefronts", segments, a.n_waves);
   const uint32_t runs = (uint32_t)a.bs / (head_size <= 128 ? 16 : 8);
   const uint32_t negate = a.scale_log2e < 0.f ? 0x80008000u : 0u;
   a.scale_log2e = fabsf(a.scale_log2e);
-  const Fp8Args fa = {a, k_scales, v_scales, negate, runs, 0xffffffffu / runs};
+  const Fp8Args fa = {a, k_scales, v_scales, negate, runs, 0xffffffffu / runs, parts, arrived};
   const bool ok = head_size == 64 ? launch_fp8_d64(&fa, st) : head_size == 128 ? launch_fp8_d128(&fa, st) : launch_fp8_d256(&fa, st);
   hipEvent_t ev0, ev1;
   take_profile_events(ev0, ev1);  // still armed only if the launch did not happen
   if (!ok) return fail(TTPA_ERR_LAUNCH, "fp8 decode: cannot configure the kernel");
-  if (!a.direct) launch_combine(a, a.users * a.hkv, g, head_size, st);
+  if (!a.direct) launch_combine(a, segments, g, head_size, st);
   return check_launch("paged_fp8_decode");
 }
 
@@ -380,16 +523,18 @@ int check_decode(const void *out, int64_t out_us, int64_t out_hs, const void *q,
 
 // A sparse call's scratch behind the attention's: the scores' keys, the tables, the positions.
 struct SparseLayout {
-  size_t decode, keys, table, total;
+  size_t slots, keys, table, total;
 };
 SparseLayout sparse_layout(int users, int q_heads, int kv_heads, int head_size, int table_width, int kept) {
   const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   const size_t segments = (size_t)users * kv_heads;
+  // (segments x parts: fewer than CUs and segments, or no part but one and no slot)
+  const size_t slots = (size_t)std::max(device_cus(), 256) + segments;
   SparseLayout l;
-  l.decode = up(ttpa_paged_decode_workspace_bytes((int32_t)segments, q_heads / kv_heads, 1, head_size));
-  l.keys = up(segments * (size_t)table_width * 8);
+  l.slots = up(slots * slot_floats_for(q_heads / kv_heads, head_size) * sizeof(float));
+  l.keys = up(segments * (size_t)table_width * 8);  // scores, and as much for exact ones
   l.table = up(segments * (size_t)kept * 4);
-  l.total = l.decode + l.keys + l.table + up(segments * 4);
+  l.total = l.slots + 2 * l.keys + l.table + 2 * up(segments * 4);
   return l;
 }
 constexpr int kSparseSegments = kMaxUsers;  // (user, KV head) pairs per pass
@@ -425,7 +570,7 @@ extern "C" int ttpa_paged_fp8_decode(void *out, int64_t out_user_stride, int64_t
   a.ws_seg = static_cast<int *>(workspace);
   a.ws_slots = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + header_bytes(users, kv_heads));
   a.window = sliding_window, a.sink = attention_sink;
-  return attend(a, k_scales, v_scales, head_size, static_cast<hipStream_t>(stream));
+  return attend(a, k_scales, v_scales, head_size, nullptr, static_cast<hipStream_t>(stream));
 }
 
 extern "C" size_t ttpa_paged_fp8_sparse_decode_workspace_bytes(int32_t users, int32_t q_heads, int32_t kv_heads, int32_t head_size,
@@ -459,18 +604,13 @@ extern "C" int ttpa_paged_fp8_sparse_decode(void *out, int64_t out_head_stride, 
     s.pt = page_table + u0 * page_table_row_stride, s.pt_rs = page_table_row_stride;
     s.cur = static_cast<const uint8_t *>(cur_pos) + (int64_t)u0 * (cur_pos_is_i64 ? 8 : 4), s.cur_i64 = cur_pos_is_i64;
     s.users = n, s.hkv = kv_heads, s.g = g, s.bs = block_size, s.w = table_width, s.nb = num_blocks, s.kept = kept_blocks;
-    s.keys = reinterpret_cast<uint64_t *>(ws + l.decode);
-    s.table = reinterpret_cast<int32_t *>(ws + l.decode + l.keys);
-    s.pos = reinterpret_cast<int32_t *>(ws + l.decode + l.keys + l.table);
+    s.scores = reinterpret_cast<float2 *>(ws + l.slots);
+    s.keys = reinterpret_cast<uint64_t *>(ws + l.slots + l.keys);
+    s.table = reinterpret_cast<int32_t *>(ws + l.slots + 2 * l.keys);
+    s.pos = reinterpret_cast<int32_t *>(ws + l.slots + 2 * l.keys + l.table);
+    s.arrived = s.pos + (segments + 63) / 64 * 64;
     s.columns = columns + (int64_t)u0 * kv_heads * kept_blocks;
-    if (table_width > kept_blocks) {
-      if (head_size == 64) launch_scores<64>(s, st);
-      else if (head_size == 128) launch_scores<128>(s, st);
-      else launch_scores<256>(s, st);
-      if (const int rc = check_launch("fp8 sparse decode (scores)")) return rc;
-    }
-    choose_blocks_kernel<<<dim3(segments), dim3(256), 0, st>>>(s);
-    if (const int rc = check_launch("fp8 sparse decode (choice)")) return rc;
+    if (const int rc = head_size == 64 ? launch_choice<64>(s, st) : head_size == 128 ? launch_choice<128>(s, st) : launch_choice<256>(s, st)) return rc;
     DecodeArgs a = {};
     a.out = static_cast<uint16_t *>(out) + (int64_t)u0 * q_heads * out_head_stride, a.out_us = g * out_head_stride, a.out_hs = out_head_stride;
     a.q = s.q, a.q_us = g * q_head_stride, a.q_hs = q_head_stride;
@@ -478,9 +618,8 @@ extern "C" int ttpa_paged_fp8_sparse_decode(void *out, int64_t out_head_stride, 
     a.pt = s.table, a.pt_rs = kept_blocks, a.cur = s.pos, a.cur_i64 = 0;
     a.users = segments, a.hq = g, a.hkv = 1, a.bs = block_size, a.w = kept_blocks, a.nb = num_blocks * kv_heads;
     a.scale_log2e = scale * 1.4426950408889634f;
-    a.ws_seg = reinterpret_cast<int *>(ws);
-    a.ws_slots = reinterpret_cast<float *>(ws + header_bytes(segments, 1));
-    if (const int rc = attend(a, k_scales, v_scales, head_size, st)) return rc;
+    a.ws_slots = reinterpret_cast<float *>(ws);
+    if (const int rc = attend(a, k_scales, v_scales, head_size, s.arrived, st)) return rc;
   }
   return TTPA_OK;
 }

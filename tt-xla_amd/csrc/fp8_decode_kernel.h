@@ -34,11 +34,15 @@ namespace ttpa {
 namespace decode {
 namespace {
 
+constexpr int kMostParts = 32;  // workgroups that share a segment
 struct Fp8Args {
   DecodeArgs d;  // scale_log2e: its magnitude
   const float *k_scales, *v_scales;
   uint32_t negate;     // 0x80008000 where the scale is negative: the queries' signs are turned instead
   uint32_t runs, runs_inv;  // runs of tokens per block, and floor((2^32 - 1) / runs)
+  // DIRECT: a segment's tiles are shared by `parts` workgroups; `arrived` [segments] counts those that have left their results, from zero
+  int parts;
+  int *arrived;
 };
 
 template <int D>
@@ -66,6 +70,98 @@ __device__ __forceinline__ int fp8_kkey(int row) {
   return 4 * ((row >> 3) & 3) + (row & 3);
 }
 
+// Stores and loads that pass by the XCD's own L2 copy, of values that a workgroup of another XCD reads or has written in the same launch.  (An
+// acquire and release of all memory, which writes back and drops a whole L2 per workgroup, cost 10 us of a launch of 256.)
+__device__ __forceinline__ void store_shared(float *p, float v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ float load_shared(const float *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// The end of a segment that several workgroups have read: their wavefronts' results meet in LDS as in merge_waves, the workgroups' in memory
+// (slots [segment][part]: G * D values, G maxima, G sums), and the workgroup that arrives last merges those of all, in their order.
+template <int D, int WAVES>
+__device__ __forceinline__ void merge_parts(const DecodeArgs &a, int seg, int G, int active, int part, int parts, int slots, int *arrived, uint8_t *own,
+                                            const uint8_t *all, int pitch, const floatx4 (&acc)[D / 16], float m, float l) {
+  __shared__ float s_m[WAVES][16], s_l[WAVES][16];
+  __shared__ int s_last;
+  const int lane = threadIdx.x & 63, wib = threadIdx.x >> 6;
+  if (wib < active) {
+#pragma unroll
+    for (int db = 0; db < D / 16; ++db)
+      *reinterpret_cast<float4 *>(own + db * 1024 + lane * 16) = make_float4(acc[db][0], acc[db][1], acc[db][2], acc[db][3]);
+    if (lane < 16) s_m[wib][lane] = m, s_l[wib][lane] = l;
+  }
+  __syncthreads();
+  float *const first = a.ws_slots + (int64_t)seg * slots * a.slot_floats, *const slot = first + (int64_t)part * a.slot_floats;
+  const int gshift = G <= 1 ? 0 : 32 - __builtin_clz(G - 1);
+  for (int i = threadIdx.x; i < (D / 4) << gshift; i += kWave * WAVES) {
+    const int g = i & ((1 << gshift) - 1), d4 = i >> gshift;
+    if (g >= G) continue;
+    float mall = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w)
+      if (w < active) mall = fmaxf(mall, s_m[w][g]);
+    const float ref = merge_reference(mall);
+    float num[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w)
+      if (w < active) {
+        const float wgt = __builtin_amdgcn_exp2f(s_m[w][g] - ref);
+        const float4 x = *reinterpret_cast<const float4 *>(all + w * pitch + d4 * 256 + g * 16);
+        num[0] = fmaf(wgt, x.x, num[0]), num[1] = fmaf(wgt, x.y, num[1]);
+        num[2] = fmaf(wgt, x.z, num[2]), num[3] = fmaf(wgt, x.w, num[3]);
+        den = fmaf(wgt, s_l[w][g], den);
+      }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) store_shared(slot + g * D + 4 * d4 + r, num[r]);
+    if (d4 == 0) store_shared(slot + G * D + g, mall), store_shared(slot + G * D + G + g, den);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the thread's results have arrived where other XCDs see them
+  __syncthreads();
+  if (threadIdx.x == 0) s_last = __hip_atomic_fetch_add(arrived + seg, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
+  __syncthreads();
+  if (!s_last) return;
+  // two round trips: every part's maxima and sums, then the values, eight parts at a time
+  const int u = seg / a.hkv, h = seg - u * a.hkv;
+  float *const s_w = reinterpret_cast<float *>(const_cast<uint8_t *>(all)), *const s_den = s_w + kMostParts * 16;  // (the tiles are done with)
+  for (int i = threadIdx.x; i < parts * G; i += kWave * WAVES) {
+    const int p = i / G, g = i - p * G;
+    const float *sl = first + (int64_t)p * a.slot_floats + G * D + g;
+    s_w[p * 16 + g] = load_shared(sl), s_den[p * 16 + g] = load_shared(sl + G);
+  }
+  __syncthreads();
+  if (threadIdx.x < G) {
+    const int g = threadIdx.x;
+    float mall = -INFINITY, den = 0.f;
+    for (int p = 0; p < parts; ++p) mall = fmaxf(mall, s_w[p * 16 + g]);
+    const float ref = merge_reference(mall);
+    for (int p = 0; p < parts; ++p) {
+      const float wgt = __builtin_amdgcn_exp2f(s_w[p * 16 + g] - ref);
+      s_w[p * 16 + g] = wgt, den = fmaf(wgt, s_den[p * 16 + g], den);
+    }
+    s_den[g] = den;
+  }
+  __syncthreads();
+  for (int i = 2 * threadIdx.x; i < G * D; i += 2 * kWave * WAVES) {
+    const int g = i / D;
+    float num[2] = {0.f, 0.f};
+    for (int p0 = 0; p0 < parts; p0 += 8) {
+      uint64_t v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        v[j] = __hip_atomic_load(reinterpret_cast<const uint64_t *>(first + (int64_t)min(p0 + j, parts - 1) * a.slot_floats + i), __ATOMIC_RELAXED,
+                                 __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (p0 + j < parts) {
+          const float wgt = s_w[(p0 + j) * 16 + g];
+          num[0] = fmaf(wgt, __builtin_bit_cast(float, (uint32_t)v[j]), num[0]);
+          num[1] = fmaf(wgt, __builtin_bit_cast(float, (uint32_t)(v[j] >> 32)), num[1]);
+        }
+    }
+    uint16_t *dst = a.out + u * a.out_us + (int64_t)(h * G + g) * a.out_hs + (i - g * D);
+    dst[0] = (uint16_t)f32_to_bf16_bits(num[0] / s_den[g]), dst[1] = (uint16_t)f32_to_bf16_bits(num[1] / s_den[g]);
+  }
+}
+
 template <int D, int DIRECT>
 __global__ __launch_bounds__(DIRECT ? kWave *DIRECT : 256) __attribute__((amdgpu_waves_per_eu(2, 8)))
 void paged_decode_fp8_kernel(Fp8Args fa, const int32_t *__restrict__ page_table, const void *__restrict__ cur_pos) {
@@ -87,12 +183,15 @@ void paged_decode_fp8_kernel(Fp8Args fa, const int32_t *__restrict__ page_table,
   const int n = lane & 15, quad = lane >> 4;
   const int wave = blockIdx.x * kWavesPerBlock + wib;
   int64_t total = 0, x = 0, x_hi = 0;
-  int n_eff = 0, n_tiles = 0;
+  int n_eff = 0, n_tiles = 0, seg = 0, part = 0, parts = 1;
   Cursor cur;
   if constexpr (DIRECT > 0) {
-    cur.u = (int)blockIdx.x / a.hkv;
-    cur.h = (int)blockIdx.x - cur.u * a.hkv;
+    seg = (int)blockIdx.x / fa.parts, part = (int)blockIdx.x - seg * fa.parts;
+    cur.u = seg / a.hkv;
+    cur.h = seg - cur.u * a.hkv;
     n_tiles = tiles_of_user<TILE>(a, cur_pos, cur.u, cur.len);
+    parts = min(fa.parts, (n_tiles + DIRECT - 1) / DIRECT);
+    if (part >= max(parts, 1)) return;
     if (n_tiles == 0) {  // a padded row: NaN, like softmax over nothing
       const int g_all = a.hq / a.hkv;
       for (int i = threadIdx.x; i < g_all * D; i += kWave * DIRECT)
@@ -100,8 +199,8 @@ void paged_decode_fp8_kernel(Fp8Args fa, const int32_t *__restrict__ page_table,
       return;
     }
     cur.lo = window_lo(a, cur.len);
-    cur.t = cur.lo / TILE + wib;
-    cur.tiles_left = n_tiles - wib;
+    cur.t = cur.lo / TILE + part * DIRECT + wib;
+    cur.tiles_left = n_tiles - (part * DIRECT + wib);
   } else {
     const int total_units = __builtin_amdgcn_readfirstlane(s_pref[a.users]);
     const Share share = share_of(total_units, a.hkv, n_ranges, seg_units, wave);
@@ -185,13 +284,13 @@ void paged_decode_fp8_kernel(Fp8Args fa, const int32_t *__restrict__ page_table,
   // ---- the walk over the list ------------------------------------------------------------------
   // The cursor and unit of the tile behind (cu, at); behind the last one (of the range, or of the wavefront's part of a segment) that itself.
   auto is_last = [&](const Cursor &cu, int64_t at) {
-    if constexpr (DIRECT > 0) return cu.tiles_left <= DIRECT;
+    if constexpr (DIRECT > 0) return cu.tiles_left <= DIRECT * parts;
     return at + (cu.tiles_left > 1 ? 1 : 1 + seg_units) >= x_hi;
   };
   auto advance = [&](Cursor &cu, int64_t &at) {
     if (is_last(cu, at)) return;
     if constexpr (DIRECT > 0) {
-      cu.t += DIRECT, cu.tiles_left -= DIRECT;
+      cu.t += DIRECT * parts, cu.tiles_left -= DIRECT * parts;
     } else if (cu.tiles_left > 1) {
       ++cu.t, --cu.tiles_left, ++at;
     } else {
@@ -341,16 +440,20 @@ void paged_decode_fp8_kernel(Fp8Args fa, const int32_t *__restrict__ page_table,
     while (!is_last(cur, x)) process_tile(std::true_type{});
     process_tile(std::false_type{});
   }
-  if constexpr (DIRECT > 0)
-    merge_waves<D, DIRECT>(a, (int)blockIdx.x / a.hkv, (int)blockIdx.x % a.hkv, G, std::min(n_tiles, DIRECT), k_tile, tiles, fp8_lds_bytes<D>(), acc, 1.f,
-                           m_run, l_acc[0]);
+  if constexpr (DIRECT > 0) {
+    const int active = std::min(n_tiles - part * DIRECT, DIRECT);
+    if (parts > 1)
+      merge_parts<D, DIRECT>(a, seg, G, active, part, parts, fa.parts, fa.arrived, k_tile, tiles, fp8_lds_bytes<D>(), acc, m_run, l_acc[0]);
+    else
+      merge_waves<D, DIRECT>(a, cur.u, cur.h, G, active, k_tile, tiles, fp8_lds_bytes<D>(), acc, 1.f, m_run, l_acc[0]);
+  }
 }
 
 template <int D, int DIRECT>
 bool launch_fp8_form(const Fp8Args &fa, hipStream_t st) {
   const DecodeArgs &a = fa.d;
   constexpr int kWaves = DIRECT ? DIRECT : kWavesPerBlock;
-  const int blocks = DIRECT ? a.users * a.hkv : a.n_waves / kWavesPerBlock;
+  const int blocks = DIRECT ? a.users * a.hkv * fa.parts : a.n_waves / kWavesPerBlock;
   const auto lds_for = [](int users) { return (size_t)kWaves * fp8_lds_bytes<D>() + (DIRECT ? 0 : (2 * (size_t)users + 1) * sizeof(int)); };
   static std::atomic<uint64_t> lds_ready{0};
   const auto kernel = &paged_decode_fp8_kernel<D, DIRECT>;
