@@ -155,6 +155,7 @@ struct Rotation {
     weights_f32 = f32;
     const auto plain = [&](const OptTensor &w) {
       if (!w) return Tensor();
+      if (w->dim() == 1 && has_rows(*w) && (w->scalar_type() == at::kFloat) == f32) return *w;  // (a view would cost as much as the launch)
       Tensor t = (f32 ? w->to(at::kFloat) : *w).reshape({-1}).contiguous();
       return aligned16(t) ? t : t.clone();
     };
@@ -259,7 +260,7 @@ void paged_fill_fp8_cache_(const Tensor &k_cache, const Tensor &v_cache, const T
   const int64_t users = k_fill.size(0), s = k_fill.size(2);
   Tensor bidx;
   if (batch_idx) {
-    bidx = indices(c, batch_idx->reshape({-1}), "batch_idx");
+    bidx = indices(c, batch_idx->dim() == 1 ? *batch_idx : batch_idx->reshape({-1}), "batch_idx");
     TORCH_CHECK_VALUE(bidx.size(0) == users, c.name(), ": batch_idx must have one entry per fill row");
   } else {
     TORCH_CHECK_VALUE(users <= 1, c.name(), ": batch_idx is required when the fill holds more than one user");
@@ -302,7 +303,7 @@ void decode_into(const Call &c, const Tensor &out, const Tensor &query, const Ca
   if (sink) {
     c.see(*sink, "attention_sink");
     TORCH_CHECK_VALUE(sink->numel() == hq, c.name(), ": attention_sink must hold one logit per query head (", hq, ")");
-    logits = sink->reshape({hq}).to(at::kFloat).contiguous();
+    logits = sink->scalar_type() == at::kFloat && sink->is_contiguous() ? *sink : sink->to(at::kFloat).contiguous();
   }
   if (users == 0) return;
   const Tensor q = rows(query), target = storable(out);
@@ -398,7 +399,7 @@ void chunk_into(const Call &c, const Tensor &out, const Tensor &query, const Cac
   TORCH_CHECK_VALUE(most_keys >= 0, c.name(), ": most_keys must not be negative");
   const int64_t users = query.size(0), hq = query.size(1), s = query.size(2);
   if (users == 0 || s == 0) return;
-  const Tensor start = chunk_start.reshape({-1}).to(at::kInt).contiguous();
+  const Tensor start = chunk_start.scalar_type() == at::kInt ? chunk_start : chunk_start.to(at::kInt);
   const Tensor q = rows(query), target = storable(out);
   // as many users at a time as the copies of their blocks have room for
   const auto bytes_of = [&](int64_t n) {

@@ -7,10 +7,12 @@
 // Bound by memory: a row is read and written once.  A head row lies in D / 16 lanes as two chunks of eight features that
 // are `rotary / 2` apart, so that both features of a pair are a lane's own and the norm's sum is a few
 // cross-lane moves; 16-byte loads and stores, 128 consecutive bytes of a row at a time.  A wavefront takes U
-// groups of 1024 / D heads of one token: its cosines and sines are read once for all of them, and 2 U loads of rows are in flight.
+// groups of 1024 / D heads of one token: its cosines, sines and weights are read once for all of them, and 2 U loads of rows are in flight.
+// 8192 tokens of 32 + 8 heads of 128: 168 MB in 32.5 us, 5.2 TB/s (a large copy by torch reaches 4.9).
 #include "fp8_rows.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace ttpa {
 namespace {
@@ -157,30 +159,32 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeArgs a, int parts
   const Place<D> p(a);
   const int r = (int)(threadIdx.x & 63) / LPR, heads = a.hq + a.hk;
   RowPart x[U];
-  bool is_q[U], live[U];
-  int head[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int h = min((part * U + u) * R + r, heads - 1);  // (rows past the last head: that one again, and not stored)
+    x[u] = h < a.hq ? load_part(a.q + token * a.q_ts + h * a.q_hs, p.fa, p.fb) : load_part(a.k + token * a.k_ts + (h - a.hq) * a.k_hs, p.fa, p.fb);
+  }
+  const Angles t = angles_of<D>(a, p, load_index(a.positions, a.positions_i64, token));
+  Weights wq, wk;
+  if (a.q_weight) load_weights<D>(a.q_weight, a.weights_f32, p, wq);
+  if (a.k_weight) load_weights<D>(a.k_weight, a.weights_f32, p, wk);
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int h = (part * U + u) * R + r;
-    live[u] = h < heads;
-    is_q[u] = h < a.hq;
-    head[u] = is_q[u] ? h : h - a.hq;
-    if (live[u])
-      x[u] = is_q[u] ? load_part(a.q + token * a.q_ts + head[u] * a.q_hs, p.fa, p.fb) : load_part(a.k + token * a.k_ts + head[u] * a.k_hs, p.fa, p.fb);
-    else
-      x[u] = RowPart{};
-  }
-  const Angles t = angles_of<D>(a, p, load_index(a.positions, a.positions_i64, token));
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const void *weight = is_q[u] ? a.q_weight : a.k_weight;
+    const bool is_q = h < a.hq;
     Weights w;
-    if (weight) load_weights<D>(weight, a.weights_f32, p, w);
-    const RowPart y = turn_row<D>(a, p, x[u], weight != nullptr, w, t);
-    if (live[u]) {
-      uint16_t *dst = is_q[u] ? a.q_out + token * a.qo_ts + head[u] * a.qo_hs : a.k_out + token * a.ko_ts + head[u] * a.ko_hs;
-      *reinterpret_cast<u32x4 *>(dst + p.fa) = y.a;
-      *reinterpret_cast<u32x4 *>(dst + p.fb) = y.b;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w.a[i] = is_q ? wq.a[i] : wk.a[i], w.b[i] = is_q ? wq.b[i] : wk.b[i];
+    const RowPart y = turn_row<D>(a, p, x[u], (is_q ? a.q_weight : a.k_weight) != nullptr, w, t);
+    if (h < heads) {
+      uint16_t *dst = is_q ? a.q_out + token * a.qo_ts + h * a.qo_hs : a.k_out + token * a.ko_ts + (h - a.hq) * a.ko_hs;
+      if constexpr (U > 1) {
+        __builtin_nontemporal_store(y.a, reinterpret_cast<u32x4 *>(dst + p.fa));
+        __builtin_nontemporal_store(y.b, reinterpret_cast<u32x4 *>(dst + p.fb));
+      } else {
+        *reinterpret_cast<u32x4 *>(dst + p.fa) = y.a;
+        *reinterpret_cast<u32x4 *>(dst + p.fb) = y.b;
+      }
     }
   }
 }
@@ -260,9 +264,20 @@ int launch_rope(const RopeArgs &a, hipStream_t st) {
     const int64_t waves = (int64_t)a.tokens * parts;
     qk_norm_rope_kernel<D, U><<<dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, st>>>(a, parts);
   };
-  if (groups >= 4 && (int64_t)a.tokens * groups >= 16384) go(std::integral_constant<int, 4>{});
-  else if (groups >= 2 && (int64_t)a.tokens * groups >= 8192) go(std::integral_constant<int, 2>{});
-  else go(std::integral_constant<int, 1>{});
+  // Few rows want to be everywhere at once; many, as many groups per wavefront as there are registers for, with no slots left over: its angles and
+  // weights are read once.  8192 tokens of 32 + 8 heads of 128 (168 MB), us a pass with 1 / 2 / 3 / 5 groups 44.1 / 41.4 / 36.8 / 32.5; with ordinary
+  // stores 44.5 / 41.9 / 39.0 / 36.9.  (Those of few rows are ordinary: what is read next is read from L2.)
+  int best = 1;
+  if ((int64_t)a.tokens * groups >= 8192)
+    for (int u = 2; u <= 5; ++u)
+      if ((groups + u - 1) / u * u <= (groups + best - 1) / best * best || (u == 5 && best == 1)) best = u;
+  switch (best) {
+    case 1: go(std::integral_constant<int, 1>{}); break;
+    case 2: go(std::integral_constant<int, 2>{}); break;
+    case 3: go(std::integral_constant<int, 3>{}); break;
+    case 4: go(std::integral_constant<int, 4>{}); break;
+    default: go(std::integral_constant<int, 5>{}); break;
+  }
   return check_launch("qk_norm_rope");
 }
 
