@@ -72,15 +72,17 @@ struct Caches {
   const int32_t *pt;
   int64_t pt_rs;
   int hkv, bs, w, nb;
+  uint32_t bs_inv;  // floor((2^32 - 1) / bs)
 };
+inline uint32_t block_inverse(int bs) { return bs > 0 ? 0xffffffffu / (uint32_t)bs : 0u; }
 
-// Block and row of position `pos` of a table row; false: negative, outside the table, or a block outside the cache.
-__device__ __forceinline__ bool slot_of(const Caches &c, int64_t table_row, int64_t pos, int &phys, int &row) {
-  const int64_t col = pos / c.bs;
-  if (pos < 0 || col >= c.w) return false;
-  phys = c.pt[table_row * c.pt_rs + col];
-  row = (int)(pos - col * c.bs);
-  return (unsigned)phys < (unsigned)c.nb;
+// Column and row of position `pos` of a table row; false: negative or outside the table.  (A table row holds less than 2^31 tokens.)
+__device__ __forceinline__ bool place_of(const Caches &c, int64_t pos, int &col, int &row) {
+  const uint32_t p = (uint32_t)pos;
+  uint32_t q = __umulhi(p, c.bs_inv), r = p - q * (uint32_t)c.bs;  // one too few at most
+  if (r >= (uint32_t)c.bs) ++q, r -= (uint32_t)c.bs;
+  col = (int)q, row = (int)r;
+  return pos >= 0 && pos < (int64_t)c.w * c.bs;
 }
 
 }  // namespace fp8

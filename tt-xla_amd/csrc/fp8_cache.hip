@@ -141,7 +141,7 @@ extern "C" int ttpa_paged_fill_fp8_cache(void *k_cache, void *v_cache, float *k_
                "fp8 fill: rows and bounds must be 16-byte aligned, strides multiples of 8 elements");
   if (fill_users == 0 || seq_len == 0) return TTPA_OK;
   fp8::FillArgs a = {{static_cast<uint8_t *>(k_cache), static_cast<uint8_t *>(v_cache), k_scales, v_scales, static_cast<uint16_t *>(key_bounds),
-                      page_table, page_table_row_stride, kv_heads, block_size, table_width, num_blocks},
+                      page_table, page_table_row_stride, kv_heads, block_size, table_width, num_blocks, fp8::block_inverse(block_size)},
                      static_cast<const uint16_t *>(k_fill), static_cast<const uint16_t *>(v_fill), k_user_stride, k_head_stride, k_token_stride,
                      v_user_stride, v_head_stride, v_token_stride, batch_idx, batch_idx_is_i64, table_rows, seq_len,
                      (seq_len + block_size - 1) / block_size};

@@ -36,13 +36,33 @@ __device__ __forceinline__ void rescale_rows(uint8_t *slab, int rows, float rati
   }
 }
 
+// What the block holds already for the lane's row: its scale and, where there are any, the bounds of the lane's features.
+struct Held {
+  float scale;
+  u32x4 low[2], high[2];
+};
+template <int D>
+__device__ __forceinline__ Held load_held(const float *scales, const uint16_t *bounds, const Caches &c, int head, int phys, int row, int fa, int fb) {
+  const int64_t slab = (int64_t)phys * c.hkv + head;
+  Held h = {};
+  if (row > 0) {
+    h.scale = scales[slab];
+    if (bounds) {
+      const uint16_t *low = bounds + slab * 2 * D, *high = low + D;
+      h.low[0] = *reinterpret_cast<const u32x4 *>(low + fa), h.low[1] = *reinterpret_cast<const u32x4 *>(low + fb);
+      h.high[0] = *reinterpret_cast<const u32x4 *>(high + fa), h.high[1] = *reinterpret_cast<const u32x4 *>(high + fb);
+    }
+  }
+  return h;
+}
+
 // Writes the wavefront's rows (KV heads `head` of one token; `live`: the lane's row is one) into row `row` of block `phys`.
 // Chunk a of the lane starts at feature fa, chunk b at fb.  Row 0 begins the block: its scale and bounds are the row's own.  A later row may
 // make the scale grow; the rows before it are then rounded again, by the whole wavefront, head after head (a block's largest
 // magnitude rarely crosses a power of two behind its first rows).
 template <int D>
 __device__ __forceinline__ void write_row(uint8_t *cache, float *scales, uint16_t *bounds, const Caches &c, int head, bool live, int phys,
-                                          int row, const RowPart &x, int fa, int fb) {
+                                          int row, const RowPart &x, const Held &held, int fa, int fb) {
   constexpr int LPR = D / 16;
   const int lane = threadIdx.x & 63;
   uint32_t most = 0;
@@ -51,7 +71,7 @@ __device__ __forceinline__ void write_row(uint8_t *cache, float *scales, uint16_
   most = row_max<D>(most);
   const int64_t slab = (int64_t)phys * c.hkv + head;
   const float need = scale_for(most);
-  const float old = live && row > 0 ? scales[slab] : 0.f;
+  const float old = row > 0 ? held.scale : 0.f;
   const float scale = row > 0 ? fmaxf(old, need) : need;
   if (row > 0) {
     uint64_t grown = __builtin_amdgcn_ballot_w64(live && scale > old);
@@ -77,10 +97,7 @@ __device__ __forceinline__ void write_row(uint8_t *cache, float *scales, uint16_
     for (int half = 0; half < 2; ++half) {
       const u32x4 v = half ? x.b : x.a;
       const int f = half ? fb : fa;
-      u32x4 lo = v, hi = v;
-      if (row > 0) {
-        lo = *reinterpret_cast<const u32x4 *>(low + f), hi = *reinterpret_cast<const u32x4 *>(high + f);
-      }
+      u32x4 lo = held.low[half], hi = held.high[half];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         // (a NaN is no bound: fminf and fmaxf return the other operand; a first NaN leaves a bound that nothing passes)
@@ -96,38 +113,51 @@ __device__ __forceinline__ void write_row(uint8_t *cache, float *scales, uint16_
   }
 }
 
-// The users of a step whose tokens go to the same block: they write in turn, all of them by the first one's wavefront.
-// Returns false where the token of user u is written by another one's wavefront, or nowhere.
+// The users of a step whose tokens go to the same block write in turn, all of them by the first one's wavefront.  Every wavefront
+// therefore looks where everybody's token goes: a user per lane, four at a time, so that the look-ups of a step of up to 256 users are two round
+// trips, beside the wavefront's own.
 struct Turn {
   const void *pos;
   int pos_i64, users;
   __device__ __forceinline__ int64_t position(int u) const { return load_index(pos, pos_i64, u); }
 };
-// The next user behind u (whose block is `phys`) that writes into the same block, or `users`; `before`: whether one in front of u does.
-__device__ inline int next_in_block(const Caches &c, const Turn &t, int u, int phys, bool &before) {
+constexpr int kTurnBatch = 4, kTurnUsers = 64 * kTurnBatch;
+struct Blocks {
+  int64_t pos[kTurnBatch];
+  int block[kTurnBatch];
+};
+__device__ __forceinline__ void request_positions(const Turn &t, int first, Blocks &b) {
+#pragma unroll
+  for (int j = 0; j < kTurnBatch; ++j) b.pos[j] = t.position(min(first + 64 * j + (int)(threadIdx.x & 63), t.users - 1));
+}
+__device__ __forceinline__ void request_blocks(const Caches &c, const Turn &t, int first, Blocks &b) {
+#pragma unroll
+  for (int j = 0; j < kTurnBatch; ++j) {
+    const int v = first + 64 * j + (int)(threadIdx.x & 63);
+    int col, row;
+    b.block[j] = -1;
+    if (v < t.users && place_of(c, b.pos[j], col, row)) b.block[j] = c.pt[v * c.pt_rs + col];
+  }
+}
+// Whether a user in front of u writes into its block `phys`, too, and the next one behind it that does (`users`: nobody).  `b`: the first look-ups.
+__device__ inline int next_in_block(const Caches &c, const Turn &t, int u, int phys, Blocks b, bool &before) {
   const int lane = threadIdx.x & 63;
   before = false;
   int next = t.users;
-  constexpr int kBatch = 4;  // independent look-ups in flight
-  for (int at = 0; at < t.users && next == t.users; at += 64 * kBatch) {
-    int block[kBatch];
+  for (int at = 0;;) {
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
+    for (int j = 0; j < kTurnBatch; ++j) {
       const int v = at + 64 * j + lane;
-      int row;
-      block[j] = -1;
-      if (v < t.users && v != u && !slot_of(c, v, t.position(v), block[j], row)) block[j] = -1;
-    }
-#pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-      const int v = at + 64 * j + lane;
-      const uint64_t same = __builtin_amdgcn_ballot_w64(block[j] == phys && v < u);
-      const uint64_t later = __builtin_amdgcn_ballot_w64(block[j] == phys && v > u);
-      before |= same != 0;
+      const uint64_t earlier = __builtin_amdgcn_ballot_w64(b.block[j] == phys && v < u);
+      const uint64_t later = __builtin_amdgcn_ballot_w64(b.block[j] == phys && v > u);
+      before |= earlier != 0;
       if (later && next == t.users) next = at + 64 * j + __builtin_ctzll(later);
     }
+    at += kTurnUsers;
+    if (at >= t.users || next != t.users) return next;
+    request_positions(t, at, b);
+    request_blocks(c, t, at, b);
   }
-  return next;
 }
 
 }  // namespace fp8

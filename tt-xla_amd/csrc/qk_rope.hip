@@ -198,9 +198,10 @@ struct StepArgs {
 };
 
 // A step's write: one token per user, its keys (turned first, if `rotate`) and values into the cache; with the turned queries
-// written out by the wavefronts in front.  Bound by latency: position, page, scale, and the row are chains of
-// two or three reads, all of a few KiB; so every wavefront has one group of heads of one operand, and a
-// workgroup is one wavefront.  Users whose tokens go to the same block write in turn, by the first one's wavefront.
+// written out by the wavefronts in front.  Bound by latency: position, page, scale and bounds are a chain of three reads, of a few
+// KiB in all; so every wavefront has one group of heads of one operand, a workgroup is one wavefront, and whatever a read does not wait for is asked
+// for before it: the row and the weights beside the position, the angles beside the page.  Users whose tokens go to the same block write in
+// turn, by the first one's wavefront.
 template <int D>
 __global__ __launch_bounds__(64) void step_write_kernel(StepArgs a, int q_parts, int kv_parts) {
   constexpr int LPR = D / 16, R = 64 / LPR;
@@ -209,15 +210,15 @@ __global__ __launch_bounds__(64) void step_write_kernel(StepArgs a, int q_parts,
   const RopeArgs &ra = a.rope;
   const Place<D> p(ra);
   const int r = (int)threadIdx.x / LPR;
+  const fp8::Turn turn{ra.positions, ra.positions_i64, ra.tokens};
   if (part < q_parts) {
-    const int h = part * R + r;
-    const bool live = h < ra.hq;
-    const RowPart x = live ? load_part(ra.q + token * ra.q_ts + h * ra.q_hs, p.fa, p.fb) : RowPart{};
+    const int h = min(part * R + r, ra.hq - 1);  // (rows past the last head: that one again, and not stored)
+    const RowPart x = load_part(ra.q + token * ra.q_ts + h * ra.q_hs, p.fa, p.fb);
     Weights w;
     if (ra.q_weight) load_weights<D>(ra.q_weight, ra.weights_f32, p, w);
-    const Angles t = angles_of<D>(ra, p, load_index(ra.positions, ra.positions_i64, token));
+    const Angles t = angles_of<D>(ra, p, turn.position(token));
     const RowPart y = turn_row<D>(ra, p, x, ra.q_weight != nullptr, w, t);
-    if (live) {
+    if (part * R + r < ra.hq) {
       uint16_t *dst = ra.q_out + token * ra.qo_ts + h * ra.qo_hs;
       *reinterpret_cast<u32x4 *>(dst + p.fa) = y.a;
       *reinterpret_cast<u32x4 *>(dst + p.fb) = y.b;
@@ -226,31 +227,45 @@ __global__ __launch_bounds__(64) void step_write_kernel(StepArgs a, int q_parts,
   }
   const bool is_v = part >= q_parts + kv_parts;
   const int h = (part - q_parts - (is_v ? kv_parts : 0)) * R + r;
-  const bool live = h < a.c.hkv;
+  const bool live = h < a.c.hkv, turned = !is_v && a.rotate;
   const int head = live ? h : 0;
-  const fp8::Turn turn{ra.positions, ra.positions_i64, ra.tokens};
-  int phys, row;
+  uint8_t *const cache = is_v ? a.c.v : a.c.k;
+  float *const scales = is_v ? a.c.v_scales : a.c.k_scales;
+  uint16_t *const bounds = is_v ? nullptr : a.c.bounds;
+  const auto load_row = [&](int u) {
+    return is_v ? load_part(a.v + u * a.v_ts + head * a.v_hs, p.fa, p.fb) : load_part(ra.k + u * ra.k_ts + head * ra.k_hs, p.fa, p.fb);
+  };
   int u = token;
-  if (!fp8::slot_of(a.c, u, turn.position(u), phys, row)) return;
+  RowPart x = load_row(u);
+  Weights w;
+  if (turned && ra.k_weight) load_weights<D>(ra.k_weight, ra.weights_f32, p, w);
+  fp8::Blocks blocks;
+  fp8::request_positions(turn, 0, blocks);
+  int64_t pos = turn.position(u);
+  int col, row;
+  if (!fp8::place_of(a.c, pos, col, row)) return;
+  int phys = a.c.pt[u * a.c.pt_rs + col];
+  fp8::request_blocks(a.c, turn, 0, blocks);
+  Angles t;
+  if (turned) t = angles_of<D>(ra, p, pos);
+  if ((unsigned)phys >= (unsigned)a.c.nb) return;
+  fp8::Held held = fp8::load_held<D>(scales, bounds, a.c, head, phys, row, p.fa, p.fb);
   bool before;
-  int next = fp8::next_in_block(a.c, turn, u, phys, before);
+  int next = fp8::next_in_block(a.c, turn, u, phys, blocks, before);
   if (before) return;  // an earlier user's wavefront writes this one's token, too
   for (;;) {
-    RowPart x = is_v ? load_part(a.v + u * a.v_ts + head * a.v_hs, p.fa, p.fb) : load_part(ra.k + u * ra.k_ts + head * ra.k_hs, p.fa, p.fb);
-    if (!is_v && a.rotate) {
-      Weights w;
-      if (ra.k_weight) load_weights<D>(ra.k_weight, ra.weights_f32, p, w);
-      x = turn_row<D>(ra, p, x, ra.k_weight != nullptr, w, angles_of<D>(ra, p, turn.position(u)));
-    }
-    fp8::write_row<D>(is_v ? a.c.v : a.c.k, is_v ? a.c.v_scales : a.c.k_scales, is_v ? nullptr : a.c.bounds, a.c, head, live, phys, row, x,
-                      p.fa, p.fb);
+    if (turned) x = turn_row<D>(ra, p, x, ra.k_weight != nullptr, w, t);
+    fp8::write_row<D>(cache, scales, bounds, a.c, head, live, phys, row, x, held, p.fa, p.fb);
     if (next == ra.tokens) return;
-    // what has been written is read again by other lanes of the wavefront
+    // what has been written is read again, by other lanes of the wavefront, too
     __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");
     u = next;
-    (void)fp8::slot_of(a.c, u, turn.position(u), phys, row);
-    bool some;
-    next = fp8::next_in_block(a.c, turn, u, phys, some);
+    x = load_row(u);
+    pos = turn.position(u);
+    (void)fp8::place_of(a.c, pos, col, row);  // (of the same block)
+    if (turned) t = angles_of<D>(ra, p, pos);
+    held = fp8::load_held<D>(scales, bounds, a.c, head, phys, row, p.fa, p.fb);
+    next = fp8::next_in_block(a.c, turn, u, phys, blocks, before);
   }
 }
 
@@ -373,7 +388,7 @@ extern "C" int ttpa_qk_norm_rope_update_fp8(
                  cos_sin_is_f32, weights_are_f32, max_positions, positions, positions_is_i64, q_weight, k_weight, eps, users, q_heads, kv_heads,
                  rotary, interleaved},
                 {static_cast<uint8_t *>(k_cache), static_cast<uint8_t *>(v_cache), k_scales, v_scales, static_cast<uint16_t *>(key_bounds),
-                 page_table, page_table_row_stride, kv_heads, block_size, table_width, num_blocks},
+                 page_table, page_table_row_stride, kv_heads, block_size, table_width, num_blocks, fp8::block_inverse(block_size)},
                 static_cast<const uint16_t *>(v), v_token_stride, v_head_stride, 1};
   if (int rc = check_rope(a.rope, head_size, false)) return rc;
   if (int rc = fp8::check_cache(k_cache, v_cache, k_scales, v_scales, page_table, kv_heads, head_size, block_size, table_width, num_blocks)) return rc;
@@ -397,7 +412,7 @@ extern "C" int ttpa_paged_update_fp8_cache(void *k_cache, void *v_cache, float *
   a.rope.positions = update_indices, a.rope.positions_i64 = indices_is_i64;
   a.rope.tokens = users, a.rope.rotary = head_size;
   a.c = {static_cast<uint8_t *>(k_cache), static_cast<uint8_t *>(v_cache), k_scales, v_scales, static_cast<uint16_t *>(key_bounds), page_table,
-         page_table_row_stride, kv_heads, block_size, table_width, num_blocks};
+         page_table_row_stride, kv_heads, block_size, table_width, num_blocks, fp8::block_inverse(block_size)};
   a.v = static_cast<const uint16_t *>(v_fill), a.v_ts = v_user_stride, a.v_hs = v_head_stride;
   return step_write(a, head_size, static_cast<hipStream_t>(stream));
 }
