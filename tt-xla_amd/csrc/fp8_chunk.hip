@@ -2,8 +2,10 @@
 // (exactly: an element times its block's power of two is a bfloat16 value), and the bfloat16 prefill kernels run over the copies.
 //
 // A chunk is bound by its matrix products, 4 D q_heads operations per (row, key) pair, and every workgroup of 128 rows reads every key, so keys
-// are expanded once here and not once per workgroup; the copies cost 1 byte read and 2 written per element.  Memory bound: a
-// wavefront asks for four pieces of 512 elements before it writes the first.
+// are expanded once here and not once per workgroup; the copies cost 1 byte read and 2 written per element, at the rate of a large
+// copy: 22 us for 4 x 4608 keys of 8 heads (113 MB; 27 when every piece of 512 elements looked its block up), 13 for 8704 (53 MB).
+// (Back to back with the attention the difference is within the noise: such a pass takes 298 us either way, held up by the matrix products.)
+// The blocks are read by streaming loads and the copies written by ordinary stores: what follows reads them from the caches.
 //
 // The prefill kernels take keys by tiles of 64 and give what is behind the last row's own position weight zero, whatever it is, so it has to be
 // numbers: rows behind the chunk are copied as zeros, up to the end of the tile, and block 0 of the copies, which stands in for
@@ -30,45 +32,46 @@ struct ExpandArgs {
   int batch, w, hkv, bs, nb, q_len, d;
 };
 
-constexpr int kExpandWorkgroups = 2048, kPieces = 4;
+constexpr int kExpandWorkgroups = 16384, kPieces = 4;
 
+// A workgroup takes blocks of one head and operand (blockIdx.y), by pieces of 2048 elements.
 __global__ __launch_bounds__(256) void fp8_expand_kernel(ExpandArgs e) {
   // keys 0 .. chunk_start + q_len - 1 are read, in tiles of 64
   const int64_t end = (int64_t)(e.chunk_start ? max(*e.chunk_start, 0) : 0) + e.q_len;
-  const int cols = (int)min((int64_t)e.w, ((end + 63) / 64 * 64 + e.bs - 1) / e.bs);
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)e.batch * e.w; i += (int64_t)gridDim.x * 256)
-    e.table[i] = (int)(i % e.w) < cols ? (int)i + 1 : 0;
-  const int per_slab = e.bs * e.d / 512;  // pieces of 64 lanes x 8 elements
-  const uint32_t slabs = 2u * e.hkv, per_block = slabs * per_slab;
-  const int64_t pieces = ((int64_t)e.batch * cols + 1) * per_block;
-  const int lane = threadIdx.x & 63;
-  const int64_t step = (int64_t)gridDim.x * 4 * kPieces;
-  for (int64_t at = ((int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6)) * kPieces; at < pieces; at += step) {
-    u32x2 raw[kPieces];
-    float scale[kPieces];
-    bool zero[kPieces];
-    uint16_t *dst[kPieces];
+  const uint32_t cols = (uint32_t)min((int64_t)e.w, ((end + 63) / 64 * 64 + e.bs - 1) / e.bs);
+  const int slab = blockIdx.y;
+  if (slab == 0)
+    for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < (uint32_t)e.batch * e.w; i += gridDim.x * 256)
+      e.table[i] = i % (uint32_t)e.w < cols ? (int)i + 1 : 0;
+  const bool is_v = slab >= e.hkv;
+  const int h = slab - (is_v ? e.hkv : 0);
+  const uint8_t *src = is_v ? e.v : e.k;
+  const float *scales = is_v ? e.v_scales : e.k_scales;
+  uint16_t *copy = is_v ? e.v_copy : e.k_copy;
+  const int elements = e.bs * e.d, pieces = elements / 2048;
+  const uint32_t blocks = (uint32_t)e.batch * cols + 1;
+  for (uint32_t r = blockIdx.x; r < blocks; r += gridDim.x) {
+    // r = 0: the block of zeros; then the users' columns
+    const uint32_t b = r ? (r - 1) / cols : 0, col = r ? r - 1 - b * cols : 0;
+    const int64_t x = r ? (int64_t)b * e.w + col + 1 : 0;
+    int phys = e.pt[(int64_t)b * e.pt_rs + col];
+    if ((unsigned)phys >= (unsigned)e.nb) phys = 0;
+    const int64_t from = (int64_t)phys * e.hkv + h;
+    const uint8_t *in = src + from * elements;
+    uint16_t *out = copy + (x * e.hkv + h) * elements;
+    const int64_t left = r ? (end - (int64_t)col * e.bs) * e.d : 0;  // elements of the block in front of the chunk's end
+    const float scale = scales[from];
+    for (int p = 0; p < pieces; p += kPieces) {
+      u32x2 raw[kPieces];
 #pragma unroll
-    for (int j = 0; j < kPieces; ++j) {
-      const int64_t p = min(at + j, pieces - 1);
-      const uint32_t r = (uint32_t)(p / per_block), in_block = (uint32_t)(p - (int64_t)r * per_block);
-      const uint32_t slab = in_block / per_slab, element = 512 * (in_block - slab * per_slab) + 8 * lane;
-      // r = 0: the block of zeros; then the users' columns
-      const int b = r ? (int)((r - 1) / (uint32_t)cols) : 0, col = r ? (int)(r - 1 - (uint32_t)b * cols) : 0;
-      const int64_t x = r ? (int64_t)b * e.w + col + 1 : 0;
-      const bool is_v = slab >= (uint32_t)e.hkv;
-      const int h = (int)slab - (is_v ? e.hkv : 0);
-      int phys = e.pt[(int64_t)b * e.pt_rs + col];
-      if ((unsigned)phys >= (unsigned)e.nb) phys = 0;
-      const int64_t from = (int64_t)phys * e.hkv + h, elements = (int64_t)e.bs * e.d;
-      raw[j] = *reinterpret_cast<const u32x2 *>((is_v ? e.v : e.k) + from * elements + element);
-      scale[j] = (is_v ? e.v_scales : e.k_scales)[from];
-      zero[j] = r == 0 || (int64_t)col * e.bs + (int)(element / (uint32_t)e.d) >= end;
-      dst[j] = (is_v ? e.v_copy : e.k_copy) + (x * e.hkv + h) * elements + element;
+      for (int j = 0; j < kPieces; ++j)
+        raw[j] = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(in + 2048 * min(p + j, pieces - 1)) + threadIdx.x);
+#pragma unroll
+      for (int j = 0; j < kPieces; ++j) {
+        const int at = 2048 * (p + j) + 8 * (int)threadIdx.x;
+        if (p + j < pieces) *reinterpret_cast<u32x4 *>(out + at) = at < left ? decode8(raw[j].x, raw[j].y, scale) : u32x4{0, 0, 0, 0};
+      }
     }
-#pragma unroll
-    for (int j = 0; j < kPieces; ++j)
-      if (at + j < pieces) *reinterpret_cast<u32x4 *>(dst[j]) = zero[j] ? u32x4{0, 0, 0, 0} : decode8(raw[j].x, raw[j].y, scale[j]);
   }
 }
 
@@ -117,17 +120,16 @@ extern "C" int ttpa_chunked_fp8_attention(void *out, int64_t out_batch_stride, i
   if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u))
     return fail(TTPA_ERR_WORKSPACE, "fp8 chunk: workspace of %lld bytes (256-byte aligned) required, got %lld", (long long)need,
                 (long long)workspace_bytes);
-  TTPA_REQUIRE((int64_t)batch * l.width < (1ll << 31) - 2, "fp8 chunk: too many blocks");
+  TTPA_REQUIRE((int64_t)batch * l.width < (1ll << 31) - 2 && kv_heads < 32768, "fp8 chunk: too many blocks or heads");
   uint8_t *ws = static_cast<uint8_t *>(workspace);
   fp8::ExpandArgs e = {static_cast<const uint8_t *>(k_cache), static_cast<const uint8_t *>(v_cache), k_scales, v_scales,
                        reinterpret_cast<uint16_t *>(ws), reinterpret_cast<uint16_t *>(ws + l.copy), reinterpret_cast<int32_t *>(ws + 2 * l.copy),
                        page_table, page_table_row_stride, chunk_start, batch, l.width, kv_heads, block_size, num_blocks, q_len, head_size};
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const int64_t pieces = ((int64_t)batch * l.width + 1) * 2 * kv_heads * (block_size * head_size / 512);
   // armed events: the pair brackets both launches
   hipEvent_t before, after;
   take_profile_events(before, after);
-  const dim3 grid((unsigned)std::min<int64_t>((pieces + 4 * fp8::kPieces - 1) / (4 * fp8::kPieces), fp8::kExpandWorkgroups));
+  const dim3 grid((unsigned)std::min<int64_t>((int64_t)batch * l.width + 1, std::max(1, fp8::kExpandWorkgroups / (2 * kv_heads))), 2 * kv_heads);
   if (before)
     hipExtLaunchKernelGGL(fp8::fp8_expand_kernel, grid, dim3(256), 0u, st, before, nullptr, 0u, e);
   else
