@@ -151,6 +151,19 @@ def test_long_ragged_contexts_default_choice():
     _check(out, q, cache, table, cur, d**-0.5)
 
 
+@pytest.mark.parametrize("users, tokens", [(24, 2304), (24, 1000), (70, 800), (70, 300)])
+def test_long_and_short_lists_at_head_size_64_on_wide_tables(users, tokens):
+    """Tables wide enough for the larger grid; lists that use all of it, and lists that leave half of it empty."""
+    lengths = [max(0, tokens - 37 * (u % 9)) for u in range(users)]
+    lengths[3], lengths[5] = 0, 1
+    cache, table, cur, q, _ = _setup(users, 8, 2, 64, 64, lengths, users + tokens)
+    wide = torch.full((users, 80), -1, dtype=torch.int32)
+    wide[:, : table.shape[1]] = table
+    cache = _void(cache, wide, lengths, [0] * users)
+    out = _run(q, cache, wide, cur)
+    _check(out, q, cache, wide, cur, 64**-0.5)
+
+
 def test_more_users_than_a_wavefront_has_lanes_and_positions_beyond_the_table():
     d, bs, hkv, grp, users = 64, 32, 2, 2, 150
     g = torch.Generator().manual_seed(9)

@@ -458,7 +458,10 @@ int launch_choice(const ScoreArgs &a, hipStream_t st) {
 }
 
 // ---- the attention's launch ----------------------------------------------------------------------------
-// Wavefronts of the workgroup that reads a whole segment, or 0 (see direct_waves in decode.hip).
+// Wavefronts of the workgroup that reads a whole segment, or 0.  The limit is where lists of few segments turn (us a pass whole / cut, one user of
+// 32/8 heads of 128: 1024 tokens 8.1 / 10.9, 2048 14.1 / 10.8; 8 users 11.1 / 10.8 and 17.3 / 12.4).  With a segment for every CU and contexts about
+// alike whole segments stay ahead beyond it (128 users, 1024 ... 2048 tokens 67.5 / 75.2), but not over ragged ones, and the host cannot
+// tell them apart (64 users of 32 ... 2048 24.5 / 20.2).
 int fp8_direct_waves(int users, int kv_heads, int head_size, int64_t tokens) {
   const int64_t segments = (int64_t)users * kv_heads, bytes = tokens * head_size * 2;
   const char *forced_name = getenv("TTPA_DECODE_KERNEL");
@@ -491,7 +494,14 @@ int attend(DecodeArgs a, const float *k_scales, const float *v_scales, int head_
     a.direct = head_size <= 128 ? 8 : 4;
     parts = std::max(1, std::min({(cus + segments - 1) / segments, (tiles + a.direct - 1) / a.direct, kMostParts}));
   }
+  // Four wavefronts per CU, and eight over a long list at head size 64, whose tiles are half as large.  How long the list is the kernel
+  // knows, and then leaves half of the ranges empty.  us a pass at four / eight, 32/8 heads of 64: 8 users of 2048 ... 4096 tokens (3000 tiles) 11.8 / 12.7,
+  // 24 of 32 ... 4096 (6000) 12.0 / 12.2, 24 of 32 ... 8192 (12 000) 15.4 / 14.3, 32 of 8000 ... 16384 (49 000) 74.4 / 67.5; at 128 and 256 lists of
+  // 50 000 tiles gain 1 %, shorter ones lose 3 - 15 %.
+  const int larger_grid = waves_for_device(8.0);
   a.n_waves = waves_for_device(4.0);
+  a.many_from = 3 * (int64_t)larger_grid;
+  if (head_size == 64 && segments * ((tokens + 63) / 64 + 1) >= a.many_from) a.few_ranges = a.n_waves, a.n_waves = larger_grid;
   a.seg_units = segment_units(1);
   if (!segment_units_forced()) a.seg_free_tiles = a.n_waves;
   if (!a.direct && segments > (int64_t)a.n_waves * kWave)
