@@ -654,8 +654,10 @@ int ttpa_qk_norm_rope_update_fp8(void *q_out, int64_t q_out_token_stride, int64_
 
 /*
  * Prompts: ttpa_paged_fill_cache for both 8-bit caches.  Token t of fill row i goes to block t / block_size of page-table row batch_idx[i]
- * (NULL: row 0, of one fill row); every block's scale and bounds are those of the rows written.  Rows behind seq_len keep their bytes.  No block
- * may be named twice among the columns written: which of the writers its scale then belongs to is not defined.
+ * (NULL: row 0, of one fill row); every block's scale and bounds are those of the rows written, all seq_len of them (a padded prompt's padding, too: it
+ * is finite, or NaN).  Rows behind seq_len keep their bytes.  Of fill rows with one index the last one is written.  No block may be named twice among
+ * the columns written, unless with the same rows: whose its elements and scale then are is not defined (a block that stands for padding and is never
+ * attended may be).  Fill rows with an index outside the table and blocks outside the cache are not written.
  */
 int ttpa_paged_fill_fp8_cache(void *k_cache, void *v_cache, float *k_scales, float *v_scales, void *key_bounds, const void *k_fill,
                               int64_t k_user_stride, int64_t k_head_stride, int64_t k_token_stride, const void *v_fill, int64_t v_user_stride,
@@ -677,7 +679,7 @@ int ttpa_paged_fp8_decode(void *out, int64_t out_user_stride, int64_t out_head_s
  * The decode over `kept_blocks` (at least 2) of each user's blocks, chosen for each KV head: the first, the one that holds cur_pos, and of the others
  * those with the largest
  *   score = max over the KV head's query heads of  sum_d  max(q_d, 0) * high_d + min(q_d, 0) * low_d
- * (a bound of q . k over the block), in 64 bits; of equal scores the lower column; a score that is no finite number counts as the
+ * (a bound of q . k over the block), in 64 bits; of equal scores the lower column; a score that is NaN or +infinity counts as the
  * largest.  columns [users, kv_heads, kept_blocks] receives the page-table columns in order, then -1.  A context of no more blocks is attended whole.
  * q and out are [users, q_heads, head_size] with users q_heads * head stride apart.
  */

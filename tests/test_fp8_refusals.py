@@ -103,6 +103,12 @@ def test_refused_before_any_launch(lib, call, wrong, status, says):
     assert says in lib.ttpa_last_error(), lib.ttpa_last_error()
 
 
+@pytest.mark.parametrize("call, wrong", [(_rope, dict(tokens=1 << 25)), (_update, dict(users=1 << 25)), (_fill, dict(s=1 << 30, bs=16, w=1 << 26))])
+def test_more_than_one_launch_takes_is_refused(lib, call, wrong):
+    assert call(lib, **wrong) == -1
+    assert b"too many" in lib.ttpa_last_error(), lib.ttpa_last_error()
+
+
 def test_nothing_to_do_is_no_error(lib):
     assert _rope(lib, tokens=0) == 0 and _fill(lib, users=0) == 0 and _fill(lib, s=0) == 0 and _update(lib, users=0) == 0
 

@@ -194,3 +194,23 @@ def test_refusals():
             fill(*cache, *args)
     with pytest.raises(NotImplementedError):
         fill(*cache, p[:1, :, :5].clone().requires_grad_(), p[:1, :, :5], table)
+
+
+def test_one_row_of_the_table_filled_twice_and_one_tensor_for_both_caches():
+    hkv, d, bs = 2, 128, 32
+    cache, b, g = _noise(20, hkv, bs, d, 3)
+    want = R.Cache(*cache, b)
+    k, v = (torch.randn(70, hkv, 3 * bs - 5, d, generator=g).to(torch.bfloat16) for _ in range(2))
+    table = torch.arange(15, dtype=torch.int32).view(5, 3)
+    rows = torch.tensor([2, 4, 2, 9] + [1] * 60 + [4, 0, -1, 2, 1, 9])
+    last = [max(i for i, r in enumerate(rows.tolist()) if r == row) for row in range(5) if row in rows.tolist()]
+    want.fill(k[last], v[last], table, rows[last])
+    torch.ops.tt.paged_fill_fp8_cache_(*cache, k.cuda(), v.cuda(), table.cuda(), rows.cuda(), b)
+    assert want.differences(*cache, b) == {}
+    ke, ve, ks, vs = cache
+    idx = torch.zeros(5, dtype=torch.int32, device="cuda")
+    for bad in [(ke, ke, ks, vs), (ke, ve, ks, ks)]:
+        with pytest.raises(ValueError, match="share"):
+            torch.ops.tt.paged_update_fp8_cache_(*bad, k[None, :5, :, 0].cuda(), v[None, :5, :, 0].cuda(), idx, table.cuda())
+        with pytest.raises(ValueError, match="share"):
+            torch.ops.tt.paged_fill_fp8_cache_(*bad, k[:1].cuda(), v[:1].cuda(), table.cuda())

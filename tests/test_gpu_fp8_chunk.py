@@ -106,3 +106,63 @@ def test_refusals():
     with pytest.raises(NotImplementedError):
         op(q.clone().requires_grad_(), k, v, ks, vs, table, start)
     assert op(q[:, :, :0], k, v, ks, vs, table, start).shape == (1, 4, 0, 64)
+
+
+def test_users_in_several_passes():
+    """A table so wide that the copies of three users' blocks do not fit the scratch at once: two passes, of two users and of one."""
+    d, bs, hkv, grp, s, start = 128, 64, 8, 2, 70, 300
+    g = torch.Generator().manual_seed(9)
+    cache = _cache(20, hkv, bs, d, g)
+    table = torch.full((3, 11500), -1, dtype=torch.int32)
+    table[:, :6] = (torch.randperm(18, generator=g) + 1).view(3, 6).int()
+    q = torch.randn(3, hkv * grp, s, d, generator=g).to(torch.bfloat16)
+    args = [t.cuda() for t in cache]
+    op, at = torch.ops.tt.chunked_fp8_attention, torch.tensor([start]).cuda()
+    out = op(q.cuda(), *args, table.cuda(), at)
+    _check(out.cpu(), q, cache, table, start, d**-0.5)
+
+
+def test_captured_prompts_and_chunks():
+    """A prompt's write and a chunk over it in one graph, replayed at other starts and with other keys; every replay against the eager calls."""
+    d, bs, hkv, grp, s = 128, 32, 2, 4, 64
+    g = torch.Generator().manual_seed(10)
+    state = [t.cuda() for t in _cache(40, hkv, bs, d, g)]
+    table = (torch.randperm(39, generator=g) + 1)[:24].view(2, 12).int().cuda()
+    fill = (torch.arange(2 * 2) + 36).view(2, 2).int().cuda()
+    k, v = (torch.randn(2, hkv, s, d, generator=g).to(torch.bfloat16).cuda() for _ in range(2))
+    q = torch.randn(2, hkv * grp, s, d, generator=g).to(torch.bfloat16).cuda()
+    rows, start = torch.tensor([0, 1]).cuda(), torch.tensor([64]).cuda()
+    tt = torch.ops.tt
+
+    def run(cache):
+        tt.paged_fill_fp8_cache_(*cache, k, v, fill, rows)
+        return tt.chunked_fp8_attention(q, *cache, table, start)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run([t.clone() for t in state])
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(state)
+    for n, at in enumerate((0, 128, 32, 320, 64)):
+        start.fill_(at)
+        fill[:, 0] = table[:, (n + 1) % 4]
+        fill[:, 1] = table[:, 10]
+        for t in (k, v, q):
+            t.copy_(torch.randn(t.shape, generator=g).to(torch.bfloat16))
+        copy = [t.clone() for t in state]
+        graph.replay()
+        want = run(copy)
+        if n % 2:
+            torch.cuda.synchronize()
+        assert torch.equal(out, want) and all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(state, copy))
+
+
+def test_expanded_outputs_are_refused():
+    cache = [t.cuda() for t in _cache(4, 2, 32, 64, torch.Generator().manual_seed(5))]
+    q = torch.zeros(2, 4, 8, 64, dtype=torch.bfloat16, device="cuda")
+    table, start = torch.zeros(2, 3, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="expanded"):
+        torch.ops.tt.chunked_fp8_attention_out(q, *cache, table, start, q[:1].clone().expand(2, -1, -1, -1))

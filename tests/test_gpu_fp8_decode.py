@@ -338,6 +338,22 @@ def test_sparse_more_segments_than_one_pass_takes():
     _check_sparse(out, cols, q, cache, bounds, table, cur, 3, d**-0.5)
 
 
+@pytest.mark.parametrize("d, blocks", [(64, 8300), (128, 9001)])
+def test_sparse_tables_beyond_what_is_held(d, blocks):
+    """More columns than scores and pages are kept on the chip for, short contexts among the long ones."""
+    bs, hkv, grp, nb = 16, 1, 4, 300
+    g = torch.Generator().manual_seed(blocks)
+    cache = _cache(nb, hkv, bs, d, g)
+    bounds = _bounds(cache)
+    table = torch.randint(0, nb, (4, blocks), generator=g).int()
+    table[0, 5000:6000] = 17  # (ties across the last place)
+    cur = torch.tensor([blocks * bs - 3, 40 * bs, 3, -1])
+    q = torch.randn(4, hkv * grp, d, generator=g).to(torch.bfloat16)
+    for kept in (2, 33, 600):
+        out, cols = _sparse(q, cache, bounds, table, cur, kept, scale=0.05)
+        _check_sparse(out, cols, q, cache, bounds, table, cur, kept, 0.05)
+
+
 def test_sparse_strides():
     d, bs, hkv, grp = 128, 32, 2, 4
     cache, table, cur, q, g = _setup(4, hkv, grp, d, bs, [300, 3, 64, 200], 8)
@@ -374,3 +390,12 @@ def test_refusals():
         torch.ops.tt.paged_fp8_attention_decode_out(q, k, v, ks, vs, table, cur, torch.empty_like(q)[:, :1])
     with pytest.raises(NotImplementedError):
         op(q.clone().requires_grad_(), k, v, ks, vs, table, cur)
+
+
+def test_expanded_outputs_are_refused():
+    cache, table, cur, q, _ = _setup(2, 2, 2, 64, 32, [40, 50], 1)
+    on, out = [t.cuda() for t in cache], torch.zeros(1, 1, 4, 64, dtype=torch.bfloat16, device="cuda").expand(-1, 2, -1, -1)
+    with pytest.raises(ValueError, match="expanded"):
+        torch.ops.tt.paged_fp8_attention_decode_out(q.cuda()[None], *on, table.cuda(), cur.cuda(), out)
+    with pytest.raises(ValueError, match="expanded"):
+        torch.ops.tt.paged_fp8_sparse_attention_decode_out(q.cuda()[None], *on, _bounds(cache).cuda(), table.cuda(), cur.cuda(), out, 2)

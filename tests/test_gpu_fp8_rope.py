@@ -133,3 +133,14 @@ def test_refusals():
         op(q.clone().requires_grad_(), k, table, pos)
     with torch.no_grad():
         op(q.clone().requires_grad_(), k, table, pos)
+
+
+def test_operands_that_overlap_are_not_turned_in_place():
+    x = torch.zeros(3, 6, 64, dtype=torch.bfloat16, device="cuda")
+    table, pos = _table(4, 64).cuda(), torch.zeros(3, dtype=torch.int32, device="cuda")
+    op = torch.ops.tt.qk_norm_rope_
+    for q, k in [(x[:1].expand(3, -1, -1), x[:, :2].clone()), (x[:, :2].clone(), x[:, :1].expand(-1, 4, -1)), (x, x), (x[:, :4], x[:, :2]),
+                 (x[:2], x[1:])]:
+        with pytest.raises(ValueError):
+            op(q, k, table, pos[: q.shape[0]])
+    op(x[:, :4], x[:, 4:], table, pos)  # (views of one projection)

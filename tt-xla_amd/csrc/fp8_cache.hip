@@ -33,7 +33,7 @@ __global__ __launch_bounds__(256) void fill_kernel(FillArgs a) {
   __shared__ uint32_t s_most[4];
   __shared__ float s_low[4][D], s_high[4][D];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int col = blockIdx.x, user = blockIdx.z >> 1, h = blockIdx.y;
+  const int col = blockIdx.x, user = blockIdx.z >> 1, users = gridDim.z >> 1, h = blockIdx.y;
   const bool is_v = blockIdx.z & 1;
   const int first = col * a.c.bs, rows = min(a.c.bs, a.s - first);
   const int64_t ts = is_v ? a.v_ts : a.k_ts;
@@ -67,6 +67,11 @@ __global__ __launch_bounds__(256) void fill_kernel(FillArgs a) {
   // (uniform in the workgroup, like the next)
   const int64_t table_row = a.bidx ? load_index(a.bidx, a.bidx_i64, user) : 0;
   if (table_row < 0 || table_row >= a.table_rows) return;
+  // (of fill rows with one index the last one counts: blocks are written whole, and never with another row's scale)
+  for (int j = user + 1; j < users; j += 64) {
+    const int v = j + lane;
+    if (__builtin_amdgcn_ballot_w64(v < users && load_index(a.bidx, a.bidx_i64, min(v, users - 1)) == table_row)) return;
+  }
   const int phys = a.c.pt[table_row * a.c.pt_rs + col];
   if ((unsigned)phys >= (unsigned)a.c.nb) return;
   if constexpr (PIECES > 0) {
@@ -140,7 +145,7 @@ extern "C" int ttpa_paged_fill_fp8_cache(void *k_cache, void *v_cache, float *k_
   TTPA_REQUIRE(batch_idx != nullptr || fill_users <= 1, "fp8 fill: batch_idx may only be omitted for a single user");
   TTPA_REQUIRE((int64_t)seq_len <= (int64_t)table_width * block_size, "fp8 fill: seq_len %d does not fit %d page-table columns of %d tokens",
                seq_len, table_width, block_size);
-  TTPA_REQUIRE(fill_users < 32768 && kv_heads < 65536, "fp8 fill: too many users or heads for one launch");
+  TTPA_REQUIRE(fill_users < 32768 && kv_heads < 65536 && (seq_len - 1) / block_size < (1 << 23), "fp8 fill: too many users, heads or blocks for one launch");
   TTPA_REQUIRE(aligned16(k_fill) && aligned16(v_fill) && (!key_bounds || aligned16(key_bounds)) && k_user_stride % 8 == 0 && k_head_stride % 8 == 0 &&
                    k_token_stride % 8 == 0 && v_user_stride % 8 == 0 && v_head_stride % 8 == 0 && v_token_stride % 8 == 0,
                "fp8 fill: rows and bounds must be 16-byte aligned, strides multiples of 8 elements");

@@ -5,12 +5,14 @@
 // the caching allocator on that stream, call by call, so streams, threads and graph captures need no care of their own.  Nothing here has a
 // backward pass: a call that autograd would have to watch is refused.
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <cmath>
 #include <limits>
 #include <optional>
@@ -92,6 +94,11 @@ void written(const Tensor &t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
+// A tensor that is written: no element may stand for several.
+void single(const Call &c, const Tensor &t, const char *what) {
+  TORCH_CHECK_VALUE(at::has_internal_overlap(t) != at::MemOverlap::Yes, c.name(), ": ", what, " is written and must not be expanded");
+}
+
 // The caches of a layer.
 struct Cache {
   Tensor k, v, ks, vs;
@@ -110,6 +117,10 @@ struct Cache {
       TORCH_CHECK_VALUE(t->dim() == 2 && t->is_contiguous() && t->size(0) == nb && t->size(1) == hkv, c.name(),
                         ": a cache's scales must be a contiguous [num_blocks, kv_heads] tensor");
     }
+  }
+  // What a writer needs besides: four tensors, not one twice.
+  void writable(const Call &c) const {
+    TORCH_CHECK_VALUE(k.data_ptr() != v.data_ptr() && ks.data_ptr() != vs.data_ptr(), c.name(), ": K and V caches must not share memory");
   }
   float *k_scales() const { return static_cast<float *>(ks.data_ptr()); }
   float *v_scales() const { return static_cast<float *>(vs.data_ptr()); }
@@ -191,6 +202,9 @@ void qk_norm_rope_(const Tensor &query, const Tensor &key, const Tensor &cos_sin
   const Call c("tt::qk_norm_rope_", query);
   const Rotation r(c, query, key, cos_sin, positions, q_weight, k_weight);
   if (query.size(0) == 0) return;
+  single(c, query, "query"), single(c, key, "key");
+  TORCH_CHECK_VALUE(query.data_ptr() != key.data_ptr() && at::get_overlap_status(query, key) != at::MemOverlapStatus::Partial, c.name(),
+                    ": query and key must not overlap");
   const Tensor q = rows(query), k = rows(key);
   turn(c, r, q, k, q, k, eps, interleaved);
   if (!q.is_same(query)) query.copy_(q);
@@ -206,6 +220,7 @@ Tensor qk_norm_rope_update_fp8_(const Tensor &query, const Tensor &key, const Te
   const Call c("tt::qk_norm_rope_update_fp8_", query);
   const Rotation r(c, query, key, cos_sin, positions, q_weight, k_weight);
   const Cache cache(c, k_cache, v_cache, k_scales, v_scales);
+  cache.writable(c);
   void *bounds = cache.bounds(c, key_bounds);
   c.type(value, at::kBFloat16, "value");
   const int64_t users = query.size(0), hq = query.size(1);
@@ -231,6 +246,7 @@ void paged_update_fp8_cache_(const Tensor &k_cache, const Tensor &v_cache, const
                              const Tensor &v_fill, const Tensor &update_indices, const Tensor &page_table, const OptTensor &key_bounds) {
   const Call c("tt::paged_update_fp8_cache_", k_cache);
   const Cache cache(c, k_cache, v_cache, k_scales, v_scales);
+  cache.writable(c);
   void *bounds = cache.bounds(c, key_bounds);
   c.type(k_fill, at::kBFloat16, "k_fill");
   c.type(v_fill, at::kBFloat16, "v_fill");
@@ -254,6 +270,7 @@ void paged_fill_fp8_cache_(const Tensor &k_cache, const Tensor &v_cache, const T
                            const Tensor &v_fill, const Tensor &page_table, const OptTensor &batch_idx, const OptTensor &key_bounds) {
   const Call c("tt::paged_fill_fp8_cache_", k_cache);
   const Cache cache(c, k_cache, v_cache, k_scales, v_scales);
+  cache.writable(c);
   void *bounds = cache.bounds(c, key_bounds);
   c.type(k_fill, at::kBFloat16, "k_fill");
   c.type(v_fill, at::kBFloat16, "v_fill");
@@ -284,6 +301,7 @@ void paged_fill_fp8_cache_(const Tensor &k_cache, const Tensor &v_cache, const T
 Tensor storable(const Tensor &out) { return has_rows(out, 4) ? out : at::empty(out.sizes(), out.options()); }
 void check_out(const Call &c, const Tensor &out, const Tensor &query) {
   c.type(out, at::kBFloat16, "out");
+  single(c, out, "out");
   TORCH_CHECK_VALUE(out.sizes() == query.sizes(), c.name(), ": out must have the query's shape ", query.sizes(), ", got ", out.sizes());
 }
 void check_query(const Call &c, const Tensor &query, const Cache &cache, const Tensor &pt, const Tensor &cur) {
@@ -410,7 +428,7 @@ void chunk_into(const Call &c, const Tensor &out, const Tensor &query, const Cac
   };
   int64_t per = users;
   while (per > 1 && bytes_of(per) > kScratchLimit) per = (per + 1) / 2;
-  const int64_t bytes = bytes_of(per);
+  const int64_t rest = users % per, bytes = std::max(bytes_of(per), rest ? bytes_of(rest) : 0);  // (fewer users may want more parts)
   const Tensor ws = c.scratch(bytes);
   for (int64_t u = 0; u < users; u += per) {
     const int64_t n = std::min(per, users - u);

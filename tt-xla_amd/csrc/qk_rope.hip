@@ -318,7 +318,7 @@ int check_rope(RopeArgs &a, int head_size, bool outputs_k) {
   TTPA_REQUIRE(a.q_ts % 8 == 0 && a.q_hs % 8 == 0 && a.k_ts % 8 == 0 && a.k_hs % 8 == 0 && a.qo_ts % 8 == 0 && a.qo_hs % 8 == 0 &&
                    a.ko_ts % 8 == 0 && a.ko_hs % 8 == 0 && a.angle_rs % 8 == 0,
                "qk_norm_rope: strides must be multiples of 8 elements");
-  TTPA_REQUIRE((int64_t)a.tokens * ((a.hq + a.hk) / (1024 / head_size) + 3) < (1ll << 31), "qk_norm_rope: too many rows for one launch");
+  TTPA_REQUIRE((int64_t)a.tokens * ((a.hq + a.hk) / (1024 / head_size) + 3) < (1ll << 26), "qk_norm_rope: too many rows for one launch");
   return TTPA_OK;
 }
 
@@ -367,7 +367,7 @@ extern "C" int ttpa_qk_norm_rope(void *q_out, int64_t q_out_token_stride, int64_
 
 static int step_write(StepArgs &a, int head_size, hipStream_t st) {
   const int64_t waves = (int64_t)a.rope.tokens * ((a.rope.hq + 2 * a.c.hkv) / (1024 / head_size) + 3);
-  TTPA_REQUIRE(waves < (1ll << 31), "fp8 step write: too many rows for one launch");
+  TTPA_REQUIRE(waves < (1ll << 26), "fp8 step write: too many rows for one launch");  // (a grid has less than 2^32 threads)
   if (a.rope.tokens == 0) return TTPA_OK;
   switch (head_size) {
     case 64: return launch_step<64>(a, st);
