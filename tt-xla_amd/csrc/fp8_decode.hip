@@ -178,7 +178,6 @@ struct Choice {
   int ties;
 };
 constexpr int kThreads = 512, kWaves = kThreads / 64;
-constexpr int kHeldColumns = 8192;  // contexts of up to so many blocks: scores and pages in LDS
 struct ChoiceLds {
   uint32_t bins[kBins];
   uint64_t cand[kRanked], high[kWaves], low[kWaves];
@@ -186,14 +185,13 @@ struct ChoiceLds {
   float size[kWaves];
   uint8_t kept[kRanked];
 };
-// This thread's places in two running counts over the workgroup, and the counts of all.
+// This thread's places in two running counts over the workgroup, and the counts of all.  (Between two calls lies a barrier.)
 struct Counts {
   int before[2], all[2];
 };
 __device__ __forceinline__ Counts running_counts(ChoiceLds &s, int x, int y) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int ix = wave_prefix_sum(x), iy = wave_prefix_sum(y);
-  __syncthreads();
   if (lane == 63) s.num[0][wave] = ix, s.num[1][wave] = iy;
   __syncthreads();
   Counts c = {{ix - x, iy - y}, {0, 0}};
@@ -205,38 +203,38 @@ __device__ __forceinline__ Counts running_counts(ChoiceLds &s, int x, int y) {
   return c;
 }
 
-// Where the `need` largest of the keys key_at(1) .. key_at(n - 2) with `among` end; all threads.  A histogram over the keys' range finds the bin; the keys
-// in it are ranked, or its range is the next histogram's.
-template <typename Key, typename KeyAt, typename Among>
-__device__ __forceinline__ Choice last_kept(ChoiceLds &s, int n, int need, const KeyAt &key_at, const Among &among) {
-  constexpr int OWN = kBins / kThreads;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  Key hi = 0, lo = ~(Key)0;
-#pragma unroll 1
-  for (int c = 1 + tid; c < n - 1; c += kThreads)
-    if (among(c)) {
-      const Key k = key_at(c);
-      hi = max(hi, k), lo = min(lo, k);
-    }
+__device__ __forceinline__ void clear_bins(ChoiceLds &s) {
+#pragma unroll
+  for (int j = 0; j < kBins / kThreads; ++j) s.bins[threadIdx.x + j * kThreads] = 0;
+  if (threadIdx.x == 0) s.next = 0;
+}
+// The largest and the least of the workgroup's keys, and the largest of `size`; also in front of whatever the bins are used for.
+template <typename Key>
+__device__ __forceinline__ void extent(ChoiceLds &s, Key &hi, Key &lo, float &size) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   hi = wave_max(hi), lo = ~wave_max((Key)~lo);
+  // (magnitudes: their order is that of their bits)
+  size = __builtin_bit_cast(float, wave_max_u32(__builtin_bit_cast(uint32_t, size)));
+  if (lane == 0) s.high[wave] = hi, s.low[wave] = lo, s.size[wave] = size;
+  clear_bins(s);
   __syncthreads();
-  if (lane == 0) s.high[wave] = hi, s.low[wave] = lo;
-  __syncthreads();
-  for (int w = 0; w < kWaves; ++w) hi = max(hi, (Key)s.high[w]), lo = min(lo, (Key)s.low[w]);
+  for (int w = 0; w < kWaves; ++w) hi = max(hi, (Key)s.high[w]), lo = min(lo, (Key)s.low[w]), size = fmaxf(size, s.size[w]);
+}
+
+// Where the `need` largest of the keys between lo and hi end; all threads.  visit(f) calls f for every key that the thread has.  A
+// histogram over the keys' range finds the bin; the keys in it are ranked, or its range is the next histogram's.  The bins come cleared.
+template <typename Key, typename Visit>
+__device__ __forceinline__ Choice last_kept(ChoiceLds &s, int need, Key hi, Key lo, const Visit &visit) {
+  constexpr int OWN = kBins / kThreads;
+  const int tid = threadIdx.x;
 #pragma unroll 1
   for (;;) {
     if (need == 0) return {hi, 0};
     if (lo == hi) return {lo, need};
     const int shift = max(0, 64 - __builtin_clzll((uint64_t)(hi - lo)) - 10);  // (hi - lo) >> shift < 1024
-#pragma unroll
-    for (int j = 0; j < OWN; ++j) s.bins[tid + j * kThreads] = 0;
-    if (tid == 0) s.next = 0;
-    __syncthreads();
-#pragma unroll 1
-    for (int c = 1 + tid; c < n - 1; c += kThreads) {
-      const Key k = key_at(c);
-      if (among(c) && k >= lo && k <= hi) atomicAdd(&s.bins[(k - lo) >> shift], 1u);
-    }
+    visit([&](Key k) {
+      if (k >= lo && k <= hi) atomicAdd(&s.bins[(k - lo) >> shift], 1u);
+    });
     __syncthreads();
     // the bin, from the top, where the count reaches `need`: each thread owns neighbouring bins
     const int base = kBins - OWN * (tid + 1);
@@ -257,11 +255,9 @@ __device__ __forceinline__ Choice last_kept(ChoiceLds &s, int n, int need, const
     hi = hi - lo < span ? hi : lo + span;  // (the last bin may reach past the largest number)
     if (shift == 0) return {lo, need};     // all of the bin are alike
     if (count <= kRanked) {
-#pragma unroll 1
-      for (int c = 1 + tid; c < n - 1; c += kThreads) {
-        const Key k = key_at(c);
-        if (among(c) && k >= lo && k <= hi) s.cand[atomicAdd(&s.next, 1)] = k;
-      }
+      visit([&](Key k) {
+        if (k >= lo && k <= hi) s.cand[atomicAdd(&s.next, 1)] = k;
+      });
       __syncthreads();
       if (tid < count) {
         // the need-th largest: fewer than `need` keys are larger, and with its equals there are enough
@@ -274,6 +270,7 @@ __device__ __forceinline__ Choice last_kept(ChoiceLds &s, int n, int need, const
       __syncthreads();
       return {s.high[0], s.over};
     }
+    clear_bins(s);
     __syncthreads();
   }
 }
@@ -306,29 +303,37 @@ __device__ __forceinline__ uint64_t exact_key(const ScoreArgs &a, int u, int h, 
   return score_key(s);
 }
 
-// One workgroup per (user, KV head); what bounds it is its own chain (four round trips to memory, a dozen barriers) and, as every launch begins with a cold
-// instruction cache, its code: loops are not unrolled, scores and pages lie in LDS.  (Unrolled, in registers, 1024 threads took 21 us over 1500 blocks.)
-template <int D>
+// One workgroup per (user, KV head); what bounds it is its own chain (three round trips to memory, a dozen barriers) and, as every launch begins with a cold
+// instruction cache, its code.  HELD: tables of up to kHeld columns per thread, whose scores and pages every thread has in registers, asked for before it is
+// known how many there are; the scores of wider ones lie in LDS, up to kLdsColumns, or stay where they are.  128 (user, head) pairs of 64 ... 512 blocks 6.5 us,
+// 32 of 1024 ... 2048 9.2 (scores and pages in LDS throughout 7.1 and 12.4; unrolled over sixteen columns and with 1024 threads 21); a pass over 8192 columns,
+// in LDS / where they lie, 46.1 / 51.8.
+constexpr int kHeld = 4, kLdsColumns = 8192;
+template <int D, bool HELD>
 __global__ __launch_bounds__(kThreads) void choose_blocks_kernel(ScoreArgs a) {
   __shared__ ChoiceLds s;
-  extern __shared__ float s_held[];  // [columns], then the pages
+  extern __shared__ float s_score[];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int seg = blockIdx.x, u = seg / a.hkv, h = seg - u * a.hkv;
   const int32_t *pt = a.pt + u * a.pt_rs;
   const float2 *scores = a.scores + (int64_t)seg * a.w;
-  const bool held = a.w <= kHeldColumns;
-  int *const s_page = reinterpret_cast<int *>(s_held) + a.w;
-  float size = 0.f;  // largest sum of magnitudes
+  // Each thread has neighbouring columns, so that the chosen ones come out in order behind running counts.
+  const int held_per = (a.w + kThreads - 1) / kThreads;
+  float2 x[HELD ? kHeld : 1];
+  int id[HELD ? kHeld : 1];
+  if constexpr (HELD) {
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+      const int c = min(tid * held_per + min(j, held_per - 1), a.w - 1);
+      x[j] = scores[c], id[j] = pt[c];  // (scores that nobody has written are not used)
+    }
+  }
   int64_t pos = load_index(a.cur, a.cur_i64, u);
-  // (the first columns are asked for before it is known how many there are)
-  const int c_first = min(tid, a.w - 1);
-  const float2 first_score = a.w > a.kept ? scores[c_first] : make_float2(0.f, 0.f);
-  const int first_page = pt[c_first];
   const int nblk = blocks_of(a, u, pos);
   int32_t *table = a.table + (int64_t)seg * a.kept, *columns = a.columns + (int64_t)seg * a.kept;
   const int chosen = min(nblk, a.kept);
-  const auto emit = [&](int at, int c, int id) {
-    table[at] = ((unsigned)id < (unsigned)a.nb ? id : 0) * a.hkv + h;
+  const auto emit = [&](int at, int c, int page) {
+    table[at] = ((unsigned)page < (unsigned)a.nb ? page : 0) * a.hkv + h;
     columns[at] = c;
   };
 #pragma unroll 1
@@ -342,21 +347,52 @@ __global__ __launch_bounds__(kThreads) void choose_blocks_kernel(ScoreArgs a) {
     for (int c = tid; c < nblk; c += kThreads) emit(c, c, pt[c]);
     return;
   }
+  if (tid == 0) emit(0, 0, pt[0]), emit(a.kept - 1, nblk - 1, pt[nblk - 1]);
+  const int per = HELD ? held_per : (nblk + kThreads - 1) / kThreads;
+  const int first = tid * per, from = max(min(first, nblk), 1), to = min(first + per, nblk - 1);  // of the blocks but the first and the last
+  const bool in_lds = !HELD && a.w <= kLdsColumns;
+  const auto score = [&](int c) { return in_lds ? s_score[c] : scores[c].x; };
+  // f(column, score, place in `id`) for the thread's own, in order
+  const auto own = [&](const auto &f) {
+    if constexpr (HELD) {
+#pragma unroll
+      for (int j = 0; j < kHeld; ++j)
+        if (first + j >= from && first + j < to) f(first + j, x[j].x, j);
+    } else {
 #pragma unroll 1
-  for (int c = tid; c < nblk; c += kThreads) {
-    const float2 v = c == tid ? first_score : scores[c];
-    size = fmaxf(size, v.y);
-    if (held) s_held[c] = v.x, s_page[c] = c == tid ? first_page : pt[c];
+      for (int c = from; c < to; ++c) f(c, score(c), c);
+    }
+  };
+  // f(column, score) for the columns between the workgroup's threads in any order
+  const auto any = [&](const auto &f) {
+    if constexpr (HELD) {
+      own([&](int c, float v, int) { f(c, v); });
+    } else {
+#pragma unroll 1
+      for (int c = 1 + tid; c < nblk - 1; c += kThreads) f(c, score(c));
+    }
+  };
+  const auto page = [&](int j) {
+    if constexpr (HELD) return id[j];
+    return pt[j];
+  };
+  uint32_t hi = 0, lo = ~0u;
+  float size = 0.f;  // largest sum of magnitudes
+  if constexpr (HELD) {
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j)
+      if (first + j >= from && first + j < to) size = fmaxf(size, x[j].y), hi = max(hi, float_key(x[j].x)), lo = min(lo, float_key(x[j].x));
+  } else {
+#pragma unroll 4
+    for (int c = 1 + tid; c < nblk - 1; c += kThreads) {
+      const float2 v = scores[c];
+      if (in_lds) s_score[c] = v.x;
+      size = fmaxf(size, v.y), hi = max(hi, float_key(v.x)), lo = min(lo, float_key(v.x));
+    }
   }
-  // (magnitudes: their order is that of their bits)
-  size = __builtin_bit_cast(float, wave_max_u32(__builtin_bit_cast(uint32_t, size)));
-  if (lane == 0) s.size[wave] = size;
-  __syncthreads();
-  for (int w = 0; w < kWaves; ++w) size = fmaxf(size, s.size[w]);
-  const auto score = [&](int c) { return held ? s_held[c] : scores[c].x; };
-  const auto page = [&](int c) { return held ? s_page[c] : pt[c]; };
-  const int need = a.kept - 2;  // of the blocks but the first and the last
-  const Choice approx = last_kept<uint32_t>(s, nblk, need, [&](int c) { return float_key(score(c)); }, [](int) { return true; });
+  extent(s, hi, lo, size);
+  const int need = a.kept - 2;
+  const Choice approx = last_kept<uint32_t>(s, need, hi, lo, [&](const auto &f) { any([&](int, float v) { f(float_key(v)); }); });
   // T, and how far a score may be from the exact one: at most 512 additions, each off by at most a unit in the last place of what the magnitudes
   // add up to (2^-23), twice that for what the matrix pipe's own order and rounding may be; and what falls below the smallest normal number.
   const uint32_t tb = (uint32_t)approx.threshold;
@@ -364,13 +400,10 @@ __global__ __launch_bounds__(kThreads) void choose_blocks_kernel(ScoreArgs a) {
   const float e = size * 0x1p-13f + 0x1p-100f;
   const bool exact_all = !(size < INFINITY) || !(fabsf(t) < INFINITY);  // infinities among the scores: no bound says anything
   const float sure = exact_all ? INFINITY : t + 2.f * e, out = exact_all ? -INFINITY : t - 2.f * e;
-  const auto kept_surely = [&](int c) { return !exact_all && need > 0 && score(c) > sure; };
-  const auto in_question = [&](int c) { return exact_all || (need > 0 && score(c) >= out && !(score(c) > sure)); };
-  // Each thread has neighbouring columns from here on, so that the chosen ones come out in order behind running counts.
-  const int per = (nblk + kThreads - 1) / kThreads, from = max(min(tid * per, nblk), 1), to = min(tid * per + per, nblk - 1);
+  const auto kept_surely = [&](float v) { return !exact_all && need > 0 && v > sure; };
+  const auto in_question = [&](float v) { return exact_all || (need > 0 && v >= out && !(v > sure)); };
   int sure_mine = 0, open_mine = 0;
-#pragma unroll 1
-  for (int c = from; c < to; ++c) sure_mine += kept_surely(c), open_mine += in_question(c);
+  own([&](int, float v, int) { sure_mine += kept_surely(v), open_mine += in_question(v); });
   const Counts n = running_counts(s, sure_mine, open_mine);
   const int open = n.all[1], need_open = need - n.all[0];
   constexpr int GROUPS = 256 / D;  // of lanes with a score of their own, in a wavefront
@@ -380,14 +413,14 @@ __global__ __launch_bounds__(kThreads) void choose_blocks_kernel(ScoreArgs a) {
   if (open <= kRanked) {
     // few in question: their exact scores and ranks in LDS
     int at = n.before[1];
-#pragma unroll 1
-    for (int c = from; c < to; ++c)
-      if (in_question(c)) s.column[at] = c, s.cand[at] = 0, ++at;
+    own([&](int c, float v, int j) {
+      if (in_question(v)) s.column[at] = page(j), s.cand[at] = 0, ++at;
+    });
     __syncthreads();
 #pragma unroll 1
     for (int i = group; i - group < open * a.g; i += kWaves * GROUPS) {
-      const int x = min(i, open * a.g - 1), o = x / a.g;
-      const uint64_t k = exact_key<D>(a, u, h, x - o * a.g, page(s.column[o]));
+      const int y = min(i, open * a.g - 1), o = y / a.g;
+      const uint64_t k = exact_key<D>(a, u, h, y - o * a.g, s.column[o]);
       if (lane % (D / 4) == 0 && i < open * a.g) atomicMax(reinterpret_cast<unsigned long long *>(&s.cand[o]), (unsigned long long)k);
     }
     __syncthreads();
@@ -399,15 +432,15 @@ __global__ __launch_bounds__(kThreads) void choose_blocks_kernel(ScoreArgs a) {
       s.kept[tid] = better < need_open;
     }
     __syncthreads();
+    if (sure_mine + open_mine == 0) return;
 #pragma unroll 1
     for (int i = 0; i < n.before[1]; ++i) place += s.kept[i];
     at = n.before[1];
-#pragma unroll 1
-    for (int c = from; c < to; ++c) {
-      bool is = kept_surely(c);
-      if (in_question(c)) is = s.kept[at++];
-      if (is) emit(place++, c, page(c));
-    }
+    own([&](int c, float v, int j) {
+      bool is = kept_surely(v);
+      if (in_question(v)) is = s.kept[at++];
+      if (is) emit(place++, c, page(j));
+    });
   } else {
     // many (scores alike, infinities): exact scores of all in memory, and the choice among those in question by them
 #pragma unroll 1
@@ -415,30 +448,37 @@ __global__ __launch_bounds__(kThreads) void choose_blocks_kernel(ScoreArgs a) {
       const int c = min(i, nblk - 1);
       uint64_t k = 0;
 #pragma unroll 1
-      for (int g = 0; g < a.g; ++g) k = max(k, exact_key<D>(a, u, h, g, page(c)));
+      for (int g = 0; g < a.g; ++g) k = max(k, exact_key<D>(a, u, h, g, pt[c]));
       if (lane % (D / 4) == 0 && i < nblk) keys[i] = k;
     }
     __syncthreads();
-    const Choice exact = last_kept<uint64_t>(s, nblk, need_open, [&](int c) { return keys[c]; }, in_question);
+    const auto visit = [&](const auto &f) {
+      any([&](int c, float v) {
+        if (in_question(v)) f(keys[c]);
+      });
+    };
+    uint64_t high = 0, low = ~0ull;
+    visit([&](uint64_t k) { high = max(high, k), low = min(low, k); });
+    extent(s, high, low, size);
+    const Choice exact = last_kept<uint64_t>(s, need_open, high, low, visit);
     // of the blocks tied for the last places the first ones win
     int above = 0, tied = 0;
-#pragma unroll 1
-    for (int c = from; c < to; ++c)
-      if (in_question(c)) above += keys[c] > exact.threshold, tied += keys[c] == exact.threshold;
+    own([&](int c, float v, int) {
+      if (in_question(v)) above += keys[c] > exact.threshold, tied += keys[c] == exact.threshold;
+    });
+    __syncthreads();
     const Counts m = running_counts(s, above, tied);
     int t_at = m.before[1];
     place += m.before[0] + min(t_at, exact.ties);
-#pragma unroll 1
-    for (int c = from; c < to; ++c) {
-      bool is = kept_surely(c);
-      if (in_question(c)) {
+    own([&](int c, float v, int j) {
+      bool is = kept_surely(v);
+      if (in_question(v)) {
         is = keys[c] > exact.threshold || (keys[c] == exact.threshold && t_at < exact.ties);
         t_at += keys[c] == exact.threshold;
       }
-      if (is) emit(place++, c, page(c));
-    }
+      if (is) emit(place++, c, page(j));
+    });
   }
-  if (tid == 0) emit(0, 0, page(0)), emit(a.kept - 1, nblk - 1, page(nblk - 1));
 }
 
 template <int D>
@@ -449,11 +489,10 @@ int launch_choice(const ScoreArgs &a, hipStream_t st) {
     block_scores_kernel<D><<<dim3((a.w + kBlocks - 1) / kBlocks, segments), dim3(256), 0, st>>>(a);
     if (const int rc = check_launch("fp8 sparse decode (scores)")) return rc;
   }
-  const size_t lds = a.w <= kHeldColumns ? (size_t)a.w * 8 : 0;
-  static std::atomic<uint64_t> lds_ready{0};
-  if (!ensure_dynamic_lds(reinterpret_cast<const void *>(&choose_blocks_kernel<D>), kHeldColumns * 8, lds_ready))
-    return fail(TTPA_ERR_LAUNCH, "fp8 sparse decode: cannot configure the choice of blocks");
-  choose_blocks_kernel<D><<<dim3(segments), dim3(kThreads), lds, st>>>(a);
+  if (a.w <= kHeld * kThreads)
+    choose_blocks_kernel<D, true><<<dim3(segments), dim3(kThreads), 0, st>>>(a);
+  else
+    choose_blocks_kernel<D, false><<<dim3(segments), dim3(kThreads), a.w <= kLdsColumns ? 4 * (size_t)a.w : 0, st>>>(a);
   return check_launch("fp8 sparse decode (choice)");
 }
 
