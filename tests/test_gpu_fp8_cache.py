@@ -209,7 +209,8 @@ def test_one_row_of_the_table_filled_twice_and_one_tensor_for_both_caches():
     assert want.differences(*cache, b) == {}
     ke, ve, ks, vs = cache
     idx = torch.zeros(5, dtype=torch.int32, device="cuda")
-    for bad in [(ke, ke, ks, vs), (ke, ve, ks, ks)]:
+    both = torch.zeros(30, hkv, bs, d, dtype=torch.uint8, device="cuda").view(ke.dtype)
+    for bad in [(ke, ke, ks, vs), (ke, ve, ks, ks), (both[:20], both[10:], ks, vs)]:
         with pytest.raises(ValueError, match="share"):
             torch.ops.tt.paged_update_fp8_cache_(*bad, k[None, :5, :, 0].cuda(), v[None, :5, :, 0].cuda(), idx, table.cuda())
         with pytest.raises(ValueError, match="share"):

@@ -399,3 +399,6 @@ def test_expanded_outputs_are_refused():
         torch.ops.tt.paged_fp8_attention_decode_out(q.cuda()[None], *on, table.cuda(), cur.cuda(), out)
     with pytest.raises(ValueError, match="expanded"):
         torch.ops.tt.paged_fp8_sparse_attention_decode_out(q.cuda()[None], *on, _bounds(cache).cuda(), table.cuda(), cur.cuda(), out, 2)
+    into = torch.zeros(600, dtype=torch.bfloat16, device="cuda").as_strided((1, 2, 4, 64), (0, 128, 64, 1))
+    with pytest.raises(ValueError, match="overlap itself"):
+        torch.ops.tt.paged_fp8_attention_decode_out(q.cuda()[None], *on, table.cuda(), cur.cuda(), into)

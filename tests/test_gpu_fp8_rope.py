@@ -140,7 +140,32 @@ def test_operands_that_overlap_are_not_turned_in_place():
     table, pos = _table(4, 64).cuda(), torch.zeros(3, dtype=torch.int32, device="cuda")
     op = torch.ops.tt.qk_norm_rope_
     for q, k in [(x[:1].expand(3, -1, -1), x[:, :2].clone()), (x[:, :2].clone(), x[:, :1].expand(-1, 4, -1)), (x, x), (x[:, :4], x[:, :2]),
-                 (x[:2], x[1:])]:
+                 (x[:2], x[1:]), (x[:, :4], x[:, 3:]), (x[:, 2:4], x[:, 1:]), (x[:, ::2], x[:, 1:3]),
+                 (x.as_strided((3, 3, 64), (128, 64, 1)), x[:, :2].clone()), (x.as_strided((3, 4, 64), (384, 32, 1)), x[:, :2].clone())]:
         with pytest.raises(ValueError):
             op(q, k, table, pos[: q.shape[0]])
-    op(x[:, :4], x[:, 4:], table, pos)  # (views of one projection)
+
+
+def test_views_of_one_projection_are_turned_in_place():
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(3, 6, 64, generator=g).to(torch.bfloat16).cuda()
+    table, pos = _table(4, 64).cuda(), torch.tensor([0, 3, 1], dtype=torch.int32, device="cuda")
+    op = torch.ops.tt.qk_norm_rope_
+    for q, k in [(slice(0, 4), slice(4, 6)), (slice(4, 6), slice(0, 4)), (slice(0, 6, 2), slice(1, 6, 2)), (slice(0, 3), slice(5, 6))]:
+        want = torch.ops.tt.qk_norm_rope(x[:, q].contiguous(), x[:, k].contiguous(), table, pos)
+        y = x.clone()
+        op(y[:, q], y[:, k], table, pos)
+        assert torch.equal(y[:, q], want[0]) and torch.equal(y[:, k], want[1])
+    y = x.clone()  # (tokens behind tokens)
+    want = torch.ops.tt.qk_norm_rope(x[:1], x[1:2], table, pos[:1])
+    op(y[:1], y[1:2], table, pos[:1])
+    assert torch.equal(y[:1], want[0]) and torch.equal(y[1:2], want[1])
+
+
+def test_tangents_are_refused():
+    import torch.autograd.forward_ad as fwd
+
+    q = torch.zeros(2, 4, 64, dtype=torch.bfloat16, device="cuda")
+    table, pos = _table(4, 64).cuda(), torch.zeros(2, dtype=torch.int32, device="cuda")
+    with fwd.dual_level(), pytest.raises(NotImplementedError, match="tangent"):
+        torch.ops.tt.qk_norm_rope(fwd.make_dual(q, torch.ones_like(q)), q, table, pos)

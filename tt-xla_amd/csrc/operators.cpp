@@ -5,7 +5,6 @@
 // the caching allocator on that stream, call by call, so streams, threads and graph captures need no care of their own.  Nothing here has a
 // backward pass: a call that autograd would have to watch is refused.
 #include <ATen/ATen.h>
-#include <ATen/MemoryOverlap.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
@@ -44,6 +43,7 @@ class Call {
     TORCH_CHECK_VALUE(t.device() == device_, name_, ": ", what, " is on ", t.device(), ", not on ", device_);
     TORCH_CHECK_NOT_IMPLEMENTED(!(at::GradMode::is_enabled() && t.requires_grad()), name_, " has no backward pass, and ", what,
                                 " requires a gradient: call it under torch.no_grad()");
+    TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), name_, " has no derivative, and ", what, " carries a tangent");
   }
   void see(const OptTensor &t, const char *what) const {
     if (t) see(*t, what);
@@ -94,9 +94,36 @@ void written(const Tensor &t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
-// A tensor that is written: no element may stand for several.
+// A tensor that is written: no element may stand for several.  (Strides in order, each at least as long as what lies inside it: what is laid out
+// in another way without overlapping is refused, too.)
 void single(const Call &c, const Tensor &t, const char *what) {
-  TORCH_CHECK_VALUE(at::has_internal_overlap(t) != at::MemOverlap::Yes, c.name(), ": ", what, " is written and must not be expanded");
+  int64_t end = 1, last = 0;  // elements that the dimensions so far reach over
+  for (int64_t n = 0; n < t.dim(); ++n) {
+    int64_t stride = std::numeric_limits<int64_t>::max(), size = 1;  // the next longer stride's
+    for (int64_t i = 0; i < t.dim(); ++i)
+      if (t.size(i) > 1 && t.stride(i) > last && t.stride(i) < stride) stride = t.stride(i), size = t.size(i);
+    for (int64_t i = 0; i < t.dim(); ++i)
+      TORCH_CHECK_VALUE(t.size(i) <= 1 || t.stride(i) > 0, c.name(), ": ", what, " is written and must not be expanded");
+    if (size == 1) break;
+    TORCH_CHECK_VALUE(stride >= end, c.name(), ": ", what, " is written and must not overlap itself");
+    end += (size - 1) * stride, last = stride;
+  }
+}
+// Whether two [tokens, heads, head_size] tensors of one shape but for the heads, neither overlapping itself, have an element in common;
+// true also where that is not looked into (different token strides, tokens that reach into each other).
+bool overlap(const Tensor &x, const Tensor &y) {
+  if (!x.is_alias_of(y)) return false;
+  const int64_t d = x.size(2), tokens = x.size(0), xs = x.storage_offset(), ys = y.storage_offset();
+  const int64_t xh = step_of(x, 1), yh = step_of(y, 1), xt = step_of(x, 0), yt = step_of(y, 0);
+  const int64_t xe = xs + (x.size(1) - 1) * xh + (d - 1) * x.stride(2) + 1, ye = ys + (y.size(1) - 1) * yh + (d - 1) * y.stride(2) + 1;
+  if (xe + (tokens - 1) * xt <= ys || ye + (tokens - 1) * yt <= xs) return false;
+  if (xt != yt || (tokens > 1 && std::max(xe, ye) - std::min(xs, ys) > xt)) return true;
+  if (xe <= ys || ye <= xs) return false;
+  if (x.stride(2) != 1 || y.stride(2) != 1) return true;
+  for (int64_t i = 0; i < x.size(1); ++i)
+    for (int64_t j = 0; j < y.size(1); ++j)
+      if (std::abs(xs + i * xh - ys - j * yh) < d) return true;
+  return false;
 }
 
 // The caches of a layer.
@@ -120,7 +147,11 @@ struct Cache {
   }
   // What a writer needs besides: four tensors, not one twice.
   void writable(const Call &c) const {
-    TORCH_CHECK_VALUE(k.data_ptr() != v.data_ptr() && ks.data_ptr() != vs.data_ptr(), c.name(), ": K and V caches must not share memory");
+    const auto apart = [](const Tensor &x, const Tensor &y) {  // (contiguous, of one shape)
+      const char *const a = static_cast<const char *>(x.data_ptr()), *const b = static_cast<const char *>(y.data_ptr());
+      return std::abs(a - b) >= (int64_t)x.nbytes();
+    };
+    TORCH_CHECK_VALUE(apart(k, v) && apart(ks, vs), c.name(), ": K and V caches must not share memory");
   }
   float *k_scales() const { return static_cast<float *>(ks.data_ptr()); }
   float *v_scales() const { return static_cast<float *>(vs.data_ptr()); }
@@ -203,8 +234,7 @@ void qk_norm_rope_(const Tensor &query, const Tensor &key, const Tensor &cos_sin
   const Rotation r(c, query, key, cos_sin, positions, q_weight, k_weight);
   if (query.size(0) == 0) return;
   single(c, query, "query"), single(c, key, "key");
-  TORCH_CHECK_VALUE(query.data_ptr() != key.data_ptr() && at::get_overlap_status(query, key) != at::MemOverlapStatus::Partial, c.name(),
-                    ": query and key must not overlap");
+  TORCH_CHECK_VALUE(!overlap(query, key), c.name(), ": query and key must not overlap");
   const Tensor q = rows(query), k = rows(key);
   turn(c, r, q, k, q, k, eps, interleaved);
   if (!q.is_same(query)) query.copy_(q);
