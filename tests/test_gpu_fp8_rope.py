@@ -64,6 +64,25 @@ def test_rows(tokens, hq, hk, d, rotary):
             assert torch.equal(v2, dev[:, (hq + hk) * d :])
 
 
+@pytest.mark.parametrize("hq, hk, d, rotary, tokens", [(8, 2, 64, 32, 8195), (1, 1, 64, 64, 8200), (8, 1, 128, 128, 4100), (5, 1, 128, 64, 8193), (2, 2, 256, 256, 8192),
+                                                       (3, 2, 256, 96, 4111), (14, 3, 128, 128, 2731), (30, 3, 128, 128, 1700), (63, 2, 64, 64, 1650), (25, 3, 128, 96, 2100)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_many_tokens_of_few_heads(hq, hk, d, rotary, tokens, interleaved):
+    """Rows of neighbouring tokens in one wavefront, views of a projection, positions in no order and outside the table."""
+    g = torch.Generator().manual_seed(tokens + hq)
+    both = torch.randn(tokens, hq + hk + 1, d, generator=g).to(torch.bfloat16)
+    q, k = both[:, :hq], both[:, hq : hq + hk]
+    table = _table(300, rotary)
+    pos = torch.randint(-2, 305, (tokens,), generator=g)
+    qw, kw = (1 + 0.2 * torch.randn(d, generator=g) for _ in range(2))
+    on = both.cuda()
+    got = torch.ops.tt.qk_norm_rope(on[:, :hq], on[:, hq : hq + hk], table.cuda(), pos.cuda(), qw.cuda(), None, 1e-6, interleaved)
+    _check(got[0].cpu(), q, qw, table, pos, 1e-6, interleaved)
+    _check(got[1].cpu(), k, None, table, pos, 1e-6, interleaved)
+    torch.ops.tt.qk_norm_rope_(on[:, :hq], on[:, hq : hq + hk], table.cuda(), pos.cuda(), qw.cuda(), None, 1e-6, interleaved)
+    assert torch.equal(on[:, :hq], got[0]) and torch.equal(on[:, hq : hq + hk], got[1]) and torch.equal(on[:, hq + hk :].cpu(), both[:, hq + hk :])
+
+
 def test_table_in_bfloat16_long_positions_and_positions_outside():
     tokens, hq, hk, d = 6, 4, 2, 128
     qkv, _ = _inputs(tokens, hq, hk, d, 3)

@@ -189,6 +189,54 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeArgs a, int parts
   }
 }
 
+// The same over the rows of all tokens in order (row = token * heads + head), U * R consecutive ones per wavefront, each with angles of its own: for so
+// few heads that a token's own one or two wavefronts stay partly empty.  us a pass, a token's wavefronts / this: 12056 tokens of 8 + 2 heads of 64 14.1 / 8.8,
+// 16384 of 8 + 1 of 128 24.0 / 19.4 and of 4 + 1 18.2 / 12.7, 8192 of 2 + 1 of 256 11.2 / 8.4; with three wavefronts per token 8192 of 16 + 2 of 128 17.7 / 18.9.
+// (One, three and four rows per lane 10.1, 9.5 and 9.5 on the first.)
+template <int D, int U>
+__global__ __launch_bounds__(256) void qk_norm_rope_rows_kernel(RopeArgs a, uint32_t heads_inv) {
+  constexpr int LPR = D / 16, R = 64 / LPR;
+  const Place<D> p(a);
+  const uint32_t heads = a.hq + a.hk, rows = (uint32_t)a.tokens * heads;
+  const uint32_t first = (blockIdx.x * 4 + (threadIdx.x >> 6)) * (U * R) + (threadIdx.x & 63) / LPR;
+  RowPart x[U];
+  int token[U], head[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t row = min(first + u * R, rows - 1);  // (rows past the last: that one again, and not stored)
+    uint32_t n = __umulhi(row, heads_inv), h = row - n * heads;  // one too few at most
+    if (h >= heads) ++n, h -= heads;
+    token[u] = (int)n, head[u] = (int)h;
+  }
+  int64_t pos[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) pos[u] = load_index(a.positions, a.positions_i64, token[u]);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int h = head[u] - a.hq;
+    x[u] = load_part(h < 0 ? a.q + token[u] * a.q_ts + head[u] * a.q_hs : a.k + token[u] * a.k_ts + h * a.k_hs, p.fa, p.fb);
+  }
+  Angles t[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) t[u] = angles_of<D>(a, p, pos[u]);
+  Weights wq, wk;
+  if (a.q_weight) load_weights<D>(a.q_weight, a.weights_f32, p, wq);
+  if (a.k_weight) load_weights<D>(a.k_weight, a.weights_f32, p, wk);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int h = head[u] - a.hq;
+    Weights w;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w.a[i] = h < 0 ? wq.a[i] : wk.a[i], w.b[i] = h < 0 ? wq.b[i] : wk.b[i];
+    const RowPart y = turn_row<D>(a, p, x[u], (h < 0 ? a.q_weight : a.k_weight) != nullptr, w, t[u]);
+    if (first + u * R < rows) {
+      uint16_t *dst = h < 0 ? a.q_out + token[u] * a.qo_ts + head[u] * a.qo_hs : a.k_out + token[u] * a.ko_ts + h * a.ko_hs;
+      __builtin_nontemporal_store(y.a, reinterpret_cast<u32x4 *>(dst + p.fa));
+      __builtin_nontemporal_store(y.b, reinterpret_cast<u32x4 *>(dst + p.fb));
+    }
+  }
+}
+
 struct StepArgs {
   RopeArgs rope;
   fp8::Caches c;
@@ -283,12 +331,18 @@ int launch_rope(const RopeArgs &a, hipStream_t st) {
   // weights are read once.  8192 tokens of 32 + 8 heads of 128 (168 MB), us a pass with 1 / 2 / 3 / 5 groups 44.1 / 41.4 / 36.8 / 32.5; with ordinary
   // stores 44.5 / 41.9 / 39.0 / 36.9.  (Those of few rows are ordinary: what is read next is read from L2.)
   int best = 1;
-  if ((int64_t)a.tokens * groups >= 8192)
-    for (int u = 2; u <= 5; ++u)
+  if ((int64_t)a.tokens * groups >= 8192) {
+    if (groups <= 2) {
+      constexpr int U = 2, PER = 4 * U * R;  // rows of a workgroup
+      const int64_t rows = (int64_t)a.tokens * (a.hq + a.hk);
+      qk_norm_rope_rows_kernel<D, U><<<dim3((unsigned)((rows + PER - 1) / PER)), dim3(256), 0, st>>>(a, 0xffffffffu / (uint32_t)(a.hq + a.hk));
+      return check_launch("qk_norm_rope");
+    }
+    for (int u = 3; u <= std::min(groups, 5); ++u)
       if ((groups + u - 1) / u * u <= (groups + best - 1) / best * best || (u == 5 && best == 1)) best = u;
+  }
   switch (best) {
     case 1: go(std::integral_constant<int, 1>{}); break;
-    case 2: go(std::integral_constant<int, 2>{}); break;
     case 3: go(std::integral_constant<int, 3>{}); break;
     case 4: go(std::integral_constant<int, 4>{}); break;
     default: go(std::integral_constant<int, 5>{}); break;
