@@ -517,7 +517,6 @@ int fp8_direct_waves(int users, int kv_heads, int head_size, int64_t tokens) {
 int attend(DecodeArgs a, const float *k_scales, const float *v_scales, int head_size, int *arrived, hipStream_t st) {
   const int g = a.hq / a.hkv;
   int64_t tokens = (int64_t)a.w * a.bs;
-  a.bs_magic = block_magic(tokens, a.bs);
   if (a.window > 0) tokens = std::min<int64_t>(tokens, a.window);
   a.slot_floats = slot_floats_for(g, head_size);
   a.kv_format = -1;
