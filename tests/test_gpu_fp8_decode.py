@@ -402,3 +402,27 @@ def test_expanded_outputs_are_refused():
     into = torch.zeros(600, dtype=torch.bfloat16, device="cuda").as_strided((1, 2, 4, 64), (0, 128, 64, 1))
     with pytest.raises(ValueError, match="overlap itself"):
         torch.ops.tt.paged_fp8_attention_decode_out(q.cuda()[None], *on, table.cuda(), cur.cuda(), into)
+
+
+def test_sparse_decode_and_chunks_over_a_cache_beyond_four_gibibytes():
+    d, bs, hkv, grp = 128, 64, 8, 2
+    lengths = [700, 64]
+    cache, table, cur, q, g = _setup(2, hkv, grp, d, bs, lengths, 13)
+    nb, few = (1 << 32) // (hkv * d * bs) + 20, cache[0].shape[0]
+
+    def far(t):
+        big = torch.zeros(nb, *t.shape[1:], dtype=t.dtype, device="cuda") if t.dtype != torch.float8_e4m3fn else torch.empty(
+            nb, *t.shape[1:], dtype=torch.uint8, device="cuda").view(t.dtype)
+        big.view(torch.uint8)[nb - few :] = t.contiguous().view(torch.uint8).cuda()
+        return big
+
+    bounds = _bounds(cache)
+    moved = torch.where(table >= 0, table + (nb - few), table).cuda()
+    near, there = [t.cuda() for t in (*cache, bounds)], [far(t) for t in (*cache, bounds)]
+    tt, on = torch.ops.tt, q.cuda()[None]
+    want = tt.paged_fp8_sparse_attention_decode(on, *near, table.cuda(), cur.cuda(), 4)
+    got = tt.paged_fp8_sparse_attention_decode(on, *there, moved, cur.cuda(), 4)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    rows = torch.randn(2, hkv * grp, 40, d, generator=g).to(torch.bfloat16).cuda()
+    start = torch.tensor([20]).cuda()
+    assert torch.equal(tt.chunked_fp8_attention(rows, *there[:4], moved[:, :1], start), tt.chunked_fp8_attention(rows, *near[:4], table[:, :1].cuda(), start))
