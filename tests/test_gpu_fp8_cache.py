@@ -110,7 +110,8 @@ def test_the_step_in_one_launch(hq, hkv, d, bs, rotary, users):
                 assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip((*one, b1), (*two, b2)))
 
 
-@pytest.mark.parametrize("hkv, d, bs", SHAPES + [(2, 128, 256), (1, 256, 512), (2, 64, 4096)])
+@pytest.mark.parametrize("hkv, d, bs", SHAPES + [(2, 128, 256), (1, 256, 512), (2, 64, 4096), (5, 64, 16), (3, 128, 16), (2, 128, 32), (7, 64, 64),
+                                                    (1, 64, 48), (9, 64, 128), (2, 256, 64)])
 @pytest.mark.parametrize("users, blocks, short", [(1, 1, 1), (1, 2, 0), (3, 2, 5), (2, 3, -1)])
 @pytest.mark.parametrize("bounds", [False, True])
 def test_prompts(hkv, d, bs, users, blocks, short, bounds):
