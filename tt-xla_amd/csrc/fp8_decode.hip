@@ -538,8 +538,10 @@ int attend(DecodeArgs a, const float *k_scales, const float *v_scales, int head_
   // 50 000 tiles gain 1 %, shorter ones lose 3 - 15 %.
   const int larger_grid = waves_for_device(8.0);
   a.n_waves = waves_for_device(4.0);
-  a.many_from = 3 * (int64_t)larger_grid;
-  if (head_size == 64 && segments * ((tokens + 63) / 64 + 1) >= a.many_from) a.few_ranges = a.n_waves, a.n_waves = larger_grid;
+  // (few_ranges also keeps the merge in whole pieces where its slices do not fit the chip at once, with 128 segments and wide groups: 32 users of
+  // 2000 ... 6000 tokens, 64/4 heads of 128 36.4 / 33.1, of 256 62.1 / 55.9.)
+  a.few_ranges = a.n_waves, a.many_from = 0;
+  if (head_size == 64 && segments * ((tokens + 63) / 64 + 1) >= 3 * (int64_t)larger_grid) a.n_waves = larger_grid, a.many_from = 3 * (int64_t)larger_grid;
   a.seg_units = segment_units(1);
   if (!segment_units_forced()) a.seg_free_tiles = a.n_waves;
   if (!a.direct && segments > (int64_t)a.n_waves * kWave)
