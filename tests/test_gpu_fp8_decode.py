@@ -338,6 +338,20 @@ def test_sparse_more_segments_than_one_pass_takes():
     _check_sparse(out, cols, q, cache, bounds, table, cur, 3, d**-0.5)
 
 
+@pytest.mark.parametrize("d, width", [(64, 400), (128, 2500), (256, 1300)])
+def test_sparse_many_contexts_of_many_blocks_on_wide_tables(d, width):
+    """A workgroup scores several parts of a context; tables that go on behind the contexts."""
+    bs, hkv, grp, nb, users = 16, 8, 2, 60, 150
+    g = torch.Generator().manual_seed(d)
+    cache = _cache(nb, hkv, bs, d, g)
+    bounds = _bounds(cache)
+    table = torch.randint(0, nb, (users, width), generator=g).int()
+    cur = torch.randint(-1, 300 * bs, (users,), generator=g)
+    q = torch.randn(users, hkv * grp, d, generator=g).to(torch.bfloat16)
+    out, cols = _sparse(q, cache, bounds, table, cur, 7, scale=0.05)
+    _check_sparse(out, cols, q, cache, bounds, table, cur, 7, 0.05)
+
+
 @pytest.mark.parametrize("d, blocks", [(64, 8300), (128, 9001)])
 def test_sparse_tables_beyond_what_is_held(d, blocks):
     """More columns than scores and pages are kept on the chip for, short contexts among the long ones."""

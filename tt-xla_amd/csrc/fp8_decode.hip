@@ -44,8 +44,9 @@ struct ScoreArgs {
   const void *cur;
   int cur_i64;
   int users, hkv, g, bs, w, nb, kept;
-  float2 *scores;  // [users * hkv][w]: score in 32 bits, sum of its products' magnitudes
-  uint64_t *keys;  // [users * hkv][w]: exact scores, where too many are in question for LDS
+  int64_t row;     // elements of a row of the next two
+  float2 *scores;  // [users * hkv][row]: score in 32 bits, sum of its products' magnitudes
+  uint64_t *keys;  // [users * hkv][row]: exact scores, where too many are in question for LDS
   int32_t *table;  // [users * hkv][kept]
   int32_t *pos;    // [users * hkv]
   int32_t *columns;  // [users, hkv, kept], the caller's
@@ -87,8 +88,8 @@ __global__ __launch_bounds__(256) void block_scores_kernel(ScoreArgs a) {
   constexpr int KSTEPS = D / 32, TILES = score_tiles<D>();
   const int lane = threadIdx.x & 63, n = lane & 15, quad = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int seg = blockIdx.y, u = seg / a.hkv, h = seg - u * a.hkv;
-  const int c0 = ((int)blockIdx.x * 4 + wave) * 16 * TILES;
+  const int seg = blockIdx.x, u = seg / a.hkv, h = seg - u * a.hkv;
+  int c0 = ((int)blockIdx.y * 4 + wave) * 16 * TILES;
   // (the table row is as wide for every user: a page that the context does not reach is looked up, too, and goes no further)
   int page[TILES];
 #pragma unroll
@@ -104,54 +105,61 @@ __global__ __launch_bounds__(256) void block_scores_kernel(ScoreArgs a) {
   int64_t pos;
   const int nblk = blocks_of(a, u, pos);
   if (nblk <= a.kept || c0 >= nblk) return;  // (up to `kept` blocks: all are attended)
-  u32x4 low[TILES][KSTEPS], high[TILES][KSTEPS];
+#pragma unroll 1
+  for (;;) {
+    u32x4 low[TILES][KSTEPS], high[TILES][KSTEPS];
 #pragma unroll
-  for (int t = 0; t < TILES; ++t) {
-    const int64_t slab = (int64_t)((unsigned)page[t] < (unsigned)a.nb ? page[t] : 0) * a.hkv + h;
-    const uint16_t *b = a.bounds + slab * (2 * D) + 8 * quad;
+    for (int t = 0; t < TILES; ++t) {
+      const int64_t slab = (int64_t)((unsigned)page[t] < (unsigned)a.nb ? page[t] : 0) * a.hkv + h;
+      const uint16_t *b = a.bounds + slab * (2 * D) + 8 * quad;
 #pragma unroll
-    for (int s = 0; s < KSTEPS; ++s) low[t][s] = *reinterpret_cast<const u32x4 *>(b + 32 * s);
+      for (int s = 0; s < KSTEPS; ++s) low[t][s] = *reinterpret_cast<const u32x4 *>(b + 32 * s);
 #pragma unroll
-    for (int s = 0; s < KSTEPS; ++s) high[t][s] = *reinterpret_cast<const u32x4 *>(b + D + 32 * s);
-  }
-  floatx4 sum[TILES], size[TILES];
+      for (int s = 0; s < KSTEPS; ++s) high[t][s] = *reinterpret_cast<const u32x4 *>(b + D + 32 * s);
+    }
+    floatx4 sum[TILES], size[TILES];
 #pragma unroll
-  for (int t = 0; t < TILES; ++t) sum[t] = size[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < TILES; ++t) sum[t] = size[t] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int s = 0; s < KSTEPS; ++s) {
-    // the parts of the queries; a NaN stays one in both (it counts as positive and as negative)
-    u32x4 plus, minus, less;
+    for (int s = 0; s < KSTEPS; ++s) {
+      // the parts of the queries; a NaN stays one in both (it counts as positive and as negative)
+      u32x4 plus, minus, less;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t w = q[s][i];
-      const uint32_t lo_nan = (w & 0x7fffu) > 0x7f80u ? 0xffffu : 0u, hi_nan = (w & 0x7fff0000u) > 0x7f800000u ? 0xffff0000u : 0u;
-      const uint32_t negative = ((w >> 15) & 0x00010001u) * 0xffffu;
-      plus[i] = w & (~negative | lo_nan | hi_nan), minus[i] = w & (negative | lo_nan | hi_nan), less[i] = minus[i] & 0x7fff7fffu;
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t w = q[s][i];
+        const uint32_t lo_nan = (w & 0x7fffu) > 0x7f80u ? 0xffffu : 0u, hi_nan = (w & 0x7fff0000u) > 0x7f800000u ? 0xffff0000u : 0u;
+        const uint32_t negative = ((w >> 15) & 0x00010001u) * 0xffffu;
+        plus[i] = w & (~negative | lo_nan | hi_nan), minus[i] = w & (negative | lo_nan | hi_nan), less[i] = minus[i] & 0x7fff7fffu;
+      }
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) {
+        u32x4 low_size, high_size;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) low_size[i] = low[t][s][i] & 0x7fff7fffu, high_size[i] = high[t][s][i] & 0x7fff7fffu;
+        sum[t] = mma16<false>(high[t][s], plus, sum[t]);
+        size[t] = mma16<false>(high_size, plus, size[t]);
+        sum[t] = mma16<false>(low[t][s], minus, sum[t]);
+        size[t] = mma16<false>(low_size, less, size[t]);
+      }
     }
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
-      u32x4 low_size, high_size;
+      // lane (head n, quad) holds blocks 4 quad + r: the largest over the heads; a sum that is no number is as good as infinite
+      float best[4], most[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) low_size[i] = low[t][s][i] & 0x7fff7fffu, high_size[i] = high[t][s][i] & 0x7fff7fffu;
-      sum[t] = mma16<false>(high[t][s], plus, sum[t]);
-      size[t] = mma16<false>(high_size, plus, size[t]);
-      sum[t] = mma16<false>(low[t][s], minus, sum[t]);
-      size[t] = mma16<false>(low_size, less, size[t]);
+      for (int r = 0; r < 4; ++r) {
+        best[r] = row16_max(n < a.g ? (sum[t][r] == sum[t][r] ? sum[t][r] : INFINITY) : -INFINITY);
+        most[r] = row16_max(n < a.g ? (size[t][r] == size[t][r] ? size[t][r] : INFINITY) : 0.f);
+      }
+      const int c = c0 + 16 * t + 4 * quad + n;
+      if (n < 4 && c < nblk)
+        a.scores[seg * a.row + c] = make_float2(n == 0 ? best[0] : n == 1 ? best[1] : n == 2 ? best[2] : best[3],
+                                                       n == 0 ? most[0] : n == 1 ? most[1] : n == 2 ? most[2] : most[3]);
     }
-  }
+    c0 += (int)gridDim.y * 64 * TILES;
+    if (c0 >= nblk) return;
 #pragma unroll
-  for (int t = 0; t < TILES; ++t) {
-    // lane (head n, quad) holds blocks 4 quad + r: the largest over the heads; a sum that is no number is as good as infinite
-    float best[4], most[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      best[r] = row16_max(n < a.g ? (sum[t][r] == sum[t][r] ? sum[t][r] : INFINITY) : -INFINITY);
-      most[r] = row16_max(n < a.g ? (size[t][r] == size[t][r] ? size[t][r] : INFINITY) : 0.f);
-    }
-    const int c = c0 + 16 * t + 4 * quad + n;
-    if (n < 4 && c < nblk)
-      a.scores[(int64_t)seg * a.w + c] = make_float2(n == 0 ? best[0] : n == 1 ? best[1] : n == 2 ? best[2] : best[3],
-                                                     n == 0 ? most[0] : n == 1 ? most[1] : n == 2 ? most[2] : most[3]);
+    for (int t = 0; t < TILES; ++t) page[t] = a.pt[u * a.pt_rs + min(c0 + 16 * t + n, a.w - 1)];
   }
 }
 
@@ -178,28 +186,42 @@ struct Choice {
   int ties;
 };
 constexpr int kThreads = 512, kWaves = kThreads / 64;
+constexpr int kHeld = 4, kLdsColumns = 8192;
 struct ChoiceLds {
   uint32_t bins[kBins];
   uint64_t cand[kRanked], high[kWaves], low[kWaves];
-  int num[2][kWaves], column[kRanked], bin, over, count, next;
+  int num[kHeld][kWaves], column[kRanked], bin, over, count, next;
   float size[kWaves];
   uint8_t kept[kRanked];
 };
-// This thread's places in two running counts over the workgroup, and the counts of all.  (Between two calls lies a barrier.)
+// This thread's places in the first `used` of N running counts over the workgroup, and the counts of all.  (Between two calls lies a barrier.)
+template <int N>
 struct Counts {
-  int before[2], all[2];
+  int before[N], all[N];
 };
-__device__ __forceinline__ Counts running_counts(ChoiceLds &s, int x, int y) {
+template <int N>
+__device__ __forceinline__ Counts<N> running_counts(ChoiceLds &s, const int (&x)[N], int used = N) {
+  static_assert(N <= kHeld, "");
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int ix = wave_prefix_sum(x), iy = wave_prefix_sum(y);
-  if (lane == 63) s.num[0][wave] = ix, s.num[1][wave] = iy;
-  __syncthreads();
-  Counts c = {{ix - x, iy - y}, {0, 0}};
-  for (int w = 0; w < kWaves; ++w) {
-    const int nx = s.num[0][w], ny = s.num[1][w];
-    if (w < wave) c.before[0] += nx, c.before[1] += ny;
-    c.all[0] += nx, c.all[1] += ny;
+  Counts<N> c;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    c.before[i] = c.all[i] = 0;
+    if (i < used) {
+      const int upto = wave_prefix_sum(x[i]);
+      if (lane == 63) s.num[i][wave] = upto;
+      c.before[i] = upto - x[i];
+    }
   }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i < used)
+      for (int w = 0; w < kWaves; ++w) {
+        const int n = s.num[i][w];
+        if (w < wave) c.before[i] += n;
+        c.all[i] += n;
+      }
   return c;
 }
 
@@ -241,7 +263,7 @@ __device__ __forceinline__ Choice last_kept(ChoiceLds &s, int need, Key hi, Key 
     int mine[OWN], sum = 0;
 #pragma unroll
     for (int j = 0; j < OWN; ++j) mine[j] = (int)s.bins[base + j], sum += mine[j];
-    int above = running_counts(s, sum, 0).before[0];
+    int above = running_counts<1>(s, {sum}).before[0];
     if (above < need && above + sum >= need) {  // one thread
       int b = OWN - 1;
       while (above + mine[b] < need) above += mine[b], --b;
@@ -303,31 +325,183 @@ __device__ __forceinline__ uint64_t exact_key(const ScoreArgs &a, int u, int h, 
   return score_key(s);
 }
 
-// One workgroup per (user, KV head); what bounds it is its own chain (three round trips to memory, a dozen barriers) and, as every launch begins with a cold
-// instruction cache, its code.  HELD: tables of up to kHeld columns per thread, whose scores and pages every thread has in registers, asked for before it is
-// known how many there are; the scores of wider ones lie in LDS, up to kLdsColumns, or stay where they are.  128 (user, head) pairs of 64 ... 512 blocks 6.5 us,
-// 32 of 1024 ... 2048 9.2 (scores and pages in LDS throughout 7.1 and 12.4; unrolled over sixteen columns and with 1024 threads 21); a pass over 8192 columns,
-// in LDS / where they lie, 46.1 / 51.8.
-constexpr int kHeld = 4, kLdsColumns = 8192;
-template <int D, bool HELD>
-__global__ __launch_bounds__(kThreads) void choose_blocks_kernel(ScoreArgs a) {
-  __shared__ ChoiceLds s;
-  extern __shared__ float s_score[];
+// The choice among the blocks but the first and the last of a context of nblk > kept, each handed to `emit`.  HELD: contexts of up to kHeld blocks
+// per thread, whose scores and pages every thread has in registers (column tid + kThreads j; x0, id0: those of the first); the scores of longer ones lie in LDS,
+// where the table has up to kLdsColumns, or stay where they are, and each thread has neighbouring columns.
+template <int D, bool HELD, typename Emit>
+__device__ __forceinline__ void choose_among(const ScoreArgs &a, ChoiceLds &s, float *s_score, int seg, int u, int h, int nblk, float2 x0, int id0,
+                                             const Emit &emit) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int seg = blockIdx.x, u = seg / a.hkv, h = seg - u * a.hkv;
   const int32_t *pt = a.pt + u * a.pt_rs;
-  const float2 *scores = a.scores + (int64_t)seg * a.w;
-  // Each thread has neighbouring columns, so that the chosen ones come out in order behind running counts.
-  const int held_per = (a.w + kThreads - 1) / kThreads;
+  const float2 *scores = a.scores + seg * a.row;
+  const int held = HELD ? (nblk + kThreads - 1) / kThreads : 0;  // of the registers
   float2 x[HELD ? kHeld : 1];
   int id[HELD ? kHeld : 1];
   if constexpr (HELD) {
+    x[0] = x0, id[0] = id0;
 #pragma unroll
-    for (int j = 0; j < kHeld; ++j) {
-      const int c = min(tid * held_per + min(j, held_per - 1), a.w - 1);
-      x[j] = scores[c], id[j] = pt[c];  // (scores that nobody has written are not used)
+    for (int j = 1; j < kHeld; ++j)
+      if (j < held) x[j] = scores[min(tid + kThreads * j, nblk - 1)], id[j] = pt[min(tid + kThreads * j, nblk - 1)];
+  }
+  // The thread's columns, of the blocks but the first and the last: visit(f) calls f(column, score, place in `id`).
+  const int per = (nblk + kThreads - 1) / kThreads, from = max(min(tid * per, nblk), 1), to = min(tid * per + per, nblk - 1);  // (not HELD)
+  const bool in_lds = !HELD && a.w <= kLdsColumns;
+  const auto visit = [&](const auto &f) {
+    if constexpr (HELD) {
+#pragma unroll
+      for (int j = 0; j < kHeld; ++j) {
+        const int c = tid + kThreads * j;
+        if (j < held && c > 0 && c < nblk - 1) f(c, x[j].x, j);
+      }
+    } else {
+#pragma unroll 1
+      for (int c = from; c < to; ++c) f(c, in_lds ? s_score[c] : scores[c].x, c);
+    }
+  };
+  const auto page = [&](int j) {
+    if constexpr (HELD) return id[j];
+    return pt[j];
+  };
+  uint32_t hi = 0, lo = ~0u;
+  float size = 0.f;  // largest sum of magnitudes
+  if constexpr (HELD) {
+    visit([&](int, float v, int j) { size = fmaxf(size, x[j].y), hi = max(hi, float_key(v)), lo = min(lo, float_key(v)); });
+  } else {
+#pragma unroll 4
+    for (int c = 1 + tid; c < nblk - 1; c += kThreads) {
+      const float2 v = scores[c];
+      if (in_lds) s_score[c] = v.x;
+      size = fmaxf(size, v.y), hi = max(hi, float_key(v.x)), lo = min(lo, float_key(v.x));
     }
   }
+  extent(s, hi, lo, size);
+  const int need = a.kept - 2;
+  const Choice approx = last_kept<uint32_t>(s, need, hi, lo, [&](const auto &f) { visit([&](int, float v, int) { f(float_key(v)); }); });
+  // T, and how far a score may be from the exact one: at most 512 additions, each off by at most a unit in the last place of what the magnitudes
+  // add up to (2^-23), twice that for what the matrix pipe's own order and rounding may be; and what falls below the smallest normal number.
+  const uint32_t tb = (uint32_t)approx.threshold;
+  const float t = __builtin_bit_cast(float, (tb >> 31) ? tb & 0x7fffffffu : ~tb);
+  const float e = size * 0x1p-13f + 0x1p-100f;
+  const bool exact_all = !(size < INFINITY) || !(fabsf(t) < INFINITY);  // infinities among the scores: no bound says anything
+  const float sure = exact_all ? INFINITY : t + 2.f * e, out = exact_all ? -INFINITY : t - 2.f * e;
+  const auto kept_surely = [&](float v) { return !exact_all && need > 0 && v > sure; };
+  const auto in_question = [&](float v) { return exact_all || (need > 0 && v >= out && !(v > sure)); };
+  // Two running counts over the columns in order, of those that p and q hold for: the counts in front of the thread's columns (HELD: of each), and of all.
+  struct Places {
+    int p[HELD ? kHeld : 1], q[HELD ? kHeld : 1], all_p, all_q;
+  };
+  const auto count = [&](const auto &p, const auto &q) {
+    Places o;
+    if constexpr (HELD) {
+      // (for each row of kThreads columns both counts in a word)
+      int n[kHeld] = {};
+      visit([&](int c, float v, int j) { n[j] = (int)p(c, v) | (int)q(c, v) << 16; });
+      const Counts<kHeld> r = running_counts<kHeld>(s, n, held);
+      o.all_p = o.all_q = 0;
+#pragma unroll
+      for (int j = 0; j < kHeld; ++j) {
+        o.p[j] = o.all_p + (r.before[j] & 0xffff), o.q[j] = o.all_q + (r.before[j] >> 16);
+        o.all_p += r.all[j] & 0xffff, o.all_q += r.all[j] >> 16;
+      }
+    } else {
+      int n[2] = {0, 0};
+      visit([&](int c, float v, int) { n[0] += p(c, v), n[1] += q(c, v); });
+      const Counts<2> r = running_counts<2>(s, n);
+      o.p[0] = r.before[0], o.q[0] = r.before[1], o.all_p = r.all[0], o.all_q = r.all[1];
+    }
+    return o;
+  };
+  // f(column, score, place in `id`, the two counts in front of it)
+  const auto walk = [&](const Places &o, const auto &p, const auto &q, const auto &f) {
+    if constexpr (HELD) {
+      visit([&](int c, float v, int j) { f(c, v, j, o.p[j], o.q[j]); });
+    } else {
+      int np = o.p[0], nq = o.q[0];
+      visit([&](int c, float v, int j) {
+        f(c, v, j, np, nq);
+        np += p(c, v), nq += q(c, v);
+      });
+    }
+  };
+  const auto is_sure = [&](int, float v) { return kept_surely(v); };
+  const auto is_open = [&](int, float v) { return in_question(v); };
+  const Places n = count(is_sure, is_open);
+  const int open = n.all_q, need_open = need - n.all_p;
+  constexpr int GROUPS = 256 / D;  // of lanes with a score of their own, in a wavefront
+  const int group = wave * GROUPS + lane / (D / 4);
+  uint64_t *const keys = a.keys + seg * a.row;
+  if (open <= kRanked) {
+    // few in question: their exact scores and ranks in LDS
+    walk(n, is_sure, is_open, [&](int, float v, int j, int, int at) {
+      if (in_question(v)) s.column[at] = page(j), s.cand[at] = 0;
+    });
+    __syncthreads();
+#pragma unroll 1
+    for (int i = group; i - group < open * a.g; i += kWaves * GROUPS) {
+      const int y = min(i, open * a.g - 1), o = y / a.g;
+      const uint64_t k = exact_key<D>(a, u, h, y - o * a.g, s.column[o]);
+      if (lane % (D / 4) == 0 && i < open * a.g) atomicMax(reinterpret_cast<unsigned long long *>(&s.cand[o]), (unsigned long long)k);
+    }
+    __syncthreads();
+    if (tid < open) {
+      const uint64_t k = s.cand[tid];
+      int better = 0;  // (columns are in order: of equals the first ones)
+#pragma unroll 1
+      for (int i = 0; i < open; ++i) better += s.cand[i] > k || (s.cand[i] == k && i < tid);
+      s.kept[tid] = better < need_open;
+    }
+    __syncthreads();
+    walk(n, is_sure, is_open, [&](int c, float v, int j, int at, int open_at) {
+      if (!kept_surely(v) && !(in_question(v) && s.kept[open_at])) return;
+      ++at;  // (column 0 is in front)
+#pragma unroll 1
+      for (int i = 0; i < open_at; ++i) at += s.kept[i];
+      emit(at, c, page(j));
+    });
+  } else {
+    // many (scores alike, infinities): exact scores of all in memory, and the choice among those in question by them
+#pragma unroll 1
+    for (int i = group; i - group < nblk; i += kWaves * GROUPS) {
+      const int c = min(i, nblk - 1);
+      uint64_t k = 0;
+#pragma unroll 1
+      for (int g = 0; g < a.g; ++g) k = max(k, exact_key<D>(a, u, h, g, pt[c]));
+      if (lane % (D / 4) == 0 && i < nblk) keys[i] = k;
+    }
+    __syncthreads();
+    const auto those = [&](const auto &f) {
+      visit([&](int c, float v, int) {
+        if (in_question(v)) f(keys[c]);
+      });
+    };
+    uint64_t high = 0, low = ~0ull;
+    those([&](uint64_t k) { high = max(high, k), low = min(low, k); });
+    extent(s, high, low, size);
+    const Choice exact = last_kept<uint64_t>(s, need_open, high, low, those);
+    // what is kept for sure or by its exact score; of the blocks tied for the last places the first ones
+    const auto is_kept = [&](int c, float v) { return kept_surely(v) || (in_question(v) && keys[c] > exact.threshold); };
+    const auto is_tied = [&](int c, float v) { return in_question(v) && keys[c] == exact.threshold; };
+    __syncthreads();
+    walk(count(is_kept, is_tied), is_kept, is_tied, [&](int c, float v, int j, int at, int tied_at) {
+      if (is_kept(c, v) || (is_tied(c, v) && tied_at < exact.ties)) emit(1 + at + min(tied_at, exact.ties), c, page(j));
+    });
+  }
+}
+
+// One workgroup per (user, KV head); what bounds it is its own chain (three round trips to memory, a dozen barriers) and, as every launch begins with a cold
+// instruction cache, its code.  128 (user, head) pairs of 64 ... 512 blocks 6.5 us, 32 of 1024 ... 2048 9.2 (scores and pages in LDS throughout 7.1 and 12.4; unrolled
+// over sixteen columns and with 1024 threads 21); a pass over 8192 columns, in LDS / where they lie, 46.1 / 51.8.  Scores made in the same workgroup instead of a
+// launch of their own: 35.2 / 32.5 the first pass, 54.9 / 30.4 the second.
+template <int D, bool LONG>
+__global__ __launch_bounds__(kThreads) void choose_blocks_kernel(ScoreArgs a) {
+  __shared__ ChoiceLds s;
+  extern __shared__ float s_score[];
+  const int tid = threadIdx.x;
+  const int seg = blockIdx.x, u = seg / a.hkv, h = seg - u * a.hkv;
+  const int32_t *pt = a.pt + u * a.pt_rs;
+  // (asked for before it is known how many there are; scores that nobody has written are not used)
+  const float2 x0 = a.scores[seg * a.row + min(tid, a.w - 1)];
+  const int id0 = pt[min(tid, a.w - 1)];
   int64_t pos = load_index(a.cur, a.cur_i64, u);
   const int nblk = blocks_of(a, u, pos);
   int32_t *table = a.table + (int64_t)seg * a.kept, *columns = a.columns + (int64_t)seg * a.kept;
@@ -348,151 +522,32 @@ __global__ __launch_bounds__(kThreads) void choose_blocks_kernel(ScoreArgs a) {
     return;
   }
   if (tid == 0) emit(0, 0, pt[0]), emit(a.kept - 1, nblk - 1, pt[nblk - 1]);
-  const int per = HELD ? held_per : (nblk + kThreads - 1) / kThreads;
-  const int first = tid * per, from = max(min(first, nblk), 1), to = min(first + per, nblk - 1);  // of the blocks but the first and the last
-  const bool in_lds = !HELD && a.w <= kLdsColumns;
-  const auto score = [&](int c) { return in_lds ? s_score[c] : scores[c].x; };
-  // f(column, score, place in `id`) for the thread's own, in order
-  const auto own = [&](const auto &f) {
-    if constexpr (HELD) {
-#pragma unroll
-      for (int j = 0; j < kHeld; ++j)
-        if (first + j >= from && first + j < to) f(first + j, x[j].x, j);
-    } else {
-#pragma unroll 1
-      for (int c = from; c < to; ++c) f(c, score(c), c);
-    }
-  };
-  // f(column, score) for the columns between the workgroup's threads in any order
-  const auto any = [&](const auto &f) {
-    if constexpr (HELD) {
-      own([&](int c, float v, int) { f(c, v); });
-    } else {
-#pragma unroll 1
-      for (int c = 1 + tid; c < nblk - 1; c += kThreads) f(c, score(c));
-    }
-  };
-  const auto page = [&](int j) {
-    if constexpr (HELD) return id[j];
-    return pt[j];
-  };
-  uint32_t hi = 0, lo = ~0u;
-  float size = 0.f;  // largest sum of magnitudes
-  if constexpr (HELD) {
-#pragma unroll
-    for (int j = 0; j < kHeld; ++j)
-      if (first + j >= from && first + j < to) size = fmaxf(size, x[j].y), hi = max(hi, float_key(x[j].x)), lo = min(lo, float_key(x[j].x));
-  } else {
-#pragma unroll 4
-    for (int c = 1 + tid; c < nblk - 1; c += kThreads) {
-      const float2 v = scores[c];
-      if (in_lds) s_score[c] = v.x;
-      size = fmaxf(size, v.y), hi = max(hi, float_key(v.x)), lo = min(lo, float_key(v.x));
+  if constexpr (LONG) {
+    if (nblk > kHeld * kThreads) {
+      choose_among<D, false>(a, s, s_score, seg, u, h, nblk, x0, id0, emit);
+      return;
     }
   }
-  extent(s, hi, lo, size);
-  const int need = a.kept - 2;
-  const Choice approx = last_kept<uint32_t>(s, need, hi, lo, [&](const auto &f) { any([&](int, float v) { f(float_key(v)); }); });
-  // T, and how far a score may be from the exact one: at most 512 additions, each off by at most a unit in the last place of what the magnitudes
-  // add up to (2^-23), twice that for what the matrix pipe's own order and rounding may be; and what falls below the smallest normal number.
-  const uint32_t tb = (uint32_t)approx.threshold;
-  const float t = __builtin_bit_cast(float, (tb >> 31) ? tb & 0x7fffffffu : ~tb);
-  const float e = size * 0x1p-13f + 0x1p-100f;
-  const bool exact_all = !(size < INFINITY) || !(fabsf(t) < INFINITY);  // infinities among the scores: no bound says anything
-  const float sure = exact_all ? INFINITY : t + 2.f * e, out = exact_all ? -INFINITY : t - 2.f * e;
-  const auto kept_surely = [&](float v) { return !exact_all && need > 0 && v > sure; };
-  const auto in_question = [&](float v) { return exact_all || (need > 0 && v >= out && !(v > sure)); };
-  int sure_mine = 0, open_mine = 0;
-  own([&](int, float v, int) { sure_mine += kept_surely(v), open_mine += in_question(v); });
-  const Counts n = running_counts(s, sure_mine, open_mine);
-  const int open = n.all[1], need_open = need - n.all[0];
-  constexpr int GROUPS = 256 / D;  // of lanes with a score of their own, in a wavefront
-  const int group = wave * GROUPS + lane / (D / 4);
-  uint64_t *const keys = a.keys + (int64_t)seg * a.w;
-  int place = 1 + n.before[0];  // of the thread's first kept column (column 0 is in front)
-  if (open <= kRanked) {
-    // few in question: their exact scores and ranks in LDS
-    int at = n.before[1];
-    own([&](int c, float v, int j) {
-      if (in_question(v)) s.column[at] = page(j), s.cand[at] = 0, ++at;
-    });
-    __syncthreads();
-#pragma unroll 1
-    for (int i = group; i - group < open * a.g; i += kWaves * GROUPS) {
-      const int y = min(i, open * a.g - 1), o = y / a.g;
-      const uint64_t k = exact_key<D>(a, u, h, y - o * a.g, s.column[o]);
-      if (lane % (D / 4) == 0 && i < open * a.g) atomicMax(reinterpret_cast<unsigned long long *>(&s.cand[o]), (unsigned long long)k);
-    }
-    __syncthreads();
-    if (tid < open) {
-      const uint64_t k = s.cand[tid];
-      int better = 0;  // (columns are in order: of equals the first ones)
-#pragma unroll 1
-      for (int i = 0; i < open; ++i) better += s.cand[i] > k || (s.cand[i] == k && i < tid);
-      s.kept[tid] = better < need_open;
-    }
-    __syncthreads();
-    if (sure_mine + open_mine == 0) return;
-#pragma unroll 1
-    for (int i = 0; i < n.before[1]; ++i) place += s.kept[i];
-    at = n.before[1];
-    own([&](int c, float v, int j) {
-      bool is = kept_surely(v);
-      if (in_question(v)) is = s.kept[at++];
-      if (is) emit(place++, c, page(j));
-    });
-  } else {
-    // many (scores alike, infinities): exact scores of all in memory, and the choice among those in question by them
-#pragma unroll 1
-    for (int i = group; i - group < nblk; i += kWaves * GROUPS) {
-      const int c = min(i, nblk - 1);
-      uint64_t k = 0;
-#pragma unroll 1
-      for (int g = 0; g < a.g; ++g) k = max(k, exact_key<D>(a, u, h, g, pt[c]));
-      if (lane % (D / 4) == 0 && i < nblk) keys[i] = k;
-    }
-    __syncthreads();
-    const auto visit = [&](const auto &f) {
-      any([&](int c, float v) {
-        if (in_question(v)) f(keys[c]);
-      });
-    };
-    uint64_t high = 0, low = ~0ull;
-    visit([&](uint64_t k) { high = max(high, k), low = min(low, k); });
-    extent(s, high, low, size);
-    const Choice exact = last_kept<uint64_t>(s, need_open, high, low, visit);
-    // of the blocks tied for the last places the first ones win
-    int above = 0, tied = 0;
-    own([&](int c, float v, int) {
-      if (in_question(v)) above += keys[c] > exact.threshold, tied += keys[c] == exact.threshold;
-    });
-    __syncthreads();
-    const Counts m = running_counts(s, above, tied);
-    int t_at = m.before[1];
-    place += m.before[0] + min(t_at, exact.ties);
-    own([&](int c, float v, int j) {
-      bool is = kept_surely(v);
-      if (in_question(v)) {
-        is = keys[c] > exact.threshold || (keys[c] == exact.threshold && t_at < exact.ties);
-        t_at += keys[c] == exact.threshold;
-      }
-      if (is) emit(place++, c, page(j));
-    });
-  }
+  choose_among<D, true>(a, s, s_score, seg, u, h, nblk, x0, id0, emit);
 }
 
+constexpr int kScoreWorkgroups = 1024;
 template <int D>
 int launch_choice(const ScoreArgs &a, hipStream_t st) {
   const int segments = a.users * a.hkv;
   if (a.w > a.kept) {
+    // Tables are wide where contexts may grow long: not more workgroups than are at work at once about, each of which goes on until its context ends, and
+    // a context's workgroups as far apart as there are contexts, so that those that have work are on all XCDs.  (Side by side, and as many as the table is
+    // wide, 16 users of 4096 ... 32768 tokens took 31.9 us where the table ended with them and 68 in a table of 16384 columns; so 31.6 and 32.1.)
     constexpr int kBlocks = 4 * 16 * score_tiles<D>();
-    block_scores_kernel<D><<<dim3((a.w + kBlocks - 1) / kBlocks, segments), dim3(256), 0, st>>>(a);
+    const int most = std::max(kScoreWorkgroups / segments, 1);
+    block_scores_kernel<D><<<dim3(segments, std::min((a.w + kBlocks - 1) / kBlocks, most)), dim3(256), 0, st>>>(a);
     if (const int rc = check_launch("fp8 sparse decode (scores)")) return rc;
   }
   if (a.w <= kHeld * kThreads)
-    choose_blocks_kernel<D, true><<<dim3(segments), dim3(kThreads), 0, st>>>(a);
+    choose_blocks_kernel<D, false><<<dim3(segments), dim3(kThreads), 0, st>>>(a);
   else
-    choose_blocks_kernel<D, false><<<dim3(segments), dim3(kThreads), a.w <= kLdsColumns ? 4 * (size_t)a.w : 0, st>>>(a);
+    choose_blocks_kernel<D, true><<<dim3(segments), dim3(kThreads), a.w <= kLdsColumns ? 4 * (size_t)a.w : 0, st>>>(a);
   return check_launch("fp8 sparse decode (choice)");
 }
 
@@ -573,7 +628,7 @@ int check_decode(const void *out, int64_t out_us, int64_t out_hs, const void *q,
 
 // A sparse call's scratch behind the attention's: the scores' keys, the tables, the positions.
 struct SparseLayout {
-  size_t slots, keys, table, total;
+  size_t slots, row, keys, table, total;
 };
 SparseLayout sparse_layout(int users, int q_heads, int kv_heads, int head_size, int table_width, int kept) {
   const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
@@ -582,7 +637,9 @@ SparseLayout sparse_layout(int users, int q_heads, int kv_heads, int head_size, 
   const size_t slots = (size_t)std::max(device_cus(), 256) + segments;
   SparseLayout l;
   l.slots = up(slots * slot_floats_for(q_heads / kv_heads, head_size) * sizeof(float));
-  l.keys = up(segments * (size_t)table_width * 8);  // scores, and as much for exact ones
+  l.row = ((size_t)table_width + 15) / 16 | 1;  // (an odd number of lines: rows that begin on the same channels of the memory wait for each other)
+  l.row *= 16;
+  l.keys = up(segments * l.row * 8);  // scores, and as much for exact ones
   l.table = up(segments * (size_t)kept * 4);
   l.total = l.slots + 2 * l.keys + l.table + 2 * up(segments * 4);
   return l;
@@ -654,6 +711,7 @@ extern "C" int ttpa_paged_fp8_sparse_decode(void *out, int64_t out_head_stride, 
     s.pt = page_table + u0 * page_table_row_stride, s.pt_rs = page_table_row_stride;
     s.cur = static_cast<const uint8_t *>(cur_pos) + (int64_t)u0 * (cur_pos_is_i64 ? 8 : 4), s.cur_i64 = cur_pos_is_i64;
     s.users = n, s.hkv = kv_heads, s.g = g, s.bs = block_size, s.w = table_width, s.nb = num_blocks, s.kept = kept_blocks;
+    s.row = (int64_t)l.row;
     s.scores = reinterpret_cast<float2 *>(ws + l.slots);
     s.keys = reinterpret_cast<uint64_t *>(ws + l.slots + l.keys);
     s.table = reinterpret_cast<int32_t *>(ws + l.slots + 2 * l.keys);
