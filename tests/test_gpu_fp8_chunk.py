@@ -42,7 +42,10 @@ def _check(out, q, cache, table, start, scale):
 @pytest.mark.parametrize("users, hkv, grp, s, start", [(1, 2, 4, 32, 0), (2, 1, 1, 64, 96), (1, 8, 4, 96, 1000), (3, 2, 2, 33, 64), (1, 1, 8, 1, 130),
                                                        (1, 2, 5, 160, 64)])
 @pytest.mark.parametrize("known", [False, True])
-def test_chunks(d, bs, users, hkv, grp, s, start, known):
+@pytest.mark.parametrize("form", ["few", "copies", None])
+def test_chunks(d, bs, users, hkv, grp, s, start, known, form, monkeypatch):
+    if form:
+        monkeypatch.setenv("TTPA_CHUNK_FORM", form)
     g = torch.Generator().manual_seed(d + bs + s)
     width = -(-(start + s) // bs) + 2
     nb = users * width + 3
@@ -108,8 +111,9 @@ def test_refusals():
     assert op(q[:, :, :0], k, v, ks, vs, table, start).shape == (1, 4, 0, 64)
 
 
-def test_users_in_several_passes():
+def test_users_in_several_passes(monkeypatch):
     """A table so wide that the copies of three users' blocks do not fit the scratch at once: two passes, of two users and of one."""
+    monkeypatch.setenv("TTPA_CHUNK_FORM", "copies")
     d, bs, hkv, grp, s, start = 128, 64, 8, 2, 70, 300
     g = torch.Generator().manual_seed(9)
     cache = _cache(20, hkv, bs, d, g)
@@ -122,8 +126,10 @@ def test_users_in_several_passes():
     _check(out.cpu(), q, cache, table, start, d**-0.5)
 
 
-def test_captured_prompts_and_chunks():
+@pytest.mark.parametrize("form", ["few", "copies"])
+def test_captured_prompts_and_chunks(form, monkeypatch):
     """A prompt's write and a chunk over it in one graph, replayed at other starts and with other keys; every replay against the eager calls."""
+    monkeypatch.setenv("TTPA_CHUNK_FORM", form)
     d, bs, hkv, grp, s = 128, 32, 2, 4, 64
     g = torch.Generator().manual_seed(10)
     state = [t.cuda() for t in _cache(40, hkv, bs, d, g)]
@@ -166,3 +172,37 @@ def test_expanded_outputs_are_refused():
     table, start = torch.zeros(2, 3, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
     with pytest.raises(ValueError, match="expanded"):
         torch.ops.tt.chunked_fp8_attention_out(q, *cache, table, start, q[:1].clone().expand(2, -1, -1, -1))
+
+
+@pytest.mark.parametrize("d, hq, hkv", [(64, 8, 1), (128, 16, 2), (256, 4, 4)])
+@pytest.mark.parametrize("form", ["few", "copies"])
+def test_chunks_that_begin_before_the_prompt_or_end_behind_the_table(d, hq, hkv, form, monkeypatch):
+    """Rows in front of the prompt attend nothing; rows behind the table attend what it holds."""
+    monkeypatch.setenv("TTPA_CHUNK_FORM", form)
+    g = torch.Generator().manual_seed(d)
+    bs, s = 32, 40
+    cache = _cache(6, hkv, bs, d, g)
+    table = torch.tensor([[2, 5, 1, 4]], dtype=torch.int32)
+    q = torch.randn(1, hq, s, d, generator=g).to(torch.bfloat16)
+    on = [t.cuda() for t in cache]
+    for start in (-7, 100, 127, 400):
+        out = torch.ops.tt.chunked_fp8_attention(q.cuda(), *on, table.cuda(), torch.tensor([start]).cuda()).cpu()
+        if start < 0:
+            assert torch.isnan(out[:, :, : -start]).all()
+            _check(out[:, :, -start:], q[:, :, -start:], cache, table, 0, d**-0.5)
+        else:
+            _check(out, q, cache, table, start, d**-0.5)
+
+
+def test_few_rows_over_many_parts_and_many_blocks_of_rows(monkeypatch):
+    monkeypatch.setenv("TTPA_CHUNK_FORM", "few")
+    g = torch.Generator().manual_seed(11)
+    for d, hq, hkv, users, s, start in ((64, 2, 1, 1, 3, 9000), (128, 8, 4, 2, 100, 4000), (256, 6, 2, 1, 50, 5000), (128, 40, 8, 3, 7, 300)):
+        bs, width = 64, -(-(start + s) // 64) + 5
+        cache = _cache(width + 4, hkv, bs, d, g)
+        table = torch.stack([torch.randperm(width + 4, generator=g)[:width] for _ in range(users)]).int()
+        q = torch.randn(users, s, hq, d, generator=g).to(torch.bfloat16).transpose(1, 2)
+        on = [t.cuda() for t in cache]
+        for known in (0, start + s):
+            out = torch.ops.tt.chunked_fp8_attention(q.cuda(), *on, table.cuda(), torch.tensor([start]).cuda(), most_keys=known)
+            _check(out.cpu(), q, cache, table, start, d**-0.5)

@@ -1,5 +1,5 @@
-// Attention of a prompt's chunk over the 8-bit cache: the blocks that the pass reads become bfloat16 copies in the caller's scratch
-// (exactly: an element times its block's power of two is a bfloat16 value), and the bfloat16 prefill kernels run over the copies.
+// Attention of a prompt's chunk over the 8-bit cache: the blocks that the pass reads become bfloat16 copies in the caller's scratch, unless the chunk has few rows
+// (fp8_chunk_few.hip); exactly, as an element times its block's power of two is a bfloat16 value.  The bfloat16 prefill kernels run over the copies.
 //
 // A chunk is bound by its matrix products, 4 D q_heads operations per (row, key) pair, and every workgroup of 128 rows reads every key, so keys
 // are expanded once here and not once per workgroup; the copies cost 1 byte read and 2 written per element, at the rate of a large
@@ -13,13 +13,42 @@
 #include "fp8.h"
 
 #include <algorithm>
+#include <cstdlib>
+#include <cstring>
 
 namespace ttpa {
 namespace fp8 {
 int check_cache(const void *k_cache, const void *v_cache, const float *k_scales, const float *v_scales, const int32_t *page_table, int kv_heads,
                 int head_size, int block_size, int table_width, int num_blocks);
 
+// A chunk of few rows (fp8_chunk_few.hip).
+int64_t chunk_few_bytes(int batch, int q_heads, int kv_heads, int q_len, int head_size, int64_t keys);
+double chunk_few_us(int batch, int q_heads, int kv_heads, int q_len, int head_size, int64_t keys);
+int chunk_few(void *out, int64_t out_batch_stride, int64_t out_head_stride, int64_t out_token_stride, const void *q, int64_t q_batch_stride,
+              int64_t q_head_stride, int64_t q_token_stride, const void *k_cache, const void *v_cache, const float *k_scales, const float *v_scales,
+              const int32_t *page_table, int64_t page_table_row_stride, const int32_t *chunk_start, int batch, int q_heads, int kv_heads, int q_len,
+              int head_size, int block_size, int table_width, int num_blocks, float scale, int64_t keys, void *workspace, hipStream_t st);
+
 namespace {
+
+// Keys that the host knows a pass to read at most.
+int64_t keys_at_most(int block_size, int table_width, int64_t most_keys) {
+  const int64_t room = (int64_t)table_width * block_size;
+  return most_keys > 0 ? std::min(most_keys, room) : room;
+}
+// Whether the cache is read as it is, and not by copies; TTPA_CHUNK_FORM=few|copies (read on every call) overrides.  By what the two are expected to
+// take: the copies 18 us, their bytes at the rate of a large copy and the products at 1 PFLOP/s (32/8 heads of 128, one user: 128 rows of a KV head behind 8192
+// tokens 37, expected 33, 512 45 (46), 768 54 (54); five users behind 4096: 128 51 (55), 256 62 (66)).  Chosen so, us copies / few rows: 320 rows behind 8192 41 / 36,
+// 384 40.5 / 47; five users, 192 rows 62 / 47, 256 62 / 81; behind 1000 tokens 512 rows 23 / 17.  (Left to the copies, and 10 ... 30 % better off without: more rows
+// behind as few tokens, 768 rows 27 / 18.)
+bool few_rows(int batch, int q_heads, int kv_heads, int q_len, int head_size, int64_t keys) {
+  const char *form = getenv("TTPA_CHUNK_FORM");
+  if (form && !strcmp(form, "few")) return true;
+  if (form && !strcmp(form, "copies")) return false;
+  if ((int64_t)batch * kv_heads * ((int64_t)(q_heads / kv_heads) * q_len / 32 + 1) >= (1 << 18)) return false;  // (more than its grid takes)
+  const double values = (double)batch * kv_heads * keys * head_size, flops = 4.0 * batch * q_heads * q_len * (double)keys * head_size;
+  return chunk_few_us(batch, q_heads, kv_heads, q_len, head_size, keys) < 18.0 + 6.0 * values / 4.9e6 + flops / 1e9;
+}
 
 struct ExpandArgs {
   const uint8_t *k, *v;
@@ -99,6 +128,8 @@ extern "C" int64_t ttpa_chunked_fp8_attention_workspace_bytes(int32_t batch, int
                                                               int32_t block_size, int32_t table_width, int64_t most_keys) {
   if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || q_len <= 0 || head_size <= 0 || block_size <= 0 || table_width <= 0)
     return 0;
+  const int64_t keys = fp8::keys_at_most(block_size, table_width, most_keys);
+  if (fp8::few_rows(batch, q_heads, kv_heads, q_len, head_size, keys)) return fp8::chunk_few_bytes(batch, q_heads, kv_heads, q_len, head_size, keys);
   const fp8::ChunkLayout l = fp8::chunk_layout(batch, q_heads, kv_heads, q_len, head_size, block_size, table_width, most_keys);
   return 2 * l.copy + l.table + l.parts;
 }
@@ -115,11 +146,22 @@ extern "C" int ttpa_chunked_fp8_attention(void *out, int64_t out_batch_stride, i
   TTPA_REQUIRE(batch > 0 && q_heads > 0 && q_len > 0 && most_keys >= 0, "fp8 chunk: non-positive dimension");
   TTPA_REQUIRE(q_heads % kv_heads == 0, "fp8 chunk: q_heads %d not divisible by kv_heads %d", q_heads, kv_heads);
   if (block_size % 32) return fail(TTPA_ERR_UNSUPPORTED, "fp8 chunk: block_size %d must be a multiple of 32", block_size);
-  const fp8::ChunkLayout l = fp8::chunk_layout(batch, q_heads, kv_heads, q_len, head_size, block_size, table_width, most_keys);
-  const int64_t need = 2 * l.copy + l.table + l.parts;
+  const int64_t keys = fp8::keys_at_most(block_size, table_width, most_keys);
+  const bool few = fp8::few_rows(batch, q_heads, kv_heads, q_len, head_size, keys);
+  const fp8::ChunkLayout l = few ? fp8::ChunkLayout{} : fp8::chunk_layout(batch, q_heads, kv_heads, q_len, head_size, block_size, table_width, most_keys);
+  const int64_t need = ttpa_chunked_fp8_attention_workspace_bytes(batch, q_heads, kv_heads, q_len, head_size, block_size, table_width, most_keys);
   if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u))
     return fail(TTPA_ERR_WORKSPACE, "fp8 chunk: workspace of %lld bytes (256-byte aligned) required, got %lld", (long long)need,
                 (long long)workspace_bytes);
+  if (few) {
+    TTPA_REQUIRE(aligned16(q) && q_batch_stride % 8 == 0 && q_head_stride % 8 == 0 && q_token_stride % 8 == 0 &&
+                     (reinterpret_cast<uintptr_t>(out) & 7u) == 0 && out_batch_stride % 4 == 0 && out_head_stride % 4 == 0 && out_token_stride % 4 == 0 && scale > 0,
+                 "fp8 chunk: q must be 16-byte aligned, its strides multiples of 8 elements, the output's of 4, the scale positive");
+    return fp8::chunk_few(out, out_batch_stride, out_head_stride, out_token_stride, q, q_batch_stride, q_head_stride, q_token_stride, k_cache, v_cache,
+                          k_scales, v_scales, page_table, page_table_row_stride, chunk_start, batch, q_heads, kv_heads, q_len, head_size, block_size,
+                          table_width, num_blocks, scale, keys, workspace,
+                          static_cast<hipStream_t>(stream));
+  }
   TTPA_REQUIRE((int64_t)batch * l.width < (1ll << 31) - 2 && kv_heads < 32768, "fp8 chunk: too many blocks or heads");
   uint8_t *ws = static_cast<uint8_t *>(workspace);
   fp8::ExpandArgs e = {static_cast<const uint8_t *>(k_cache), static_cast<const uint8_t *>(v_cache), k_scales, v_scales,
