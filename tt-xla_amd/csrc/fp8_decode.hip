@@ -568,6 +568,10 @@ int fp8_direct_waves(int users, int kv_heads, int head_size, int64_t tokens) {
   return head_size > 128 || segments > cus || tokens <= 4 * tile ? 4 : 8;
 }
 
+// Workgroups that a sparse pass's scratch has room for, beyond one per segment: so many may share a segment.
+int sparse_slots() { return 4 * std::max(device_cus(), 256); }
+int most_sparse_parts(int segments) { return sparse_slots() / segments; }
+
 // arrived: counters of the segments, at zero, with which several workgroups may share a segment of equal ones; or null.
 int attend(DecodeArgs a, const float *k_scales, const float *v_scales, int head_size, int *arrived, hipStream_t st) {
   const int g = a.hq / a.hkv;
@@ -579,13 +583,17 @@ int attend(DecodeArgs a, const float *k_scales, const float *v_scales, int head_
   const int segments = a.users * a.hkv;
   int parts = 1;
   if (arrived) {
-    // Segments of one length, about: as many workgroups each as there are CUs for, and tiles for their wavefronts.  us a pass by wavefronts of a
-    // workgroup and workgroups of a segment, 128 segments of 2048 tokens 4/1 38.7, 4/2 36.2, 4/4 36.4, 8/1 37.2, 8/2 35.7, 8/4 40.6; 32 of 4096
-    // 4/4 37.9, 4/8 35.9, 4/16 38.6, 8/2 42.8, 8/4 36.9, 8/8 35.1.
-    const int tile = head_size <= 128 ? 64 : 32, tiles = (int)((tokens + tile - 1) / tile);
-    const int cus = std::max(device_cus(), 1);
+    // Segments of one length, about: as many workgroups each as make the rounds of workgroups, one per CU, times a wavefront's tiles and about two more for
+    // its beginning and end fewest.  us a pass, as many as there are CUs for, rounded up / so, 32 blocks of 64 tokens of 32/8 heads of 128: 10 users 33.4 / 27.2, 20
+    // 44.2 / 35.1, 24 45.8 / 37.7; of 64: 10 users 26.7 / 22.7, 24 33.1 / 26.3; 16/4 heads of 256: 33 users 57.6 / 51.6.  (Two per CU, which there is room for at 64 and
+    // 256: 16 users of 64 25.0 / 28.9, 4 of 256 29.9 / 33.6.)  Wavefronts: 128 segments of 2048 tokens 4 x 2 36.2, 8 x 2 35.7; 32 of 4096 4 x 8 35.9, 8 x 8 35.1.
+    const int tile = head_size <= 128 ? 64 : 32, tiles = (int)((tokens + tile - 1) / tile), cus = std::max(device_cus(), 1);
     a.direct = head_size <= 128 ? 8 : 4;
-    parts = std::max(1, std::min({(cus + segments - 1) / segments, (tiles + a.direct - 1) / a.direct, kMostParts}));
+    int64_t best = INT64_MAX;
+    for (int p = 1; p <= std::min({(tiles + a.direct - 1) / a.direct, kMostParts, std::max(most_sparse_parts(segments), 1)}); ++p) {
+      const int64_t cost = ((int64_t)segments * p + cus - 1) / cus * ((tiles + a.direct * p - 1) / (a.direct * p) + 2);
+      if (cost < best) best = cost, parts = p;
+    }
   }
   // Four wavefronts per CU, and eight over a long list at head size 64, whose tiles are half as large.  How long the list is the kernel
   // knows, and then leaves half of the ranges empty.  us a pass at four / eight, 32/8 heads of 64: 8 users of 2048 ... 4096 tokens (3000 tiles) 11.8 / 12.7,
@@ -633,8 +641,7 @@ struct SparseLayout {
 SparseLayout sparse_layout(int users, int q_heads, int kv_heads, int head_size, int table_width, int kept) {
   const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   const size_t segments = (size_t)users * kv_heads;
-  // (segments x parts: fewer than CUs and segments, or no part but one and no slot)
-  const size_t slots = (size_t)std::max(device_cus(), 256) + segments;
+  const size_t slots = (size_t)sparse_slots() + segments;
   SparseLayout l;
   l.slots = up(slots * slot_floats_for(q_heads / kv_heads, head_size) * sizeof(float));
   l.row = ((size_t)table_width + 15) / 16 | 1;  // (an odd number of lines: rows that begin on the same channels of the memory wait for each other)
