@@ -332,7 +332,7 @@ void paged_decode_fp8_kernel(Fp8Args fa, const int32_t *__restrict__ page_table,
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
         const int row = i * RPL + l_row;
-        const uint32_t keep = (row < nvalid) & (row >= nbelow) ? 0xffffffffu : 0u;
+        const uint32_t keep = ((row < nvalid) & (row >= nbelow)) ? 0xffffffffu : 0u;
         *reinterpret_cast<u32x4 *>(v_tile + vw[i]) = u32x4{vraw[i].x & keep, vraw[i].y & keep, vraw[i].z & keep, vraw[i].w & keep};
       }
     } else {
@@ -384,7 +384,7 @@ void paged_decode_fp8_kernel(Fp8Args fa, const int32_t *__restrict__ page_table,
       for (int r = 0; r < 4; ++r) sc[4 * b + r] = st[b][r];
     if (partial) {
 #pragma unroll
-      for (int i = 0; i < 4 * KBLK; ++i) sc[i] = (i >= nvalid) | (i < nbelow) ? -INFINITY : sc[i];
+      for (int i = 0; i < 4 * KBLK; ++i) sc[i] = ((i >= nvalid) | (i < nbelow)) ? -INFINITY : sc[i];
     }
     float mloc = -INFINITY;
 #pragma unroll
