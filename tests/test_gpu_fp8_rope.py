@@ -160,7 +160,8 @@ def test_operands_that_overlap_are_not_turned_in_place():
     op = torch.ops.tt.qk_norm_rope_
     for q, k in [(x[:1].expand(3, -1, -1), x[:, :2].clone()), (x[:, :2].clone(), x[:, :1].expand(-1, 4, -1)), (x, x), (x[:, :4], x[:, :2]),
                  (x[:2], x[1:]), (x[:, :4], x[:, 3:]), (x[:, 2:4], x[:, 1:]), (x[:, ::2], x[:, 1:3]),
-                 (x.as_strided((3, 3, 64), (128, 64, 1)), x[:, :2].clone()), (x.as_strided((3, 4, 64), (384, 32, 1)), x[:, :2].clone())]:
+                 (x.as_strided((3, 3, 64), (128, 64, 1)), x[:, :2].clone()), (x.as_strided((3, 4, 64), (384, 32, 1)), x[:, :2].clone()),
+                 (x.as_strided((3, 4, 64), (64, 64, 1)), x[:, :2].clone()), (x[:, :2].clone(), x.as_strided((3, 2, 64), (8, 128, 1)))]:
         with pytest.raises(ValueError):
             op(q, k, table, pos[: q.shape[0]])
 

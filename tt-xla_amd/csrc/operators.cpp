@@ -99,13 +99,17 @@ void written(const Tensor &t) {
 void single(const Call &c, const Tensor &t, const char *what) {
   int64_t end = 1, last = 0;  // elements that the dimensions so far reach over
   for (int64_t n = 0; n < t.dim(); ++n) {
-    int64_t stride = std::numeric_limits<int64_t>::max(), size = 1;  // the next longer stride's
-    for (int64_t i = 0; i < t.dim(); ++i)
-      if (t.size(i) > 1 && t.stride(i) > last && t.stride(i) < stride) stride = t.stride(i), size = t.size(i);
-    for (int64_t i = 0; i < t.dim(); ++i)
-      TORCH_CHECK_VALUE(t.size(i) <= 1 || t.stride(i) > 0, c.name(), ": ", what, " is written and must not be expanded");
+    int64_t stride = std::numeric_limits<int64_t>::max(), size = 1, alike = 0;  // the next longer stride's
+    for (int64_t i = 0; i < t.dim(); ++i) {
+      if (t.size(i) <= 1 || t.stride(i) <= last) {
+        TORCH_CHECK_VALUE(t.size(i) <= 1 || t.stride(i) > 0, c.name(), ": ", what, " is written and must not be expanded");
+        continue;
+      }
+      if (t.stride(i) < stride) stride = t.stride(i), size = t.size(i), alike = 0;
+      alike += t.stride(i) == stride;
+    }
     if (size == 1) break;
-    TORCH_CHECK_VALUE(stride >= end, c.name(), ": ", what, " is written and must not overlap itself");
+    TORCH_CHECK_VALUE(stride >= end && alike == 1, c.name(), ": ", what, " is written and must not overlap itself");
     end += (size - 1) * stride, last = stride;
   }
 }
