@@ -37,17 +37,16 @@ int64_t keys_at_most(int block_size, int table_width, int64_t most_keys) {
   return most_keys > 0 ? std::min(most_keys, room) : room;
 }
 // Whether the cache is read as it is, and not by copies; TTPA_CHUNK_FORM=few|copies (read on every call) overrides.  By what the two are expected to
-// take: the copies 18 us, their bytes at the rate of a large copy and the products at 1 PFLOP/s (32/8 heads of 128, one user: 128 rows of a KV head behind 8192
-// tokens 37, expected 33, 512 45 (46), 768 54 (54); five users behind 4096: 128 51 (55), 256 62 (66)).  Chosen so, us copies / few rows: 320 rows behind 8192 41 / 36,
-// 384 40.5 / 47; five users, 192 rows 62 / 47, 256 62 / 81; behind 1000 tokens 512 rows 23 / 17.  (Left to the copies, and 10 ... 30 % better off without: more rows
-// behind as few tokens, 768 rows 27 / 18.)
+// take: the copies 20 us (24 at head size 256), their bytes at the rate of a large copy and the products at 1.2 PFLOP/s (32/8 heads of 128, one user: 128 rows of a
+// KV head behind 8192 tokens 37, expected 34, 512 45 (45), 768 54 (52); five users behind 4096: 128 51 (55), 512 82 (84)).  Chosen so, us copies / few rows: 512 rows
+// behind 8192 45 / 41, 768 54 / 62; five users, 384 rows 72 / 60, 512 82 / 87; behind 1000 tokens 512 rows 23 / 17, 768 26 / 20; of 256, 256 rows behind 8192 58 / 53, 384 64 / 80.
 bool few_rows(int batch, int q_heads, int kv_heads, int q_len, int head_size, int64_t keys) {
   const char *form = getenv("TTPA_CHUNK_FORM");
   if (form && !strcmp(form, "few")) return true;
   if (form && !strcmp(form, "copies")) return false;
   if ((int64_t)batch * kv_heads * ((int64_t)(q_heads / kv_heads) * q_len / 32 + 1) >= (1 << 18)) return false;  // (more than its grid takes)
   const double values = (double)batch * kv_heads * keys * head_size, flops = 4.0 * batch * q_heads * q_len * (double)keys * head_size;
-  return chunk_few_us(batch, q_heads, kv_heads, q_len, head_size, keys) < 18.0 + 6.0 * values / 4.9e6 + flops / 1e9;
+  return chunk_few_us(batch, q_heads, kv_heads, q_len, head_size, keys) < (head_size <= 128 ? 20.0 : 24.0) + 6.0 * values / 4.9e6 + flops / 1.2e9;
 }
 
 struct ExpandArgs {

@@ -7,8 +7,8 @@
 //   causal     a row attends chunk_start + its token + 1 keys: a limit per lane and group
 // The wavefronts' results meet in LDS, the parts' in memory, merged by a kernel of its own.  Blocks of rows of one KV head and part have
 // workgroups on one XCD, which then reads its keys once.  Four groups at head size 128 spill (one token of 32/8 heads behind 8192 28 us, two groups 17.4, three
-// 36 with 32 tokens where two take 21.6).  Against copies (fp8_chunk.hip), us a pass copies / this, 8/8 heads of 64, four users, 64 rows behind 10112 tokens
-// 49 / 24; 16/16 of 128, four users, 64 behind 4096 66 / 32; 32/8 of 256, one user, 32 behind 8192 55 / 35; 64/8 of 128, 32 behind 6912 34 / 27.
+// 36 with 32 tokens where two take 21.6).  Against copies (fp8_chunk.hip), us a pass copies / this: 8/8 heads of 64, four users, 64 rows behind 10112 tokens
+// 49 / 24; 16/16 of 128, four users, 64 behind 4096 66 / 24; 32/8 of 256, one user, 32 behind 8192 55 / 35; 64/8 of 128, 32 behind 6912 34 / 27.
 #include "fp8_decode_kernel.h"
 
 #include <algorithm>
@@ -37,6 +37,12 @@ template <int D>
 constexpr int few_groups() {
   return D == 64 ? 4 : 2;
 }
+// Workgroups per CU: two at head size 128, in whose 256 registers two groups fit (five users, 256 rows of a KV head behind 4096 tokens: 53.7 us, 78 with one; 768 rows
+// 110, 168); with one each the others need more (64 in 256: 192 rows behind 60000 tokens 64 us as in 366, but 32 rows 43 and not 33).
+template <int D>
+constexpr int few_per_cu() {
+  return D == 128 ? 2 : 1;
+}
 template <int D>
 constexpr int few_slot_floats() {
   return 16 * few_groups<D>() * (D + 2);
@@ -53,7 +59,7 @@ __device__ __forceinline__ int few_parts(const FewArgs &a, int keys) {
 }
 
 template <int D>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 2))) void few_rows_kernel(FewArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(few_per_cu<D>(), 2))) void few_rows_kernel(FewArgs a) {
   constexpr int TILE = fp8_tile<D>(), RUN = TILE / 4, RG = few_groups<D>(), ROWS = 16 * RG;
   constexpr int KBLK = TILE / 16, KP = D / 64, DBLK = D / 16, PSTEPS = TILE / 32;
   constexpr int CPR = D / 16, RPL = 16 / CPR, NL = RUN / RPL;
@@ -351,27 +357,28 @@ int launch_few(FewArgs &a, hipStream_t st) {
 
 namespace fp8 {
 
-// Blocks of rows per KV head, and parts of the keys.  A CU takes one workgroup, so what counts is rounds of workgroups, each as long as a wavefront's tiles
-// and about three more for its beginning and end (264 workgroups took nearly twice as long as 256).  Returns that number of tiles.
+// Blocks of rows per KV head, and parts of the keys.  What counts is rounds of workgroups, each as long as a wavefront's tiles and about three more for its
+// beginning and end (264 workgroups took nearly twice as long as 256).  Returns that number of tiles.
 static int64_t few_split(int batch, int kv_heads, int64_t rows, int head_size, int64_t keys, int &row_blocks, int &parts) {
   const int per = head_size == 64 ? 64 : 32, tile = head_size <= 128 ? 64 : 32;
   row_blocks = (int)((rows + per - 1) / per);
-  const int64_t segments = (int64_t)batch * kv_heads * row_blocks, tiles = (keys + tile - 1) / tile, cus = std::max(device_cus(), 1);
+  const int64_t segments = (int64_t)batch * kv_heads * row_blocks, tiles = (keys + tile - 1) / tile;
+  const int64_t at_once = std::max(device_cus(), 1) * (head_size == 128 ? decode::few_per_cu<128>() : 1);
   int64_t best = INT64_MAX;
   parts = 1;
   for (int64_t p = 1; p <= std::min<int64_t>(32, (tiles + 3) / 4); ++p) {
-    const int64_t cost = (segments * p + cus - 1) / cus * ((tiles + 4 * p - 1) / (4 * p) + 3);
+    const int64_t cost = (segments * p + at_once - 1) / at_once * ((tiles + 4 * p - 1) / (4 * p) + 3);
     if (cost < best) best = cost, parts = (int)p;
   }
   return best;
 }
 
-// us that this form is expected to take, of which the other one's (copies, then the prefill kernels) is compared.  32/8 heads of 128, one user: 128 rows of a KV
-// head behind 8192 tokens 23.1 (expected 23), 256 30.5 (31), 512 47.8 (46), 768 78.5 (76); five users behind 4096: 256 80.6 (84).
+// us that this form is expected to take, with which the other one's (copies, then the prefill kernels) is compared.  32/8 heads of 128, one user: 128 rows of a KV
+// head behind 8192 tokens 23.9 (expected 23.9), 256 29.8 (29.2), 512 40.6 (39.8), 768 62.3 (61.0); five users behind 4096: 256 53.7 (55.7), 768 110 (114).
 double chunk_few_us(int batch, int q_heads, int kv_heads, int q_len, int head_size, int64_t keys) {
   int row_blocks, parts;
   const int64_t tiles = few_split(batch, kv_heads, (int64_t)(q_heads / kv_heads) * q_len, head_size, keys, row_blocks, parts);
-  return 8.0 + (head_size <= 128 ? 1.9 : 2.25) * (double)tiles;
+  return 8.0 + (head_size == 64 ? 1.9 : head_size == 128 ? 2.65 : 2.25) * (double)tiles;
 }
 
 int64_t chunk_few_bytes(int batch, int q_heads, int kv_heads, int q_len, int head_size, int64_t keys) {
