@@ -237,3 +237,25 @@ def test_tracing_sees_shapes():
         assert tt.qk_norm_rope_update_fp8_(f["q"], f["k"], f["v"], f["angles"], f["pos"], *kv[:4], f["table"]).shape == f["q"].shape
         a, b = tt.qk_norm_rope(f["q"], f["k"], f["angles"], f["pos"])
         assert a.shape == f["q"].shape and b.shape == f["k"].shape
+
+
+@pytest.mark.parametrize("hq, hkv, d, bs, start, s", [(8, 2, 64, 32, 64, 64), (32, 8, 128, 64, 128, 32), (4, 4, 256, 32, 32, 70)])
+@pytest.mark.parametrize("known", [True, False])
+def test_a_continuation_chunk_of_a_layer_that_shares_a_cache(hq, hkv, d, bs, start, s, known):
+    """Its rows attend the whole prefix and the chunk's keys as the layer that owns the cache has written them, and write nothing."""
+    from tt_xla_amd import TTAttentionBackendImpl, TTMetadata
+
+    users, width = 2, -(-(start + s) // bs) + 2
+    cache, table, _, _, g = _setup(users, hkv, hq // hkv, d, bs, [width * bs] * users, d + s)
+    kv = [t.cuda() for t in cache]
+    before = [t.clone() for t in kv]
+    impl = TTAttentionBackendImpl(hq, d, d**-0.5, hkv, kv_cache_dtype="fp8", kv_sharing_target_layer_name="other")
+    q = torch.randn(users * s, hq * d, generator=g).to(torch.bfloat16)
+    new = torch.randn(users * s, hkv * d, generator=g).to(torch.bfloat16).cuda()
+    out = torch.empty(users * s, hq * d, dtype=torch.bfloat16, device="cuda")
+    meta = TTMetadata(page_table=table.cuda(), num_users=users, batch_idx=torch.arange(users, dtype=torch.int32).cuda(),
+                      chunk_start_idx=torch.tensor([start], dtype=torch.int32).cuda(), chunk_end=start + s if known else None)
+    impl.forward(None, q.cuda(), new, new, kv, meta, output=out)
+    rows = [t.view(users, s, hq, d).transpose(1, 2) for t in (out.cpu(), q)]
+    check_chunk(*rows, cache, table, start, d**-0.5)
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(kv, before))

@@ -412,7 +412,8 @@ class TTAttentionBackendImpl(_ImplBase):
                     batch_idx = batch_idx % (k.shape[0] // attn_metadata.dp_size)
                 ops.paged_fill_fp8_cache_(*cache, k, v, attn_metadata.fill_page_table, batch_idx, bounds)
             q, target = inputs.query.transpose(1, 2), into.transpose(1, 2)
-            if attn_metadata.chunk_start_idx is not None and writes:
+            if attn_metadata.chunk_start_idx is not None and cache[0].numel() > 0:
+                # keys come from the cache, prefix included: also where another layer has written them
                 # (what a graph captures is replayed for other chunks: it has to have room for all that the table holds)
                 known = 0 if torch.cuda.is_current_stream_capturing() else attn_metadata.chunk_end or 0
                 ops.chunked_fp8_attention_out(q, *cache, attn_metadata.page_table, attn_metadata.chunk_start_idx, target,
