@@ -259,3 +259,32 @@ def test_a_continuation_chunk_of_a_layer_that_shares_a_cache(hq, hkv, d, bs, sta
     rows = [t.view(users, s, hq, d).transpose(1, 2) for t in (out.cpu(), q)]
     check_chunk(*rows, cache, table, start, d**-0.5)
     assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(kv, before))
+
+
+def test_windows_of_continuation_chunks():
+    """A window that may leave out a key is refused, and nothing is written; one that cannot is none."""
+    from tt_xla_amd import TTAttentionBackendImpl, TTMetadata
+
+    hq, hkv, d, bs, start, s = 8, 2, 64, 32, 96, 32
+    cache, table, _, _, g = _setup(1, hkv, hq // hkv, d, bs, [6 * bs], 4)
+    kv = [t.cuda() for t in cache]
+    q = torch.randn(s, hq * d, generator=g).to(torch.bfloat16)
+    k, v = (torch.randn(s, hkv * d, generator=g).to(torch.bfloat16).cuda() for _ in range(2))
+    room = table.shape[1] * bs
+    for shared in (None, "other"):
+        for window, end in ((1, start + s), (start + s - 1, start + s), (start + s, None), (room - 1, None), (start + s, start + s), (room, None),
+                            (room, room + 70)):
+            impl = TTAttentionBackendImpl(hq, d, d**-0.5, hkv, sliding_window=window, kv_cache_dtype="fp8", kv_sharing_target_layer_name=shared)
+            own = [t.clone() for t in kv]
+            out = torch.zeros(s, hq * d, dtype=torch.bfloat16, device="cuda")
+            meta = TTMetadata(page_table=table.cuda(), fill_page_table=table[:, start // bs :].contiguous().cuda(), num_users=1,
+                              batch_idx=torch.zeros(1, dtype=torch.int32).cuda(), chunk_start_idx=torch.tensor([start], dtype=torch.int32).cuda(),
+                              chunk_end=end)
+            if window < min(end or room, room):
+                with pytest.raises(NotImplementedError, match="sliding window"):
+                    impl.forward(None, q.cuda(), k, v, own, meta, output=out)
+                assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(own, kv)) and int(out.count_nonzero()) == 0
+                continue
+            impl.forward(None, q.cuda(), k, v, own, meta, output=out)
+            rows = [t.view(1, s, hq, d).transpose(1, 2) for t in (out.cpu(), q)]
+            check_chunk(*rows, [t.cpu() for t in own], table, start, d**-0.5)

@@ -405,6 +405,13 @@ class TTAttentionBackendImpl(_ImplBase):
         else:
             assert self.sinks is None, "Attention sink is unsupported in SDPA prefill"
             k, v = inputs.key.transpose(1, 2), inputs.value.transpose(1, 2)
+            chunk = attn_metadata.chunk_start_idx is not None and cache[0].numel() > 0
+            # (what a graph captures is replayed for other chunks: it has to have room for all that the table holds)
+            known = 0 if not chunk or torch.cuda.is_current_stream_capturing() else attn_metadata.chunk_end or 0
+            if chunk and self.sliding_window is not None:
+                room = attn_metadata.page_table.shape[1] * cache[0].shape[2]
+                if self.sliding_window < (min(known, room) if known else room):
+                    raise NotImplementedError("continuation chunks over an 8-bit cache are built without sliding windows")
             if writes:
                 batch_idx = attn_metadata.batch_idx
                 assert batch_idx is not None, "batch_idx must be provided for prefill."
@@ -412,10 +419,8 @@ class TTAttentionBackendImpl(_ImplBase):
                     batch_idx = batch_idx % (k.shape[0] // attn_metadata.dp_size)
                 ops.paged_fill_fp8_cache_(*cache, k, v, attn_metadata.fill_page_table, batch_idx, bounds)
             q, target = inputs.query.transpose(1, 2), into.transpose(1, 2)
-            if attn_metadata.chunk_start_idx is not None and cache[0].numel() > 0:
+            if chunk:
                 # keys come from the cache, prefix included: also where another layer has written them
-                # (what a graph captures is replayed for other chunks: it has to have room for all that the table holds)
-                known = 0 if torch.cuda.is_current_stream_capturing() else attn_metadata.chunk_end or 0
                 ops.chunked_fp8_attention_out(q, *cache, attn_metadata.page_table, attn_metadata.chunk_start_idx, target,
                                               scale=self.scale, most_keys=known)
             else:
