@@ -288,3 +288,21 @@ def test_windows_of_continuation_chunks():
             impl.forward(None, q.cuda(), k, v, own, meta, output=out)
             rows = [t.view(1, s, hq, d).transpose(1, 2) for t in (out.cpu(), q)]
             check_chunk(*rows, [t.cpu() for t in own], table, start, d**-0.5)
+
+
+@pytest.mark.parametrize("wrong", [dict(bounds=False), dict(sliding_window=40), dict(sinks=True)])
+def test_a_refused_sparse_step_writes_nothing(wrong):
+    from tt_xla_amd import TTAttentionBackendImpl, TTMetadata
+
+    hq, hkv, d, bs = 8, 2, 64, 32
+    cache, table, cur, q, g = _setup(2, hkv, hq // hkv, d, bs, [100, 50], 3)
+    kv = [t.cuda() for t in cache] + ([_bounds(cache).cuda()] if wrong.pop("bounds", True) else [])
+    if wrong.pop("sinks", False):
+        wrong["sinks"] = torch.randn(hq, generator=g).cuda()
+    before = [t.clone() for t in kv]
+    impl = TTAttentionBackendImpl(hq, d, d**-0.5, hkv, kv_cache_dtype="fp8", sparse_kept_blocks=2, **wrong)
+    new = torch.randn(2, hkv * d, generator=g).to(torch.bfloat16).cuda()
+    out = torch.zeros(2, hq * d, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(NotImplementedError, match="sparse"):
+        impl.forward(None, q.flatten(1).cuda(), new, new, kv, TTMetadata(cache_position=cur.cuda(), page_table=table.cuda(), num_users=2), output=out)
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(kv, before)) and int(out.count_nonzero()) == 0

@@ -392,12 +392,13 @@ class TTAttentionBackendImpl(_ImplBase):
         into = torch.empty(inputs.query.shape, dtype=query.dtype, device=query.device) if out is None else out
         if not inputs.is_prefill:
             positions, table = attn_metadata.cache_position, attn_metadata.page_table
+            sparse = self.sparse_kept_blocks is not None
+            if sparse and (bounds is None or self.sinks is not None or self.sliding_window is not None):
+                raise NotImplementedError("sparse decode needs key bounds, and is built without sinks and sliding windows")
             if writes:
                 ops.paged_update_fp8_cache_(*cache, inputs.key.transpose(0, 1), inputs.value.transpose(0, 1), positions, table, bounds)
             q, target = inputs.query.transpose(0, 1), into.transpose(0, 1)
-            if self.sparse_kept_blocks is not None:
-                if bounds is None or self.sinks is not None or self.sliding_window is not None:
-                    raise NotImplementedError("sparse decode needs key bounds, and is built without sinks and sliding windows")
+            if sparse:
                 ops.paged_fp8_sparse_attention_decode_out(q, *cache, bounds, table, positions, target, self.sparse_kept_blocks, scale=self.scale)
             else:
                 ops.paged_fp8_attention_decode_out(q, *cache, table, positions, target, attention_sink=self.sinks, scale=self.scale,
