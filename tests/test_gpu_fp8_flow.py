@@ -306,3 +306,31 @@ def test_a_refused_sparse_step_writes_nothing(wrong):
     with pytest.raises(NotImplementedError, match="sparse"):
         impl.forward(None, q.flatten(1).cuda(), new, new, kv, TTMetadata(cache_position=cur.cuda(), page_table=table.cuda(), num_users=2), output=out)
     assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(kv, before)) and int(out.count_nonzero()) == 0
+
+
+@pytest.mark.parametrize("tensors", [2, 4, 5])
+@pytest.mark.parametrize("shared", [None, "other"])
+@pytest.mark.parametrize("start", [None, 64])
+@pytest.mark.parametrize("kw", [{}, dict(sliding_window=20), dict(sparse_kept_blocks=4)])
+def test_prompts_with_caches_that_are_still_empty(tensors, shared, start, kw):
+    """What vLLM runs to see how much memory a pass takes: attention of the pass's own keys and values, as with any other type of cache."""
+    from tt_xla_amd import TTAttentionBackendImpl, TTMetadata
+
+    hq, hkv, d, bs, users, s = 8, 2, 64, 32, 2, 64
+    kv = _layer(0, hkv, bs, d)[:tensors]
+    g = torch.Generator().manual_seed(tensors)
+    q = torch.randn(users * s, hq * d, generator=g).to(torch.bfloat16)
+    k, v = (torch.randn(users * s, hkv * d, generator=g).to(torch.bfloat16) for _ in range(2))
+    meta = TTMetadata(page_table=torch.zeros(users, 4, dtype=torch.int32).cuda(), num_users=users, batch_idx=torch.arange(users, dtype=torch.int32).cuda(),
+                      chunk_start_idx=None if start is None else torch.tensor([start], dtype=torch.int32).cuda())
+    impl = TTAttentionBackendImpl(hq, d, d**-0.5, hkv, kv_cache_dtype="fp8", kv_sharing_target_layer_name=shared, **kw)
+    out = torch.zeros(users * s, hq * d, dtype=torch.bfloat16, device="cuda")
+    impl.forward(None, q.cuda(), k.cuda(), v.cuda(), kv, meta, output=out)
+    got, q = (t.view(users, s, hq, d) for t in (out.cpu(), q))
+    k, v = (t.view(users, s, hkv, d).double() for t in (k, v))
+    at = torch.arange(s)
+    allowed = (at[None, :] <= at[:, None]) & (at[None, :] > at[:, None] - kw.get("sliding_window", s))
+    for u in range(users):
+        for h in range(hq):
+            one, size = R.softmax_rows(q[u, :, h], k[u, :, h * hkv // hq], v[u, :, h * hkv // hq], allowed, d**-0.5)
+            assert bool(((got[u, :, h].double() - one).abs() <= 2.0**-8 * one.abs() + 0.0085 * size).all())

@@ -283,7 +283,8 @@ class TTAttentionBackendImpl(_ImplBase):
         the result is written into ``output`` [tokens, Hq*D]."""
         assert attn_metadata is not None, "TT attention requires metadata."
         assert output is not None, "TT attention requires an output buffer."
-        if isinstance(kv_cache, (list, tuple)) and kv_cache[0].dtype == torch.float8_e4m3fn:
+        # (empty caches stand in while vLLM profiles memory, of any type: such a pass is the ordinary one without a cache)
+        if isinstance(kv_cache, (list, tuple)) and kv_cache[0].dtype == torch.float8_e4m3fn and kv_cache[0].numel() > 0:
             self._fp8_pass(query, key, value, kv_cache, attn_metadata, output)
             return
         if self._native_pass(query, key, value, kv_cache, attn_metadata, output):
@@ -387,7 +388,6 @@ class TTAttentionBackendImpl(_ImplBase):
         ops, cache, bounds = torch.ops.tt, tuple(kv_cache[:4]), kv_cache[4] if len(kv_cache) == 5 else None
         inputs = self._prepare_inputs(query, key, value, attn_metadata)
         shared = self.kv_sharing_target_layer_name is not None
-        writes = not shared and cache[0].numel() > 0  # (an empty cache stands in while vLLM profiles memory)
         out = self._output_view(output, inputs)
         into = torch.empty(inputs.query.shape, dtype=query.dtype, device=query.device) if out is None else out
         if not inputs.is_prefill:
@@ -395,7 +395,7 @@ class TTAttentionBackendImpl(_ImplBase):
             sparse = self.sparse_kept_blocks is not None
             if sparse and (bounds is None or self.sinks is not None or self.sliding_window is not None):
                 raise NotImplementedError("sparse decode needs key bounds, and is built without sinks and sliding windows")
-            if writes:
+            if not shared:
                 ops.paged_update_fp8_cache_(*cache, inputs.key.transpose(0, 1), inputs.value.transpose(0, 1), positions, table, bounds)
             q, target = inputs.query.transpose(0, 1), into.transpose(0, 1)
             if sparse:
@@ -406,14 +406,14 @@ class TTAttentionBackendImpl(_ImplBase):
         else:
             assert self.sinks is None, "Attention sink is unsupported in SDPA prefill"
             k, v = inputs.key.transpose(1, 2), inputs.value.transpose(1, 2)
-            chunk = attn_metadata.chunk_start_idx is not None and cache[0].numel() > 0
+            chunk = attn_metadata.chunk_start_idx is not None
             # (what a graph captures is replayed for other chunks: it has to have room for all that the table holds)
             known = 0 if not chunk or torch.cuda.is_current_stream_capturing() else attn_metadata.chunk_end or 0
             if chunk and self.sliding_window is not None:
                 room = attn_metadata.page_table.shape[1] * cache[0].shape[2]
                 if self.sliding_window < (min(known, room) if known else room):
                     raise NotImplementedError("continuation chunks over an 8-bit cache are built without sliding windows")
-            if writes:
+            if not shared:
                 batch_idx = attn_metadata.batch_idx
                 assert batch_idx is not None, "batch_idx must be provided for prefill."
                 if attn_metadata.dp_size > 1:
