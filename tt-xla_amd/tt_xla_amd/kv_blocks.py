@@ -1,10 +1,11 @@
 """Moving whole KV blocks between a host-side cache and the device cache (block swap for
 preemption / offload).  Same call surface and no-op rules as ``copy_kv_blocks`` in tt-xla's
 ``integrations/vllm_plugin/vllm_tt/model_runner.py:5433-5474``: caches are dicts
-``layer name -> tensor`` or ``layer name -> (k_cache, v_cache)`` with blocks on dim 0, and
-block ``src_block_ids[i]`` of every source tensor lands in block ``dst_block_ids[i]`` of the
-matching destination tensor.  Pure block copies: torch's gather / scatter on dim 0 plus one
-transfer per tensor; nothing is computed.
+``layer name -> tensor`` or ``layer name -> (k_cache, v_cache)`` with blocks on dim 0 (an
+8-bit layer: all of its kv_cache, scales and key bounds too), and block ``src_block_ids[i]``
+of every source tensor lands in block ``dst_block_ids[i]`` of the matching destination
+tensor.  Pure block copies: torch's gather / scatter on dim 0 plus one transfer per tensor;
+nothing is computed.
 """
 
 from __future__ import annotations
@@ -21,6 +22,8 @@ def _device_of(value: Cache) -> torch.device:
 
 
 def _move(src: torch.Tensor, dst: torch.Tensor, src_idx: torch.Tensor, dst_idx: torch.Tensor) -> None:
+    if src.dtype == dst.dtype and src.dtype.itemsize == 1:  # (torch gathers and scatters bytes everywhere, 8-bit floats not on the host)
+        src, dst = src.view(torch.uint8), dst.view(torch.uint8)
     picked = src.index_select(0, src_idx)
     dst.index_copy_(0, dst_idx, picked.to(dst.device, non_blocking=False))
 
@@ -49,6 +52,8 @@ def copy_kv_blocks(
     for name, src in src_kv_caches.items():
         dst = dst_kv_caches[name]
         if isinstance(src, (list, tuple)):
+            if len(src) != len(dst):
+                raise ValueError(f"layer {name!r} has {len(src)} tensors on one side and {len(dst)} on the other")
             for s, d in zip(src, dst):
                 _move(s, d, src_idx, dst_idx)
         else:
