@@ -334,3 +334,21 @@ def test_prompts_with_caches_that_are_still_empty(tensors, shared, start, kw):
         for h in range(hq):
             one, size = R.softmax_rows(q[u, :, h], k[u, :, h * hkv // hq], v[u, :, h * hkv // hq], allowed, d**-0.5)
             assert bool(((got[u, :, h].double() - one).abs() <= 2.0**-8 * one.abs() + 0.0085 * size).all())
+
+
+@pytest.mark.parametrize("kind", ["bfloat16", "block-float-8"])
+@pytest.mark.parametrize("s", [1, 32])
+def test_sparse_passes_over_other_caches_are_refused(kind, s):
+    from tt_xla_amd import TTAttentionBackendImpl, TTMetadata, custom_ops
+
+    hq, hkv, d, bs, nb = 8, 2, 64, 32, 6
+    shape, dtype = ((nb, hkv, bs, d), torch.bfloat16) if kind == "bfloat16" else (custom_ops.bfp8_cache_shape(nb, hkv, bs, d), torch.uint8)
+    kv = [torch.zeros(shape, dtype=dtype, device="cuda") for _ in range(2)]
+    impl = TTAttentionBackendImpl(hq, d, d**-0.5, hkv, sparse_kept_blocks=2)
+    q, k = (torch.ones(s, h * d, dtype=torch.bfloat16, device="cuda") for h in (hq, hkv))
+    out = torch.zeros_like(q)
+    meta = TTMetadata(cache_position=torch.zeros(1, dtype=torch.int32).cuda(), page_table=torch.zeros(1, 4, dtype=torch.int32).cuda(), num_users=1,
+                      batch_idx=torch.zeros(1, dtype=torch.int32).cuda())
+    with pytest.raises(NotImplementedError, match="sparse"):
+        impl.forward(None, q, k, k, kv, meta, output=out)
+    assert not any(int(t.count_nonzero()) for t in (*kv, out))

@@ -237,7 +237,7 @@ class TTAttentionBackendImpl(_ImplBase):
         sparse_kept_blocks: Optional[int] = None,
     ) -> None:
         """sparse_kept_blocks: decode passes over an 8-bit cache with key bounds attend that many blocks of each context, chosen
-        per KV head, instead of all of them."""
+        per KV head, instead of all of them; passes over other caches are refused."""
         self.num_heads = num_heads
         self.head_size = head_size
         self.scale = float(scale)
@@ -287,6 +287,8 @@ class TTAttentionBackendImpl(_ImplBase):
         if isinstance(kv_cache, (list, tuple)) and kv_cache[0].dtype == torch.float8_e4m3fn and kv_cache[0].numel() > 0:
             self._fp8_pass(query, key, value, kv_cache, attn_metadata, output)
             return
+        if self.sparse_kept_blocks is not None and isinstance(kv_cache, (list, tuple)) and kv_cache[0].numel() > 0:
+            raise NotImplementedError(f"sparse decode is built for 8-bit caches with key bounds, not for {kv_cache[0].dtype} caches")
         if self._native_pass(query, key, value, kv_cache, attn_metadata, output):
             return
         inputs = self._prepare_inputs(query, key, value, attn_metadata)
