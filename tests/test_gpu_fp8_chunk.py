@@ -206,3 +206,20 @@ def test_few_rows_over_many_parts_and_many_blocks_of_rows(monkeypatch):
         for known in (0, start + s):
             out = torch.ops.tt.chunked_fp8_attention(q.cuda(), *on, table.cuda(), torch.tensor([start]).cuda(), most_keys=known)
             _check(out.cpu(), q, cache, table, start, d**-0.5)
+
+
+@pytest.mark.parametrize("form", ["few", "copies", None])
+@pytest.mark.parametrize("d, hq, hkv", [(64, 8, 2), (128, 8, 1), (256, 4, 4)])
+def test_a_bound_below_the_chunk_ends_the_table(d, hq, hkv, form, monkeypatch):
+    """most_keys is a promise; where it is not kept, both forms attend what the table holds up to the block of the last promised key."""
+    if form:
+        monkeypatch.setenv("TTPA_CHUNK_FORM", form)
+    g = torch.Generator().manual_seed(d)
+    bs, s, start = 32, 40, 88
+    cache = _cache(9, hkv, bs, d, g)
+    table = torch.tensor([[2, 5, 1, 4, 7, 3], [6, 8, 1, 2, 4, 5]], dtype=torch.int32)
+    q = torch.randn(2, hq, s, d, generator=g).to(torch.bfloat16)
+    on = [t.cuda() for t in cache]
+    for most in (1, 32, 33, 64, 95, 96, 97, 127, 128, 129):
+        out = torch.ops.tt.chunked_fp8_attention(q.cuda(), *on, table.cuda(), torch.tensor([start]).cuda(), most_keys=most).cpu()
+        _check(out, q, cache, table[:, : -(-most // bs)], start, d**-0.5)

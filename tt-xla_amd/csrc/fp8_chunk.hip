@@ -31,7 +31,7 @@ int chunk_few(void *out, int64_t out_batch_stride, int64_t out_head_stride, int6
 
 namespace {
 
-// Keys that the host knows a pass to read at most.
+// Keys that the host knows a pass to read at most.  (Both forms take the table as if it ended with the block that holds the last of them.)
 int64_t keys_at_most(int block_size, int table_width, int64_t most_keys) {
   const int64_t room = (int64_t)table_width * block_size;
   return most_keys > 0 ? std::min(most_keys, room) : room;
@@ -158,8 +158,7 @@ extern "C" int ttpa_chunked_fp8_attention(void *out, int64_t out_batch_stride, i
                  "fp8 chunk: q must be 16-byte aligned, its strides multiples of 8 elements, the output's of 4, the scale positive");
     return fp8::chunk_few(out, out_batch_stride, out_head_stride, out_token_stride, q, q_batch_stride, q_head_stride, q_token_stride, k_cache, v_cache,
                           k_scales, v_scales, page_table, page_table_row_stride, chunk_start, batch, q_heads, kv_heads, q_len, head_size, block_size,
-                          table_width, num_blocks, scale, keys, workspace,
-                          static_cast<hipStream_t>(stream));
+                          (int)((keys + block_size - 1) / block_size), num_blocks, scale, keys, workspace, static_cast<hipStream_t>(stream));
   }
   TTPA_REQUIRE((int64_t)batch * l.width < (1ll << 31) - 2 && kv_heads < 32768, "fp8 chunk: too many blocks or heads");
   uint8_t *ws = static_cast<uint8_t *>(workspace);
