@@ -352,3 +352,51 @@ def test_sparse_passes_over_other_caches_are_refused(kind, s):
     with pytest.raises(NotImplementedError, match="sparse"):
         impl.forward(None, q, k, k, kv, meta, output=out)
     assert not any(int(t.count_nonzero()) for t in (*kv, out))
+
+
+def _odd(t):
+    """The same values in a contiguous tensor whose address is no multiple of 16."""
+    x = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")[1:].view(t.shape)
+    x.copy_(t)
+    assert x.is_contiguous() and x.data_ptr() % 16
+    return x
+
+
+def test_operands_at_odd_addresses():
+    """Contiguous tensors that vector loads cannot take: the results of aligned ones, in place and in the caches too."""
+    tt, s = torch.ops.tt, _state(9)
+    users = s["q"].shape[0]
+    g = torch.Generator().manual_seed(12)
+    rope = [s[n] for n in ("q", "k", "angles", "pos", "qw", "kw")]
+    odd = [_odd(t) if t.is_floating_point() else t for t in rope]
+    want = tt.qk_norm_rope(*rope)
+    for i in range(len(rope)):
+        got = tt.qk_norm_rope(*rope[:i], odd[i], *rope[i + 1 :])
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    q, k = _odd(s["q"]), _odd(s["k"])
+    tt.qk_norm_rope_(q, k, *rope[2:])
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+
+    def same(call, *args):
+        """call(caches, *args) gives the same results and caches whichever operand lies at an odd address."""
+        def once(*a):
+            kv = [t.clone() for t in s["kv"]]
+            out = call(kv, *a)
+            return [t for t in (out if isinstance(out, (list, tuple)) else [out]) if t is not None] + kv
+
+        want = once(*args)
+        for i in range(len(args)):
+            got = once(*args[:i], _odd(args[i]), *args[i + 1 :])
+            assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(got, want)), i
+
+    table, pos = s["table"], s["pos"]
+    same(lambda kv, q, k, v: tt.qk_norm_rope_update_fp8_(q, k, v, s["angles"], pos, *kv[:4], table, s["qw"], s["kw"], kv[4]), s["q"], s["k"], s["v"])
+    same(lambda kv, k, v: tt.paged_update_fp8_cache_(*kv[:4], k, v, pos, table, kv[4]), s["k"][None], s["v"][None])
+    prompts = [torch.randn(2, 4, 45, 128, generator=g).to(torch.bfloat16).cuda() for _ in range(2)]
+    same(lambda kv, k, v: tt.paged_fill_fp8_cache_(*kv[:4], k, v, table[:2, :2].contiguous(), torch.tensor([1, 0]).cuda(), kv[4]), *prompts)
+    same(lambda kv, q: tt.paged_fp8_attention_decode(q, *kv[:4], table, pos), s["q"][None])
+    same(lambda kv, q: tt.paged_fp8_sparse_attention_decode(q, *kv, table, pos, 3), s["q"][None])
+    rows = torch.randn(users, 16, 40, 128, generator=g).to(torch.bfloat16).cuda()
+    same(lambda kv, q: tt.chunked_fp8_attention(q, *kv[:4], table, torch.tensor([20]).cuda()), rows)
+    sink = torch.randn(16, generator=g).cuda()
+    same(lambda kv, x: tt.paged_fp8_attention_decode(s["q"][None], *kv[:4], table, pos, x), sink)

@@ -73,7 +73,12 @@ bool has_rows(const Tensor &t, int64_t unit = 8) {
     if (t.size(i) > 1 && t.stride(i) % unit) return false;
   return true;
 }
-Tensor rows(const Tensor &t) { return has_rows(t) ? t : t.contiguous(); }
+// (a contiguous tensor at an odd address comes back from contiguous() as it is)
+Tensor compact(const Tensor &t) {
+  const Tensor c = t.contiguous();
+  return aligned16(c) ? c : c.clone(at::MemoryFormat::Contiguous);
+}
+Tensor rows(const Tensor &t) { return has_rows(t) ? t : compact(t); }
 // A stride for the kernels: of a dimension of one element it is never used, and torch may leave anything there.
 int64_t step_of(const Tensor &t, int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; }
 Tensor indices(const Call &c, const Tensor &t, const char *what) {
@@ -404,7 +409,7 @@ Tensor sparse_into(const Call &c, const Tensor &out, const Tensor &query, const 
   if (users == 0) return columns;
   // (users and heads in one row of heads: a (user, KV head) is a user of the attention)
   const auto packed = [&](const Tensor &t) { return has_rows(t, 8) && (users == 1 || step_of(t, 1) == hq * (hq > 1 ? t.stride(2) : t.stride(1))); };
-  const Tensor q = packed(query) ? query : query.contiguous(), target = packed(out) ? out : at::empty(out.sizes(), out.options());
+  const Tensor q = packed(query) ? query : compact(query), target = packed(out) ? out : at::empty(out.sizes(), out.options());
   const auto head_stride = [&](const Tensor &t) { return hq > 1 ? t.stride(2) : users > 1 ? t.stride(1) : cache.d; };
   const size_t bytes = ttpa_paged_fp8_sparse_decode_workspace_bytes(i32(users), i32(hq), i32(cache.hkv), i32(cache.d), i32(pt.size(1)), i32(kept));
   const Tensor ws = c.scratch((int64_t)bytes);
