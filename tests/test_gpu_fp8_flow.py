@@ -400,3 +400,47 @@ def test_operands_at_odd_addresses():
     same(lambda kv, q: tt.chunked_fp8_attention(q, *kv[:4], table, torch.tensor([20]).cuda()), rows)
     sink = torch.randn(16, generator=g).cuda()
     same(lambda kv, x: tt.paged_fp8_attention_decode(s["q"][None], *kv[:4], table, pos, x), sink)
+
+
+def test_outputs_in_the_memory_of_the_query():
+    """The query itself and views beside it are written; what would overwrite rows that are still to be read is refused."""
+    tt, s = torch.ops.tt, _state(13)
+    users, hq, d = s["q"].shape
+    g = torch.Generator().manual_seed(14)
+    rows, start = torch.randn(users, hq, 40, d, generator=g).to(torch.bfloat16).cuda(), torch.tensor([20]).cuda()
+    calls = [(s["q"][None], lambda q, out: tt.paged_fp8_attention_decode_out(q, *s["kv"][:4], s["table"], s["pos"], out)),
+             (s["q"][None], lambda q, out: tt.paged_fp8_sparse_attention_decode_out(q, *s["kv"], s["table"], s["pos"], out, 3)),
+             (rows, lambda q, out: tt.chunked_fp8_attention_out(q, *s["kv"][:4], s["table"], start, out))]
+    for q, call in calls:
+        want = torch.empty_like(q)
+        call(q, want)
+        own = q.clone()
+        call(own, own)
+        assert torch.equal(own.view(torch.int16), want.view(torch.int16))
+
+        def views():
+            """(query, out, whether that can be served): two views of one memory."""
+            for dim in range(1, q.dim()):
+                size = q.shape[dim]
+                both = torch.cat([q, q], dim).contiguous()
+                yield both.narrow(dim, 0, size), both.narrow(dim, size, size), True
+                if size > 1:
+                    yield both.narrow(dim, size, size), both.narrow(dim, 1, size), False
+                    yield both.narrow(dim, 0, size), both.narrow(dim, 1, size), False
+            two = torch.stack([q, q], -2)
+            yield two[..., 0, :], two[..., 1, :], True
+            flat = torch.cat([q.flatten(), q.flatten()])
+            yield flat[: q.numel()].view(q.shape), flat[q.numel() :].view(q.shape), True
+            yield flat[: q.numel()].view(q.shape), flat[d : q.numel() + d].view(q.shape), False
+            yield flat[: q.numel()].view(q.shape), flat[8 : q.numel() + 8].view(q.shape), False
+            swapped = (q.shape[0], q.shape[2], q.shape[1], d)
+            yield flat[: q.numel()].view(q.shape), flat[: q.numel()].view(swapped).transpose(1, 2), False
+
+        for query, out, served in views():
+            if served:
+                query.copy_(q)
+                call(query, out)
+                assert torch.equal(out.contiguous().view(torch.int16), want.contiguous().view(torch.int16)) and torch.equal(query, q)
+            else:
+                with pytest.raises(ValueError, match="overlap"):
+                    call(query, out)

@@ -338,10 +338,40 @@ void paged_fill_fp8_cache_(const Tensor &k_cache, const Tensor &v_cache, const T
 // ---- attention --------------------------------------------------------------------------------------
 // An output handed in by the caller: [.., heads, head_size] bfloat16; what the kernels' stores cannot take is copied to.
 Tensor storable(const Tensor &out) { return has_rows(out, 4) ? out : at::empty(out.sizes(), out.options()); }
+// Whether `distance` elements lie between two elements of t, whose dimensions `dims` from `at` on are in order, the longest stride first, each stride
+// at least as long as what lies inside it.
+bool apart_by(const Tensor &t, int64_t distance, const c10::SmallVector<int64_t, 6> &dims, size_t at = 0) {
+  if (at == dims.size()) return distance == 0;
+  const int64_t stride = t.stride(dims[at]), size = t.size(dims[at]);
+  const int64_t below = distance / stride - (distance % stride < 0);
+  for (int64_t i = below; i <= below + 1; ++i)
+    if (std::abs(i) < size && apart_by(t, distance - i * stride, dims, at + 1)) return true;
+  return false;
+}
+// Whether a call that reads `query` while it writes `out`, of one shape, would find its results there: they have elements in common, and not each its own.
+// (out does not overlap itself.  True also where that is not looked into: views of one memory with different strides that reach into each other.)
+bool collide(const Tensor &out, const Tensor &query) {
+  if (!out.is_alias_of(query) || out.numel() == 0) return false;
+  const int64_t distance = query.storage_offset() - out.storage_offset();
+  int64_t out_reach = 0, query_reach = 0;
+  bool alike = true;
+  c10::SmallVector<int64_t, 6> dims;
+  for (int64_t i = 0; i < out.dim(); ++i) {
+    if (out.size(i) <= 1) continue;
+    out_reach += (out.size(i) - 1) * out.stride(i), query_reach += (query.size(i) - 1) * query.stride(i);
+    alike = alike && out.stride(i) == query.stride(i);
+    dims.push_back(i);
+  }
+  if (distance > out_reach || -distance > query_reach) return false;
+  if (!alike) return true;
+  std::sort(dims.begin(), dims.end(), [&](int64_t a, int64_t b) { return out.stride(a) > out.stride(b); });
+  return distance != 0 && apart_by(out, distance, dims);
+}
 void check_out(const Call &c, const Tensor &out, const Tensor &query) {
   c.type(out, at::kBFloat16, "out");
   single(c, out, "out");
   TORCH_CHECK_VALUE(out.sizes() == query.sizes(), c.name(), ": out must have the query's shape ", query.sizes(), ", got ", out.sizes());
+  TORCH_CHECK_VALUE(query.scalar_type() != at::kBFloat16 || !collide(out, query), c.name(), ": out and query must be one view or not overlap");
 }
 void check_query(const Call &c, const Tensor &query, const Cache &cache, const Tensor &pt, const Tensor &cur) {
   c.type(query, at::kBFloat16, "query");
