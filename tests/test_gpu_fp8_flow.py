@@ -402,8 +402,10 @@ def test_operands_at_odd_addresses():
     same(lambda kv, x: tt.paged_fp8_attention_decode(s["q"][None], *kv[:4], table, pos, x), sink)
 
 
-def test_outputs_in_the_memory_of_the_query():
+@pytest.mark.parametrize("form", ["few", "copies"])
+def test_outputs_in_the_memory_of_the_query(form, monkeypatch):
     """The query itself and views beside it are written; what would overwrite rows that are still to be read is refused."""
+    monkeypatch.setenv("TTPA_CHUNK_FORM", form)
     tt, s = torch.ops.tt, _state(13)
     users, hq, d = s["q"].shape
     g = torch.Generator().manual_seed(14)

@@ -189,3 +189,26 @@ def test_tangents_are_refused():
     table, pos = _table(4, 64).cuda(), torch.zeros(2, dtype=torch.int32, device="cuda")
     with fwd.dual_level(), pytest.raises(NotImplementedError, match="tangent"):
         torch.ops.tt.qk_norm_rope(fwd.make_dual(q, torch.ones_like(q)), q, table, pos)
+
+
+@pytest.mark.parametrize("hq, hk, d, rotary, tokens", [(40, 8, 128, 128, 1367), (64, 8, 128, 64, 911), (32, 32, 128, 128, 1025), (16, 8, 256, 256, 1366), (48, 8, 128, 128, 1171),
+                                                       (129, 8, 128, 96, 483), (90, 7, 64, 64, 1173), (21, 3, 256, 32, 1366), (64, 64, 64, 64, 1030)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_many_tokens_of_many_heads(hq, hk, d, rotary, tokens, interleaved):
+    """Several wavefronts per token with several groups of heads in each, the last of them full or not; also in place."""
+    g = torch.Generator().manual_seed(tokens + hq)
+    both = torch.randn(tokens, hq + hk + 1, d, generator=g).to(torch.bfloat16)
+    q, k = both[:, :hq], both[:, hq : hq + hk]
+    table = _table(300, rotary)
+    pos = torch.randint(-2, 305, (tokens,), generator=g, dtype=torch.int32)
+    qw, kw = (1 + 0.2 * torch.randn(d, generator=g) for _ in range(2))
+    on = both.cuda()
+    for weights in ((None, kw), (qw, kw.to(torch.bfloat16))):
+        w = [None if t is None else t.cuda() for t in weights]
+        args = (table.cuda(), pos.cuda(), *w, 1e-6, interleaved)
+        got = torch.ops.tt.qk_norm_rope(on[:, :hq], on[:, hq : hq + hk], *args)
+        _check(got[0].cpu(), q, weights[0], table, pos, 1e-6, interleaved)
+        _check(got[1].cpu(), k, weights[1], table, pos, 1e-6, interleaved)
+        own = on.clone()
+        torch.ops.tt.qk_norm_rope_(own[:, :hq], own[:, hq : hq + hk], *args)
+        assert torch.equal(own[:, :hq], got[0]) and torch.equal(own[:, hq : hq + hk], got[1]) and torch.equal(own[:, hq + hk :].cpu(), both[:, hq + hk :])
