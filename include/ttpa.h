@@ -679,7 +679,7 @@ int ttpa_paged_fp8_decode(void *out, int64_t out_user_stride, int64_t out_head_s
  * The decode over `kept_blocks` (at least 2) of each user's blocks, chosen for each KV head: the first, the one that holds cur_pos, and of the others
  * those with the largest
  *   score = max over the KV head's query heads of  sum_d  max(q_d, 0) * high_d + min(q_d, 0) * low_d
- * (a bound of q . k over the block), in 64 bits; of equal scores the lower column; a score that is NaN or +infinity counts as the
+ * (a bound of q . k over the block's keys as they were written, before their rounding to e4m3), in 64 bits; of equal scores the lower column; a score that is NaN or +infinity counts as the
  * largest.  columns [users, kv_heads, kept_blocks] receives the page-table columns in order, then -1.  A context of no more blocks is attended whole.
  * q and out are [users, q_heads, head_size] with users q_heads * head stride apart.
  */

@@ -4,7 +4,7 @@
 // A chunk is bound by its matrix products, 4 D q_heads operations per (row, key) pair, and every workgroup of 128 rows reads every key, so keys
 // are expanded once here and not once per workgroup; the copies cost 1 byte read and 2 written per element, at the rate of a large
 // copy: 22 us for 4 x 4608 keys of 8 heads (113 MB; 27 when every piece of 512 elements looked its block up), 13 for 8704 (53 MB).
-// The pass as a whole takes 292 us there, 298 before.
+// The pass as a whole takes 284 us there (where both were timed in turn, 292, and 298 with the piece-wise look-up).
 // The blocks are read by streaming loads and the copies written by ordinary stores: what follows reads them from the caches.
 //
 // The prefill kernels take keys by tiles of 64 and give what is behind the last row's own position weight zero, whatever it is, so it has to be

@@ -2,7 +2,7 @@
 //
 // Sparse form.  For every (user, KV head) the blocks of the context are scored by what their key bounds allow,
 //   score(block) = max over the group's heads of  sum_d  max(q_d, 0) high_d + min(q_d, 0) low_d,
-// an upper bound of q . k over the block's keys; the block that holds the newest token, the first block and the best of the others are
+// an upper bound of q . k over the block's keys as they were written (their rounding to e4m3 may pass it by a little); the block that holds the newest token, the first block and the best of the others are
 // attended, `kept` in all, of equal scores the lower column.  A choice flips with the last bit of a score, so scores are
 // sums in 64 bits: products of bfloat16 values are exact there and a sum of 512 of them keeps 28 bits to spare, so that neither
 // the order of the sum nor its split matters in practice.  But 64-bit sums for all blocks took 13 and 21 us (27 000 blocks with four heads, 46 000

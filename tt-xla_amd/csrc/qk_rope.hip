@@ -328,7 +328,7 @@ int launch_rope(const RopeArgs &a, hipStream_t st) {
     const int64_t waves = (int64_t)a.tokens * parts;
     qk_norm_rope_kernel<D, U><<<dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, st>>>(a, parts);
   };
-  // Few rows want to be everywhere at once; many, as many groups per wavefront as there are registers for, with no slots left over: its angles and
+  // Few rows want to be everywhere at once; many, three to five groups per wavefront, as many as leave no slot without a group, or else five: its angles and
   // weights are read once.  8192 tokens of 32 + 8 heads of 128 (168 MB), us a pass with 1 / 2 / 3 / 5 groups 44.1 / 41.4 / 36.8 / 32.5; with ordinary
   // stores 44.5 / 41.9 / 39.0 / 36.9.  (Those of few rows are ordinary: what is read next is read from L2.)
   int best = 1;
