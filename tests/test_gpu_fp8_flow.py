@@ -446,3 +446,30 @@ def test_outputs_in_the_memory_of_the_query(form, monkeypatch):
             else:
                 with pytest.raises(ValueError, match="overlap"):
                     call(query, out)
+
+
+def test_block_ids_and_starts_beyond_32_bits():
+    """Numbers that lose their upper half would name a block of the cache, or a start in it: they are outside, like other ids that are too large."""
+    tt, hq, hkv, d, bs = torch.ops.tt, 8, 2, 64, 32
+    cache, table, cur, q, g = _setup(2, hkv, hq // hkv, d, bs, [100, 70], 3)
+    bounds = _bounds(cache)
+    kv, b = [t.cuda() for t in cache], bounds.cuda()
+    before = [t.clone() for t in (*kv, b)]
+    for far in (1 << 32, -(1 << 32)):
+        ids = table.long() + far
+        x = torch.randn(2, hkv, d, generator=g).to(torch.bfloat16).cuda()
+        tt.paged_update_fp8_cache_(*kv, x[None], x[None], cur.cuda(), ids.cuda(), b)
+        prompt = torch.randn(2, hkv, 40, d, generator=g).to(torch.bfloat16).cuda()
+        tt.paged_fill_fp8_cache_(*kv, prompt, prompt, ids.cuda(), torch.arange(2).cuda(), b)
+        assert all(torch.equal(a.view(torch.uint8), c.view(torch.uint8)) for a, c in zip((*kv, b), before))
+        zeros = torch.zeros_like(table)  # what is outside the cache reads block 0
+        out = tt.paged_fp8_attention_decode(q.cuda()[None], *kv, ids.cuda(), cur.cuda())[0].cpu()
+        _check(out, q, cache, zeros, cur, d**-0.5)
+        out, cols = tt.paged_fp8_sparse_attention_decode(q.cuda()[None], *kv, b, ids.cuda(), cur.cuda(), 3)
+        _check_sparse(out[0].cpu(), cols.cpu(), q, cache, bounds, zeros, cur, 3, d**-0.5)
+    rows = torch.randn(2, hq, 20, d, generator=g).to(torch.bfloat16)
+    ids = table.clamp(min=0)
+    room = ids.shape[1] * bs
+    out = tt.chunked_fp8_attention(rows.cuda(), *kv, ids.cuda(), torch.tensor([1 << 32]).cuda()).cpu()
+    check_chunk(out, rows, cache, ids, room, d**-0.5)
+    assert torch.isnan(tt.chunked_fp8_attention(rows.cuda(), *kv, ids.cuda(), torch.tensor([-(1 << 32)]).cuda())).all()

@@ -87,11 +87,17 @@ Tensor indices(const Call &c, const Tensor &t, const char *what) {
   return (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong ? t : t.to(at::kLong)).contiguous();
 }
 int is_i64(const Tensor &t) { return t.scalar_type() == at::kLong; }
+// Whole numbers as 32-bit ones; what does not fit stays outside every table and cache.
+Tensor narrow(const Tensor &t) {
+  if (t.scalar_type() == at::kInt) return t;
+  if (t.scalar_type() != at::kLong) return t.to(at::kInt);
+  return t.clamp(std::numeric_limits<int32_t>::min(), std::numeric_limits<int32_t>::max()).to(at::kInt);
+}
 Tensor table(const Call &c, const Tensor &t) {
   c.see(t, "page_table");
   TORCH_CHECK_VALUE(t.dim() == 2 && t.size(1) > 0, c.name(), ": page_table must be [users, blocks_per_user]");
   TORCH_CHECK_VALUE(at::isIntegralType(t.scalar_type(), false), c.name(), ": page_table must hold whole numbers");
-  const Tensor p = t.scalar_type() == at::kInt ? t : t.to(at::kInt);
+  const Tensor p = narrow(t);
   return p.size(1) == 1 || p.stride(1) == 1 ? p : p.contiguous();
 }
 const int32_t *int_ptr(const Tensor &t) { return static_cast<const int32_t *>(t.data_ptr()); }
@@ -489,7 +495,7 @@ void chunk_into(const Call &c, const Tensor &out, const Tensor &query, const Cac
   TORCH_CHECK_VALUE(most_keys >= 0, c.name(), ": most_keys must not be negative");
   const int64_t users = query.size(0), hq = query.size(1), s = query.size(2);
   if (users == 0 || s == 0) return;
-  const Tensor start = chunk_start.scalar_type() == at::kInt ? chunk_start : chunk_start.to(at::kInt);
+  const Tensor start = narrow(chunk_start);
   const Tensor q = rows(query), target = storable(out);
   // as many users at a time as the copies of their blocks have room for
   const auto bytes_of = [&](int64_t n) {
