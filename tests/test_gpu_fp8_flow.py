@@ -473,3 +473,53 @@ def test_block_ids_and_starts_beyond_32_bits():
     out = tt.chunked_fp8_attention(rows.cuda(), *kv, ids.cuda(), torch.tensor([1 << 32]).cuda()).cpu()
     check_chunk(out, rows, cache, ids, room, d**-0.5)
     assert torch.isnan(tt.chunked_fp8_attention(rows.cuda(), *kv, ids.cuda(), torch.tensor([-(1 << 32)]).cuda())).all()
+
+
+@pytest.mark.parametrize("sparse", [None, 3])
+def test_captured_passes_of_the_backend(sparse):
+    """A prompt, a continuation chunk of an owning and of a sharing layer and a step in one graph, replayed with other tokens, places and starts;
+    every replay against the eager passes on a copy."""
+    from tt_xla_amd import TTAttentionBackendImpl, TTMetadata
+
+    hq, hkv, d, bs, users, s = 8, 2, 128, 32, 2, 64
+    g = torch.Generator().manual_seed(21)
+    cache, table, _, _, _ = _setup(users, hkv, hq // hkv, d, bs, [10 * bs] * users, 5)
+    kv, table = [t.cuda() for t in (*cache, _bounds(cache))], table.cuda()
+    fill, rows, start = table[:, :2].contiguous(), torch.arange(users, dtype=torch.int32).cuda(), torch.tensor([4 * bs], dtype=torch.int32).cuda()
+    place, pos = table[:, 4:6].contiguous(), torch.tensor([6 * bs, 7 * bs + 5], dtype=torch.int32).cuda()
+    own = TTAttentionBackendImpl(hq, d, d**-0.5, hkv, kv_cache_dtype="fp8", sparse_kept_blocks=sparse)
+    sharing = TTAttentionBackendImpl(hq, d, d**-0.5, hkv, kv_cache_dtype="fp8", kv_sharing_target_layer_name="other")
+    tokens = {n: [torch.randn(users * n, h * d, generator=g).to(torch.bfloat16).cuda() for h in (hq, hkv, hkv)] for n in (1, s)}
+
+    def passes(kv):
+        out = [torch.zeros(users * n, hq * d, dtype=torch.bfloat16, device="cuda") for n in (s, s, s, 1)]
+        one = dict(page_table=table, batch_idx=rows, num_users=users)
+        own.forward(None, *tokens[s], kv, TTMetadata(fill_page_table=fill, **one), output=out[0])
+        own.forward(None, *tokens[s], kv, TTMetadata(fill_page_table=place, chunk_start_idx=start, **one), output=out[1])
+        sharing.forward(None, *tokens[s], kv, TTMetadata(fill_page_table=place, chunk_start_idx=start, **one), output=out[2])
+        own.forward(None, *tokens[1], kv, TTMetadata(page_table=table, cache_position=pos, num_users=users), output=out[3])
+        return out
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        passes([t.clone() for t in kv])
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = passes(kv)
+    for n, at in enumerate((4, 2, 6, 0, 8)):
+        start.fill_(at * bs)
+        place.copy_(table[:, at : at + 2])
+        pos.copy_(torch.tensor([n * 40, -1 if n == 2 else 200 + n]))
+        for ts in tokens.values():
+            for t in ts:
+                t.copy_(torch.randn(t.shape, generator=g).to(torch.bfloat16))
+        copy = [t.clone() for t in kv]
+        graph.replay()
+        want = passes(copy)
+        if n % 2:
+            torch.cuda.synchronize()
+        assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(outs, want)), n
+        assert torch.equal(want[1], want[2])  # (the sharing layer sees what the owner has written)
+        assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(kv, copy))
