@@ -694,7 +694,8 @@ int ttpa_paged_fp8_sparse_decode(void *out, int64_t out_head_stride, int32_t *co
 /*
  * The paged causal form of ttpa_sdpa_prefill (a prompt's continuation chunk) over the 8-bit cache; block_size a multiple of 32.  most_keys > 0: a
  * bound of chunk_start + q_len that the caller knows: the pass takes the page table as if it ended with the block of key most_keys - 1, and the
- * workspace has room for no more.
+ * workspace has room for no more.  As in ttpa_sdpa_prefill, a NaN among the chunk's own values also reaches rows in front of its token that share a
+ * tile with it: their weight for it is zero, and zero times NaN is NaN.
  */
 int64_t ttpa_chunked_fp8_attention_workspace_bytes(int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t q_len, int32_t head_size,
                                                    int32_t block_size, int32_t table_width, int64_t most_keys);
