@@ -64,7 +64,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(few_per_cu<
   constexpr int KBLK = TILE / 16, KP = D / 64, DBLK = D / 16, PSTEPS = TILE / 32;
   constexpr int CPR = D / 16, RPL = 16 / CPR, NL = RUN / RPL;
   extern __shared__ __attribute__((aligned(16))) uint8_t tiles[];
-  __shared__ float2 s_ml[4][ROWS];  // maximum and sum (of two arrays [4][ROWS] the compiler, ROCm 7.2, stored both by one two-address LDS instruction with a wrong second offset)
+  __shared__ float2 s_ml[4][ROWS];  // maximum and sum (of two arrays [4][ROWS] the compiler, ROCm 7.2, put two stores into a two-address LDS instruction with a wrong offset for one: the maxima of the first 16 rows went elsewhere)
   // workgroup -> (user, KV head, part) and block of rows, the blocks of one unit eight workgroups apart
   const uint32_t span = 8u * a.row_blocks, set = blockIdx.x / span, in_set = blockIdx.x - set * span;
   const int rb = (int)(in_set >> 3), unit = (int)(set * 8 + (in_set & 7));
