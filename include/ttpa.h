@@ -706,6 +706,50 @@ int ttpa_chunked_fp8_attention(void *out, int64_t out_batch_stride, int64_t out_
                                int32_t block_size, int32_t table_width, int32_t num_blocks, float scale, int64_t most_keys, void *workspace,
                                int64_t workspace_bytes, void *stream);
 
+/*
+ * ttpa_qk_norm_rope with positions on several axes (time, height, width): positions [axes][tokens], an axis positions_axis_stride numbers from the
+ * next, and pair_axes [rotary / 2] int32, the axis whose position turns a pair of features; axes from 1 to 4.  Row p of cos_sin holds what position p turns
+ * every pair by, whatever its axis.  A pair whose axis does not exist, or whose position is outside the table, is not turned.
+ */
+int ttpa_qk_norm_rope_axes(void *q_out, int64_t q_out_token_stride, int64_t q_out_head_stride, void *k_out, int64_t k_out_token_stride,
+                           int64_t k_out_head_stride, const void *q, int64_t q_token_stride, int64_t q_head_stride, const void *k,
+                           int64_t k_token_stride, int64_t k_head_stride, const void *cos_sin, int cos_sin_is_f32, int64_t cos_sin_row_stride,
+                           int64_t max_positions, const void *positions, int positions_is_i64, int64_t positions_axis_stride, int32_t axes,
+                           const int32_t *pair_axes, const void *q_weight, const void *k_weight, int weights_are_f32, float eps, int32_t tokens,
+                           int32_t q_heads, int32_t k_heads, int32_t head_size, int32_t rotary, int interleaved, void *stream);
+
+/*
+ * Attention of q_len tokens per batch entry to an encoder's states in a paged bfloat16 cache: all tokens see keys 0 .. encoder_lens[b] - 1 (no causal
+ * limit); of a length of zero or less the result is zeros, a length beyond the page table's room counts as that.  What the cache holds behind the last
+ * key is not used, whatever it is.  Ids outside [0, num_blocks) read block 0.  block_size a multiple of 32, head sizes 64, 128 and 256, scale > 0.
+ * most_keys > 0: a bound of the lengths that the caller knows; the pass takes the page table as if it ended with the block of key most_keys - 1.
+ */
+int64_t ttpa_paged_cross_attention_workspace_bytes(int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t q_len, int32_t head_size,
+                                                   int32_t block_size, int32_t table_width, int64_t most_keys);
+int ttpa_paged_cross_attention(void *out, int64_t out_batch_stride, int64_t out_head_stride, int64_t out_token_stride, const void *q,
+                               int64_t q_batch_stride, int64_t q_head_stride, int64_t q_token_stride, const void *k_cache, const void *v_cache,
+                               const int32_t *page_table, int64_t page_table_row_stride, const void *encoder_lens, int lens_is_i64, int32_t batch,
+                               int32_t q_heads, int32_t kv_heads, int32_t q_len, int32_t head_size, int32_t block_size, int32_t table_width,
+                               int32_t num_blocks, float scale, int64_t most_keys, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * Copies blocks inside caches: of every cache, n_caches tensors [num_blocks][block_bytes], block source_blocks[j] to target_blocks[j], as if j went from 0 on
+ * (a block may be the target of one pair and the source of a later one).  Pairs with an id outside [0, num_blocks) are skipped.  caches_host is an array of
+ * device pointers in host memory, read before the call returns.
+ */
+int ttpa_copy_cache_blocks(void *const *caches_host, int32_t n_caches, int64_t block_bytes, const int32_t *source_blocks, const int32_t *target_blocks,
+                           int32_t pairs, int32_t num_blocks, void *stream);
+
+/*
+ * Compacts sequences inside caches [num_blocks][heads][block_size] of rows of row_bytes (a multiple of 16): in every cache and head, position first[u] + i
+ * of user u receives what position kept[u][i] held before the call, i < kept_lens[u] (at most most_kept).  An entry below its own place (tokens do not move
+ * back), outside the page table's room or in a block outside the caches is skipped.  Other positions stay as they are.  first: null for zeros.  Pages that
+ * the call writes belong to one user and occur once in its row.
+ */
+int ttpa_keep_cache_tokens(void *const *caches_host, int32_t n_caches, const int32_t *page_table, int64_t page_table_row_stride, const int32_t *kept,
+                           int64_t kept_row_stride, const int32_t *kept_lens, const int32_t *first, int32_t users, int32_t most_kept, int32_t heads,
+                           int32_t row_bytes, int32_t block_size, int32_t table_width, int32_t num_blocks, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

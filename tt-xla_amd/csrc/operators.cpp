@@ -1,4 +1,4 @@
-// torch.ops.tt.* around the 8-bit cache and the rotation, over the C ABI.
+// torch.ops.tt.* around the 8-bit cache, the rotation, cross attention and moves inside caches, over the C ABI.
 //
 // Registered from C++ because most of these calls are a few microseconds of GPU time: through Python views, checks and ctypes a call
 // is issued in 15 .. 30 us, from here in 3 .. 5.  Every operator runs on its tensors' device, on that device's current stream; scratch comes from
@@ -15,6 +15,7 @@
 #include <cmath>
 #include <limits>
 #include <optional>
+#include <vector>
 
 #include "ttpa.h"
 
@@ -188,7 +189,8 @@ struct Cache {
 struct Rotation {
   Tensor angles, positions, qw, kw;
   int weights_f32 = 0;
-  Rotation(const Call &c, const Tensor &query, const Tensor &key, const Tensor &cos_sin, const Tensor &pos, const OptTensor &q_weight,
+  // (pos: a position per token, or none: there are several, Axes)
+  Rotation(const Call &c, const Tensor &query, const Tensor &key, const Tensor &cos_sin, const OptTensor &pos, const OptTensor &q_weight,
            const OptTensor &k_weight) {
     c.type(query, at::kBFloat16, "query");
     c.type(key, at::kBFloat16, "key");
@@ -201,8 +203,10 @@ struct Rotation {
     TORCH_CHECK_VALUE(cos_sin.dim() == 2 && cos_sin.size(0) > 0 && cos_sin.size(1) <= query.size(2) && cos_sin.size(1) > 0 && cos_sin.size(1) % 16 == 0,
                       c.name(), ": cos_sin must be [positions, rotary], rotary a multiple of 16 up to the head size");
     angles = rows(cos_sin);
-    positions = indices(c, pos, "positions");
-    TORCH_CHECK_VALUE(positions.dim() == 1 && positions.size(0) == query.size(0), c.name(), ": positions must hold one number per token");
+    if (pos) {
+      positions = indices(c, *pos, "positions");
+      TORCH_CHECK_VALUE(positions.dim() == 1 && positions.size(0) == query.size(0), c.name(), ": positions must hold one number per token");
+    }
     c.see(q_weight, "q_weight");
     c.see(k_weight, "k_weight");
     bool f32 = false;
@@ -252,6 +256,62 @@ void qk_norm_rope_(const Tensor &query, const Tensor &key, const Tensor &cos_sin
   TORCH_CHECK_VALUE(!overlap(query, key), c.name(), ": query and key must not overlap");
   const Tensor q = rows(query), k = rows(key);
   turn(c, r, q, k, q, k, eps, interleaved);
+  if (!q.is_same(query)) query.copy_(q);
+  if (!k.is_same(key)) key.copy_(k);
+  written(query), written(key);
+}
+
+// ---- the same with positions on several axes ----------------------------------------------------------
+// `positions` [axes, tokens] and the axis of every pair of features.
+struct Axes {
+  Tensor positions, pairs;
+  Axes(const Call &c, const Tensor &query, const Tensor &cos_sin, const Tensor &pos, const Tensor &pair_axes) {
+    TORCH_CHECK_VALUE(pos.dim() == 2 && pos.size(0) > 0, c.name(), ": positions must be [axes, tokens]");
+    TORCH_CHECK_VALUE(pos.size(0) <= 4, c.name(), ": positions on up to 4 axes are supported, got ", pos.size(0));
+    TORCH_CHECK_VALUE(query.dim() != 3 || pos.size(1) == query.size(0), c.name(), ": positions must hold one number per axis and token");
+    c.see(pos, "positions");
+    TORCH_CHECK_VALUE(at::isIntegralType(pos.scalar_type(), false), c.name(), ": positions must hold whole numbers");
+    positions = pos.scalar_type() == at::kInt || pos.scalar_type() == at::kLong ? pos : pos.to(at::kLong);
+    if (positions.size(1) > 1 && positions.stride(1) != 1) positions = positions.contiguous();
+    c.see(pair_axes, "pair_axes");
+    TORCH_CHECK_VALUE(at::isIntegralType(pair_axes.scalar_type(), false), c.name(), ": pair_axes must hold whole numbers");
+    TORCH_CHECK_VALUE(pair_axes.dim() == 1 && cos_sin.dim() == 2 && 2 * pair_axes.size(0) == cos_sin.size(1), c.name(),
+                      ": pair_axes must hold one axis for each of the rotary / 2 pairs");
+    pairs = compact(narrow(pair_axes));
+  }
+};
+
+void turn_axes(const Call &c, const Rotation &r, const Axes &x, const Tensor &q_out, const Tensor &k_out, const Tensor &q, const Tensor &k, double eps,
+               bool interleaved) {
+  ok("ttpa_qk_norm_rope_axes",
+     ttpa_qk_norm_rope_axes(q_out.data_ptr(), step_of(q_out, 0), step_of(q_out, 1), k_out.data_ptr(), step_of(k_out, 0), step_of(k_out, 1), q.data_ptr(),
+                            step_of(q, 0), step_of(q, 1), k.data_ptr(), step_of(k, 0), step_of(k, 1), r.angles.data_ptr(), r.f32(),
+                            step_of(r.angles, 0), r.angles.size(0), x.positions.data_ptr(), is_i64(x.positions), step_of(x.positions, 0),
+                            i32(x.positions.size(0)), int_ptr(x.pairs), r.q_weight(), r.k_weight(), r.weights_f32, (float)eps, i32(q.size(0)),
+                            i32(q.size(1)), i32(k.size(1)), i32(q.size(2)), i32(r.angles.size(1)), interleaved, c.stream()));
+}
+
+std::tuple<Tensor, Tensor> qk_norm_rope_axes(const Tensor &query, const Tensor &key, const Tensor &cos_sin, const Tensor &positions,
+                                             const Tensor &pair_axes, const OptTensor &q_weight, const OptTensor &k_weight, double eps,
+                                             bool interleaved) {
+  const Call c("tt::qk_norm_rope_axes", query);
+  const Axes x(c, query, cos_sin, positions, pair_axes);
+  const Rotation r(c, query, key, cos_sin, std::nullopt, q_weight, k_weight);
+  const Tensor q_out = c.fresh(query.sizes()), k_out = c.fresh(key.sizes());
+  if (query.size(0)) turn_axes(c, r, x, q_out, k_out, rows(query), rows(key), eps, interleaved);
+  return {q_out, k_out};
+}
+
+void qk_norm_rope_axes_(const Tensor &query, const Tensor &key, const Tensor &cos_sin, const Tensor &positions, const Tensor &pair_axes,
+                        const OptTensor &q_weight, const OptTensor &k_weight, double eps, bool interleaved) {
+  const Call c("tt::qk_norm_rope_axes_", query);
+  const Axes x(c, query, cos_sin, positions, pair_axes);
+  const Rotation r(c, query, key, cos_sin, std::nullopt, q_weight, k_weight);
+  if (query.size(0) == 0) return;
+  single(c, query, "query"), single(c, key, "key");
+  TORCH_CHECK_VALUE(!overlap(query, key), c.name(), ": query and key must not overlap");
+  const Tensor q = rows(query), k = rows(key);
+  turn_axes(c, r, x, q, k, q, k, eps, interleaved);
   if (!q.is_same(query)) query.copy_(q);
   if (!k.is_same(key)) key.copy_(k);
   written(query), written(key);
@@ -537,6 +597,129 @@ void chunked_fp8_attention_out(const Tensor &query, const Tensor &k_cache, const
   written(out);
 }
 
+// ---- cross attention --------------------------------------------------------------------------------
+void cross_into(const Call &c, const Tensor &out, const Tensor &query, const Tensor &k_cache, const Tensor &v_cache, const Tensor &page_table,
+                const Tensor &encoder_lens, const std::optional<double> &scale, int64_t most_keys) {
+  c.type(query, at::kBFloat16, "query");
+  for (const Tensor *t : {&k_cache, &v_cache}) {
+    c.type(*t, at::kBFloat16, "a cache");
+    TORCH_CHECK_VALUE(t->dim() == 4 && t->is_contiguous() && t->numel() > 0, c.name(),
+                      ": a cache must be a contiguous [num_blocks, kv_heads, block_size, head_size] tensor");
+  }
+  TORCH_CHECK_VALUE(k_cache.sizes() == v_cache.sizes(), c.name(), ": K and V caches must have the same shape");
+  const int64_t nb = k_cache.size(0), hkv = k_cache.size(1), bs = k_cache.size(2), d = k_cache.size(3);
+  TORCH_CHECK_VALUE(query.dim() == 4 && query.size(3) == d && query.size(1) > 0 && query.size(1) % hkv == 0, c.name(), ": query ", query.sizes(),
+                    " must be [users, heads, tokens, head_size] and match the caches' kv_heads=", hkv, ", head_size=", d);
+  const Tensor pt = table(c, page_table), lens = indices(c, encoder_lens, "encoder_lens");
+  const int64_t users = query.size(0), hq = query.size(1), s = query.size(2);
+  TORCH_CHECK_VALUE(pt.size(0) == users && lens.dim() == 1 && lens.size(0) == users, c.name(), ": page_table / encoder_lens must have one row per user");
+  TORCH_CHECK_VALUE(!scale || *scale > 0, c.name(), ": scale must be positive");
+  TORCH_CHECK_VALUE(most_keys >= 0, c.name(), ": most_keys must not be negative");
+  if (users == 0 || s == 0) return;
+  const Tensor q = rows(query), target = storable(out), k = aligned16(k_cache) ? k_cache : compact(k_cache), v = aligned16(v_cache) ? v_cache : compact(v_cache);
+  const int64_t bytes = ttpa_paged_cross_attention_workspace_bytes(i32(users), i32(hq), i32(hkv), i32(s), i32(d), i32(bs), i32(pt.size(1)), most_keys);
+  const Tensor ws = c.scratch(bytes);
+  ok("ttpa_paged_cross_attention",
+     ttpa_paged_cross_attention(target.data_ptr(), step_of(target, 0), step_of(target, 1), step_of(target, 2), q.data_ptr(), step_of(q, 0), step_of(q, 1),
+                                step_of(q, 2), k.data_ptr(), v.data_ptr(), int_ptr(pt), step_of(pt, 0), lens.data_ptr(), is_i64(lens), i32(users),
+                                i32(hq), i32(hkv), i32(s), i32(d), i32(bs), i32(pt.size(1)), i32(nb), scale_of(scale, d), most_keys, ws.data_ptr(),
+                                bytes, c.stream()));
+  if (!target.is_same(out)) out.copy_(target);
+}
+
+Tensor paged_cross_attention(const Tensor &query, const Tensor &key, const Tensor &value, const Tensor &page_table, const Tensor &encoder_lens,
+                             std::optional<double> scale, int64_t most_keys) {
+  const Call c("tt::paged_cross_attention", query);
+  const Tensor out = at::empty_like(query);  // keeps the query's (possibly token-major) strides
+  cross_into(c, out, query, key, value, page_table, encoder_lens, scale, most_keys);
+  return out;
+}
+
+void paged_cross_attention_out(const Tensor &query, const Tensor &key, const Tensor &value, const Tensor &page_table, const Tensor &encoder_lens,
+                               const Tensor &out, std::optional<double> scale, int64_t most_keys) {
+  const Call c("tt::paged_cross_attention_out", query);
+  check_out(c, out, query);
+  cross_into(c, out, query, key, value, page_table, encoder_lens, scale, most_keys);
+  written(out);
+}
+
+// ---- moves inside caches ----------------------------------------------------------------------------
+// Tensors that one call writes, blocks on dim 0: contiguous, as many blocks each, none of them in another's memory.
+void check_written_caches(const Call &c, at::TensorList caches) {
+  std::vector<std::pair<const char *, const char *>> spans;
+  spans.reserve(caches.size());
+  for (const Tensor &t : caches) {
+    c.see(t, "a cache");
+    TORCH_CHECK_VALUE(t.dim() >= 2 && t.is_contiguous() && t.size(0) == caches[0].size(0), c.name(),
+                      ": caches must be contiguous tensors of equally many blocks (dim 0), got ", t.sizes());
+    const char *p = static_cast<const char *>(t.data_ptr());
+    if (t.numel()) spans.emplace_back(p, p + t.nbytes());
+  }
+  std::sort(spans.begin(), spans.end());
+  for (size_t i = 1; i < spans.size(); ++i)
+    TORCH_CHECK_VALUE(spans[i - 1].second <= spans[i].first, c.name(), ": caches must not share memory");
+}
+Tensor list_of_ids(const Call &c, const Tensor &t, const char *what) {
+  c.see(t, what);
+  TORCH_CHECK_VALUE(at::isIntegralType(t.scalar_type(), false) && t.dim() == 1, c.name(), ": ", what, " must be a list of whole numbers");
+  return narrow(t).contiguous();
+}
+
+void copy_cache_blocks_(at::TensorList caches, const Tensor &source_blocks, const Tensor &target_blocks) {
+  TORCH_CHECK_VALUE(!caches.empty(), "tt::copy_cache_blocks_: no caches");
+  const Call c("tt::copy_cache_blocks_", caches[0]);
+  check_written_caches(c, caches);
+  const Tensor source = list_of_ids(c, source_blocks, "source_blocks"), target = list_of_ids(c, target_blocks, "target_blocks");
+  TORCH_CHECK_VALUE(source.size(0) == target.size(0), c.name(), ": as many source_blocks as target_blocks, got ", source.size(0), " and ", target.size(0));
+  const int64_t nb = caches[0].size(0);
+  if (source.size(0) == 0 || nb == 0) return;
+  std::vector<std::pair<int64_t, void *>> of_size;  // a launch takes caches whose blocks are of one size
+  of_size.reserve(caches.size());
+  for (const Tensor &t : caches)
+    if (t.numel()) of_size.emplace_back((int64_t)t.nbytes() / nb, t.data_ptr());
+  std::stable_sort(of_size.begin(), of_size.end(), [](const auto &x, const auto &y) { return x.first > y.first; });
+  std::vector<void *> some;
+  some.reserve(of_size.size());
+  for (size_t i = 0; i < of_size.size();) {
+    const int64_t bytes = of_size[i].first;
+    some.clear();
+    for (; i < of_size.size() && of_size[i].first == bytes; ++i) some.push_back(of_size[i].second);
+    ok("ttpa_copy_cache_blocks",
+       ttpa_copy_cache_blocks(some.data(), i32(some.size()), bytes, int_ptr(source), int_ptr(target), i32(source.size(0)), i32(nb), c.stream()));
+  }
+  for (const Tensor &t : caches) written(t);
+}
+
+void keep_cache_tokens_(at::TensorList caches, const Tensor &page_table, const Tensor &kept, const Tensor &kept_lens, const OptTensor &first) {
+  TORCH_CHECK_VALUE(!caches.empty(), "tt::keep_cache_tokens_: no caches");
+  const Call c("tt::keep_cache_tokens_", caches[0]);
+  check_written_caches(c, caches);
+  for (const Tensor &t : caches) {
+    TORCH_CHECK_NOT_IMPLEMENTED(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf, c.name(), " moves rows of bfloat16 or float16 caches, not of ",
+                                t.scalar_type(), " ones (whose rows share scales)");
+    TORCH_CHECK_VALUE(t.dim() == 4 && t.sizes() == caches[0].sizes(), c.name(), ": caches must be [num_blocks, kv_heads, block_size, head_size] of one shape");
+  }
+  const Tensor &one = caches[0];
+  const Tensor pt = table(c, page_table);
+  c.see(kept, "kept");
+  TORCH_CHECK_VALUE(at::isIntegralType(kept.scalar_type(), false) && kept.dim() == 2 && kept.size(0) == pt.size(0), c.name(),
+                    ": kept must be whole numbers [users, entries], users as page_table's");
+  Tensor entries = narrow(kept);
+  if (entries.size(1) > 1 && entries.stride(1) != 1) entries = entries.contiguous();
+  const Tensor lens = list_of_ids(c, kept_lens, "kept_lens");
+  const Tensor from = first ? list_of_ids(c, *first, "first") : Tensor();
+  TORCH_CHECK_VALUE(lens.size(0) == pt.size(0) && (!first || from.size(0) == pt.size(0)), c.name(), ": kept_lens and first must have one number per user");
+  if (one.numel() == 0 || pt.size(0) == 0 || entries.size(1) == 0) return;
+  std::vector<void *> all;
+  all.reserve(caches.size());
+  for (const Tensor &t : caches) all.push_back(t.data_ptr());
+  ok("ttpa_keep_cache_tokens",
+     ttpa_keep_cache_tokens(all.data(), i32(all.size()), int_ptr(pt), step_of(pt, 0), int_ptr(entries), step_of(entries, 0), int_ptr(lens),
+                            first ? int_ptr(from) : nullptr, i32(pt.size(0)), i32(entries.size(1)), i32(one.size(1)), i32(one.size(3) * 2), i32(one.size(2)),
+                            i32(pt.size(1)), i32(one.size(0)), c.stream()));
+  for (const Tensor &t : caches) written(t);
+}
+
 #define TT_ROPE "Tensor cos_sin, Tensor positions"
 #define TT_CACHE "Tensor k_cache, Tensor v_cache, Tensor k_scales, Tensor v_scales"
 #define TT_CACHE_W "Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) k_scales, Tensor(d!) v_scales"
@@ -546,6 +729,16 @@ TORCH_LIBRARY_FRAGMENT(tt, m) {
         "bool interleaved=False) -> (Tensor, Tensor)");
   m.def("qk_norm_rope_(Tensor(a!) query, Tensor(b!) key, " TT_ROPE ", Tensor? q_weight=None, Tensor? k_weight=None, float eps=1e-06, "
         "bool interleaved=False) -> ()");
+  m.def("qk_norm_rope_axes(Tensor query, Tensor key, " TT_ROPE ", Tensor pair_axes, Tensor? q_weight=None, Tensor? k_weight=None, "
+        "float eps=1e-06, bool interleaved=False) -> (Tensor, Tensor)");
+  m.def("qk_norm_rope_axes_(Tensor(a!) query, Tensor(b!) key, " TT_ROPE ", Tensor pair_axes, Tensor? q_weight=None, Tensor? k_weight=None, "
+        "float eps=1e-06, bool interleaved=False) -> ()");
+  m.def("paged_cross_attention(Tensor query, Tensor key, Tensor value, Tensor page_table, Tensor encoder_lens, float? scale=None, "
+        "int most_keys=0) -> Tensor");
+  m.def("paged_cross_attention_out(Tensor query, Tensor key, Tensor value, Tensor page_table, Tensor encoder_lens, Tensor(a!) out, "
+        "float? scale=None, int most_keys=0) -> ()");
+  m.def("copy_cache_blocks_(Tensor(a!)[] caches, Tensor source_blocks, Tensor target_blocks) -> ()");
+  m.def("keep_cache_tokens_(Tensor(a!)[] caches, Tensor page_table, Tensor kept, Tensor kept_lens, Tensor? first=None) -> ()");
   m.def("qk_norm_rope_update_fp8_(Tensor query, Tensor key, Tensor value, " TT_ROPE ", " TT_CACHE_W ", Tensor page_table, "
         "Tensor? q_weight=None, Tensor? k_weight=None, Tensor(e!)? key_bounds=None, float eps=1e-06, bool interleaved=False) -> Tensor");
   m.def("paged_update_fp8_cache_(" TT_CACHE_W ", Tensor k_fill, Tensor v_fill, Tensor update_indices, Tensor page_table, "
@@ -569,6 +762,12 @@ TORCH_LIBRARY_FRAGMENT(tt, m) {
 TORCH_LIBRARY_IMPL(tt, CUDA, m) {
   m.impl("qk_norm_rope", &qk_norm_rope);
   m.impl("qk_norm_rope_", &qk_norm_rope_);
+  m.impl("qk_norm_rope_axes", &qk_norm_rope_axes);
+  m.impl("qk_norm_rope_axes_", &qk_norm_rope_axes_);
+  m.impl("paged_cross_attention", &paged_cross_attention);
+  m.impl("paged_cross_attention_out", &paged_cross_attention_out);
+  m.impl("copy_cache_blocks_", &copy_cache_blocks_);
+  m.impl("keep_cache_tokens_", &keep_cache_tokens_);
   m.impl("qk_norm_rope_update_fp8_", &qk_norm_rope_update_fp8_);
   m.impl("paged_update_fp8_cache_", &paged_update_fp8_cache_);
   m.impl("paged_fill_fp8_cache_", &paged_fill_fp8_cache_);

@@ -1,0 +1,266 @@
+// Moves inside paged caches, for all layers in one call: copies of whole blocks (forks of sequences, moves of pages) and compaction of sequences
+// (chosen tokens move together).  Bytes are moved as they are, so any element type will do.  Both are bound by memory: read once, written once.
+#include "common.h"
+
+#include <algorithm>
+
+namespace ttpa {
+namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kMostCaches = 192;        // of one launch: their addresses are arguments
+constexpr int kMostPairs = 4096;        // of one launch: a longer list takes several, one after the other
+constexpr int kMostMarks = 1 << 18;     // blocks of a cache that a workgroup can mark (32 KiB of LDS)
+constexpr int kThreads = 256, kChunks = 4, kAtOnce = 4;  // 16-byte chunks of a block per thread, pairs on their way at a time
+
+struct CopyArgs {
+  uint8_t *caches[kMostCaches];
+  const int32_t *source, *target;
+  int pairs, nb, parts;
+  int64_t block_bytes;
+};
+
+__device__ __forceinline__ bool copies(const CopyArgs &a, int s, int t) { return (unsigned)s < (unsigned)a.nb && (unsigned)t < (unsigned)a.nb && s != t; }
+
+// Whether a block is the target of two pairs, or of one and the source of another: only then does the order of the pairs matter.
+__device__ __forceinline__ bool order_matters(const CopyArgs &a, uint32_t *marks) {
+  if (a.pairs == 1) return false;
+  const int lane = threadIdx.x & 63;
+  if (a.pairs <= 64) {
+    int s = -1, t = -1;
+    if (lane < a.pairs) s = a.source[lane], t = a.target[lane];
+    const bool mine = lane < a.pairs && copies(a, s, t);
+    bool found = false;
+    for (int i = 0; i < a.pairs; ++i) {
+      const int other = __builtin_amdgcn_readlane(t, i), live = __builtin_amdgcn_readlane((int)mine, i);
+      found = found || (live && mine && lane != i && (s == other || t == other));
+    }
+    return __builtin_amdgcn_ballot_w64(found) != 0;
+  }
+  __shared__ int s_found;
+  if (threadIdx.x == 0) s_found = 0;
+  for (int i = threadIdx.x; i < (a.nb + 31) / 32; i += kThreads) marks[i] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.pairs; i += kThreads) {
+    const int s = a.source[i], t = a.target[i];
+    if (copies(a, s, t) && (atomicOr(marks + (t >> 5), 1u << (t & 31)) >> (t & 31) & 1u)) s_found = 1;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.pairs; i += kThreads) {
+    const int s = a.source[i], t = a.target[i];
+    if (copies(a, s, t) && (marks[s >> 5] >> (s & 31) & 1u)) s_found = 1;
+  }
+  __syncthreads();
+  return s_found != 0;
+}
+
+// A workgroup has kThreads * kChunks chunks of every block of one cache, and every `parts`-th run of kAtOnce pairs.  A thread has the same bytes of every block,
+// so pairs that depend on each other are its own business: where the order matters, the workgroups of part 0 take all pairs one by one.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void copy_blocks_kernel(CopyArgs a) {
+  extern __shared__ uint32_t marks[];
+  const int part = blockIdx.z;
+  const bool ordered = order_matters(a, marks);
+  if (ordered && part > 0) return;
+  uint8_t *const cache = a.caches[blockIdx.y];
+  const int64_t first = ((int64_t)blockIdx.x * (kThreads * kChunks) + threadIdx.x) * (int64_t)sizeof(T);
+  constexpr int kStep = kThreads * (int)sizeof(T);
+  if (ordered) {
+    for (int j = 0; j < a.pairs; ++j) {
+      const int s = a.source[j], t = a.target[j];
+      if (!copies(a, s, t)) continue;
+      T x[kChunks];
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c)
+        if (first + c * kStep < a.block_bytes) x[c] = *reinterpret_cast<const T *>(cache + s * a.block_bytes + first + c * kStep);
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c)
+        if (first + c * kStep < a.block_bytes) *reinterpret_cast<T *>(cache + t * a.block_bytes + first + c * kStep) = x[c];
+    }
+    return;
+  }
+  for (int j0 = part * kAtOnce; j0 < a.pairs; j0 += a.parts * kAtOnce) {
+    T x[kAtOnce][kChunks];
+    int s[kAtOnce], t[kAtOnce];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int j = min(j0 + i, a.pairs - 1);
+      s[i] = a.source[j], t[i] = a.target[j];
+      if (j0 + i >= a.pairs) t[i] = -1;
+    }
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i)
+      if (copies(a, s[i], t[i])) {
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c)
+          if (first + c * kStep < a.block_bytes) x[i][c] = *reinterpret_cast<const T *>(cache + s[i] * a.block_bytes + first + c * kStep);
+      }
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i)
+      if (copies(a, s[i], t[i])) {
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c)
+          if (first + c * kStep < a.block_bytes) *reinterpret_cast<T *>(cache + t[i] * a.block_bytes + first + c * kStep) = x[i][c];
+      }
+  }
+}
+
+struct KeepArgs {
+  uint8_t *caches[kMostCaches];
+  const int32_t *pt, *kept, *kept_lens, *first;
+  int64_t pt_rs, kept_rs;
+  int most, hkv, bs, w, nb, row_bytes;
+  int col_shift;  // log2 of the 16-byte chunks of a row that a workgroup takes
+};
+
+// Rows of one user and head of one cache: row first + i takes what row kept[i] held, i in batches of B rows.  A row never moves back (an entry that would is
+// skipped), so no row is read behind the batch that overwrites it, and all rows of a batch are read before one of them is written: a barrier per batch.
+// Three batches are on their way: the rows of one, the pages of the next, the entries of the one behind.
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void keep_rows_kernel(KeepArgs a) {
+  constexpr int U = 8;
+  __shared__ int64_t s_from[2][THREADS], s_to[2][THREADS];
+  const int u = blockIdx.x / a.hkv, h = blockIdx.x - u * a.hkv;
+  const int cols = 1 << a.col_shift, col = threadIdx.x & (cols - 1), row = (int)threadIdx.x >> a.col_shift;
+  const int per = THREADS >> a.col_shift, batch = min(per * U, THREADS);  // rows of a pass, of a batch
+  const int n = max(min(a.kept_lens[u], a.most), 0);
+  if (n == 0) return;
+  const int64_t first = a.first ? a.first[u] : 0;
+  const int32_t *const kept = a.kept + (int64_t)u * a.kept_rs, *const pt = a.pt + (int64_t)u * a.pt_rs;
+  uint8_t *const cache = a.caches[blockIdx.y] + (int64_t)(((int)blockIdx.z << a.col_shift) + col) * 16;
+  const bool plans = (int)threadIdx.x < batch;
+  const int64_t room = (int64_t)a.w * a.bs;
+  // thread j plans row j of a batch: its entry, its pages, its offsets
+  const auto entry = [&](int b) {
+    const int64_t i = (int64_t)b * batch + threadIdx.x;
+    return plans && i < n ? kept[i] : -1;
+  };
+  struct Pages {
+    int from, to;
+  };
+  const auto moves = [&](int b, int s) {
+    const int64_t d = first + (int64_t)b * batch + threadIdx.x;
+    return plans && d >= 0 && (int64_t)s > d && s < room;
+  };
+  const auto pages = [&](int b, int s) {
+    Pages p = {-1, -1};
+    if (moves(b, s)) p.from = pt[s / a.bs], p.to = pt[(int)(first + (int64_t)b * batch + threadIdx.x) / a.bs];
+    return p;
+  };
+  const auto plan = [&](int b, int s, const Pages &p) {
+    if (!plans) return;
+    int64_t from = -1, to = -1;
+    if (moves(b, s) && (unsigned)p.from < (unsigned)a.nb && (unsigned)p.to < (unsigned)a.nb) {
+      const int d = (int)(first + (int64_t)b * batch + threadIdx.x);
+      from = (((int64_t)p.from * a.hkv + h) * a.bs + s % a.bs) * a.row_bytes;
+      to = (((int64_t)p.to * a.hkv + h) * a.bs + d % a.bs) * a.row_bytes;
+    }
+    s_from[b & 1][threadIdx.x] = from, s_to[b & 1][threadIdx.x] = to;
+  };
+  const int batches = (n + batch - 1) / batch;
+  u32x4 x[U];
+  const auto load = [&](int b) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int r = row + i * per;
+      const int64_t from = r < batch ? s_from[b & 1][r] : -1;
+      if (from >= 0) x[i] = *reinterpret_cast<const u32x4 *>(cache + from);
+    }
+  };
+  int s0 = entry(0), s1 = entry(1);
+  plan(0, s0, pages(0, s0));
+  Pages p1 = pages(1, s1);
+  int s2 = entry(2);
+  __syncthreads();  // the first plan is there
+  for (int b = 0; b < batches; ++b) {
+    load(b);
+#pragma unroll
+    for (int i = 0; i < U; ++i) asm volatile("" : "+v"(x[i]));  // (they have arrived)
+    int64_t to[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) to[i] = row + i * per < batch ? s_to[b & 1][row + i * per] : -1;
+    plan(b + 1, s1, p1);
+    s1 = s2, p1 = pages(b + 2, s1), s2 = entry(b + 3);
+    __syncthreads();  // everybody has read batch b, and the next plan is there
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (to[i] >= 0) *reinterpret_cast<u32x4 *>(cache + to[i]) = x[i];
+  }
+}
+
+int check_caches(const char *what, void *const *caches, int n) {
+  TTPA_REQUIRE(n >= 0 && (n == 0 || caches), "%s: null pointer argument", what);
+  for (int i = 0; i < n; ++i) TTPA_REQUIRE(caches[i], "%s: null cache", what);
+  return TTPA_OK;
+}
+
+template <typename T>
+int launch_copy(CopyArgs &a, int caches, hipStream_t st) {
+  const int64_t chunks = a.block_bytes / (int64_t)sizeof(T), slices = (chunks + kThreads * kChunks - 1) / (kThreads * kChunks);
+  TTPA_REQUIRE(slices < (1ll << 22), "copy_cache_blocks: a block of %lld bytes is too large", (long long)a.block_bytes);
+  // workgroups for every CU a few times over, a run of pairs each at least
+  const int64_t runs = (a.pairs + kAtOnce - 1) / kAtOnce, want = (8ll * std::max(device_cus(), 1) + slices * caches - 1) / (slices * caches);
+  a.parts = (int)std::max<int64_t>(1, std::min(runs, want));
+  const size_t lds = a.pairs > 64 ? (size_t)(a.nb + 31) / 32 * 4 : 0;
+  copy_blocks_kernel<T><<<dim3((unsigned)slices, (unsigned)caches, (unsigned)a.parts), dim3(kThreads), lds, st>>>(a);
+  return check_launch("copy_cache_blocks");
+}
+
+}  // namespace
+}  // namespace ttpa
+
+using namespace ttpa;
+
+extern "C" int ttpa_copy_cache_blocks(void *const *caches_host, int32_t n_caches, int64_t block_bytes, const int32_t *source_blocks,
+                                      const int32_t *target_blocks, int32_t pairs, int32_t num_blocks, void *stream) {
+  if (int rc = check_caches("copy_cache_blocks", caches_host, n_caches)) return rc;
+  TTPA_REQUIRE(source_blocks && target_blocks, "copy_cache_blocks: null pointer argument");
+  TTPA_REQUIRE(block_bytes > 0 && num_blocks > 0 && pairs >= 0, "copy_cache_blocks: non-positive dimension");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  CopyArgs a = {};
+  a.nb = num_blocks, a.block_bytes = block_bytes;
+  const int32_t most = num_blocks <= kMostMarks ? kMostPairs : 64;  // (more blocks than can be marked: pairs that a wavefront compares)
+  for (int32_t p0 = 0; p0 < pairs; p0 += std::min(pairs - p0, most))
+    for (int32_t c0 = 0; c0 < n_caches; c0 += kMostCaches) {
+      const int n = std::min(n_caches - c0, kMostCaches);
+      uint64_t unit = (uint64_t)block_bytes;
+      for (int i = 0; i < n; ++i) a.caches[i] = static_cast<uint8_t *>(caches_host[c0 + i]), unit |= reinterpret_cast<uint64_t>(a.caches[i]);
+      a.source = source_blocks + p0, a.target = target_blocks + p0, a.pairs = std::min(pairs - p0, most);
+      const int rc = unit % 16 == 0 ? launch_copy<u32x4>(a, n, st) : unit % 4 == 0 ? launch_copy<uint32_t>(a, n, st) : launch_copy<uint8_t>(a, n, st);
+      if (rc) return rc;
+    }
+  return TTPA_OK;
+}
+
+extern "C" int ttpa_keep_cache_tokens(void *const *caches_host, int32_t n_caches, const int32_t *page_table, int64_t page_table_row_stride,
+                                      const int32_t *kept, int64_t kept_row_stride, const int32_t *kept_lens, const int32_t *first, int32_t users,
+                                      int32_t most_kept, int32_t heads, int32_t row_bytes, int32_t block_size, int32_t table_width,
+                                      int32_t num_blocks, void *stream) {
+  if (int rc = check_caches("keep_cache_tokens", caches_host, n_caches)) return rc;
+  TTPA_REQUIRE(page_table && kept && kept_lens, "keep_cache_tokens: null pointer argument");
+  TTPA_REQUIRE(users >= 0 && most_kept >= 0 && heads > 0 && row_bytes > 0 && block_size > 0 && table_width > 0 && num_blocks > 0,
+               "keep_cache_tokens: non-positive dimension");
+  if (row_bytes % 16) return fail(TTPA_ERR_UNSUPPORTED, "keep_cache_tokens: rows of %d bytes; supported are multiples of 16", row_bytes);
+  TTPA_REQUIRE((int64_t)table_width * block_size < (1ll << 31), "keep_cache_tokens: a page-table row holds too many tokens");
+  TTPA_REQUIRE((int64_t)users * heads < (1ll << 24) && row_bytes / 16 < (1 << 16), "keep_cache_tokens: too many rows for one launch");
+  for (int i = 0; i < n_caches; ++i) TTPA_REQUIRE(aligned16(caches_host[i]), "keep_cache_tokens: caches must be 16-byte aligned");
+  if (users == 0 || most_kept == 0) return TTPA_OK;
+  KeepArgs a = {};
+  a.pt = page_table, a.pt_rs = page_table_row_stride, a.kept = kept, a.kept_rs = kept_row_stride, a.kept_lens = kept_lens, a.first = first;
+  a.most = most_kept, a.hkv = heads, a.bs = block_size, a.w = table_width, a.nb = num_blocks, a.row_bytes = row_bytes;
+  const int chunks = row_bytes / 16;
+  while (a.col_shift < 4 && chunks % (2 << a.col_shift) == 0) ++a.col_shift;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  for (int32_t c0 = 0; c0 < n_caches; c0 += kMostCaches) {
+    const int n = std::min(n_caches - c0, kMostCaches);
+    for (int i = 0; i < n; ++i) a.caches[i] = static_cast<uint8_t *>(caches_host[c0 + i]);
+    const dim3 grid((unsigned)(users * heads), (unsigned)n, (unsigned)(chunks >> a.col_shift));
+    if (most_kept <= 32)
+      keep_rows_kernel<64><<<grid, dim3(64), 0, st>>>(a);
+    else
+      keep_rows_kernel<256><<<grid, dim3(256), 0, st>>>(a);
+    if (const int rc = check_launch("keep_cache_tokens")) return rc;
+  }
+  return TTPA_OK;
+}

@@ -35,6 +35,10 @@ struct RopeArgs {
   float eps;
   int tokens, hq, hk;  // hk: key heads that this launch turns
   int rotary, interleaved;
+  // positions on several axes: [axes][tokens], an axis pos_as numbers from the next, and the axis of each of the rotary / 2 pairs
+  const int32_t *pair_axes;
+  int axes;
+  int64_t pos_as;
 };
 
 // Which features a lane holds: chunks a and b, and whether they are turned.  A row's turned part and the rest have their first halves in chunks a, so that a
@@ -64,6 +68,10 @@ __device__ __forceinline__ void load4(const void *p, int is_f32, int64_t at, flo
   }
 }
 
+__device__ __forceinline__ float load1(const void *p, int is_f32, int64_t at) {
+  return is_f32 ? static_cast<const float *>(p)[at] : bf16_lo(static_cast<const uint16_t *>(p)[at]);
+}
+
 // The cosines and sines of a token for the lane's eight pairs, as four and four.  A position outside the table is not turned.
 struct Angles {
   float c[2][4], s[2][4];
@@ -82,6 +90,69 @@ __device__ __forceinline__ Angles angles_of(const RopeArgs &a, const Place<D> &p
 #pragma unroll
       for (int i = 0; i < 4; ++i) t.c[h][i] = 1.f, t.s[h][i] = 0.f;
     }
+  }
+  return t;
+}
+
+// The same where every pair has a position of its own: that of its token on its axis.  Four neighbouring pairs are mostly of one axis, if all of them are in the whole
+// wavefront they are read as four; else one by one (axes in turn along the pairs).  A pair whose axis does not exist is not turned.
+constexpr int kMostAxes = 4;
+template <int D>
+struct PairAxes {
+  int axis[2][4];
+  bool fours;
+  __device__ __forceinline__ PairAxes(const RopeArgs &a, const Place<D> &p) {
+    bool same = true;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int4 x = p.turned ? *reinterpret_cast<const int4 *>(a.pair_axes + (h ? p.cb : p.ca)) : make_int4(0, 0, 0, 0);
+      axis[h][0] = x.x, axis[h][1] = x.y, axis[h][2] = x.z, axis[h][3] = x.w;
+      same = same && x.x == x.y && x.x == x.z && x.x == x.w;
+    }
+    fours = __builtin_amdgcn_ballot_w64(!same) == 0;
+  }
+};
+struct AxisPositions {
+  int64_t at[kMostAxes];
+  __device__ __forceinline__ AxisPositions(const RopeArgs &a, int token) {
+#pragma unroll
+    for (int i = 0; i < kMostAxes; ++i) at[i] = i < a.axes ? load_index(a.positions, a.positions_i64, i * a.pos_as + token) : -1;
+  }
+  __device__ __forceinline__ int64_t of(int axis) const {
+    int64_t x = -1;
+#pragma unroll
+    for (int i = 0; i < kMostAxes; ++i) x = axis == i ? at[i] : x;
+    return x;
+  }
+};
+template <int D>
+__device__ __forceinline__ Angles angles_of(const RopeArgs &a, const Place<D> &p, const PairAxes<D> &pairs, const AxisPositions &positions) {
+  Angles t;
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t.c[h][i] = 1.f, t.s[h][i] = 0.f;
+  if (pairs.fours) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int64_t pos = positions.of(pairs.axis[h][0]);
+      if (p.turned && pos >= 0 && pos < a.max_positions) {
+        const int64_t at = pos * a.angle_rs + (h ? p.cb : p.ca);
+        load4(a.angles, a.angles_f32, at, t.c[h]);
+        load4(a.angles, a.angles_f32, at + a.rotary / 2, t.s[h]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t pos = positions.of(pairs.axis[h][i]);
+        if (p.turned && pos >= 0 && pos < a.max_positions) {
+          const int64_t at = pos * a.angle_rs + (h ? p.cb : p.ca) + i;
+          t.c[h][i] = load1(a.angles, a.angles_f32, at), t.s[h][i] = load1(a.angles, a.angles_f32, at + a.rotary / 2);
+        }
+      }
   }
   return t;
 }
@@ -150,8 +221,18 @@ __device__ __forceinline__ RowPart turn_row(const RopeArgs &a, const Place<D> &p
   return o;
 }
 
+template <int D, bool AXES>
+__device__ __forceinline__ Angles token_angles(const RopeArgs &a, const Place<D> &p, int token) {
+  if constexpr (AXES) {
+    const PairAxes<D> pairs(a, p);
+    return angles_of<D>(a, p, pairs, AxisPositions(a, token));
+  } else {
+    return angles_of<D>(a, p, load_index(a.positions, a.positions_i64, token));
+  }
+}
+
 // Wavefront `part` of a token's: heads [part * U * R, ...) of the queries' and then the keys' (R rows per wavefront).
-template <int D, int U>
+template <int D, int U, bool AXES>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeArgs a, int parts) {
   constexpr int LPR = D / 16, R = 64 / LPR;
   const int wave = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -165,7 +246,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeArgs a, int parts
     const int h = min((part * U + u) * R + r, heads - 1);  // (rows past the last head: that one again, and not stored)
     x[u] = h < a.hq ? load_part(a.q + token * a.q_ts + h * a.q_hs, p.fa, p.fb) : load_part(a.k + token * a.k_ts + (h - a.hq) * a.k_hs, p.fa, p.fb);
   }
-  const Angles t = angles_of<D>(a, p, load_index(a.positions, a.positions_i64, token));
+  const Angles t = token_angles<D, AXES>(a, p, token);
   Weights wq, wk;
   if (a.q_weight) load_weights<D>(a.q_weight, a.weights_f32, p, wq);
   if (a.k_weight) load_weights<D>(a.k_weight, a.weights_f32, p, wk);
@@ -194,7 +275,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeArgs a, int parts
 // few heads that a token's own one or two wavefronts stay partly empty.  us a pass, a token's wavefronts / this: 12056 tokens of 8 + 2 heads of 64 14.1 / 8.8,
 // 16384 of 8 + 1 of 128 24.0 / 19.4 and of 4 + 1 18.2 / 12.7, 8192 of 2 + 1 of 256 11.2 / 8.4; with three wavefronts per token 8192 of 16 + 2 of 128 17.7 / 18.9.
 // (One, three and four rows per lane 10.1, 9.5 and 9.5 on the first.)
-template <int D, int U>
+template <int D, int U, bool AXES>
 __global__ __launch_bounds__(256) void qk_norm_rope_rows_kernel(RopeArgs a, uint32_t heads_inv) {
   constexpr int LPR = D / 16, R = 64 / LPR;
   const Place<D> p(a);
@@ -210,8 +291,10 @@ __global__ __launch_bounds__(256) void qk_norm_rope_rows_kernel(RopeArgs a, uint
     token[u] = (int)n, head[u] = (int)h;
   }
   int64_t pos[U];
+  if constexpr (!AXES) {
 #pragma unroll
-  for (int u = 0; u < U; ++u) pos[u] = load_index(a.positions, a.positions_i64, token[u]);
+    for (int u = 0; u < U; ++u) pos[u] = load_index(a.positions, a.positions_i64, token[u]);
+  }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int h = head[u] - a.hq;
@@ -219,7 +302,10 @@ __global__ __launch_bounds__(256) void qk_norm_rope_rows_kernel(RopeArgs a, uint
   }
   Angles t[U];
 #pragma unroll
-  for (int u = 0; u < U; ++u) t[u] = angles_of<D>(a, p, pos[u]);
+  for (int u = 0; u < U; ++u) {
+    if constexpr (AXES) t[u] = token_angles<D, true>(a, p, token[u]);
+    else t[u] = angles_of<D>(a, p, pos[u]);
+  }
   Weights wq, wk;
   if (a.q_weight) load_weights<D>(a.q_weight, a.weights_f32, p, wq);
   if (a.k_weight) load_weights<D>(a.k_weight, a.weights_f32, p, wk);
@@ -318,7 +404,7 @@ __global__ __launch_bounds__(64) void step_write_kernel(StepArgs a, int q_parts,
   }
 }
 
-template <int D>
+template <int D, bool AXES>
 int launch_rope(const RopeArgs &a, hipStream_t st) {
   constexpr int R = 1024 / D;
   const int groups = (a.hq + a.hk + R - 1) / R;
@@ -326,7 +412,7 @@ int launch_rope(const RopeArgs &a, hipStream_t st) {
     constexpr int U = decltype(tag)::value;
     const int parts = (groups + U - 1) / U;
     const int64_t waves = (int64_t)a.tokens * parts;
-    qk_norm_rope_kernel<D, U><<<dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, st>>>(a, parts);
+    qk_norm_rope_kernel<D, U, AXES><<<dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, st>>>(a, parts);
   };
   // Few rows want to be everywhere at once; many, three to five groups per wavefront, as many as leave no slot without a group, or else five: its angles and
   // weights are read once.  8192 tokens of 32 + 8 heads of 128 (168 MB), us a pass with 1 / 2 / 3 / 5 groups 44.1 / 41.4 / 36.8 / 32.5; with ordinary
@@ -336,7 +422,7 @@ int launch_rope(const RopeArgs &a, hipStream_t st) {
     if (groups <= 2) {
       constexpr int U = 2, PER = 4 * U * R;  // rows of a workgroup
       const int64_t rows = (int64_t)a.tokens * (a.hq + a.hk);
-      qk_norm_rope_rows_kernel<D, U><<<dim3((unsigned)((rows + PER - 1) / PER)), dim3(256), 0, st>>>(a, 0xffffffffu / (uint32_t)(a.hq + a.hk));
+      qk_norm_rope_rows_kernel<D, U, AXES><<<dim3((unsigned)((rows + PER - 1) / PER)), dim3(256), 0, st>>>(a, 0xffffffffu / (uint32_t)(a.hq + a.hk));
       return check_launch("qk_norm_rope");
     }
     for (int u = 3; u <= std::min(groups, 5); ++u)
@@ -414,9 +500,33 @@ extern "C" int ttpa_qk_norm_rope(void *q_out, int64_t q_out_token_stride, int64_
   if (tokens == 0) return TTPA_OK;
   hipStream_t st = static_cast<hipStream_t>(stream);
   switch (head_size) {
-    case 64: return launch_rope<64>(a, st);
-    case 128: return launch_rope<128>(a, st);
-    default: return launch_rope<256>(a, st);
+    case 64: return launch_rope<64, false>(a, st);
+    case 128: return launch_rope<128, false>(a, st);
+    default: return launch_rope<256, false>(a, st);
+  }
+}
+
+extern "C" int ttpa_qk_norm_rope_axes(void *q_out, int64_t q_out_token_stride, int64_t q_out_head_stride, void *k_out, int64_t k_out_token_stride,
+                                      int64_t k_out_head_stride, const void *q, int64_t q_token_stride, int64_t q_head_stride, const void *k,
+                                      int64_t k_token_stride, int64_t k_head_stride, const void *cos_sin, int cos_sin_is_f32,
+                                      int64_t cos_sin_row_stride, int64_t max_positions, const void *positions, int positions_is_i64,
+                                      int64_t positions_axis_stride, int32_t axes, const int32_t *pair_axes, const void *q_weight, const void *k_weight,
+                                      int weights_are_f32, float eps, int32_t tokens, int32_t q_heads, int32_t k_heads, int32_t head_size,
+                                      int32_t rotary, int interleaved, void *stream) {
+  RopeArgs a = {static_cast<uint16_t *>(q_out), static_cast<uint16_t *>(k_out), q_out_token_stride, q_out_head_stride, k_out_token_stride,
+                k_out_head_stride, static_cast<const uint16_t *>(q), static_cast<const uint16_t *>(k), q_token_stride, q_head_stride, k_token_stride,
+                k_head_stride, cos_sin, cos_sin_row_stride, cos_sin_is_f32, weights_are_f32, max_positions, positions, positions_is_i64, q_weight,
+                k_weight, eps, tokens, q_heads, k_heads, rotary, interleaved, pair_axes, axes, positions_axis_stride};
+  TTPA_REQUIRE(k_heads > 0, "qk_norm_rope: non-positive dimension");
+  TTPA_REQUIRE(pair_axes && aligned16(pair_axes), "qk_norm_rope: pair_axes must be a 16-byte aligned pointer");
+  if (axes < 1 || axes > kMostAxes) return fail(TTPA_ERR_UNSUPPORTED, "qk_norm_rope: %d axes; supported 1 to %d", axes, kMostAxes);
+  if (int rc = check_rope(a, head_size, true)) return rc;
+  if (tokens == 0) return TTPA_OK;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  switch (head_size) {
+    case 64: return launch_rope<64, true>(a, st);
+    case 128: return launch_rope<128, true>(a, st);
+    default: return launch_rope<256, true>(a, st);
   }
 }
 
