@@ -19,6 +19,14 @@ def _pkg():
     import tt_xla_amd  # noqa: F401
 
 
+@pytest.fixture(params=["rows", "stream", None], autouse=True)
+def form(request, monkeypatch):
+    """The form for few rows, the streaming loop, and what the library chooses."""
+    if request.param:
+        monkeypatch.setenv("TTPA_CROSS_FORM", request.param)
+    return request.param
+
+
 def _check(out, q, k, v, table, lens, scale, room=None, gain=1):
     """gain: scores are that much larger, and their roundings."""
     want, spread = M.cross(q, k, v, table, lens, scale, room)

@@ -2,7 +2,8 @@
 //
 //   out[u, h, t] = sum_j softmax_j(scale q[u, h, t] . k[u, j]) v[u, j],   j < len[u];   zeros where len[u] is 0
 //
-// This file holds the form for few rows (a token per user, a few drafted ones).  All tokens of a user see the same keys, so the rows of a KV
+// This file holds the form for few rows (a token per user, a few drafted ones) and the choice; many rows are the streaming prefill loop's
+// (prefill_stream_kernel.h, kEnds).  All tokens of a user see the same keys, so the rows of a KV
 // head are its G query heads times the tokens, and a workgroup takes 16 RG of them over a part of the keys.
 // Bound by memory: K and V are read once for each block of rows.  A wavefront takes every 4 parts-th tile of TILE keys (64 at head size 64, else 32):
 //   memory -> registers -> LDS    whole lines, a tile ahead of its use; what lies behind the last key becomes zeros on the way (V) or is masked (K)
@@ -12,8 +13,11 @@
 // Statistics and accumulators are floats; weights are rounded once to bfloat16 for the matrix instruction, and the same rounded weights are summed.
 // The four wavefronts' results meet in LDS, the parts' in memory, merged by a kernel of its own.
 #include "decode_mfma16_kernel.h"
+#include "prefill_common.h"
 
 #include <algorithm>
+#include <cstdlib>
+#include <cstring>
 
 namespace ttpa {
 namespace decode {
@@ -390,6 +394,30 @@ int launch_cross_d(const CrossArgs &a, int groups, hipStream_t st) {
   return launch_cross<D, 1>(a, st);
 }
 
+// The streaming loop's arguments.  It steps through rows by unsigned 32-bit numbers of bytes and through blocks by a 32-bit inverse; what does not fit those is
+// the few rows' form's.
+bool stream_args(const CrossArgs &c, int head_size, bool keys_known, int64_t keys, PrefillArgs &a) {
+  for (const int64_t rows : {c.q_ts, c.o_ts})
+    if (rows < 0 || rows >= (int64_t)1 << 31) return false;
+  if ((int64_t)c.w * c.bs * c.bs >= (1ll << 32)) return false;
+  a = {};
+  a.out = c.out, a.out_bs = c.o_bs, a.out_hs = c.o_hs, a.out_ts = c.o_ts;
+  a.q = c.q, a.q_bs = c.q_bs, a.q_hs = c.q_hs, a.q_ts = c.q_ts;
+  a.k = c.k, a.v = c.v, a.pt = c.pt, a.pt_rs = c.pt_rs, a.lens = c.lens, a.lens_i64 = c.lens_i64;
+  a.batch = c.batch, a.hq = c.hkv * c.g, a.hkv = c.hkv, a.sq = c.s, a.skv = c.w * c.bs, a.bs = c.bs, a.w = c.w, a.nb = c.nb;
+  a.bs_magic = (uint32_t)((1ull << 32) / (uint32_t)c.bs) + 1u;
+  a.scale_log2e = c.scale_log2e, a.parts = 1, a.stream = 1;
+  a.cus = std::max(device_cus(), 1), a.keys_known = keys_known, a.keys_bound = keys;
+  return true;
+}
+
+// Which form takes a call.  TTPA_CROSS_FORM=rows|stream, read on every call, overrides.
+bool streams(const CrossArgs &c, int head_size, const PrefillArgs &a) {
+  const char *e = getenv("TTPA_CROSS_FORM");
+  if (e && (!strcmp(e, "rows") || !strcmp(e, "stream"))) return !strcmp(e, "stream");
+  return c.s >= 32;
+}
+
 // Keys that the call is laid out for.
 int64_t room_of(int block_size, int table_width, int64_t most_keys) {
   const int64_t room = (int64_t)block_size * table_width;
@@ -405,8 +433,16 @@ using namespace ttpa;
 extern "C" int64_t ttpa_paged_cross_attention_workspace_bytes(int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t q_len, int32_t head_size,
                                                               int32_t block_size, int32_t table_width, int64_t most_keys) {
   if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || q_len <= 0 || head_size <= 0 || block_size <= 0 || table_width <= 0 || q_heads % kv_heads) return 0;
-  const decode::CrossCut c = decode::cross_cut(batch, kv_heads, (int64_t)(q_heads / kv_heads) * q_len, head_size, decode::room_of(block_size, table_width, most_keys));
-  return decode::cross_bytes(c, batch, kv_heads, head_size);
+  const int64_t keys = decode::room_of(block_size, table_width, most_keys);
+  const decode::CrossCut c = decode::cross_cut(batch, kv_heads, (int64_t)(q_heads / kv_heads) * q_len, head_size, keys);
+  int64_t bytes = decode::cross_bytes(c, batch, kv_heads, head_size);
+  // (strides are not known here: what either form may want)
+  decode::CrossArgs a = {};
+  a.batch = batch, a.hkv = kv_heads, a.g = q_heads / kv_heads, a.s = q_len, a.bs = block_size, a.w = (int)((keys + block_size - 1) / block_size);
+  PrefillArgs p;
+  if ((head_size == 64 || head_size == 128 || head_size == 256) && decode::stream_args(a, head_size, most_keys > 0, keys, p) && decode::streams(a, head_size, p))
+    bytes = std::max(bytes, stream_ends_part_bytes(p, head_size));
+  return bytes;
 }
 
 extern "C" int ttpa_paged_cross_attention(void *out, int64_t out_batch_stride, int64_t out_head_stride, int64_t out_token_stride, const void *q,
@@ -427,8 +463,7 @@ extern "C" int ttpa_paged_cross_attention(void *out, int64_t out_batch_stride, i
   TTPA_REQUIRE(most_keys >= 0, "cross attention: most_keys must not be negative");
   TTPA_REQUIRE((int64_t)table_width * block_size < (1ll << 31) - 8192, "cross attention: a page-table row holds too many keys");
   TTPA_REQUIRE((int64_t)q_heads / kv_heads * q_len < (1ll << 30), "cross attention: too many rows");
-  TTPA_REQUIRE(aligned16(q) && aligned16(k_cache) && aligned16(v_cache) && (reinterpret_cast<uintptr_t>(out) & 7) == 0,
-               "cross attention: operands must be 16-byte aligned (out: 8)");
+  TTPA_REQUIRE(aligned16(q) && aligned16(k_cache) && aligned16(v_cache) && aligned16(out), "cross attention: operands must be 16-byte aligned");
   TTPA_REQUIRE(q_batch_stride % 8 == 0 && q_head_stride % 8 == 0 && q_token_stride % 8 == 0 && out_batch_stride % 4 == 0 && out_head_stride % 4 == 0 &&
                    out_token_stride % 4 == 0,
                "cross attention: strides must be multiples of 8 elements (out: 4)");
@@ -444,6 +479,13 @@ extern "C" int ttpa_paged_cross_attention(void *out, int64_t out_batch_stride, i
   a.w = (int)((keys + block_size - 1) / block_size);
   a.scale_log2e = scale * 1.4426950408889634f;
   a.runs = (uint32_t)block_size / (decode::tile_of(head_size) / 4), a.runs_inv = 0xffffffffu / a.runs;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  PrefillArgs p;
+  if (decode::stream_args(a, head_size, most_keys > 0, keys, p) && decode::streams(a, head_size, p)) {
+    TTPA_REQUIRE((int64_t)batch * q_heads * ((q_len + 31) / 32) < (1ll << 26), "cross attention: too many rows for one launch");
+    if (workspace && aligned16(workspace)) p.part_acc = static_cast<float *>(workspace), p.part_bytes = workspace_bytes;
+    return launch_stream_ends(p, head_size, st);
+  }
   const decode::CrossCut c = decode::cross_cut(batch, kv_heads, (int64_t)a.g * q_len, head_size, keys);
   a.row_blocks = c.row_blocks, a.parts = c.parts;
   TTPA_REQUIRE(((int64_t)batch * kv_heads * a.parts + 8) * a.row_blocks < (1ll << 24), "cross attention: too many rows for one launch");
@@ -451,7 +493,6 @@ extern "C" int ttpa_paged_cross_attention(void *out, int64_t out_batch_stride, i
   if (a.parts > 1 && (!workspace || !aligned16(workspace) || workspace_bytes < need))
     return fail(TTPA_ERR_WORKSPACE, "cross attention: needs %lld bytes of workspace, 16-byte aligned", (long long)need);
   a.slots = static_cast<float *>(workspace);
-  hipStream_t st = static_cast<hipStream_t>(stream);
   switch (head_size) {
     case 64: return decode::launch_cross_d<64>(a, c.groups, st);
     case 128: return decode::launch_cross_d<128>(a, c.groups, st);

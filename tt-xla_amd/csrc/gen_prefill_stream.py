@@ -60,6 +60,9 @@ Keys of 128 + 64 features: S(i) is 12 matrix instructions, an iteration 20; a bl
 is 4 KiB (one load per wavefront), in a ring of its own behind the other two.  With rings of NS = 4
 the three still fit 80 KiB, half of a CU's LDS, and a request has two iterations to arrive.
 
+Keys that end anywhere (`ends`, paged forms: an encoder's states, one length per batch entry): the masks see to the scores; V rows of the last block that
+lie behind the last key, in which anything may stand, are written over with zeros once they have landed.
+
 A workgroup may take only a part of the keys (paged forms): it starts at any block, and if the base
 of a partial result is given, the accumulators go out as they are, with the reference and the sum of
 every row, for a merge kernel.
@@ -119,7 +122,9 @@ class Registers:
         self.T = [take(1) for _ in range(4)]
         self.ORV, self.MLOC, self.MB, self.MCN = (take(1) for _ in range(4))
         self.PTREQ = take(1)                       # paged: the requested block-table entry
-        self.LOWEST, self.LOWREL = take(1), take(1)  # window: first visible key of the lane's row, minus 4 h; relative to the block
+        # window: first visible key of the lane's row, minus 4 h; relative to the block.  ends: the row of a V block that the lane's first load has, its
+        # place in LDS in slot 0 of the K ring
+        self.LOWEST, self.LOWREL = take(1), take(1)
         self.PTREQ2 = take(1)                      # blocks of 32: the entry requested in odd iterations
         self.LIMIT = take(1)                       # last visible key of the lane's row, minus 4 h
         self.LIMREL, self.NEGINF, self.VZERO = (take(1) for _ in range(3))
@@ -147,7 +152,7 @@ S_VLEFT = "s73"                # V blocks left to request
 S_MASKFROM = "s74"             # blocks whose first key is >= this are masked
 S_KEY0 = "s75"                 # first key of the block whose softmax comes next (input: of the first block)
 S_STATS, S_PART = "s[36:37]", "s[38:39]"  # paged: where (reference, sum) and the accumulators of a part go (0: the whole result)
-S_LOWTO = "s34"                # window: blocks whose first key is < this are masked from below (input)
+S_LOWTO = "s34"                # window: blocks whose first key is < this are masked from below (input); ends: rows of the last V block that hold keys
 # keys of 128 + 64 only: the second part of K, its bytes per block and the LDS address of the wavefront's segment; V's bytes per block
 S_PBASE, S_PSTRIDE, S_M0P, S_VSTRIDE = "s[30:31]", "s32", "s33", "s35"
 # paged only
@@ -181,9 +186,10 @@ KEY_CONST = [8 * (r // 4) + r % 4 for r in range(16)]
 class Form:
     """What one block of assembly serves."""
 
-    def __init__(self, name, d=128, paged=0, window=False, wide=False):
+    def __init__(self, name, d=128, paged=0, window=False, wide=False, ends=False):
         self.name, self.d = f"{name}_{d}", d
         self.paged, self.window = paged, window  # paged: 0 or the keys that share a table entry
+        self.ends = ends                    # the keys end anywhere, and what lies behind them is not to be used
         self.wide = wide                    # keys of 128 + 64 features
         self.ns = 4 if wide or d == 256 else 5  # slots per ring
         self.unroll = 4 if self.ns == 4 else 10  # lcm(2, ns): score bank and slots repeat
@@ -193,13 +199,14 @@ class Form:
         self.vring = self.ns * self.SLOT    # LDS offset of the V ring (VOFF carries it), of the second part's ring (KOFFP)
         self.pring = 2 * self.vring
         self.loads = 2 * self.tensor_loads + wide  # tile loads of an iteration
-        self.items = d == 128 and not window and not wide and paged != 32  # several row blocks in turn
+        self.items = d == 128 and not window and not wide and not ends and paged != 32  # several row blocks in turn
         self.parts = paged > 0  # may take a part of the keys
 
 
 FORMS = [Form("DENSE_WIDE", wide=True)] + [
     form for d in (64, 128, 256)
-    for form in (Form("DENSE", d), Form("DENSE_WINDOW", d, window=True), Form("PAGED", d, paged=64), Form("PAGED32", d, paged=32))]
+    for form in (Form("DENSE", d), Form("DENSE_WINDOW", d, window=True), Form("PAGED", d, paged=64), Form("PAGED32", d, paged=32),
+                 Form("ENDS", d, paged=64, ends=True), Form("ENDS32", d, paged=32, ends=True))]
 START_REFERENCE = "0xff7fffff"  # the lowest finite float
 
 
@@ -367,6 +374,25 @@ def mask_block(o, f, q, tag):
     mask_selects(o, f, q)
     o.label(f"L_nomask_{tag}")
     o.e(f"s_add_u32 {S_KEY0}, {S_KEY0}, 32")
+
+
+def zero_tail(o, f, slot, tag):
+    """The rows of the last V block behind the last key become zeros (their probabilities are, but zero times NaN is NaN): in front of the barrier that
+    publishes the block, each wavefront those that it has requested itself, whose loads it has waited for."""
+    o.e(f"s_cmp_ge_u32 {S_LOWTO}, 32")
+    o.e(f"s_cbranch_scc1 L_whole_{tag}%=")
+    rows = 1024 // (2 * f.d)  # of a load
+    for j in range(f.tensor_loads):
+        o.e(f"s_sub_u32 s90, {S_LOWTO}, {j * rows}")
+        o.e(f"v_add_u32 v{f.VT0}, 0x{f.vring + slot * f.SLOT + 1024 * j:x}, v{f.LOWREL}")
+        o.e(f"v_cmp_le_i32_e64 s[88:89], s90, v{f.LOWEST}")
+        o.e("s_nop 4")
+        o.e("s_and_saveexec_b64 s[62:63], s[88:89]")
+        o.e(f"ds_write2_b32 v{f.VT0}, v{f.VZERO}, v{f.VZERO} offset0:0 offset1:1")
+        o.e(f"ds_write2_b32 v{f.VT0}, v{f.VZERO}, v{f.VZERO} offset0:2 offset1:3")
+        o.e("s_mov_b64 exec, s[62:63]")
+    o.e("s_waitcnt lgkmcnt(0)")
+    o.label(f"L_whole_{tag}")
 
 
 def accumulators(f):
@@ -586,13 +612,15 @@ def iteration_head(o, f, p, tag):
         o.e("s_mov_b64 s[98:99], s[86:87]")
 
 
-def few_left(o, f, tag):
-    """The wait of an iteration with less than ns blocks left."""
+def few_left(o, f, p, tag):
+    """The wait of iteration i = p (mod f.unroll) with less than ns blocks left."""
     o.label(f"L_few_{tag}")
     for left in range(1, f.ns - 1):
         o.e(f"s_cmp_lg_u32 {S_NB}, {left}")
         o.e(f"s_cbranch_scc1 L_few{left}_{tag}%=")
         o.e(f"s_waitcnt vmcnt({in_flight(f, left)})")
+        if f.ends and left == 1:
+            zero_tail(o, f, p % f.ns, tag)
         o.e(f"s_branch L_bar_{tag}%=")
         o.label(f"L_few{left}_{tag}")
     o.e(f"s_waitcnt vmcnt({in_flight(f, f.ns - 1)})")
@@ -936,6 +964,11 @@ def generate(f):
     for ks in range(f.d // 16):
         o.e(f"v_add_u32 v{f.T[ks % 4]}, {S_QSLOT}, v{f.KOFF + ks}")
         o.e(f"ds_read_b128 {vr(f.QF + 4 * ks, 4)}, v{f.T[ks % 4]}")
+    if f.ends:  # (the last block is the first one, and has landed; head size 64 reads it in front of iteration 0's barrier)
+        o.e(f"s_cmp_lg_u32 {S_NB}, 1")
+        o.e("s_cbranch_scc1 L_more%=")
+        zero_tail(o, f, 0, "first")
+        o.label("L_more")
     o.e("s_waitcnt lgkmcnt(0)")
     o.e("s_barrier")
     first_request(o, f, "K", f.ns - 1, "late")
@@ -1001,7 +1034,7 @@ def generate(f):
     slow_path(o, f, 0, "L_slow_i0", "L_join_i0", first=True)
     for p in range(f.unroll):
         slow_path(o, f, p % 2, f"L_slow_p{p}", f"L_join_p{p}")
-        few_left(o, f, f"p{p}")
+        few_left(o, f, p, f"p{p}")
     o.label("L_end")
     o.e("s_nop 15")
     o.e("s_nop 15")
@@ -1046,6 +1079,8 @@ def operands(f):
         ins += [i(f.QFP, "q_second", 16), i(f.KOFFP, "po", 4)]
     if f.window:
         ins += [i(f.LOWEST, "lowest"), i(S_LOWTO, "low_to")]
+    if f.ends:
+        ins += [i(f.LOWEST, "tail_row"), i(f.LOWREL, "tail_address"), i(S_LOWTO, "tail_count")]
     if f.paged:
         outs += [io(S_CIN, "tab.read_in_block"), io(S_RIN, "tab.request_in_block"), io(S_RPTR, "tab.entry_ptr"), io(S_RLEFT, "tab.entry_requests"),
                  io(f.PTREQ, "tab.entry"), io(S_PART, "out_part.acc")] + [io(*x) for x in offs[-2:]]

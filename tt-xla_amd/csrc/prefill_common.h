@@ -89,12 +89,20 @@ struct PrefillArgs {
   int keys_known;        // ... from the caller, and not from the page table's room
   int cus;               // CUs of the device: asked for once per pass, whose rules need it several times
   int stream;            // 0: the plain loop whatever the shape (TTPA_PREFILL_STREAM=0)
+  // Cross attention (the streaming kernel's kEnds forms): keys of each batch entry, of skv that the table has room for
+  const void *lens;
+  int lens_i64;
 };
 
 // key / block_size without a division instruction sequence (about 30 instructions each, and the
 // paged tile loads need several per tile).
 __device__ __forceinline__ int div_block(const PrefillArgs &a, int key) {
   return a.bs == 1 ? key : (int)__umulhi((uint32_t)key, a.bs_magic);
+}
+
+// Keys of a batch entry of cross attention.
+__device__ __forceinline__ int entry_keys(const PrefillArgs &a, int b) {
+  return __builtin_amdgcn_readfirstlane((int)max(min(load_index(a.lens, a.lens_i64, b), (int64_t)a.skv), (int64_t)0));
 }
 
 // Position of the first query row.  It is in device memory, where no check of the host's sees it: below -sq no row
@@ -264,6 +272,11 @@ int64_t stream_part_bytes(const PrefillArgs &a, int head_size);
 int launch_stream(const PrefillArgs &a, int head_size, hipStream_t st);
 int launch_stream_d64(const PrefillArgs &a, hipStream_t st);
 int launch_stream_d256(const PrefillArgs &a, hipStream_t st);
+// ... with a length per batch entry (paged, block size a multiple of 32).
+int launch_stream_ends(const PrefillArgs &a, int head_size, hipStream_t st);
+int launch_stream_ends_d64(const PrefillArgs &a, hipStream_t st);
+int launch_stream_ends_d256(const PrefillArgs &a, hipStream_t st);
+int64_t stream_ends_part_bytes(const PrefillArgs &a, int head_size);
 // The streaming kernel for keys of 128 + 64 features (dense, causal or not, kv length a multiple of 32).
 int launch_stream_wide(const PrefillArgs &a, hipStream_t st);
 

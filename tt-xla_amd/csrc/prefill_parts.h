@@ -71,6 +71,11 @@ __device__ __forceinline__ int blocks_per_part(const PrefillArgs &a, int offset)
   return part_of_blocks(a, max(((a.causal ? min(a.skv, offset + a.sq) : a.skv) + kBlockKeys - 1) / kBlockKeys, 1));  // (of the last row block)
 }
 
+// The same for a batch entry of cross attention.
+__device__ __forceinline__ int blocks_per_part_of_keys(const PrefillArgs &a, int keys) {
+  return part_of_blocks(a, max((keys + kBlockKeys - 1) / kBlockKeys, 1));
+}
+
 // Accumulators and (reference, sum) rows of the parts: [part][batch][head][row block], the statistics
 // behind all accumulators.
 struct PartLayout {
@@ -88,16 +93,17 @@ __host__ __device__ inline PartLayout part_layout(const PrefillArgs &a) {
 // 8 group + 4 (lane / 32) .. + 3): 512 consecutive bytes per read of 32 lanes, whole 32-byte pieces of a row per
 // write.  Memory bound: 34 MB of accumulators (512 rows, 32 heads, 4 parts) in 7.9 us.  Parts past the last are zeros: repeated
 // with weight 0 they needed as long at head sizes 64 and 128 and 5 us more at 256 (128 rows of 16/8 heads behind 2048 tokens 36.7 / 31.7).
-template <int D>
+// ENDS: the keys are a batch entry's own number.
+template <int D, bool ENDS = false>
 __global__ __launch_bounds__(2 * D) void prefill_merge_kernel(PrefillArgs a) {
   const int rb = blockIdx.x, hq = blockIdx.y, b = blockIdx.z;
   const int pair = rb * a.head_group + hq - quotient(a.by_head_group, hq) * a.head_group;
   const int n = threadIdx.x & 31, g = threadIdx.x >> 5;
   const int offset = a.causal ? chunk_offset(a.chunk_start, a.sq, a.skv) : 0;
   const int wg_last_row = min(a.sq, (last_row_block(a, pair >> 2) + 1) * kRowsPerWave) - 1;
-  const int kv_end = a.causal ? min(a.skv, offset + wg_last_row + 1) : a.skv;
+  const int kv_end = ENDS ? entry_keys(a, b) : a.causal ? min(a.skv, offset + wg_last_row + 1) : a.skv;
   const int nblk = (kv_end + kBlockKeys - 1) / kBlockKeys;
-  const int share = blocks_per_part(a, offset);
+  const int share = ENDS ? blocks_per_part_of_keys(a, kv_end) : blocks_per_part(a, offset);
   if (share >= nblk) return;  // one workgroup saw all keys and wrote the output
   const int active = (nblk + share - 1) / share;
   const PartLayout lay = part_layout(a);

@@ -91,6 +91,18 @@ bool stream_expands(const PrefillArgs &a, int head_size, int64_t room) {
 
 int launch_stream_wide(const PrefillArgs &a, hipStream_t st) { return launch_form<128, kDenseWide>(a, st); }
 
+int launch_stream_ends(const PrefillArgs &a, int head_size, hipStream_t st) {
+  switch (head_size) {
+    case 64: return launch_stream_ends_d64(a, st);
+    case 128: return launch_ends_d<128>(a, st);
+    default: return launch_stream_ends_d256(a, st);
+  }
+}
+
+int64_t stream_ends_part_bytes(const PrefillArgs &a, int head_size) {
+  return part_bytes(a, head_group_size(a, head_size), stream_split(head_size), head_size);
+}
+
 int launch_stream(const PrefillArgs &a, int head_size, hipStream_t st) {
   switch (head_size) {
     case 64: return launch_stream_d64(a, st);

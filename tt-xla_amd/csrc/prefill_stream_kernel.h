@@ -16,7 +16,11 @@ namespace {
 // kDenseWide: keys of 128 + 64 features (the latent layers' prompts with K and V expanded per head): 20 matrix
 // instructions per block of 32 keys; 4 x 2048 tokens, 16 heads: 8.6e10 flop in 100 us, where the absorbed form's
 // 2.9e11 took 281
-enum StreamForm { kDense = 0, kDenseWindow = 1, kPaged = 2, kPaged32 = 3, kDenseWide = 4 };
+// kEnds, kEnds32: as kPaged and kPaged32, with a length per batch entry instead of a causal limit (cross attention)
+enum StreamForm { kDense = 0, kDenseWindow = 1, kPaged = 2, kPaged32 = 3, kDenseWide = 4, kEnds = 5, kEnds32 = 6 };
+constexpr bool form_ends(int form) { return form == kEnds || form == kEnds32; }
+constexpr bool form_tiles(int form) { return form == kPaged || form == kEnds; }  // two 32-key blocks share a table entry
+constexpr bool form_paged(int form) { return form == kPaged || form == kPaged32 || form_ends(form); }
 
 // The assembly is bound to the registers its text names through constraint strings (both written by
 // gen_prefill_stream.py, with the names that the kernel below gives the values); everything else it
@@ -97,7 +101,7 @@ constexpr int stream_lds_bytes(int d, bool wide) { return stream_p_ring(d, wide)
 
 template <int D, int FORM>
 __global__ __launch_bounds__(256, stream_wgs_per_cu(D)) void prefill_stream_kernel(PrefillArgs a) {
-  constexpr bool PAGED = FORM == kPaged || FORM == kPaged32, WIDE = FORM == kDenseWide;
+  constexpr bool PAGED = form_paged(FORM), WIDE = FORM == kDenseWide, ENDS = form_ends(FORM);
   using T = Tile<D>;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
 
@@ -132,7 +136,17 @@ __global__ __launch_bounds__(256, stream_wgs_per_cu(D)) void prefill_stream_kern
 
   // keys the workgroup can see, in blocks of 32
   const int wg_last_row = min(a.sq, (last_row_block(a, qt) + 1) * kRowsPerWave) - 1;
-  const int kv_end = a.causal ? min(a.skv, offset + wg_last_row + 1) : a.skv;
+  int skv = a.skv;
+  if constexpr (ENDS) {
+    skv = entry_keys(a, b);
+    if (skv == 0) {  // nothing to attend: zeros
+      if (part == 0)
+        for (int i = lane; i < (min(a.sq, row0 + kRowsPerWave) - row0) * (D / 4); i += 64)
+          *reinterpret_cast<uint2 *>(a.out + b * a.out_bs + hq * a.out_hs + (int64_t)(row0 + i / (D / 4)) * a.out_ts + 4 * (i % (D / 4))) = make_uint2(0u, 0u);
+      return;
+    }
+  }
+  const int kv_end = a.causal ? min(skv, offset + wg_last_row + 1) : skv;
   int first_block = FORM == kDenseWindow ? max(0, offset + quotient(a.by_head_group, 4 * qt) * kRowsPerWave - a.window + 1) / kBlockKeys : 0;
   // (at least one: the loop counts blocks down to zero.  Where no row sees a key, a chunk that starts at a negative
   // position, block 0 is read and masked, and the rows come out as NaN, softmax over nothing)
@@ -140,7 +154,7 @@ __global__ __launch_bounds__(256, stream_wgs_per_cu(D)) void prefill_stream_kern
   bool whole = true;  // this workgroup sees all keys of its rows
   if constexpr (PAGED) {
     if (a.parts > 1) {
-      const int share = __builtin_amdgcn_readfirstlane(blocks_per_part(a, offset));
+      const int share = __builtin_amdgcn_readfirstlane(ENDS ? blocks_per_part_of_keys(a, skv) : blocks_per_part(a, offset));
       whole = share >= nblk;
       first_block = part * share;
       nblk = min(share, nblk - first_block);
@@ -215,8 +229,9 @@ __global__ __launch_bounds__(256, stream_wgs_per_cu(D)) void prefill_stream_kern
   } else {
     // keys that share a table entry are a multiple of a unit (a 64-key tile, a 32-key block); the first FIRST
     // units are requested here, the loop takes raw entries from there on
-    constexpr int UNIT = FORM == kPaged ? kKeysPerTile : kBlockKeys;
-    constexpr int FIRST = FORM == kPaged ? (SLOTS + 1) / 2 : SLOTS, RAW = FORM == kPaged ? 1 : 2;
+    constexpr bool TILES = form_tiles(FORM);
+    constexpr int UNIT = TILES ? kKeysPerTile : kBlockKeys;
+    constexpr int FIRST = TILES ? (SLOTS + 1) / 2 : SLOTS, RAW = TILES ? 1 : 2;
     const int per = a.bs / UNIT, last = a.w * per - 1;  // (entries exist for every unit of the table)
     const int unit0 = first_block * kBlockKeys / UNIT;
     auto column = [&](int unit) { return div_block(a, unit * UNIT); };
@@ -239,9 +254,9 @@ __global__ __launch_bounds__(256, stream_wgs_per_cu(D)) void prefill_stream_kern
     tab.read_in_block = uni(in_block(next)), tab.request_in_block = uni(in_block(next + RAW));
     tab.entry_ptr = uni(reinterpret_cast<uint64_t>(a.pt + (int64_t)b * a.pt_rs + column(next + RAW)));
     tab.entry_requests = uni(max((nblk - 1) / (UNIT / kBlockKeys) + 1 - FIRST - RAW, 0));
-    if constexpr (FORM == kPaged && D == 64) asm volatile(TTPA_STREAM_FIRST_PAGED_64);
-    else if constexpr (FORM == kPaged && D == 128) asm volatile(TTPA_STREAM_FIRST_PAGED_128);
-    else if constexpr (FORM == kPaged) asm volatile(TTPA_STREAM_FIRST_PAGED_256);
+    if constexpr (TILES && D == 64) asm volatile(TTPA_STREAM_FIRST_PAGED_64);
+    else if constexpr (TILES && D == 128) asm volatile(TTPA_STREAM_FIRST_PAGED_128);
+    else if constexpr (TILES) asm volatile(TTPA_STREAM_FIRST_PAGED_256);
     else if constexpr (D == 64) asm volatile(TTPA_STREAM_FIRST_PAGED32_64);
     else if constexpr (D == 128) asm volatile(TTPA_STREAM_FIRST_PAGED32_128);
     else asm volatile(TTPA_STREAM_FIRST_PAGED32_256);
@@ -280,7 +295,7 @@ __global__ __launch_bounds__(256, stream_wgs_per_cu(D)) void prefill_stream_kern
   const auto vo = Words<D / 32>::of(lane_vo);
   StreamItems it;
   it.k = 0, it.j = uni(item0), it.spg = uni(spg), it.nqt = uni(nqt);
-  it.sq = uni(a.sq), it.skv = uni(a.skv), it.offset = uni(offset), it.causal = uni(a.causal);
+  it.sq = uni(a.sq), it.skv = uni(skv), it.offset = uni(offset), it.causal = uni(a.causal);
   it.q_row_bytes = uni(2u * (uint32_t)a.q_ts), it.out_row_bytes = uni(2u * (uint32_t)a.out_ts);
   it.row0 = __builtin_amdgcn_readfirstlane(row0);
   it.key0 = uni(first_block * kBlockKeys);
@@ -296,6 +311,15 @@ __global__ __launch_bounds__(256, stream_wgs_per_cu(D)) void prefill_stream_kern
     lowest = offset + min(row0 + n, a.sq - 1) - a.window + 1 - h4;
     low_to = uni(offset + row0 + kRowsPerWave - a.window);
   }
+  // rows of a V block that the wavefront has requested: the lane's first one, its place in LDS (of K slot 0), and how many rows of the last block hold keys (a
+  // part that ends in front of the last block: all)
+  int tail_row = 0, tail_count = 32;
+  uint32_t tail_address = 0;
+  if constexpr (ENDS) {
+    tail_row = LOADS * wave * T::RPI + lane / T::CPR;
+    tail_address = req.m0_base + 16u * (uint32_t)lane;
+    tail_count = uni(min(skv - (first_block + nblk - 1) * kBlockKeys, kBlockKeys));
+  }
   // Everything behind the first requests of item 0, through the stored output rows of the last item.
   if constexpr (WIDE) asm volatile(TTPA_STREAM_LOOP_DENSE_WIDE_128);
   else if constexpr (FORM == kDense && D == 64) asm volatile(TTPA_STREAM_LOOP_DENSE_64);
@@ -307,15 +331,21 @@ __global__ __launch_bounds__(256, stream_wgs_per_cu(D)) void prefill_stream_kern
   else if constexpr (FORM == kPaged && D == 64) asm volatile(TTPA_STREAM_LOOP_PAGED_64);
   else if constexpr (FORM == kPaged && D == 128) asm volatile(TTPA_STREAM_LOOP_PAGED_128);
   else if constexpr (FORM == kPaged) asm volatile(TTPA_STREAM_LOOP_PAGED_256);
-  else if constexpr (D == 64) asm volatile(TTPA_STREAM_LOOP_PAGED32_64);
-  else if constexpr (D == 128) asm volatile(TTPA_STREAM_LOOP_PAGED32_128);
-  else asm volatile(TTPA_STREAM_LOOP_PAGED32_256);
+  else if constexpr (FORM == kPaged32 && D == 64) asm volatile(TTPA_STREAM_LOOP_PAGED32_64);
+  else if constexpr (FORM == kPaged32 && D == 128) asm volatile(TTPA_STREAM_LOOP_PAGED32_128);
+  else if constexpr (FORM == kPaged32) asm volatile(TTPA_STREAM_LOOP_PAGED32_256);
+  else if constexpr (FORM == kEnds && D == 64) asm volatile(TTPA_STREAM_LOOP_ENDS_64);
+  else if constexpr (FORM == kEnds && D == 128) asm volatile(TTPA_STREAM_LOOP_ENDS_128);
+  else if constexpr (FORM == kEnds) asm volatile(TTPA_STREAM_LOOP_ENDS_256);
+  else if constexpr (D == 64) asm volatile(TTPA_STREAM_LOOP_ENDS32_64);
+  else if constexpr (D == 128) asm volatile(TTPA_STREAM_LOOP_ENDS32_128);
+  else asm volatile(TTPA_STREAM_LOOP_ENDS32_256);
 }
 
 template <int D, int FORM>
 int launch_form(const PrefillArgs &a, hipStream_t st) {
   constexpr int lds = stream_lds_bytes(D, FORM == kDenseWide);
-  constexpr bool PAGED = FORM == kPaged || FORM == kPaged32;
+  constexpr bool PAGED = form_paged(FORM);
   static std::atomic<uint64_t> lds_ready{0};
   if (!ensure_dynamic_lds(reinterpret_cast<const void *>(&prefill_stream_kernel<D, FORM>), lds, lds_ready))
     return fail(TTPA_ERR_LAUNCH, "prefill: cannot reserve %d bytes of LDS", lds);
@@ -347,7 +377,7 @@ int launch_form(const PrefillArgs &a, hipStream_t st) {
   launch_dominant(&prefill_stream_kernel<D, FORM>, dim3(grid, b.parts), dim3(256), (size_t)lds, st, b);
   if (const int rc = check_launch("sdpa_prefill")) return rc;
   if (b.parts > 1) {
-    prefill_merge_kernel<D><<<dim3((b.sq + kRowsPerWave - 1) / kRowsPerWave, b.hq, b.batch), dim3(2 * D), 0, st>>>(b);
+    prefill_merge_kernel<D, form_ends(FORM)><<<dim3((b.sq + kRowsPerWave - 1) / kRowsPerWave, b.hq, b.batch), dim3(2 * D), 0, st>>>(b);
     return check_launch("sdpa_prefill (merge of the parts)");
   }
   return TTPA_OK;
@@ -357,6 +387,11 @@ template <int D>
 int launch_stream_d(const PrefillArgs &a, hipStream_t st) {
   if (a.pt) return a.bs % kKeysPerTile == 0 ? launch_form<D, kPaged>(a, st) : launch_form<D, kPaged32>(a, st);
   return a.window > 0 ? launch_form<D, kDenseWindow>(a, st) : launch_form<D, kDense>(a, st);
+}
+
+template <int D>
+int launch_ends_d(const PrefillArgs &a, hipStream_t st) {
+  return a.bs % kKeysPerTile == 0 ? launch_form<D, kEnds>(a, st) : launch_form<D, kEnds32>(a, st);
 }
 
 }  // namespace
