@@ -9,6 +9,10 @@
 // cross-lane moves; 16-byte loads and stores, 128 consecutive bytes of a row at a time.  A wavefront takes U
 // groups of 1024 / D heads of one token: its cosines, sines and weights are read once for all of them, and 2 U loads of rows are in flight.
 // 8192 tokens of 32 + 8 heads of 128: 168 MB in 32.5 us, 5.2 TB/s (a large copy by torch reaches 4.9).
+//
+// Positions on several axes (time, height, width): pair i turns by the position on axis pair_axes[i], which takes a token's angles from one row of the table per axis.
+// A wavefront puts a token's row together in LDS once, for all of its heads (TokenRow).  8191 tokens of 32 + 8 heads of 128 in 35.5 us, of one axis 35.7; 4900 of 16 + 16
+// of 64 in 10.8.
 #include "fp8_rows.h"
 
 #include <algorithm>
@@ -94,52 +98,61 @@ __device__ __forceinline__ Angles angles_of(const RopeArgs &a, const Place<D> &p
   return t;
 }
 
-// The same where every pair has a position of its own: that of its token on its axis.  Four neighbouring pairs are mostly of one axis, if all of them are in the whole
-// wavefront they are read as four; else one by one (axes in turn along the pairs).  A pair whose axis does not exist is not turned.
+// The same where every pair has a position of its own: that of its token on its axis.  Four neighbouring pairs are mostly of one axis; if all of them are, in the whole
+// wavefront, they are read as four, else one by one (axes in turn along the pairs).  No load under a condition: what is not turned reads the table's first row, or the
+// first pairs of a row, and takes 1 and 0 instead.  A pair whose axis does not exist, or whose position is outside the table, is not turned.
 constexpr int kMostAxes = 4;
 template <int D>
 struct PairAxes {
   int axis[2][4];
-  bool fours;
+  int at[2];  // columns of the cosines
   __device__ __forceinline__ PairAxes(const RopeArgs &a, const Place<D> &p) {
-    bool same = true;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int4 x = p.turned ? *reinterpret_cast<const int4 *>(a.pair_axes + (h ? p.cb : p.ca)) : make_int4(0, 0, 0, 0);
-      axis[h][0] = x.x, axis[h][1] = x.y, axis[h][2] = x.z, axis[h][3] = x.w;
-      same = same && x.x == x.y && x.x == x.z && x.x == x.w;
+      at[h] = p.turned ? (h ? p.cb : p.ca) : 0;
+      const int4 v = *reinterpret_cast<const int4 *>(a.pair_axes + at[h]);
+      axis[h][0] = v.x, axis[h][1] = v.y, axis[h][2] = v.z, axis[h][3] = v.w;
     }
-    fours = __builtin_amdgcn_ballot_w64(!same) == 0;
+  }
+  __device__ __forceinline__ bool in_fours() const {
+    bool same = true;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) same = same && axis[h][0] == axis[h][1] && axis[h][0] == axis[h][2] && axis[h][0] == axis[h][3];
+    return __builtin_amdgcn_ballot_w64(!same) == 0;
   }
 };
-struct AxisPositions {
-  int64_t at[kMostAxes];
-  __device__ __forceinline__ AxisPositions(const RopeArgs &a, int token) {
+struct AxisRows {
+  int at[kMostAxes];  // first element of the token's row of the table on each axis, or -1
+  __device__ __forceinline__ AxisRows(const RopeArgs &a, int token) {
 #pragma unroll
-    for (int i = 0; i < kMostAxes; ++i) at[i] = i < a.axes ? load_index(a.positions, a.positions_i64, i * a.pos_as + token) : -1;
+    for (int i = 0; i < kMostAxes; ++i) {
+      at[i] = -1;
+      if (i < a.axes) {
+        const int64_t pos = load_index(a.positions, a.positions_i64, i * a.pos_as + token);
+        at[i] = pos >= 0 && pos < a.max_positions ? (int)pos * (int)a.angle_rs : -1;
+      }
+    }
   }
-  __device__ __forceinline__ int64_t of(int axis) const {
-    int64_t x = -1;
+  __device__ __forceinline__ int of(int axis) const {
+    int x = -1;
 #pragma unroll
     for (int i = 0; i < kMostAxes; ++i) x = axis == i ? at[i] : x;
     return x;
   }
 };
 template <int D>
-__device__ __forceinline__ Angles angles_of(const RopeArgs &a, const Place<D> &p, const PairAxes<D> &pairs, const AxisPositions &positions) {
+__device__ __forceinline__ Angles angles_of(const RopeArgs &a, const Place<D> &p, const PairAxes<D> &pairs, const AxisRows &rows) {
   Angles t;
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) t.c[h][i] = 1.f, t.s[h][i] = 0.f;
-  if (pairs.fours) {
+  if (pairs.in_fours()) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int64_t pos = positions.of(pairs.axis[h][0]);
-      if (p.turned && pos >= 0 && pos < a.max_positions) {
-        const int64_t at = pos * a.angle_rs + (h ? p.cb : p.ca);
-        load4(a.angles, a.angles_f32, at, t.c[h]);
-        load4(a.angles, a.angles_f32, at + a.rotary / 2, t.s[h]);
+      const int row = rows.of(pairs.axis[h][0]);
+      const uint32_t at = (uint32_t)(max(row, 0) + pairs.at[h]);
+      load4(a.angles, a.angles_f32, at, t.c[h]);
+      load4(a.angles, a.angles_f32, at + a.rotary / 2, t.s[h]);
+      if (row < 0 || !p.turned) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t.c[h][i] = 1.f, t.s[h][i] = 0.f;
       }
     }
   } else {
@@ -147,15 +160,55 @@ __device__ __forceinline__ Angles angles_of(const RopeArgs &a, const Place<D> &p
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int64_t pos = positions.of(pairs.axis[h][i]);
-        if (p.turned && pos >= 0 && pos < a.max_positions) {
-          const int64_t at = pos * a.angle_rs + (h ? p.cb : p.ca) + i;
-          t.c[h][i] = load1(a.angles, a.angles_f32, at), t.s[h][i] = load1(a.angles, a.angles_f32, at + a.rotary / 2);
-        }
+        const int row = rows.of(pairs.axis[h][i]);
+        const uint32_t at = (uint32_t)(max(row, 0) + pairs.at[h] + i);
+        const float c = load1(a.angles, a.angles_f32, at), s = load1(a.angles, a.angles_f32, at + a.rotary / 2);
+        const bool known = row >= 0 && p.turned;
+        t.c[h][i] = known ? c : 1.f, t.s[h][i] = known ? s : 0.f;
       }
   }
   return t;
 }
+
+// The same for a wavefront that has one token: its lanes read the values of the token's row, which come from one row of the table per axis, value by value, and meet in
+// LDS.  Every lane for itself, one by one where the axes take turns, 4096 tokens of 16 + 8 heads of 256 took 33.6 us (22.7 with one axis), of 64 + 8 of 128 40.9 (34.4).
+template <int D>
+struct TokenRow {
+  static constexpr int LOADS = D / 64;
+  int axis[LOADS];
+  __device__ __forceinline__ TokenRow(const RopeArgs &a) {
+    const int half = a.rotary / 2;
+#pragma unroll
+    for (int k = 0; k < LOADS; ++k) {
+      const int v = min((int)(threadIdx.x & 63) + 64 * k, a.rotary - 1);
+      axis[k] = a.pair_axes[v < half ? v : v - half];
+    }
+  }
+  // `own`: rotary floats of the wavefront's.
+  __device__ __forceinline__ Angles angles(const RopeArgs &a, const Place<D> &p, const AxisRows &rows, float *own) const {
+    const int half = a.rotary / 2;
+    float x[LOADS];
+#pragma unroll
+    for (int k = 0; k < LOADS; ++k) {
+      const int v = min((int)(threadIdx.x & 63) + 64 * k, a.rotary - 1), row = rows.of(axis[k]);
+      const float y = load1(a.angles, a.angles_f32, (uint32_t)(max(row, 0) + v));
+      x[k] = row >= 0 ? y : v < half ? 1.f : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < LOADS; ++k) own[min((int)(threadIdx.x & 63) + 64 * k, a.rotary - 1)] = x[k];  // (past the end: the last one again)
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    Angles t;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int at = p.turned ? (h ? p.cb : p.ca) : 0;
+      load4(own, 1, at, t.c[h]);
+      load4(own, 1, at + half, t.s[h]);
+    }
+    return t;
+  }
+};
 
 struct Weights {
   float a[8], b[8];
@@ -221,15 +274,10 @@ __device__ __forceinline__ RowPart turn_row(const RopeArgs &a, const Place<D> &p
   return o;
 }
 
-template <int D, bool AXES>
-__device__ __forceinline__ Angles token_angles(const RopeArgs &a, const Place<D> &p, int token) {
-  if constexpr (AXES) {
-    const PairAxes<D> pairs(a, p);
-    return angles_of<D>(a, p, pairs, AxisPositions(a, token));
-  } else {
-    return angles_of<D>(a, p, load_index(a.positions, a.positions_i64, token));
-  }
-}
+struct Unused {
+  template <typename... T>
+  __device__ __forceinline__ Unused(const T &...) {}
+};
 
 // Wavefront `part` of a token's: heads [part * U * R, ...) of the queries' and then the keys' (R rows per wavefront).
 template <int D, int U, bool AXES>
@@ -240,13 +288,20 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeArgs a, int parts
   if (token >= a.tokens) return;
   const Place<D> p(a);
   const int r = (int)(threadIdx.x & 63) / LPR, heads = a.hq + a.hk;
+  std::conditional_t<AXES, TokenRow<D>, Unused> row(a);  // (asked for in front of the rows: loads come back in order)
   RowPart x[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int h = min((part * U + u) * R + r, heads - 1);  // (rows past the last head: that one again, and not stored)
     x[u] = h < a.hq ? load_part(a.q + token * a.q_ts + h * a.q_hs, p.fa, p.fb) : load_part(a.k + token * a.k_ts + (h - a.hq) * a.k_hs, p.fa, p.fb);
   }
-  const Angles t = token_angles<D, AXES>(a, p, token);
+  Angles t;
+  if constexpr (AXES) {
+    __shared__ __attribute__((aligned(16))) float s_angles[4][D];
+    t = row.angles(a, p, AxisRows(a, token), s_angles[threadIdx.x >> 6]);
+  } else {
+    t = angles_of<D>(a, p, load_index(a.positions, a.positions_i64, token));
+  }
   Weights wq, wk;
   if (a.q_weight) load_weights<D>(a.q_weight, a.weights_f32, p, wq);
   if (a.k_weight) load_weights<D>(a.k_weight, a.weights_f32, p, wk);
@@ -290,7 +345,10 @@ __global__ __launch_bounds__(256) void qk_norm_rope_rows_kernel(RopeArgs a, uint
     if (h >= heads) ++n, h -= heads;
     token[u] = (int)n, head[u] = (int)h;
   }
+  std::conditional_t<AXES, PairAxes<D>, Unused> pairs(a, p);
   int64_t pos[U];
+  std::conditional_t<AXES, AxisRows, Unused> rows_of[U] = {{a, token[0]}, {a, token[1]}};
+  static_assert(U == 2, "a place for each row");
   if constexpr (!AXES) {
 #pragma unroll
     for (int u = 0; u < U; ++u) pos[u] = load_index(a.positions, a.positions_i64, token[u]);
@@ -303,7 +361,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_rows_kernel(RopeArgs a, uint
   Angles t[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    if constexpr (AXES) t[u] = token_angles<D, true>(a, p, token[u]);
+    if constexpr (AXES) t[u] = angles_of<D>(a, p, pairs, rows_of[u]);
     else t[u] = angles_of<D>(a, p, pos[u]);
   }
   Weights wq, wk;
@@ -419,6 +477,12 @@ int launch_rope(const RopeArgs &a, hipStream_t st) {
   // stores 44.5 / 41.9 / 39.0 / 36.9.  (Those of few rows are ordinary: what is read next is read from L2.)
   int best = 1;
   if ((int64_t)a.tokens * groups >= 8192) {
+    // (several axes: a token's row of angles is put together once per wavefront.  16384 tokens of 16 + 16 heads of 64 35.3 -> 29.7 us, 43.6 -> 29.3 with the axes in
+    // turn; 8 + 1 of 128 26.1 -> 27.2 and 39.9 -> 26.9; of half a wavefront of heads, which stays with the rows, 8 + 2 of 64 17.0 -> 19.7 and 21.0 -> 19.7)
+    if (AXES && groups == 2) {
+      go(std::integral_constant<int, 2>{});
+      return check_launch("qk_norm_rope");
+    }
     if (groups <= 2) {
       constexpr int U = 2, PER = 4 * U * R;  // rows of a workgroup
       const int64_t rows = (int64_t)a.tokens * (a.hq + a.hk);
@@ -519,6 +583,8 @@ extern "C" int ttpa_qk_norm_rope_axes(void *q_out, int64_t q_out_token_stride, i
                 k_weight, eps, tokens, q_heads, k_heads, rotary, interleaved, pair_axes, axes, positions_axis_stride};
   TTPA_REQUIRE(k_heads > 0, "qk_norm_rope: non-positive dimension");
   TTPA_REQUIRE(pair_axes && aligned16(pair_axes), "qk_norm_rope: pair_axes must be a 16-byte aligned pointer");
+  TTPA_REQUIRE(max_positions > 0 && cos_sin_row_stride >= 0 && (max_positions - 1) * cos_sin_row_stride + rotary < (1ll << 31),
+               "qk_norm_rope: a table of angles for several axes holds less than 2^31 elements");
   if (axes < 1 || axes > kMostAxes) return fail(TTPA_ERR_UNSUPPORTED, "qk_norm_rope: %d axes; supported 1 to %d", axes, kMostAxes);
   if (int rc = check_rope(a, head_size, true)) return rc;
   if (tokens == 0) return TTPA_OK;
