@@ -42,7 +42,7 @@ struct CrossArgs {
   int batch, hkv, g, s, bs, w, nb;
   float scale_log2e;
   uint32_t runs, runs_inv;  // runs of keys per block, and floor((2^32 - 1) / runs)
-  int row_blocks, parts, share;  // share: tiles of a part
+  int row_blocks, parts, share;  // share: tiles of a part at least
   float *slots;  // [batch * hkv * row_blocks][parts]: ROWS * D values, ROWS maxima, ROWS sums
 };
 
@@ -69,7 +69,7 @@ __device__ __forceinline__ int cross_vkey(int row) {
   const int run = row / RUN & 1, r = row & 3;
   return D == 64 ? 2 * ((r >> 1) + 2 * run) : 2 * (r + 4 * run);
 }
-// Parts of a user's keys, of a.share tiles or a few more each.
+// Parts of a user's keys, of a.share tiles or more each.
 template <int D>
 __device__ __forceinline__ int cross_parts(const CrossArgs &a, int keys) {
   constexpr int TILE = cross_tile<D>();

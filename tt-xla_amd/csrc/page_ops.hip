@@ -1,5 +1,8 @@
 // Moves inside paged caches, for all layers in one call: copies of whole blocks (forks of sequences, moves of pages) and compaction of sequences
-// (chosen tokens move together).  Bytes are moved as they are, so any element type will do.  Both are bound by memory: read once, written once.
+// (chosen tokens move together).  Bytes are moved as they are, so any element type will do.  Both are bound by memory: read once, written once; a large copy by torch
+// reaches 5.3 TB/s both ways together on this card.  250 blocks of 64 x 8 heads x 128 bytes in 24 caches (786 MB) 157 us, 5.0 TB/s (164 with ordinary loads and stores);
+// half of the last three quarters of 4 x 8192 tokens, K and V of 16 layers of 8 heads of 128 (1.6 GB) 328 us, 4.9; of 2048 ... 8192 tokens (867 MB), where the longest
+// user's chain of batches ends the launch, 178 us (203 with one batch on its way, 191 with streaming stores).
 #include "common.h"
 
 #include <algorithm>
@@ -94,14 +97,14 @@ __global__ __launch_bounds__(kThreads) void copy_blocks_kernel(CopyArgs a) {
       if (copies(a, s[i], t[i])) {
 #pragma unroll
         for (int c = 0; c < kChunks; ++c)
-          if (first + c * kStep < a.block_bytes) x[i][c] = *reinterpret_cast<const T *>(cache + s[i] * a.block_bytes + first + c * kStep);
+          if (first + c * kStep < a.block_bytes) x[i][c] = __builtin_nontemporal_load(reinterpret_cast<const T *>(cache + s[i] * a.block_bytes + first + c * kStep));
       }
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i)
       if (copies(a, s[i], t[i])) {
 #pragma unroll
         for (int c = 0; c < kChunks; ++c)
-          if (first + c * kStep < a.block_bytes) *reinterpret_cast<T *>(cache + t[i] * a.block_bytes + first + c * kStep) = x[i][c];
+          if (first + c * kStep < a.block_bytes) __builtin_nontemporal_store(x[i][c], reinterpret_cast<T *>(cache + t[i] * a.block_bytes + first + c * kStep));
       }
   }
 }
@@ -110,82 +113,135 @@ struct KeepArgs {
   uint8_t *caches[kMostCaches];
   const int32_t *pt, *kept, *kept_lens, *first;
   int64_t pt_rs, kept_rs;
-  int most, hkv, bs, w, nb, row_bytes;
+  int most, hkv, bs, w, nb, row_bytes, n_caches, at_once;  // at_once: caches that a workgroup of few rows takes
   int col_shift;  // log2 of the 16-byte chunks of a row that a workgroup takes
 };
 
-// Rows of one user and head of one cache: row first + i takes what row kept[i] held, i in batches of B rows.  A row never moves back (an entry that would is
-// skipped), so no row is read behind the batch that overwrites it, and all rows of a batch are read before one of them is written: a barrier per batch.
-// Three batches are on their way: the rows of one, the pages of the next, the entries of the one behind.
-template <int THREADS>
-__global__ __launch_bounds__(THREADS) void keep_rows_kernel(KeepArgs a) {
-  constexpr int U = 8;
-  __shared__ int64_t s_from[2][THREADS], s_to[2][THREADS];
-  const int u = blockIdx.x / a.hkv, h = blockIdx.x - u * a.hkv;
-  const int cols = 1 << a.col_shift, col = threadIdx.x & (cols - 1), row = (int)threadIdx.x >> a.col_shift;
-  const int per = THREADS >> a.col_shift, batch = min(per * U, THREADS);  // rows of a pass, of a batch
-  const int n = max(min(a.kept_lens[u], a.most), 0);
-  if (n == 0) return;
-  const int64_t first = a.first ? a.first[u] : 0;
-  const int32_t *const kept = a.kept + (int64_t)u * a.kept_rs, *const pt = a.pt + (int64_t)u * a.pt_rs;
-  uint8_t *const cache = a.caches[blockIdx.y] + (int64_t)(((int)blockIdx.z << a.col_shift) + col) * 16;
-  const bool plans = (int)threadIdx.x < batch;
-  const int64_t room = (int64_t)a.w * a.bs;
-  // thread j plans row j of a batch: its entry, its pages, its offsets
-  const auto entry = [&](int b) {
-    const int64_t i = (int64_t)b * batch + threadIdx.x;
-    return plans && i < n ? kept[i] : -1;
-  };
+// Where the rows of one user and head go: row first + i takes what row kept[i] held.  A row never moves back: an entry that would is skipped, and so is what stays where it
+// is, or lies outside the table's room or the cache.
+struct KeepPlan {
+  const KeepArgs &a;
+  const int u, h, n;
+  const int64_t first;
   struct Pages {
     int from, to;
   };
-  const auto moves = [&](int b, int s) {
-    const int64_t d = first + (int64_t)b * batch + threadIdx.x;
-    return plans && d >= 0 && (int64_t)s > d && s < room;
+  struct Offsets {
+    int64_t from, to;  // bytes in a cache, or -1
   };
-  const auto pages = [&](int b, int s) {
+  __device__ __forceinline__ KeepPlan(const KeepArgs &args, int user, int head)
+      : a(args), u(user), h(head), n(max(min(args.kept_lens[user], args.most), 0)), first(args.first ? args.first[user] : 0) {}
+  __device__ __forceinline__ int entry(int64_t i) const { return i < n ? a.kept[u * a.kept_rs + i] : -1; }
+  __device__ __forceinline__ bool moves(int64_t i, int s) const { return first + i >= 0 && (int64_t)s > first + i && s < (int64_t)a.w * a.bs; }
+  __device__ __forceinline__ Pages pages(int64_t i, int s) const {
     Pages p = {-1, -1};
-    if (moves(b, s)) p.from = pt[s / a.bs], p.to = pt[(int)(first + (int64_t)b * batch + threadIdx.x) / a.bs];
+    if (moves(i, s)) p.from = a.pt[u * a.pt_rs + s / a.bs], p.to = a.pt[u * a.pt_rs + (int)(first + i) / a.bs];
     return p;
-  };
-  const auto plan = [&](int b, int s, const Pages &p) {
-    if (!plans) return;
-    int64_t from = -1, to = -1;
-    if (moves(b, s) && (unsigned)p.from < (unsigned)a.nb && (unsigned)p.to < (unsigned)a.nb) {
-      const int d = (int)(first + (int64_t)b * batch + threadIdx.x);
-      from = (((int64_t)p.from * a.hkv + h) * a.bs + s % a.bs) * a.row_bytes;
-      to = (((int64_t)p.to * a.hkv + h) * a.bs + d % a.bs) * a.row_bytes;
+  }
+  __device__ __forceinline__ Offsets offsets(int64_t i, int s, const Pages &p) const {
+    Offsets o = {-1, -1};
+    if (moves(i, s) && (unsigned)p.from < (unsigned)a.nb && (unsigned)p.to < (unsigned)a.nb) {
+      o.from = (((int64_t)p.from * a.hkv + h) * a.bs + s % a.bs) * a.row_bytes;
+      o.to = (((int64_t)p.to * a.hkv + h) * a.bs + (int)(first + i) % a.bs) * a.row_bytes;
     }
-    s_from[b & 1][threadIdx.x] = from, s_to[b & 1][threadIdx.x] = to;
+    return o;
+  }
+};
+
+// Many rows of one user and head of one cache, in batches in order.  No row is read behind the batch that overwrites it (rows do not move back), and all rows of a
+// batch are read before one of them is written: a barrier per batch.  Two batches of rows are on their way, and the pages and entries of the next two.
+__global__ __launch_bounds__(256) void keep_rows_kernel(KeepArgs a) {
+  constexpr int U = 8, THREADS = 256;
+  __shared__ KeepPlan::Offsets s_plan[3][THREADS];
+  const int u = blockIdx.x / a.hkv;
+  const KeepPlan plan(a, u, blockIdx.x - u * a.hkv);
+  if (plan.n == 0) return;
+  const int cols = 1 << a.col_shift, col = threadIdx.x & (cols - 1), row = (int)threadIdx.x >> a.col_shift;
+  const int per = THREADS >> a.col_shift, batch = min(per * U, THREADS), batches = (plan.n + batch - 1) / batch;  // rows of a pass, of a batch
+  uint8_t *const cache = a.caches[blockIdx.y] + (int64_t)(((int)blockIdx.z << a.col_shift) + col) * 16;
+  // thread j plans row j of a batch
+  const auto at = [&](int b) { return (int64_t)b * batch + threadIdx.x; };
+  const bool plans = (int)threadIdx.x < batch;
+  const auto put = [&](int b, int s, const KeepPlan::Pages &p) {
+    if (plans) s_plan[b % 3][threadIdx.x] = plan.offsets(at(b), s, p);
   };
-  const int batches = (n + batch - 1) / batch;
-  u32x4 x[U];
-  const auto load = [&](int b) {
+  u32x4 x[2][U];
+  const auto load = [&](int b, u32x4 (&v)[U]) {
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const int r = row + i * per;
-      const int64_t from = r < batch ? s_from[b & 1][r] : -1;
-      if (from >= 0) x[i] = *reinterpret_cast<const u32x4 *>(cache + from);
+      const int64_t from = b < batches && r < batch ? s_plan[b % 3][r].from : -1;
+      if (from >= 0) v[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(cache + from));
     }
   };
-  int s0 = entry(0), s1 = entry(1);
-  plan(0, s0, pages(0, s0));
-  Pages p1 = pages(1, s1);
-  int s2 = entry(2);
-  __syncthreads();  // the first plan is there
-  for (int b = 0; b < batches; ++b) {
-    load(b);
-#pragma unroll
-    for (int i = 0; i < U; ++i) asm volatile("" : "+v"(x[i]));  // (they have arrived)
+  const int s0 = plan.entry(at(0)), s1 = plan.entry(at(1));
+  int s2 = plan.entry(at(2)), s3 = plan.entry(at(3));
+  put(0, s0, plan.pages(at(0), s0)), put(1, s1, plan.pages(at(1), s1));
+  KeepPlan::Pages p2 = plan.pages(at(2), s2);
+  __syncthreads();  // the first two plans are there
+  load(0, x[0]);
+  const auto step = [&](int b, u32x4 (&now)[U], u32x4 (&next)[U]) {
+    load(b + 1, next);
+    put(b + 2, s2, p2);
+    s2 = s3, p2 = plan.pages(at(b + 3), s2), s3 = plan.entry(at(b + 4));
     int64_t to[U];
 #pragma unroll
-    for (int i = 0; i < U; ++i) to[i] = row + i * per < batch ? s_to[b & 1][row + i * per] : -1;
-    plan(b + 1, s1, p1);
-    s1 = s2, p1 = pages(b + 2, s1), s2 = entry(b + 3);
-    __syncthreads();  // everybody has read batch b, and the next plan is there
+    for (int i = 0; i < U; ++i) to[i] = row + i * per < batch ? s_plan[b % 3][row + i * per].to : -1;
+#pragma unroll
+    for (int i = 0; i < U; ++i) asm volatile("" : "+v"(now[i]));  // (they have arrived)
+    __syncthreads();  // everybody has read batch b, and plan b + 2 is there
 #pragma unroll
     for (int i = 0; i < U; ++i)
-      if (to[i] >= 0) *reinterpret_cast<u32x4 *>(cache + to[i]) = x[i];
+      if (to[i] >= 0) *reinterpret_cast<u32x4 *>(cache + to[i]) = now[i];
+  };
+  for (int b = 0; b < batches; b += 2) {
+    step(b, x[0], x[1]);
+    if (b + 1 < batches) step(b + 1, x[1], x[0]);
+  }
+}
+
+// Few rows (no more than a wavefront takes in a pass of U loads): one wavefront per user and head plans them once and moves them in up to kCachesAtOnce caches, one after
+// the other with the next one's rows on their way.  32 users' six of 16 drafted tokens, K and V of 32 layers of 8 heads of 128 (50 MB): 11.2 us, 13.4 with a wavefront per
+// cache; one user's 20 of 40 3.5.
+constexpr int kCachesAtOnce = 8, kFewPasses = 8;
+__global__ __launch_bounds__(64) void keep_few_rows_kernel(KeepArgs a) {
+  constexpr int U = kFewPasses;
+  __shared__ KeepPlan::Offsets s_plan[64];
+  const int u = blockIdx.x / a.hkv;
+  const KeepPlan plan(a, u, blockIdx.x - u * a.hkv);
+  if (plan.n == 0) return;
+  const int cols = 1 << a.col_shift, col = threadIdx.x & (cols - 1), row = (int)threadIdx.x >> a.col_shift, per = 64 >> a.col_shift;
+  const int s = plan.entry(threadIdx.x);
+  s_plan[threadIdx.x] = plan.offsets(threadIdx.x, s, plan.pages(threadIdx.x, s));
+  __syncthreads();
+  int64_t from[U], to[U];
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const int r = row + i * per;
+    from[i] = r < min(plan.n, 64) ? s_plan[r].from : -1, to[i] = r < min(plan.n, 64) ? s_plan[r].to : -1;
+  }
+  const int64_t chunk = (int64_t)(((int)blockIdx.z << a.col_shift) + col) * 16;
+  const int c0 = blockIdx.y * a.at_once, end = min(c0 + a.at_once, a.n_caches);
+  u32x4 x[2][U];
+  const auto load = [&](int c, u32x4 (&v)[U]) {
+    const uint8_t *const cache = a.caches[min(c, a.n_caches - 1)] + chunk;
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (i * per < plan.n && from[i] >= 0) v[i] = *reinterpret_cast<const u32x4 *>(cache + from[i]);
+  };
+  const auto step = [&](int c, u32x4 (&now)[U], u32x4 (&next)[U]) {
+    load(c + 1, next);
+#pragma unroll
+    for (int i = 0; i < U; ++i) asm volatile("" : "+v"(now[i]));  // (all of a cache's rows have arrived before one of them is written)
+    uint8_t *const cache = a.caches[c] + chunk;
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (i * per < plan.n && to[i] >= 0) *reinterpret_cast<u32x4 *>(cache + to[i]) = now[i];
+  };
+  load(c0, x[0]);
+  for (int c = c0; c < end; c += 2) {
+    step(c, x[0], x[1]);
+    if (c + 1 < end) step(c + 1, x[1], x[0]);
   }
 }
 
@@ -251,15 +307,21 @@ extern "C" int ttpa_keep_cache_tokens(void *const *caches_host, int32_t n_caches
   a.most = most_kept, a.hkv = heads, a.bs = block_size, a.w = table_width, a.nb = num_blocks, a.row_bytes = row_bytes;
   const int chunks = row_bytes / 16;
   while (a.col_shift < 4 && chunks % (2 << a.col_shift) == 0) ++a.col_shift;
+  // narrower slices of rows, down to 128 bytes, while the workgroups leave CUs without one: one user's 4096 tokens of 8 heads of 128, half of them kept, K and V of one
+  // layer 21.6 -> 12.7 us, of four 26.5 -> 16.7 (64 bytes 11.7 and 15.7)
+  while (a.col_shift > 3 && (int64_t)users * heads * n_caches * (chunks >> a.col_shift) < std::max(device_cus(), 1)) --a.col_shift;
   hipStream_t st = static_cast<hipStream_t>(stream);
   for (int32_t c0 = 0; c0 < n_caches; c0 += kMostCaches) {
     const int n = std::min(n_caches - c0, kMostCaches);
     for (int i = 0; i < n; ++i) a.caches[i] = static_cast<uint8_t *>(caches_host[c0 + i]);
-    const dim3 grid((unsigned)(users * heads), (unsigned)n, (unsigned)(chunks >> a.col_shift));
-    if (most_kept <= 32)
-      keep_rows_kernel<64><<<grid, dim3(64), 0, st>>>(a);
+    a.n_caches = n;
+    const unsigned segments = (unsigned)(users * heads), slices = (unsigned)(chunks >> a.col_shift);
+    // (wavefronts for every SIMD twice first)
+    a.at_once = (int)std::min<int64_t>(kCachesAtOnce, std::max<int64_t>(1, (int64_t)segments * slices * n / (8 * std::max(device_cus(), 1))));
+    if (most_kept <= std::min(64, kFewPasses * (64 >> a.col_shift)))
+      keep_few_rows_kernel<<<dim3(segments, (unsigned)((n + a.at_once - 1) / a.at_once), slices), dim3(64), 0, st>>>(a);
     else
-      keep_rows_kernel<256><<<grid, dim3(256), 0, st>>>(a);
+      keep_rows_kernel<<<dim3(segments, (unsigned)n, slices), dim3(256), 0, st>>>(a);
     if (const int rc = check_launch("keep_cache_tokens")) return rc;
   }
   return TTPA_OK;
