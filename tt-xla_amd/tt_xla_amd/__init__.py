@@ -14,7 +14,9 @@ from . import fp8_ops  # noqa: F401
 from . import media_ops  # noqa: F401
 from .attention import TTAttentionBackend, TTAttentionBackendImpl, TTMetadata  # noqa: F401
 from .attention_mla import TTMLAAttentionBackend, TTMLAAttentionBackendImpl  # noqa: F401
-from .metadata import PagedMetadataBuilder  # noqa: F401
+from .kv_blocks import CachePages, copy_cache_blocks, copy_kv_blocks  # noqa: F401
+from .metadata import CrossMetadataBuilder, PagedMetadataBuilder  # noqa: F401
 
 __all__ = ["TTAttentionBackend", "TTAttentionBackendImpl", "TTMLAAttentionBackend",
-           "TTMLAAttentionBackendImpl", "TTMetadata", "PagedMetadataBuilder", "custom_ops", "fp8_ops", "media_ops"]
+           "TTMLAAttentionBackendImpl", "TTMetadata", "PagedMetadataBuilder", "CrossMetadataBuilder", "CachePages", "copy_cache_blocks",
+           "copy_kv_blocks", "custom_ops", "fp8_ops", "media_ops"]

@@ -39,10 +39,11 @@ try:  # pragma: no cover - vLLM is not part of the test image
     _DECODER = AttentionType.DECODER
     _ENCODER = AttentionType.ENCODER
     _ENCODER_ONLY = AttentionType.ENCODER_ONLY
+    _ENCODER_DECODER = AttentionType.ENCODER_DECODER
 except Exception:  # vLLM absent: same surface, no base classes
     _BackendBase = object
     _ImplBase = object
-    _DECODER, _ENCODER, _ENCODER_ONLY = "decoder", "encoder", "encoder_only"
+    _DECODER, _ENCODER, _ENCODER_ONLY, _ENCODER_DECODER = "decoder", "encoder", "encoder_only", "encoder_decoder"
 
 # Head sizes are padded to a multiple of this by the model runner (reference :37-38).
 TT_HEAD_SIZE_ALIGNMENT = 32
@@ -80,6 +81,9 @@ class TTMetadata:
     chunk_end       position behind the last row of a continuation chunk, where the host knows it: eager passes are
                     laid out for that many keys and not for all that the page table has room for.  Never what is
                     attended: chunk_start_idx says that.
+    encoder_lens    [users] int32, cross attention layers: states of each user's encoder that are in the cache, which all of its
+                    tokens attend; 0 where a user has none (its rows are zeros).
+    most_encoder_len  the largest of them, where the host knows it, as chunk_end: a bound, never what is attended.
     """
 
     cache_position: Optional[torch.Tensor]
@@ -91,6 +95,8 @@ class TTMetadata:
     batch_idx: Optional[torch.Tensor] = None
     num_users: Optional[int] = None
     chunk_end: Optional[int] = None
+    encoder_lens: Optional[torch.Tensor] = None
+    most_encoder_len: Optional[int] = None
 
     def __init__(
         self,
@@ -104,6 +110,8 @@ class TTMetadata:
         batch_idx: Optional[torch.Tensor] = None,
         num_users: Optional[int] = None,
         chunk_end: Optional[int] = None,
+        encoder_lens: Optional[torch.Tensor] = None,
+        most_encoder_len: Optional[int] = None,
     ):
         self.cache_position = cache_position
         self.attn_mask = attn_mask
@@ -115,6 +123,8 @@ class TTMetadata:
         self.num_users = num_users
         self.batch_idx = batch_idx
         self.chunk_end = chunk_end
+        self.encoder_lens = encoder_lens
+        self.most_encoder_len = most_encoder_len
 
 
 class TTAttentionMetadataBuilder:
@@ -250,10 +260,16 @@ class TTAttentionBackendImpl(_ImplBase):
         self.sparse_kept_blocks = sparse_kept_blocks
         if alibi_slopes is not None:
             raise NotImplementedError("Alibi slopes is not supported.")
-        if attn_type not in (_DECODER, _ENCODER, _ENCODER_ONLY):
+        if attn_type not in (_DECODER, _ENCODER, _ENCODER_ONLY, _ENCODER_DECODER):
             raise NotImplementedError(
-                f"TT attention only supports encoder or decoder attention, but got {attn_type}."
+                f"TT attention only supports encoder, decoder or cross attention, but got {attn_type}."
             )
+        self.cross = attn_type == _ENCODER_DECODER
+        if self.cross:
+            if sliding_window is not None or sinks is not None or sparse_kept_blocks is not None or functional_cache_ops or kv_cache_dtype not in ("auto", "bfloat16"):
+                raise NotImplementedError("cross attention is built for bfloat16 caches that are updated in place, without sliding windows, sinks and sparse decode")
+            if head_size not in (64, 128, 256):
+                raise NotImplementedError(f"cross attention is built for head sizes of 64, 128 and 256, not {head_size}")
         self.kv_cache_stored = None
         self.kv_cache_quantized_dtype = None
         if kv_cache_dtype != "auto":
@@ -283,6 +299,9 @@ class TTAttentionBackendImpl(_ImplBase):
         the result is written into ``output`` [tokens, Hq*D]."""
         assert attn_metadata is not None, "TT attention requires metadata."
         assert output is not None, "TT attention requires an output buffer."
+        if self.cross:
+            self._cross_pass(query, key, value, kv_cache, attn_metadata, output)
+            return
         # (empty caches stand in while vLLM profiles memory, of any type: such a pass is the ordinary one without a cache)
         if isinstance(kv_cache, (list, tuple)) and kv_cache[0].dtype == torch.float8_e4m3fn and kv_cache[0].numel() > 0:
             self._fp8_pass(query, key, value, kv_cache, attn_metadata, output)
@@ -434,6 +453,51 @@ class TTAttentionBackendImpl(_ImplBase):
                                                      sliding_window_size=self.sliding_window)
         if out is None:
             output.copy_(into.reshape(-1, self.num_heads * self.head_size).reshape_as(output))
+
+    def _cross_pass(self, query, key, value, kv_cache, attn_metadata: TTMetadata, output) -> None:
+        """A cross attention layer's pass, prompt or step: an encoder's new states [fill rows * tokens, Hkv*D], if any come with the pass, into the cache
+        through the rows ``batch_idx`` of the fill table, then the attention of all users' tokens to what the cache holds.  (Without a cache, while vLLM
+        profiles memory, the pass's own states are attended.)"""
+        if attn_metadata.attn_mask is not None:
+            raise NotImplementedError("cross attention is built without masks")
+        users = attn_metadata.num_users
+        assert users is not None, "num_users must be provided in attn_metadata."
+        if (key is None) != (value is None):
+            raise ValueError("a cross attention pass has keys and values, or neither")
+        ops = torch.ops.tt
+        q = self._normalize_to_attention_format(query, "query", self.num_heads, self.head_size, users)
+        caches = list(kv_cache) if isinstance(kv_cache, (list, tuple)) else [kv_cache]
+        cached = len(caches) > 0 and caches[0].numel() > 0
+        if cached:
+            if len(caches) != 2 or caches[0].dtype != torch.bfloat16 or caches[0].dim() != 4 or caches[0].shape[2] % 32:
+                raise NotImplementedError("cross attention is built for bfloat16 caches [k, v] of blocks of a multiple of 32 tokens, not for "
+                                          f"{[(tuple(t.shape), t.dtype) for t in caches]}")
+            if attn_metadata.encoder_lens is None:
+                raise ValueError("cross attention needs encoder_lens in attn_metadata")
+        elif key is None:
+            raise ValueError("cross attention without a cache needs the encoder's keys and values")
+        out = None
+        if output.dtype == torch.bfloat16 and output.is_contiguous() and output.data_ptr() % 16 == 0 and output.numel() == q.numel():
+            out = output.view(q.shape)
+        into = torch.empty(q.shape, dtype=query.dtype, device=query.device) if out is None else out
+        if cached:
+            if key is not None and self.kv_sharing_target_layer_name is None:
+                rows = attn_metadata.batch_idx
+                assert rows is not None, "batch_idx must be provided for an encoder's states."
+                k, v = (self._normalize_to_attention_format(x, n, self.num_kv_heads, self.head_size, rows.numel()) for x, n in ((key, "key"), (value, "value")))
+                ops.paged_fill_kv_cache_(caches[0], caches[1], k.transpose(1, 2), v.transpose(1, 2), attn_metadata.fill_page_table, batch_idx=rows)
+            # (what a graph captures is replayed for other lengths: it has to have room for all that the table holds)
+            most = 0 if torch.cuda.is_current_stream_capturing() else attn_metadata.most_encoder_len or 0
+            ops.paged_cross_attention_out(q.transpose(1, 2), caches[0], caches[1], attn_metadata.page_table, attn_metadata.encoder_lens,
+                                          into.transpose(1, 2), scale=self.scale, most_keys=most)
+        else:
+            k, v = (self._normalize_to_attention_format(x, n, self.num_kv_heads, self.head_size, users) for x, n in ((key, "key"), (value, "value")))
+            tokens = q.shape[1]  # (that operator takes whole blocks of 32 rows)
+            padded = torch.nn.functional.pad(q, (0, 0, 0, 0, 0, -tokens % 32))
+            into.copy_(ops.scaled_dot_product_attention(padded.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), is_causal=False,
+                                                        scale=self.scale).transpose(1, 2)[:, :tokens])
+        if out is None:
+            output.copy_(into.reshape(output.shape))
 
     def _output_view(self, output: torch.Tensor, inputs) -> Optional[torch.Tensor]:
         """``output`` as [users, tokens, heads, head_size] without a copy, or None."""

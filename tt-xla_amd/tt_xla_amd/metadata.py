@@ -1,5 +1,7 @@
 """Host-side construction of the paged-attention metadata, free of vLLM.
 
+:class:`CrossMetadataBuilder`, at the end, makes that of cross attention layers.
+
 The attention operators consume four small integer tensors per pass
 (``cache_position``, ``page_table``, ``fill_page_table``, ``chunk_start_idx``) plus
 ``batch_idx``.  In tt-xla they are produced inside the vLLM model runner's
@@ -323,3 +325,56 @@ class PagedMetadataBuilder:
             chunk_end=chunk_end,
         )
         return PassPlan(metadata, lead, padded_tokens, positions, is_decode)
+
+
+class CrossMetadataBuilder:
+    """Builds :class:`TTMetadata` for cross attention layers, whose cache holds an encoder's states, from scheduler state.  Device buffers are kept per row
+    count, as :class:`PagedMetadataBuilder` does, so that a step can be replayed from a HIP graph.
+
+    max_num_blocks_per_req  width of the page table: blocks of the longest encoder output.
+    """
+
+    def __init__(self, block_size: int, max_num_blocks_per_req: int, device: torch.device | str = "cpu"):
+        self.block_size = int(block_size)
+        self.width = int(max_num_blocks_per_req)
+        self.device = torch.device(device)
+        self._buffers: Dict[int, Tuple[torch.Tensor, torch.Tensor]] = {}
+
+    def prepare(
+        self,
+        block_table: np.ndarray,
+        encoder_lens: np.ndarray,
+        new_rows: Sequence[int] = (),
+        target_num_reqs: Optional[int] = None,
+    ) -> TTMetadata:
+        """One pass over requests ``0..len(encoder_lens)``.
+
+        block_table   [reqs, <= width] int32 physical block ids; of each row those of the request's length count
+        encoder_lens  [reqs] states per request (0: a request without an encoder's output)
+        new_rows      requests whose states come with this pass, in the order of its keys and values
+        target_num_reqs  padded row count (>= reqs); padded rows have no states
+        """
+        encoder_lens = np.asarray(encoder_lens, dtype=np.int64)
+        block_table = np.asarray(block_table)
+        reqs = int(encoder_lens.size)
+        rows = reqs if target_num_reqs is None else int(target_num_reqs)
+        assert 0 < reqs <= rows and block_table.shape[0] >= reqs, f"{reqs} requests, {rows} rows, {block_table.shape[0]} rows of the block table"
+        blocks = -(-encoder_lens // self.block_size)
+        if encoder_lens.min() < 0 or blocks.max() > min(self.width, block_table.shape[1]):
+            raise ValueError(f"encoder lengths {encoder_lens.tolist()} do not fit {min(self.width, block_table.shape[1])} blocks of {self.block_size}")
+        if any(not 0 <= r < reqs for r in new_rows):
+            raise ValueError(f"new_rows {list(new_rows)} are not among {reqs} requests")
+        # (-1 behind a request's own blocks: padding of shorter outputs in a pass is written nowhere)
+        table = torch.full((rows, self.width), -1, dtype=torch.int32)
+        lens = torch.zeros(rows, dtype=torch.int32)
+        for i, n in enumerate(blocks):
+            table[i, :n] = torch.from_numpy(np.ascontiguousarray(block_table[i, :n]).astype(np.int32))
+            lens[i] = int(encoder_lens[i])
+        if rows not in self._buffers:
+            self._buffers[rows] = tuple(torch.empty_like(x, device=self.device) for x in (table, lens))
+        table_dev, lens_dev = self._buffers[rows]
+        table_dev.copy_(table)
+        lens_dev.copy_(lens)
+        batch_idx = torch.tensor(list(new_rows), dtype=torch.int32, device=self.device) if len(new_rows) else None
+        return TTMetadata(page_table=table_dev, is_causal=False, batch_idx=batch_idx, num_users=rows, encoder_lens=lens_dev,
+                          most_encoder_len=int(encoder_lens.max()))
