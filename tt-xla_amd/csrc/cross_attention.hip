@@ -2,20 +2,21 @@
 //
 //   out[u, h, t] = sum_j softmax_j(scale q[u, h, t] . k[u, j]) v[u, j],   j < len[u];   zeros where len[u] is 0
 //
-// This file holds the form for few rows (a token per user, a few drafted ones) and the choice; many rows are the streaming prefill loop's
-// (prefill_stream_kernel.h, kEnds).  All tokens of a user see the same keys, so the rows of a KV head are its G query heads times the tokens, and a workgroup takes
-// 16 RG of them (RG 1 or 2) over a part of the keys.
+// This file holds the forms for few rows (a token per user, drafted ones, short texts) and the choice; many rows are the streaming prefill loop's
+// (prefill_stream_kernel.h, kEnds).  All tokens of a user see the same keys, so the rows of a KV head are its G query heads times the tokens.  Up to 32 rows, a workgroup's four
+// wavefronts have tiles of their own of a part of the keys and all of the rows; else, and at head size 256, they share the tiles and have 16 rows each.
 // Bound by memory: K and V are read once for each block of rows.  32 users of 32 / 8 heads of 128 over 256 ... 4096 keys (170 MB) 35 us, of which the merge is four:
-// 5.7 TB/s in the kernel; 64 users of 8 / 8 of 64 over 1500 (197 MB) 33.4, 5.9 TB/s; 96 of 64 / 8 of 128 over 512 ... 2048 (436 MB) 74, 5.9.  Between, the wavefronts' chains
-// of tiles do, 1.1 us a tile: 8 users of 32 / 8 over 1500 (49 MB) 13.4.  A wavefront takes every 4 parts-th tile of TILE keys (64 at head size 64, else 32):
-//   memory -> registers -> LDS    whole lines, a tile ahead of its use; what lies behind the last key becomes zeros on the way (V) or is masked (K).  One buffer
-//                                 takes K, then V: two workgroups share a CU.  (Three, with fewer registers, came to 5.0 TB/s: four wavefronts per SIMD ask for more than
-//                                 the memory takes well.)
+// 5.7 TB/s in the kernel; 64 users of 8 / 8 of 64 over 1500 (197 MB) 33.4, 5.9 TB/s; 96 of 64 / 8 of 128 over 512 ... 2048 (436 MB) 74, 5.9; shared, 96 of 64 / 8, 5 tokens, over
+// 1500 (590 MB) 115, 5.1; 64 of 16 / 8 of 256 over 800 (419 MB) 71, 5.9.  Between, the chains of tiles do, 1.1 us a tile of 32 keys, or of 64 that are shared:
+// 8 users of 32 / 8 over 1500 (49 MB) 13.4, 5 tokens of 64 / 8 16.0.  Tiles of TILE keys (64 at head size 64, else 32; shared 64, 32 at head size 256):
+//   memory -> registers -> LDS    whole lines, a tile ahead of its use (shared: two); what lies behind the last key becomes zeros on the way (V) or is masked (K).  One
+//                                 buffer takes K, then V: two workgroups share a CU.  (Three, with fewer registers, came to 5.0 TB/s: four wavefronts per SIMD ask for
+//                                 more than the memory takes well.)
 //   S^T = K . Q^T                 16x16x32 bfloat16; the tile is four runs of TILE / 4 keys, one per quad of lanes: row 4 j + r of block b is
 //                                 key (TILE / 4) j + 4 b + r, so lane (row, quad) ends up with its quad's run in order, which is
 //   O^T += V^T . P^T              the order in which the second product wants its weights: no moves between the two
 // Statistics and accumulators are floats; weights are rounded once to bfloat16 for the matrix instruction, and the same rounded weights are summed.
-// The four wavefronts' results meet in LDS, the parts' in memory, merged by a kernel of its own.
+// Wavefronts' results of their own tiles meet in LDS, the parts' in memory, merged by a kernel of its own.
 #include "decode_mfma16_kernel.h"
 #include "prefill_common.h"
 
@@ -42,7 +43,7 @@ struct CrossArgs {
   int batch, hkv, g, s, bs, w, nb;
   float scale_log2e;
   uint32_t runs, runs_inv;  // runs of keys per block, and floor((2^32 - 1) / runs)
-  int row_blocks, parts, share;  // share: tiles of a part at least
+  int row_blocks, parts, share;  // share: keys of a part at least
   float *slots;  // [batch * hkv * row_blocks][parts]: ROWS * D values, ROWS maxima, ROWS sums
 };
 
@@ -57,61 +58,46 @@ constexpr int cross_lds_bytes() {
 }
 // Where a row's 16-byte chunks lie: chunk c at c ^ key(row).  K is read by 16 lanes of 16 rows (four of each run) at one chunk, V by 32 lanes of eight rows (four of
 // each of two runs) at 32 bytes: rows of 256 bytes or more are every bank once or twice, two rows of 128 share that.
-template <int D>
+template <int D, int TILE>
 __device__ __forceinline__ int cross_kkey(int row) {
-  constexpr int RUN = cross_tile<D>() / 4;
+  constexpr int RUN = TILE / 4;
   const int run = row / RUN & 3, r = row & 3;
   return D == 64 ? 2 * run + (r >> 1) : 4 * run + r;
 }
-template <int D>
+template <int D, int TILE>
 __device__ __forceinline__ int cross_vkey(int row) {
-  constexpr int RUN = cross_tile<D>() / 4;
+  constexpr int RUN = TILE / 4;
   const int run = row / RUN & 1, r = row & 3;
   return D == 64 ? 2 * ((r >> 1) + 2 * run) : 2 * (r + 4 * run);
 }
-// Parts of a user's keys, of a.share tiles or more each.
-template <int D>
-__device__ __forceinline__ int cross_parts(const CrossArgs &a, int keys) {
-  constexpr int TILE = cross_tile<D>();
-  return max(1, min(a.parts, ((keys + TILE - 1) / TILE + a.share - 1) / a.share));
-}
-template <int D, int RG>
+// Parts of a user's keys, of a.share keys or more each.
+__device__ __forceinline__ int cross_parts(const CrossArgs &a, int keys) { return max(1, min(a.parts, (keys + a.share - 1) / a.share)); }
+template <int D, int ROWS>
 constexpr int cross_slot_floats() {
-  return 16 * RG * (D + 2);
-}
-// Workgroups of a CU, by the registers of one (and the LDS at head size 256).
-template <int D, int RG>
-constexpr int cross_per_cu() {
-  return D == 256 ? 1 : 2;
+  return ROWS * (D + 2);
 }
 // Keys of a user, of those that the table has room for.
 __device__ __forceinline__ int cross_keys(const CrossArgs &a, int64_t length) { return (int)max(min(length, (int64_t)a.w * a.bs), (int64_t)0); }
 
-// A wavefront's rows, its tile of keys and what it has of the result.
-template <int D, int RG>
-struct CrossTile {
-  static constexpr int TILE = cross_tile<D>(), RUN = TILE / 4, ROWS = 16 * RG;
+// A wavefront's rows and what it has of the result; what it does with a tile of TILE keys that lies in LDS.
+template <int D, int RG, int KEYS>
+struct CrossRows {
+  static constexpr int TILE = KEYS, RUN = TILE / 4, ROWS = 16 * RG;
   static constexpr int KBLK = TILE / 16, KSTEPS = D / 32, DBLK = D / 16, PSTEPS = TILE / 32;
-  static constexpr int RB = 2 * D, CPR = D / 8, NL = RUN * CPR / 16;  // row bytes, 16-byte chunks of a row, loads of a tile and tensor
+  static constexpr int RB = 2 * D, CPR = D / 8;  // row bytes, 16-byte chunks of a row
 
   const CrossArgs &a;
-  uint8_t *const tile;
   const int n, quad;
   int k_row, k_key, v_row, v_key;
   u32x4 qf[RG][KSTEPS];  // B operand of k-step i: lane (row n, quad) holds features 32 i + 8 quad + 0 .. 7
-  u32x4 kraw[NL], vraw[NL];
   floatx4 acc[RG][DBLK], l_acc[RG];
   float m_run[RG];
 
-  __device__ __forceinline__ CrossTile(const CrossArgs &args, uint8_t *lds)
-      : a(args), tile(lds), n((int)(threadIdx.x & 15)), quad((int)(threadIdx.x & 63) >> 4) {
+  __device__ __forceinline__ CrossRows(const CrossArgs &args) : a(args), n((int)(threadIdx.x & 15)), quad((int)(threadIdx.x & 63) >> 4) {
     // K operand: row RUN (n / 4) + 4 b + n % 4, chunk 4 i + quad (the key is that of every block's row: blocks are four rows apart)
-    k_row = RUN * (n >> 2) + (n & 3), k_key = cross_kkey<D>(k_row);
+    k_row = RUN * (n >> 2) + (n & 3), k_key = cross_kkey<D, TILE>(k_row);
     // V operand, transposed by the load: four rows x 16 features per quad; of step s and half t, row RUN quad + 8 s + 4 t + n / 4
-    v_row = RUN * quad + (n >> 2), v_key = cross_vkey<D>(v_row);
-    clear();
-  }
-  __device__ __forceinline__ void clear() {
+    v_row = RUN * quad + (n >> 2), v_key = cross_vkey<D, TILE>(v_row);
 #pragma unroll
     for (int rg = 0; rg < RG; ++rg) {
 #pragma unroll
@@ -130,59 +116,19 @@ struct CrossTile {
       for (int i = 0; i < KSTEPS; ++i) qf[rg][i] = *reinterpret_cast<const u32x4 *>(qp + 32 * i);
     }
   }
-  // Where the lane's run of tile t lies.  A run is in one block; its quad of lanes looks up its page and loads its rows.  (Ids out of range read block 0;
-  // tiles behind the table's room are not asked for.)
-  __device__ __forceinline__ uint64_t look_up(int u, int h, int t) const {
-    const uint32_t x = (uint32_t)(t * 4 + quad);
+  // Where run x of the keys lies: a run is in one block.  (Ids out of range read block 0; tiles behind the table's room are not asked for.)
+  __device__ __forceinline__ uint64_t place(int u, int h, uint32_t x) const {
     uint32_t col = __umulhi(x, a.runs_inv), r = x - col * a.runs;  // one too few at most
     if (r >= a.runs) ++col, r -= a.runs;
     const int page = (int)col < a.w ? a.pt[(int64_t)u * a.pt_rs + (int)col] : 0;
     const uint64_t slab = (uint64_t)((unsigned)page < (unsigned)a.nb ? page : 0) * (uint32_t)a.hkv + (uint32_t)h;
-    return slab * (uint64_t)(a.bs * RB) + r * (uint32_t)(RUN * RB) + 16 * n;
+    return slab * (uint64_t)(a.bs * RB) + r * (uint32_t)(RUN * RB);
   }
   // (non-temporal also where several blocks of rows read the same keys: 96 users of 64 / 8 heads of 128 over 2033 keys 91 -> 74 us, and three blocks of 8 users
   // over 1500 20.8 -> 19.5)
   __device__ static __forceinline__ u32x4 load(const uint8_t *p) { return __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p)); }
-  __device__ __forceinline__ void request_k(uint64_t at) {
-    const uint8_t *const kp = reinterpret_cast<const uint8_t *>(a.k) + at;
-#pragma unroll
-    for (int i = 0; i < NL; ++i) kraw[i] = load(kp + 256 * i);
-  }
-  __device__ __forceinline__ void request_v(uint64_t at) {
-    const uint8_t *const vp = reinterpret_cast<const uint8_t *>(a.v) + at;
-#pragma unroll
-    for (int i = 0; i < NL; ++i) vraw[i] = load(vp + 256 * i);
-  }
-  // Load i of a lane is chunk 16 i + n of its run.
-  __device__ __forceinline__ int run_row(int i) const { return (16 * i + n) / CPR; }
-  // Registers -> LDS (an LDS works through a wavefront's instructions in order: V overwrites K behind the last read of K); of the lane's run, `nvalid` keys
-  // are attended.
-  __device__ __forceinline__ void stage_k() {
-#pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int row = RUN * quad + run_row(i), chunk = (16 * i + n) % CPR;
-      *reinterpret_cast<u32x4 *>(tile + row * RB + ((chunk ^ cross_kkey<D>(row)) << 4)) = kraw[i];
-    }
-  }
-  __device__ __forceinline__ void stage_v(int nvalid, bool partial) {
-    if (partial) {
-#pragma unroll
-      for (int i = 0; i < NL; ++i) {
-        const uint32_t keep = run_row(i) < nvalid ? 0xffffffffu : 0u;
-        vraw[i] = u32x4{vraw[i].x & keep, vraw[i].y & keep, vraw[i].z & keep, vraw[i].w & keep};
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int row = RUN * quad + run_row(i), chunk = (16 * i + n) % CPR;
-      *reinterpret_cast<u32x4 *>(tile + row * RB + ((chunk ^ cross_vkey<D>(row)) << 4)) = vraw[i];
-    }
-  }
-  template <bool MORE>
-  __device__ __forceinline__ void attend(int nvalid, bool partial, uint64_t next) {
-    stage_k();
-    if constexpr (MORE) request_k(next);
-    // ---- S^T = K . Q^T ----
+  // S^T = K . Q^T and the weights, rounded; of the lane's run, `nvalid` keys are attended.
+  __device__ __forceinline__ void weigh(const uint8_t *tile, int nvalid, bool partial, u32x4 (&pf)[RG][PSTEPS]) {
     floatx4 st[RG][KBLK];
 #pragma unroll
     for (int b = 0; b < KBLK; ++b) {
@@ -195,9 +141,8 @@ struct CrossTile {
         for (int rg = 0; rg < RG; ++rg) st[rg][b] = mma16<false>(w, qf[rg][i], st[rg][b]);
       }
     }
-    // ---- online softmax.  The weights' reference follows the maximum only where a score is more than 2^8 ahead of it: they stay below 2^8 with
-    // all their bits, and the accumulators are rescaled in the first tile and hardly ever again. ----
-    u32x4 pf[RG][PSTEPS];
+    // The weights' reference follows the maximum only where a score is more than 2^8 ahead of it: they stay below 2^8 with all their bits, and the accumulators are
+    // rescaled in the first tile and hardly ever again.
 #pragma unroll
     for (int rg = 0; rg < RG; ++rg) {
       float sc[4 * KBLK];
@@ -226,9 +171,9 @@ struct CrossTile {
       for (int i = 0; i < 4 * KBLK; i += 2)
         pf[rg][i >> 3][(i >> 1) & 3] = pack_bf16x2(__builtin_amdgcn_exp2f(fmaf(sc[i], a.scale_log2e, minus_m)), __builtin_amdgcn_exp2f(fmaf(sc[i + 1], a.scale_log2e, minus_m)));
     }
-    stage_v(nvalid, partial);
-    if constexpr (MORE) request_v(next);
-    // ---- O^T += V^T . P^T ----
+  }
+  // O^T += V^T . P^T
+  __device__ __forceinline__ void add(const uint8_t *tile, const u32x4 (&pf)[RG][PSTEPS]) {
     typedef short shortx4 __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) shortx4 *lds_v4;
     const u32x4 ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
@@ -249,9 +194,67 @@ struct CrossTile {
   }
 };
 
+// A wavefront with tiles of its own: on their way in registers, then in its share of LDS, K first and V over it.  A quad of lanes has a run of the keys.
+template <int D, int RG>
+struct CrossTile : CrossRows<D, RG, cross_tile<D>()> {
+  using Rows = CrossRows<D, RG, cross_tile<D>()>;
+  using Rows::TILE, Rows::RUN, Rows::RB, Rows::CPR, Rows::PSTEPS, Rows::a, Rows::n, Rows::quad, Rows::load;
+  static constexpr int NL = RUN * CPR / 16;  // loads of a tile and tensor
+  uint8_t *const tile;
+  u32x4 kraw[NL], vraw[NL];
+
+  __device__ __forceinline__ CrossTile(const CrossArgs &args, uint8_t *lds) : Rows(args), tile(lds) {}
+  __device__ __forceinline__ uint64_t look_up(int u, int h, int t) const { return this->place(u, h, (uint32_t)(t * 4 + quad)) + 16 * n; }
+  __device__ __forceinline__ void request_k(uint64_t at) {
+    const uint8_t *const kp = reinterpret_cast<const uint8_t *>(a.k) + at;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) kraw[i] = load(kp + 256 * i);
+  }
+  __device__ __forceinline__ void request_v(uint64_t at) {
+    const uint8_t *const vp = reinterpret_cast<const uint8_t *>(a.v) + at;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) vraw[i] = load(vp + 256 * i);
+  }
+  // Load i of a lane is chunk 16 i + n of its run.
+  __device__ __forceinline__ int run_row(int i) const { return (16 * i + n) / CPR; }
+  // Registers -> LDS (an LDS works through a wavefront's instructions in order: V overwrites K behind the last read of K); of the lane's run, `nvalid` keys
+  // are attended.
+  __device__ __forceinline__ void stage_k() {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int row = RUN * quad + run_row(i), chunk = (16 * i + n) % CPR;
+      *reinterpret_cast<u32x4 *>(tile + row * RB + ((chunk ^ cross_kkey<D, TILE>(row)) << 4)) = kraw[i];
+    }
+  }
+  __device__ __forceinline__ void stage_v(int nvalid, bool partial) {
+    if (partial) {
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const uint32_t keep = run_row(i) < nvalid ? 0xffffffffu : 0u;
+        vraw[i] = u32x4{vraw[i].x & keep, vraw[i].y & keep, vraw[i].z & keep, vraw[i].w & keep};
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int row = RUN * quad + run_row(i), chunk = (16 * i + n) % CPR;
+      *reinterpret_cast<u32x4 *>(tile + row * RB + ((chunk ^ cross_vkey<D, TILE>(row)) << 4)) = vraw[i];
+    }
+  }
+  template <bool MORE>
+  __device__ __forceinline__ void attend(int nvalid, bool partial, uint64_t next) {
+    u32x4 pf[RG][PSTEPS];
+    stage_k();
+    if constexpr (MORE) request_k(next);
+    this->weigh(tile, nvalid, partial, pf);
+    stage_v(nvalid, partial);
+    if constexpr (MORE) request_v(next);
+    this->add(tile, pf);
+  }
+};
+
 // A workgroup per (user, KV head, block of rows): its wavefronts take the tiles in turn, and their results meet in LDS.
 template <int D, int RG>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(cross_per_cu<D, RG>(), cross_per_cu<D, RG>()))) void cross_rows_kernel(CrossArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void cross_rows_kernel(CrossArgs a) {
   using T = CrossTile<D, RG>;
   constexpr int TILE = T::TILE, ROWS = T::ROWS, DBLK = T::DBLK, CPR = T::CPR;
   extern __shared__ __attribute__((aligned(16))) uint8_t tiles[];
@@ -270,7 +273,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(cross_per_c
   const uint64_t at0 = x.look_up(u, h, t);
   x.load_q(u, h, row0);
   const int keys = __builtin_amdgcn_readfirstlane(cross_keys(a, length)), n_tiles = (keys + TILE - 1) / TILE;
-  const int parts = cross_parts<D>(a, keys), step = 4 * parts;
+  const int parts = cross_parts(a, keys), step = 4 * parts;
   if (part >= parts) return;
   if (keys == 0) {  // nothing to attend
 #pragma unroll 1
@@ -336,7 +339,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(cross_per_c
         den = fmaf(wgt, s_ml[w][row].y, den);
       }
       if (parts > 1) {
-        float *const slot = a.slots + ((int64_t)(uh * a.row_blocks + rb) * a.parts + part) * cross_slot_floats<D, RG>();
+        float *const slot = a.slots + ((int64_t)(uh * a.row_blocks + rb) * a.parts + part) * cross_slot_floats<D, ROWS>();
         *reinterpret_cast<float4 *>(slot + row * D + feature) = make_float4(num[0], num[1], num[2], num[3]);
         if (feature == 0) slot[ROWS * D + row] = mall, slot[ROWS * (D + 1) + row] = den;
         continue;
@@ -349,17 +352,127 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(cross_per_c
   }
 }
 
-// The wavefronts' shares of a segment: a workgroup per row, eight slices of the shares that meet in LDS; four features per thread.
-template <int D, int RG>
-__global__ __launch_bounds__(2 * D) void cross_merge_kernel(CrossArgs a) {
-  constexpr int ROWS = 16 * RG, SLOT = cross_slot_floats<D, RG>(), PER = D / 4, SLICES = 8, BATCH = 4;
-  __shared__ float4 s_num[SLICES][PER];
-  __shared__ float2 s_md[SLICES];
-  const int seg = blockIdx.x, m = blockIdx.y, rb = m / ROWS, row = m - rb * ROWS;
-  const int slice = threadIdx.x / PER, f = threadIdx.x - slice * PER;
+// More rows: the four wavefronts have 16 rows each and share the tiles, of which each loads a run of the keys: two tiles on their way in registers, one in LDS,
+// the next one written beside it, a barrier per tile.  (Two groups of rows per wavefront: 16 users of 32 / 8 heads over 1500 keys, 32 tokens, longer for every number of
+// parts, as are 40 and 64 rows: a tile's time is the products' and the reads of LDS.)
+template <int D>
+constexpr int shared_tile() {
+  return D == 256 ? 32 : 64;
+}
+template <int D>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void cross_shared_kernel(CrossArgs a) {
+  using T = CrossRows<D, 1, shared_tile<D>()>;
+  constexpr int TILE = T::TILE, RUN = T::RUN, RB = T::RB, CPR = T::CPR, ROWS = 64, DBLK = T::DBLK, NL = RUN * CPR / 64, BYTES = TILE * RB;
+  extern __shared__ __attribute__((aligned(16))) uint8_t tiles[];  // two of K and V
+  const uint32_t span = 8u * a.row_blocks, set = blockIdx.x / span, in_set = blockIdx.x - set * span;
+  const int rb = (int)(in_set >> 3), unit = (int)(set * 8 + (in_set & 7)), segments = a.batch * a.hkv;
+  if (unit >= segments * a.parts) return;
+  const int part = unit / segments, uh = unit - part * segments, u = uh / a.hkv, h = uh - u * a.hkv;
+  const int lane = threadIdx.x & 63, wib = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int rows = a.g * a.s, row0 = rb * ROWS + 16 * wib;
+  const bool mine = row0 < rows;  // (a wavefront without rows loads its share of the keys)
+  T x(a);
+  int t = part;
+  const auto look_up = [&](int tile) { return x.place(u, h, (uint32_t)(tile * 4 + wib)) + 16 * lane; };
+  const int64_t length = load_index(a.lens, a.lens_i64, u);
+  const uint64_t at0 = look_up(t);
+  if (mine) x.load_q(u, h, row0);
+  const int keys = __builtin_amdgcn_readfirstlane(cross_keys(a, length)), n_tiles = (keys + TILE - 1) / TILE;
+  const int parts = cross_parts(a, keys), step = parts;
+  if (part >= parts) return;
+  if (keys == 0) {  // nothing to attend
+#pragma unroll 1
+    for (int i = threadIdx.x; i < min(ROWS, rows - rb * ROWS) * CPR; i += 256) {
+      const int m = rb * ROWS + i / CPR, token = m / a.g, head = m - token * a.g;
+      uint16_t *dst = a.out + u * a.o_bs + (int64_t)(h * a.g + head) * a.o_hs + token * a.o_ts + 8 * (i % CPR);
+      *reinterpret_cast<uint2 *>(dst) = make_uint2(0u, 0u), *reinterpret_cast<uint2 *>(dst + 4) = make_uint2(0u, 0u);
+    }
+    return;
+  }
+  u32x4 kraw[2][NL], vraw[2][NL];
+  const auto request = [&](uint64_t at, u32x4 (&k)[NL], u32x4 (&v)[NL]) {
+    const uint8_t *const kp = reinterpret_cast<const uint8_t *>(a.k) + at, *const vp = reinterpret_cast<const uint8_t *>(a.v) + at;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) k[i] = T::load(kp + 1024 * i);
+#pragma unroll
+    for (int i = 0; i < NL; ++i) v[i] = T::load(vp + 1024 * i);
+  };
+  uint64_t at2 = 0;  // of the tile two steps ahead
+  const auto process = [&](int buffer, u32x4 (&k)[NL], u32x4 (&v)[NL]) {
+    uint8_t *const kt = tiles + buffer * 2 * BYTES, *const vt = kt + BYTES;
+    const bool partial = (t + 1) * TILE > keys;
+    const uint64_t at = at2;
+    if (t + 3 * step < n_tiles) at2 = look_up(t + 3 * step);
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int c = 64 * i + lane, row = RUN * wib + c / CPR;
+      *reinterpret_cast<u32x4 *>(kt + row * RB + ((c % CPR ^ cross_kkey<D, TILE>(row)) << 4)) = k[i];
+    }
+    if (partial) {
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const uint32_t keep = t * TILE + RUN * wib + (64 * i + lane) / CPR < keys ? 0xffffffffu : 0u;
+        v[i] = u32x4{v[i].x & keep, v[i].y & keep, v[i].z & keep, v[i].w & keep};
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int c = 64 * i + lane, row = RUN * wib + c / CPR;
+      *reinterpret_cast<u32x4 *>(vt + row * RB + ((c % CPR ^ cross_vkey<D, TILE>(row)) << 4)) = v[i];
+    }
+    if (t + 2 * step < n_tiles) request(at, k, v);
+    __syncthreads();  // the tile is there; whoever is ahead writes the other buffer, whose tile everybody is done with
+    if (mine) {
+      u32x4 pf[1][T::PSTEPS];
+      x.weigh(kt, keys - (t * TILE + RUN * x.quad), partial, pf);
+      x.add(vt, pf);
+    }
+    t += step;
+  };
+  if (t < n_tiles) {
+    uint64_t at1 = 0;
+    if (t + step < n_tiles) at1 = look_up(t + step);
+    if (t + 2 * step < n_tiles) at2 = look_up(t + 2 * step);
+    request(at0, kraw[0], vraw[0]);
+    if (t + step < n_tiles) request(at1, kraw[1], vraw[1]);
+    while (t < n_tiles) {
+      process(0, kraw[0], vraw[0]);
+      if (t < n_tiles) process(1, kraw[1], vraw[1]);
+    }
+  }
+  const int m = row0 + x.n, token = m / a.g, head = m - token * a.g;
+  if (m >= rows) return;
+  if (parts > 1) {
+    float *const slot = a.slots + ((int64_t)(uh * a.row_blocks + rb) * a.parts + part) * cross_slot_floats<D, ROWS>();
+    const int row = m - rb * ROWS;
+#pragma unroll
+    for (int db = 0; db < DBLK; ++db) {
+      const floatx4 &v = x.acc[0][db];
+      *reinterpret_cast<float4 *>(slot + row * D + 16 * db + 4 * x.quad) = make_float4(v[0], v[1], v[2], v[3]);
+    }
+    if (x.quad == 0) slot[ROWS * D + row] = x.m_run[0], slot[ROWS * (D + 1) + row] = x.l_acc[0][0];
+    return;
+  }
+  const float inv = 1.f / x.l_acc[0][0];
+  uint16_t *const dst = a.out + u * a.o_bs + (int64_t)(h * a.g + head) * a.o_hs + token * a.o_ts + 4 * x.quad;
+#pragma unroll
+  for (int db = 0; db < DBLK; ++db) {
+    const floatx4 &v = x.acc[0][db];
+    *reinterpret_cast<uint2 *>(dst + 16 * db) = make_uint2(pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv));
+  }
+}
+
+// The parts of a segment's rows, four features per thread: a workgroup per row, eight slices of the parts that meet in LDS, or several rows and all of a row's parts a
+// thread's own (SLICES 1), where they are few.
+template <int D, int ROWS, int SLICES>
+__global__ __launch_bounds__(256) void cross_merge_kernel(CrossArgs a) {
+  constexpr int SLOT = cross_slot_floats<D, ROWS>(), PER = D / 4, BATCH = 4, THREADS = SLICES > 1 ? SLICES * PER : 256;
+  constexpr int AT_ONCE = THREADS / (PER * SLICES);  // rows of a workgroup
+  const int slice = SLICES > 1 ? (int)threadIdx.x / PER : 0, f = threadIdx.x % PER;
+  const int seg = blockIdx.x, m = blockIdx.y * AT_ONCE + (SLICES > 1 ? 0 : (int)threadIdx.x / PER), rb = m / ROWS, row = m - rb * ROWS;
   const int u = seg / a.hkv, h = seg - u * a.hkv, token = m / a.g, head = m - token * a.g;
-  const int count = cross_parts<D>(a, cross_keys(a, load_index(a.lens, a.lens_i64, u)));
-  if (count == 1) return;  // (the one workgroup has written the output)
+  const int count = cross_parts(a, cross_keys(a, load_index(a.lens, a.lens_i64, u)));
+  if (count == 1 || m >= a.g * a.s) return;  // (the one workgroup has written the output)
   uint16_t *dst = a.out + u * a.o_bs + (int64_t)(h * a.g + head) * a.o_hs + token * a.o_ts + 4 * f;
   const float *slot = a.slots + (int64_t)(seg * a.row_blocks + rb) * a.parts * SLOT;
   float mall = -INFINITY, num[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
@@ -388,83 +501,105 @@ __global__ __launch_bounds__(2 * D) void cross_merge_kernel(CrossArgs a) {
       den = fmaf(wgt, lv[j], den);
     }
   }
-  s_num[slice][f] = make_float4(num[0], num[1], num[2], num[3]);
-  if (f == 0) s_md[slice] = make_float2(mall, den);
-  __syncthreads();
-  if (slice != 0) return;
-  mall = -INFINITY, den = 0.f;
+  if constexpr (SLICES > 1) {
+    __shared__ float4 s_num[SLICES][PER];
+    __shared__ float2 s_md[SLICES];
+    s_num[slice][f] = make_float4(num[0], num[1], num[2], num[3]);
+    if (f == 0) s_md[slice] = make_float2(mall, den);
+    __syncthreads();
+    if (slice != 0) return;
+    mall = -INFINITY, den = 0.f;
 #pragma unroll
-  for (int r = 0; r < 4; ++r) num[r] = 0.f;
-  const int used = min(count, SLICES);
-  for (int s = 0; s < used; ++s) mall = fmaxf(mall, s_md[s].x);
-  const float ref = merge_reference(mall);
-  for (int s = 0; s < used; ++s) {
-    const float wgt = __builtin_amdgcn_exp2f(s_md[s].x - ref);
-    const float4 v = s_num[s][f];
-    num[0] = fmaf(wgt, v.x, num[0]), num[1] = fmaf(wgt, v.y, num[1]), num[2] = fmaf(wgt, v.z, num[2]), num[3] = fmaf(wgt, v.w, num[3]);
-    den = fmaf(wgt, s_md[s].y, den);
+    for (int r = 0; r < 4; ++r) num[r] = 0.f;
+    const int used = min(count, SLICES);
+    for (int s = 0; s < used; ++s) mall = fmaxf(mall, s_md[s].x);
+    const float ref = merge_reference(mall);
+    for (int s = 0; s < used; ++s) {
+      const float wgt = __builtin_amdgcn_exp2f(s_md[s].x - ref);
+      const float4 v = s_num[s][f];
+      num[0] = fmaf(wgt, v.x, num[0]), num[1] = fmaf(wgt, v.y, num[1]), num[2] = fmaf(wgt, v.z, num[2]), num[3] = fmaf(wgt, v.w, num[3]);
+      den = fmaf(wgt, s_md[s].y, den);
+    }
   }
   const float inv = 1.f / den;
   *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_bf16x2(num[0] * inv, num[1] * inv), pack_bf16x2(num[2] * inv, num[3] * inv));
 }
 
-// How the rows form cuts a call: groups of 16 rows per wavefront, blocks of rows, parts of the keys and tiles of a part.
+// How a call is cut: blocks of rows, and the groups of 16 that a wavefront has of one; parts of the keys and keys of a part.
+// Wavefronts share their tiles from 33 rows on, where blocks of 32 would read the keys more than once, and at head size 256, where 32 rows are too many for a wavefront
+// and tiles of its own leave room for one workgroup on a CU.  us per call, own tiles / shared, the best parts of each: 128, 8 users of 64 / 8 heads over 512 ... 5469 keys,
+// 5 tokens 28.3 / 23.6; 96 over 1500 152 / 115; 32 of 32 / 8 over 800, 16 tokens 27.7 / 24.0; 16 over 1500, 32 tokens 37.7 / 33.9; one user over 1500, 7 tokens 9.8 / 9.4; 8, 16 tokens
+// 17.0 / 17.6; 256, 16 / 8 heads, 8 over 1500, 48 tokens 62 / 38; 2 over 6404, 20 tokens 39.9 / 26.5, one 26.0 / 23.9; 64 over 800, one 71 / 71.  Up to 32 rows: 128, 32 users over
+// 256 ... 4096, 4 rows 34.6 / 36.0; 96 over 512 ... 2048, 8 rows 74.8 / 83.5; 64 over 300, 32 rows 20.4 / 19.7; 64, 64 over 2015, 32 rows 25.5 / 31.2.
 struct CrossCut {
-  int groups, row_blocks, parts, share;
+  bool shared;
+  int groups, row_blocks, parts, share, tile;
+  int rows() const { return (shared ? 64 : 16) * groups; }
 };
-int tile_of(int head_size) { return head_size == 64 ? 64 : 32; }
 
-// The rule for the parts: the least of an estimate of the time, us behind what every launch needs, of a wavefront's tiles one after the other.  Of full tables: rounds of
-// workgroups, one per CU, or two that share its ways to memory (1.9 times as long for both); of ragged ones, of which three tenths are there: the longest
-// wavefront, or all of them.  The two are weighed 7 : 3; chains of more than eight tiles count more while the launch does not fill the chip; a split costs the merge.
-// Chosen / best of all: within 1 % over 28 shapes from 1 x 8 heads of 250 keys to 96 x 8 of 2033, 16 % at worst (8 users of 512 ... 6404 keys, 40 rows).
+// The rule for the parts: the least of an estimate of the time, us behind what every launch needs, of a chain of tiles one after the other (a wavefront's, or a workgroup's
+// that shares them).  Of full tables: rounds of workgroups, one per CU, or two that share its ways to memory; of ragged ones, of which three or four tenths are there:
+// the longest chain, or all of them.  The two are weighed 7 : 3; with tiles of their own, chains of more than eight count more while the launch does not fill the chip; a
+// split costs the merge.  Chosen / best of all: within 1 % over 28 shapes from 1 x 8 heads of 250 keys to 96 x 8 of 2033, 10 % at worst (8 x 8 of 512 ... 3597, 32
+// rows); shared, 3 % over 31 from 1 x 8 of 100 to 96 x 8 of 1500, 14 % at worst (one user of 1500, 56 rows).
 CrossCut cross_cut(int batch, int kv_heads, int64_t rows, int head_size, int64_t keys) {
-  CrossCut c;
-  c.groups = rows <= 16 || head_size == 256 ? 1 : 2;  // (two at head size 256 spill)
-  c.row_blocks = (int)((rows + 16 * c.groups - 1) / (16 * c.groups));
+  CrossCut c = {};
+  c.shared = head_size == 256 || rows > 32;
+  c.groups = c.shared || rows <= 16 ? 1 : 2;
+  c.row_blocks = (int)((rows + c.rows() - 1) / c.rows());
+  c.tile = c.shared ? (head_size == 256 ? shared_tile<256>() : shared_tile<128>()) : head_size == 64 ? cross_tile<64>() : cross_tile<128>();
   const double segments = (double)batch * kv_heads * c.row_blocks, cus = std::max(device_cus(), 1);
-  const int tiles = (int)((keys + tile_of(head_size) - 1) / tile_of(head_size));
-  const double tile_us = (head_size == 64 ? 1.2 : head_size == 128 ? 1.1 : 2.3) * (c.groups == 2 ? 1.2 : 1.0);
+  const int tiles = (int)((keys + c.tile - 1) / c.tile), chains = c.shared ? 1 : 4;  // chains of a workgroup
+  const double tile_us = c.shared ? (head_size == 64 ? 0.7 : head_size == 128 ? 1.05 : 0.95) : (head_size == 64 ? 1.2 : 1.1) * (c.groups == 2 ? 1.2 : 1.0);
+  const double two = c.shared ? 1.7 : 1.9, there = c.shared ? 0.4 : 0.3;
+  const double merged = c.shared ? segments * std::min<int64_t>(rows, 64) * 0.2e-3 : segments * 6.25e-3;
   double best = 0;
-  c.parts = 0;
-  for (int chain = (tiles + 3) / 4; chain >= 1; --chain) {
-    const int parts = std::max(1, (tiles + 4 * chain - 1) / (4 * chain));
+  for (int chain = (tiles + chains - 1) / chains; chain >= 1; --chain) {
+    const int parts = std::max(1, (tiles + chains * chain - 1) / (chains * chain));
     if (parts == c.parts) continue;  // (as many parts of fewer tiles: the same)
     if (parts > kMostCrossParts) break;
-    const int longest = (tiles + 4 * parts - 1) / (4 * parts);
-    const double groups = segments * parts, one = longest * tile_us, all = groups / cus;
-    const double full = head_size == 256 ? std::ceil(all) * one : all <= 1 ? one : 1.9 * std::ceil(all / 2) * one;
-    const double cost = 0.7 * full + 0.3 * std::max(one, 0.3 * all * one) + (segments < 2 * cus ? 0.2 * std::max(0, longest - 8) : 0.0) +
-                        (parts > 1 ? 3.0 + parts * (0.4 * segments / 64 + 0.02) : 0.0);
+    const int longest = (tiles + chains * parts - 1) / (chains * parts);
+    const double all = segments * parts / cus, one = longest * tile_us, full = all <= 1 ? one : two * std::ceil(all / 2) * one;
+    const double cost = 0.7 * full + 0.3 * std::max(one, there * all * one) + (!c.shared && segments < 2 * cus ? 0.2 * std::max(0, longest - 8) : 0.0) +
+                        (parts > 1 ? 3.0 + parts * (merged + 0.02) : 0.0);
     if (c.parts == 0 || cost < best) best = cost, c.parts = parts;
   }
   c.parts = std::max(c.parts, 1);
-  c.share = std::max((tiles + c.parts - 1) / c.parts, 4);
+  c.share = std::max((tiles + c.parts - 1) / c.parts, chains) * c.tile;
   return c;
 }
 int64_t cross_bytes(const CrossCut &c, int batch, int kv_heads, int head_size) {
-  return c.parts == 1 ? 256 : (int64_t)batch * kv_heads * c.row_blocks * c.parts * (16 * c.groups * (int64_t)(head_size + 2) * 4);
+  return c.parts == 1 ? 256 : (int64_t)batch * kv_heads * c.row_blocks * c.parts * (c.rows() * (int64_t)(head_size + 2) * 4);
 }
 
-template <int D, int RG>
+template <int D, int RG, bool SHARED>
 int launch_cross(const CrossArgs &a, hipStream_t st) {
   static std::atomic<uint64_t> lds_ready{0};
-  const size_t lds = 4 * cross_lds_bytes<D>();
-  if (!ensure_dynamic_lds(reinterpret_cast<const void *>(&cross_rows_kernel<D, RG>), lds, lds_ready))
+  constexpr auto kernel = [] {
+    if constexpr (SHARED) return &cross_shared_kernel<D>;
+    else return &cross_rows_kernel<D, RG>;
+  }();
+  const size_t lds = SHARED ? 4 * shared_tile<D>() * D * 2 : 4 * cross_lds_bytes<D>();
+  if (!ensure_dynamic_lds(reinterpret_cast<const void *>(kernel), lds, lds_ready))
     return fail(TTPA_ERR_LAUNCH, "cross attention: cannot reserve %d bytes of LDS", (int)lds);
   const int64_t units = (int64_t)a.batch * a.hkv * a.parts;
-  launch_dominant(&cross_rows_kernel<D, RG>, dim3((unsigned)((units + 7) / 8 * 8 * a.row_blocks)), dim3(256), lds, st, a);
+  launch_dominant(kernel, dim3((unsigned)((units + 7) / 8 * 8 * a.row_blocks)), dim3(256), lds, st, a);
   if (const int rc = check_launch("cross attention")) return rc;
   if (a.parts == 1) return TTPA_OK;
-  cross_merge_kernel<D, RG><<<dim3(a.batch * a.hkv, a.g * a.s), dim3(2 * D), 0, st>>>(a);
+  // slices only for many parts: 2 / 3 / 4 parts of 64 rows, 8 users of 32 / 8 heads over 1500 keys 19.8 / 23.5 / 22.3 us with them, 17.0 / 20.5 / 19.5 without; 16 the same
+  constexpr int ROWS = (SHARED ? 64 : 16) * RG, AT_ONCE = 1024 / D;
+  if (a.parts > 16)
+    cross_merge_kernel<D, ROWS, 1024 / D><<<dim3(a.batch * a.hkv, a.g * a.s), dim3(256), 0, st>>>(a);
+  else
+    cross_merge_kernel<D, ROWS, 1><<<dim3(a.batch * a.hkv, (a.g * a.s + AT_ONCE - 1) / AT_ONCE), dim3(256), 0, st>>>(a);
   return check_launch("cross attention (merge)");
 }
 
 template <int D>
-int launch_cross_d(const CrossArgs &a, int groups, hipStream_t st) {
+int launch_cross_d(const CrossArgs &a, const CrossCut &c, hipStream_t st) {
   if constexpr (D < 256)
-    if (groups == 2) return launch_cross<D, 2>(a, st);
-  return launch_cross<D, 1>(a, st);
+    if (!c.shared) return c.groups == 2 ? launch_cross<D, 2, false>(a, st) : launch_cross<D, 1, false>(a, st);
+  return launch_cross<D, 1, true>(a, st);
 }
 
 // The streaming loop's arguments.  It steps through rows by unsigned 32-bit numbers of bytes and through blocks by a 32-bit inverse; what does not fit those is
@@ -484,21 +619,21 @@ bool stream_args(const CrossArgs &c, int head_size, bool keys_known, int64_t key
   return true;
 }
 
-// Which form takes a call: the rows' where it reads every key once; while its blocks of rows have no more than 50 tiles of keys per CU to go through (25 of twice the
-// bytes at head size 256); or no more than one and a half for each that the streaming loop has.  That reads a key once for 128 rows, 32 tokens of four heads, whether there
-// are as many or not, and takes the rest.  us per call, rows / stream: 32 / 8 heads of 128, 8 users over 1500 keys, 1 token 13.4 / 22.2,
-// 16 (24 tiles per CU) 19.4 / 22.6, 32 (47) 21.0 / 22.7, 48 (70) 33.2 / 29.4, 256 105 / 51; 2 users over 6404, 24 (38) 25.5 / 23.5, 48 (75) 35.3 / 28.1; 32 over 800, 8 (25)
-// 21.6 / 25.1, 16 (50) 27.2 / 25.3, 32 (100) 44 / 26; 16 / 16 of 64, 8 over 1500, 96 (36) 20.7 / 21.8, 256 (96) 34 / 25; 16 / 8 of 256, 8 over 1500, 8 (12) 24.6 / 32.7,
-// 16 (24) 37.6 / 33.0, 64 (94) 63 / 37; tokens that leave most of the streaming loop's rows empty: 64 / 8 of 128, 8 over 512 ... 5469, 5 (86) 31 / 45, 32 over 800, 8 (50)
-// 27 / 38, 16 (100) 44 / 39.  TTPA_CROSS_FORM=rows|stream, read on every call, overrides.
+// Which form takes a call: the rows' where it reads the keys no more often than the streaming loop, which reads a key once for 128 rows, 32 tokens of four heads, whether
+// there are as many or not; and while its workgroups have no more than 28 shared tiles per CU to go through (14 at head size 128, 10 at 256).  us per call, rows / stream (row
+// blocks / groups of the loop per KV head, tiles per CU): 128, 32 / 8 heads, 8 users over 1500 keys, 16 tokens 17.6 / 22.8 (1 / 1), 32 (2 / 1, 12) 23.2 / 23.5, 48 (3 / 2, 18)
+// 31.7 / 29.5, 128 46.7 / 33.3; 32 over 800, 16 tokens 23.6 / 29.6, 24 (2 / 1, 26) 30.7 / 26.4; 64 / 8 heads, 8 over 512 ... 5469, 16 tokens (2 / 2, 43) 43.9 / 45.6, 32 (4 / 2) 77 / 45;
+// 64, 16 / 16 heads, 32 over 800, 64 tokens 22.7 / 26.1, 128 (2 / 1, 52) 37.3 / 27.1; 256, 16 / 8 heads, 2 over 6404, 32 tokens 30.2 / 37.5, 48 (2 / 1, 13) 40.6 / 39.5,
+// 96 51 / 43.  Of 525 such pairs the rule takes the slower one of 27, by 15 ... 18 % at worst (2 users over 256 keys, 2048 rows of a KV head; 64 over 300, 96 ... 128 rows).
+// TTPA_CROSS_FORM=rows|stream, read on every call, overrides.
 bool streams(const CrossArgs &c, int head_size, int64_t keys) {
   const char *e = getenv("TTPA_CROSS_FORM");
   if (e && (!strcmp(e, "rows") || !strcmp(e, "stream"))) return !strcmp(e, "stream");
   const CrossCut cut = cross_cut(c.batch, c.hkv, (int64_t)c.g * c.s, head_size, keys);
-  const int64_t tiles = (keys + tile_of(head_size) - 1) / tile_of(head_size), row_blocks = (c.s + kRowsPerWave - 1) / kRowsPerWave;
+  const int64_t tiles = (keys + cut.tile - 1) / cut.tile, row_blocks = (c.s + kRowsPerWave - 1) / kRowsPerWave;
   const int64_t groups = c.g % 4 == 0 ? c.g / 4 * row_blocks : (row_blocks * c.g + 3) / 4;  // workgroups of the streaming loop per KV head
-  if (cut.row_blocks == 1 || 2 * cut.row_blocks <= 3 * groups) return false;
-  return (int64_t)c.batch * c.hkv * cut.row_blocks * tiles > (head_size == 256 ? 25 : 50) * (int64_t)std::max(device_cus(), 1);
+  if (cut.row_blocks <= groups) return false;
+  return (int64_t)c.batch * c.hkv * cut.row_blocks * tiles > (head_size == 64 ? 28 : head_size == 128 ? 14 : 10) * (int64_t)std::max(device_cus(), 1);
 }
 
 // Keys that the call is laid out for.
@@ -561,7 +696,6 @@ extern "C" int ttpa_paged_cross_attention(void *out, int64_t out_batch_stride, i
   const int64_t keys = decode::room_of(block_size, table_width, most_keys);
   a.w = (int)((keys + block_size - 1) / block_size);
   a.scale_log2e = scale * 1.4426950408889634f;
-  a.runs = (uint32_t)block_size / (decode::tile_of(head_size) / 4), a.runs_inv = 0xffffffffu / a.runs;
   hipStream_t st = static_cast<hipStream_t>(stream);
   PrefillArgs p;
   if (decode::stream_args(a, head_size, most_keys > 0, keys, p) && decode::streams(a, head_size, keys)) {
@@ -571,6 +705,7 @@ extern "C" int ttpa_paged_cross_attention(void *out, int64_t out_batch_stride, i
   }
   const decode::CrossCut c = decode::cross_cut(batch, kv_heads, (int64_t)a.g * q_len, head_size, keys);
   a.row_blocks = c.row_blocks, a.parts = c.parts, a.share = c.share;
+  a.runs = (uint32_t)block_size / (c.tile / 4), a.runs_inv = 0xffffffffu / a.runs;
   TTPA_REQUIRE(((int64_t)batch * kv_heads * c.parts + 8) * c.row_blocks < (1ll << 24) && (c.parts == 1 || (int64_t)a.g * q_len < 65536),
                "cross attention: too many rows for one launch");
   const int64_t need = decode::cross_bytes(c, batch, kv_heads, head_size);
@@ -578,8 +713,8 @@ extern "C" int ttpa_paged_cross_attention(void *out, int64_t out_batch_stride, i
     return fail(TTPA_ERR_WORKSPACE, "cross attention: needs %lld bytes of workspace, 16-byte aligned", (long long)need);
   a.slots = static_cast<float *>(workspace);
   switch (head_size) {
-    case 64: return decode::launch_cross_d<64>(a, c.groups, st);
-    case 128: return decode::launch_cross_d<128>(a, c.groups, st);
-    default: return decode::launch_cross_d<256>(a, c.groups, st);
+    case 64: return decode::launch_cross_d<64>(a, c, st);
+    case 128: return decode::launch_cross_d<128>(a, c, st);
+    default: return decode::launch_cross_d<256>(a, c, st);
   }
 }
