@@ -733,12 +733,12 @@ int ttpa_paged_cross_attention(void *out, int64_t out_batch_stride, int64_t out_
                                int32_t num_blocks, float scale, int64_t most_keys, void *workspace, int64_t workspace_bytes, void *stream);
 
 /*
- * Copies blocks inside caches: of every cache, n_caches tensors [num_blocks][block_bytes], block source_blocks[j] to target_blocks[j], as if j went from 0 on
+ * Copies blocks inside caches: of every cache, n_caches tensors [num_blocks][block_bytes[i]], block source_blocks[j] to target_blocks[j], as if j went from 0 on
  * (a block may be the target of one pair and the source of a later one).  Pairs with an id outside [0, num_blocks) are skipped.  caches_host is an array of
- * device pointers in host memory, read before the call returns.
+ * device pointers in host memory, block_bytes_host one of bytes per block (less than 2^31), read before the call returns.
  */
-int ttpa_copy_cache_blocks(void *const *caches_host, int32_t n_caches, int64_t block_bytes, const int32_t *source_blocks, const int32_t *target_blocks,
-                           int32_t pairs, int32_t num_blocks, void *stream);
+int ttpa_copy_cache_blocks(void *const *caches_host, const int64_t *block_bytes_host, int32_t n_caches, const int32_t *source_blocks,
+                           const int32_t *target_blocks, int32_t pairs, int32_t num_blocks, void *stream);
 
 /*
  * Compacts sequences inside caches [num_blocks][heads][block_size] of rows of row_bytes (a multiple of 16): in every cache and head, position first[u] + i

@@ -75,7 +75,10 @@ def _some(n=1, p=256):
 
 
 def _copy(lib, caches=256, n=1, bytes_=64, source=16, pairs=2, nb=8):
-    return lib.ttpa_copy_cache_blocks(_some(n, caches) if caches != "none" else None, n, bytes_, source, 16, pairs, nb, None)
+    import ctypes
+
+    sizes = None if bytes_ is None else (ctypes.c_int64 * max(n, 1))(*([bytes_] * n))
+    return lib.ttpa_copy_cache_blocks(_some(n, caches) if caches != "none" else None, sizes, n, source, 16, pairs, nb, None)
 
 
 def _keep(lib, caches=256, n=1, pt=16, users=2, most=4, heads=2, row=128, bs=32, w=4, nb=8):
@@ -91,7 +94,7 @@ def _keep(lib, caches=256, n=1, pt=16, users=2, most=4, heads=2, row=128, bs=32,
     (_cross, dict(d=96), -2, b"head_size"), (_cross, dict(bs=48), -2, b"block_size"), (_cross, dict(bs=8192), -2, b"block_size"),
     (_cross, dict(scale=0.0), -1, b"scale"), (_cross, dict(scale=-1.0), -1, b"scale"), (_cross, dict(most=-1), -1, b"most_keys"), (_cross, dict(w=1 << 26), -1, b"too many keys"),
     (_cross, dict(q=24), -1, b"aligned"), (_cross, dict(stride=1028), -1, b"strides"), (_cross, dict(ws_bytes=0, users=1, w=400), -3, b"workspace"),
-    (_copy, dict(caches=None), -1, b"null"), (_copy, dict(caches="none"), -1, b"null"), (_copy, dict(source=None), -1, b"null"), (_copy, dict(bytes_=0), -1, b"dimension"),
+    (_copy, dict(caches=None), -1, b"null"), (_copy, dict(caches="none"), -1, b"null"), (_copy, dict(source=None), -1, b"null"), (_copy, dict(bytes_=0), -1, b"bytes"), (_copy, dict(bytes_=1 << 31), -1, b"bytes"), (_copy, dict(bytes_=None), -1, b"null"),
     (_copy, dict(pairs=-1), -1, b"dimension"), (_copy, dict(nb=0), -1, b"dimension"), (_copy, dict(n=-1), -1, b"null"),
     (_keep, dict(caches=None), -1, b"null"), (_keep, dict(pt=None), -1, b"null"), (_keep, dict(users=-1), -1, b"dimension"), (_keep, dict(row=24), -2, b"multiples of 16"),
     (_keep, dict(caches=264), -1, b"aligned"), (_keep, dict(w=1 << 26), -1, b"too many tokens"), (_keep, dict(heads=1 << 24), -1, b"too many rows"),

@@ -673,21 +673,13 @@ void copy_cache_blocks_(at::TensorList caches, const Tensor &source_blocks, cons
   TORCH_CHECK_VALUE(source.size(0) == target.size(0), c.name(), ": as many source_blocks as target_blocks, got ", source.size(0), " and ", target.size(0));
   const int64_t nb = caches[0].size(0);
   if (source.size(0) == 0 || nb == 0) return;
-  std::vector<std::pair<int64_t, void *>> of_size;  // a launch takes caches whose blocks are of one size
-  of_size.reserve(caches.size());
-  for (const Tensor &t : caches)
-    if (t.numel()) of_size.emplace_back((int64_t)t.nbytes() / nb, t.data_ptr());
-  if (std::any_of(of_size.begin(), of_size.end(), [&](const auto &x) { return x.first != of_size[0].first; }))
-    std::stable_sort(of_size.begin(), of_size.end(), [](const auto &x, const auto &y) { return x.first > y.first; });
   std::vector<void *> some;
-  some.reserve(of_size.size());
-  for (size_t i = 0; i < of_size.size();) {
-    const int64_t bytes = of_size[i].first;
-    some.clear();
-    for (; i < of_size.size() && of_size[i].first == bytes; ++i) some.push_back(of_size[i].second);
-    ok("ttpa_copy_cache_blocks",
-       ttpa_copy_cache_blocks(some.data(), i32(some.size()), bytes, int_ptr(source), int_ptr(target), i32(source.size(0)), i32(nb), c.stream()));
-  }
+  std::vector<int64_t> bytes;
+  some.reserve(caches.size()), bytes.reserve(caches.size());
+  for (const Tensor &t : caches)
+    if (t.numel()) some.push_back(t.data_ptr()), bytes.push_back((int64_t)t.nbytes() / nb);
+  ok("ttpa_copy_cache_blocks",
+     ttpa_copy_cache_blocks(some.data(), bytes.data(), i32(some.size()), int_ptr(source), int_ptr(target), i32(source.size(0)), i32(nb), c.stream()));
   for (const Tensor &t : caches) written(t);
 }
 
