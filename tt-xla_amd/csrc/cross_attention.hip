@@ -471,24 +471,29 @@ __global__ __launch_bounds__(256) void cross_merge_kernel(CrossArgs a) {
   const int slice = SLICES > 1 ? (int)threadIdx.x / PER : 0, f = threadIdx.x % PER;
   const int seg = blockIdx.x, m = blockIdx.y * AT_ONCE + (SLICES > 1 ? 0 : (int)threadIdx.x / PER), rb = m / ROWS, row = m - rb * ROWS;
   const int u = seg / a.hkv, h = seg - u * a.hkv, token = m / a.g, head = m - token * a.g;
-  const int count = cross_parts(a, cross_keys(a, load_index(a.lens, a.lens_i64, u)));
-  if (count == 1 || m >= a.g * a.s) return;  // (the one workgroup has written the output)
+  if (m >= a.g * a.s) return;
+  const int64_t length = load_index(a.lens, a.lens_i64, u);
   uint16_t *dst = a.out + u * a.o_bs + (int64_t)(h * a.g + head) * a.o_hs + token * a.o_ts + 4 * f;
   const float *slot = a.slots + (int64_t)(seg * a.row_blocks + rb) * a.parts * SLOT;
-  float mall = -INFINITY, num[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
-  for (int p0 = slice; p0 < count; p0 += SLICES * BATCH) {
-    float mv[BATCH], lv[BATCH];
-    float4 v[BATCH];
+  float mv[BATCH], lv[BATCH];
+  float4 v[BATCH];
+  const auto fetch = [&](int p0) {
 #pragma unroll
     for (int j = 0; j < BATCH; ++j) {
-      const float *p = slot + (int64_t)min(p0 + j * SLICES, count - 1) * SLOT;
+      const float *p = slot + (int64_t)min(p0 + j * SLICES, a.parts - 1) * SLOT;
       v[j] = *reinterpret_cast<const float4 *>(p + row * D + 4 * f);
       mv[j] = p[ROWS * D + row], lv[j] = p[ROWS * (D + 1) + row];
     }
-    // (shares past the last, the last one again, do not count)
+  };
+  fetch(slice);  // (beside the length; parts that the user does not have hold anything, and are not used)
+  const int count = cross_parts(a, cross_keys(a, length));
+  if (count == 1) return;  // (the one workgroup has written the output)
+  float mall = -INFINITY, num[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
+  for (int p0 = slice; p0 < count; p0 += SLICES * BATCH) {
+    if (p0 != slice) fetch(p0);
     float m_new = mall;
 #pragma unroll
-    for (int j = 0; j < BATCH; ++j) m_new = fmaxf(m_new, mv[j]);
+    for (int j = 0; j < BATCH; ++j) m_new = p0 + j * SLICES < count ? fmaxf(m_new, mv[j]) : m_new;
     const float ref = merge_reference(m_new), resc = __builtin_amdgcn_exp2f(mall - ref);
 #pragma unroll
     for (int r = 0; r < 4; ++r) num[r] *= resc;
