@@ -19,9 +19,9 @@ def _pkg():
     import tt_xla_amd  # noqa: F401
 
 
-@pytest.fixture(params=["rows", "stream", None], autouse=True)
+@pytest.fixture(params=["rows", "planned", "stream", None], autouse=True)
 def form(request, monkeypatch):
-    """The form for few rows, the streaming loop, and what the library chooses."""
+    """The forms for few rows, their parts by the longest user or by all users' lengths, the streaming loop, and what the library chooses."""
     if request.param:
         monkeypatch.setenv("TTPA_CROSS_FORM", request.param)
     return request.param
@@ -82,6 +82,17 @@ def test_long(d, hkv, grp, s, lens):
         q, k, v, table = _inputs(g, len(lens), hkv, grp, s, d, bs, lens, -(-max(lens) // bs) + 3)
         for kw in ({}, {"most_keys": max(lens), "scale": 0.3}):
             _check(_run(q, k, v, table, lens, **kw), q, k, v, table, lens, kw.get("scale", d**-0.5))
+
+
+@pytest.mark.parametrize("d, hq, hkv, s", [(128, 8, 2, 1), (128, 16, 2, 8), (64, 6, 3, 2), (256, 4, 2, 3), (64, 8, 1, 20)])
+@pytest.mark.parametrize("users", [64, 150])
+def test_many_users_of_all_lengths(d, hq, hkv, s, users):
+    """One long user among short ones and none, more users than a wavefront has lanes, lengths in 64 bits: every unit of the plan once."""
+    g = torch.Generator().manual_seed(users + d)
+    lens = torch.randint(0, 70, (users,), generator=g)
+    lens[users // 2], lens[0] = 3000, 0
+    q, k, v, table = _inputs(g, users, hkv, hq // hkv, s, d, 32, lens.tolist(), 94)
+    _check(_run(q, k, v, table, lens), q, k, v, table, lens, d**-0.5)
 
 
 def test_lengths_beyond_the_table_and_below_zero_and_pages_outside():

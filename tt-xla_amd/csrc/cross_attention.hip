@@ -16,7 +16,8 @@
 //                                 key (TILE / 4) j + 4 b + r, so lane (row, quad) ends up with its quad's run in order, which is
 //   O^T += V^T . P^T              the order in which the second product wants its weights: no moves between the two
 // Statistics and accumulators are floats; weights are rounded once to bfloat16 for the matrix instruction, and the same rounded weights are summed.
-// Wavefronts' results of their own tiles meet in LDS, the parts' in memory, merged by a kernel of its own.
+// Wavefronts' results of their own tiles meet in LDS, the parts' in memory, merged by a kernel of its own.  How many parts there are goes by an estimate of the time, the host's of the longest
+// user, or, where that is long enough to pay for it, the device's of all of them (cross_work).
 #include "decode_mfma16_kernel.h"
 #include "prefill_common.h"
 
@@ -45,6 +46,12 @@ struct CrossArgs {
   uint32_t runs, runs_inv;  // runs of keys per block, and floor((2^32 - 1) / runs)
   int row_blocks, parts, share;  // share: keys of a part at least
   float *slots;  // [batch * hkv * row_blocks][parts]: ROWS * D values, ROWS maxima, ROWS sums
+  // Several users: the parts go by their lengths, of which each workgroup makes the same plan (cross_work).  Slots are then [unit][row_blocks], and
+  // firsts[u] = a user's first unit over hkv, and its parts.
+  int2 *firsts;
+  int units;             // most of them: (user, KV head, part)
+  float slots_of_cus;    // workgroups of one round, one per CU, over row_blocks
+  float step_us, two, merge_us;  // the estimate of cross_cut: a step of a workgroup, two on a CU, a unit's part of the merge
 };
 
 template <int D>
@@ -78,6 +85,64 @@ constexpr int cross_slot_floats() {
 }
 // Keys of a user, of those that the table has room for.
 __device__ __forceinline__ int cross_keys(const CrossArgs &a, int64_t length) { return (int)max(min(length, (int64_t)a.w * a.bs), (int64_t)0); }
+
+// What a workgroup does: part `part` of `parts` of a user's keys for a KV head (part >= parts: nothing); the user's first unit over hkv.
+struct CrossWork {
+  int u, h, part, parts, keys, first;
+};
+// Steps of a part, of `total` steps of all users' keys per KV head, the longest user's `longest`: as many workgroups as CUs, twice as many, or one per user and KV head, by
+// the least estimate.  At least total * hkv / (2 slots_of_cus), so that there are never more than 2 slots_of_cus + batch * hkv units.
+__device__ __forceinline__ int cross_share(const CrossArgs &a, int total, int longest) {
+  const float all = (float)total * (float)a.hkv, segments = (float)(a.batch * a.hkv), one = a.slots_of_cus;
+  const auto cost = [&](float share, float units) {
+    const float rounds = units / one;
+    return share * a.step_us * (rounds <= 1.f ? 1.f : a.two * ceilf(0.5f * rounds));
+  };
+  float best = (float)longest, least = cost(best, segments);
+#pragma unroll
+  for (int k = 1; k <= 2; ++k) {
+    const float room = (float)k * one, share = fmaxf(ceilf(all / fmaxf(room - 0.5f * segments, 0.5f * room)), 1.f);
+    const float units = fminf(all / share + 0.5f * segments, room), c = cost(share, units) + units * a.merge_us + 1.f;
+    if (share < best && c < least) best = share, least = c;
+  }
+  return max((int)best, (longest + kMostCrossParts - 1) / kMostCrossParts);
+}
+// The n-th unit by the users' lengths: user after user, a user's parts one after the other, KV heads fastest.  STEP keys are what a workgroup takes at a time.
+template <int STEP>
+__device__ __forceinline__ CrossWork cross_work(const CrossArgs &a, int n) {
+  const int lane = (int)threadIdx.x & 63, x = n / a.hkv;
+  const auto keys_of = [&](int u) { return u < a.batch ? cross_keys(a, load_index(a.lens, a.lens_i64, u)) : 0; };
+  int keys = keys_of(lane), steps = (keys + STEP - 1) / STEP, total = steps, longest = steps;
+  for (int u0 = 64; u0 < a.batch; u0 += 64) {
+    const int more = (keys_of(u0 + lane) + STEP - 1) / STEP;
+    total += more, longest = max(longest, more);
+  }
+  total = __builtin_amdgcn_readlane(wave_prefix_sum(total), 63), longest = (int)wave_max_u32((uint32_t)longest);
+  const int share = max(cross_share(a, total, longest), 1);
+  CrossWork w = {0, n - x * a.hkv, 0, 0, 0, 0};
+  for (int u0 = 0, before = 0; u0 < a.batch; u0 += 64) {
+    if (u0 > 0) keys = keys_of(u0 + lane), steps = (keys + STEP - 1) / STEP;
+    const int mine = u0 + lane < a.batch ? max((steps + share - 1) / share, 1) : 0, upto = before + wave_prefix_sum(mine);
+    const uint64_t behind = __builtin_amdgcn_ballot_w64(upto > x);
+    if (behind) {
+      const int l = __builtin_ctzll(behind);
+      w.u = u0 + l, w.parts = __builtin_amdgcn_readlane(mine, l), w.keys = __builtin_amdgcn_readlane(keys, l);
+      w.first = __builtin_amdgcn_readlane(upto, l) - w.parts, w.part = x - w.first;
+      break;
+    }
+    before = __builtin_amdgcn_readlane(upto, 63);
+  }
+  return w;
+}
+// The plan for the merge, by one workgroup of a user (behind its loads: the compiler reads page tables by scalar loads only where no store comes before them.  By vector loads, which
+// are waited for behind the tiles on their way, cross_shared_kernel took 4 of 26 us more).
+__device__ __forceinline__ void cross_note(const CrossArgs &a, const CrossWork &w, int rb) {
+  if (a.firsts && rb == 0 && w.part == 0 && w.h == 0 && threadIdx.x == 0) a.firsts[w.u] = make_int2(w.first, w.parts);
+}
+// The slot of a segment's first part.
+__device__ __forceinline__ int64_t cross_slot(const CrossArgs &a, int u, int h, int rb, int first) {
+  return a.firsts ? ((int64_t)first * a.hkv + h) * a.row_blocks + rb : ((int64_t)(u * a.hkv + h) * a.row_blocks + rb) * a.parts;
+}
 
 // A wavefront's rows and what it has of the result; what it does with a tile of TILE keys that lies in LDS.
 template <int D, int RG, int KEYS>
@@ -262,20 +327,27 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   // workgroup -> (user, KV head) and block of rows, the blocks of one eight workgroups apart: on one XCD, which reads its keys once
   const uint32_t span = 8u * a.row_blocks, set = blockIdx.x / span, in_set = blockIdx.x - set * span;
   const int rb = (int)(in_set >> 3), unit = (int)(set * 8 + (in_set & 7)), segments = a.batch * a.hkv;
-  if (unit >= segments * a.parts) return;
-  const int part = unit / segments, uh = unit - part * segments, u = uh / a.hkv, h = uh - u * a.hkv;
+  if (unit >= (a.firsts ? a.units : segments * a.parts)) return;
   const int lane = threadIdx.x & 63, wib = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int rows = a.g * a.s, row0 = rb * ROWS;
+  CrossWork w;
+  if (a.firsts) {
+    w = cross_work<4 * TILE>(a, unit);
+    if (w.part >= w.parts) return;
+  } else {
+    w.part = unit / segments, w.u = (unit - w.part * segments) / a.hkv, w.h = unit - w.part * segments - w.u * a.hkv;
+  }
+  const int u = __builtin_amdgcn_readfirstlane(w.u), h = __builtin_amdgcn_readfirstlane(w.h), part = __builtin_amdgcn_readfirstlane(w.part), rows = a.g * a.s, row0 = rb * ROWS;
   // (the first page and the rows are asked for beside the length)
   T x(a, tiles + wib * cross_lds_bytes<D>());
   int t = part * 4 + wib;
-  const int64_t length = load_index(a.lens, a.lens_i64, u);
+  const int64_t length = a.firsts ? w.keys : load_index(a.lens, a.lens_i64, u);
   const uint64_t at0 = x.look_up(u, h, t);
   x.load_q(u, h, row0);
   const int keys = __builtin_amdgcn_readfirstlane(cross_keys(a, length)), n_tiles = (keys + TILE - 1) / TILE;
-  const int parts = cross_parts(a, keys), step = 4 * parts;
+  const int parts = __builtin_amdgcn_readfirstlane(a.firsts ? w.parts : cross_parts(a, keys)), step = 4 * parts;
   if (part >= parts) return;
   if (keys == 0) {  // nothing to attend
+    cross_note(a, w, rb);
 #pragma unroll 1
     for (int i = threadIdx.x; i < min(ROWS, rows - row0) * CPR; i += 256) {
       const int m = row0 + i / CPR, token = m / a.g, head = m - token * a.g;
@@ -301,6 +373,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     process_tile(std::false_type{});
   }
 
+  cross_note(a, w, rb);
   // ---- the wavefronts' results, a share of the features at a time (a wavefront's tiles hold that many) ------
   constexpr int FIT = cross_lds_bytes<D>() / (RG * 64 * 16);  // blocks of 16 features: 16 bytes per lane and group
   constexpr int BLOCKS = FIT >= 8 ? 8 : FIT >= 4 ? 4 : FIT >= 2 ? 2 : FIT;
@@ -339,7 +412,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         den = fmaf(wgt, s_ml[w][row].y, den);
       }
       if (parts > 1) {
-        float *const slot = a.slots + ((int64_t)(uh * a.row_blocks + rb) * a.parts + part) * cross_slot_floats<D, ROWS>();
+        float *const slot = a.slots + (a.firsts ? (int64_t)unit * a.row_blocks + rb : cross_slot(a, u, h, rb, 0) + part) * cross_slot_floats<D, ROWS>();
         *reinterpret_cast<float4 *>(slot + row * D + feature) = make_float4(num[0], num[1], num[2], num[3]);
         if (feature == 0) slot[ROWS * D + row] = mall, slot[ROWS * (D + 1) + row] = den;
         continue;
@@ -366,21 +439,28 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   extern __shared__ __attribute__((aligned(16))) uint8_t tiles[];  // two of K and V
   const uint32_t span = 8u * a.row_blocks, set = blockIdx.x / span, in_set = blockIdx.x - set * span;
   const int rb = (int)(in_set >> 3), unit = (int)(set * 8 + (in_set & 7)), segments = a.batch * a.hkv;
-  if (unit >= segments * a.parts) return;
-  const int part = unit / segments, uh = unit - part * segments, u = uh / a.hkv, h = uh - u * a.hkv;
+  if (unit >= (a.firsts ? a.units : segments * a.parts)) return;
   const int lane = threadIdx.x & 63, wib = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int rows = a.g * a.s, row0 = rb * ROWS + 16 * wib;
+  CrossWork w;
+  if (a.firsts) {
+    w = cross_work<TILE>(a, unit);
+    if (w.part >= w.parts) return;
+  } else {
+    w.part = unit / segments, w.u = (unit - w.part * segments) / a.hkv, w.h = unit - w.part * segments - w.u * a.hkv;
+  }
+  const int u = __builtin_amdgcn_readfirstlane(w.u), h = __builtin_amdgcn_readfirstlane(w.h), part = __builtin_amdgcn_readfirstlane(w.part), rows = a.g * a.s, row0 = rb * ROWS + 16 * wib;
   const bool mine = row0 < rows;  // (a wavefront without rows loads its share of the keys)
   T x(a);
   int t = part;
   const auto look_up = [&](int tile) { return x.place(u, h, (uint32_t)(tile * 4 + wib)) + 16 * lane; };
-  const int64_t length = load_index(a.lens, a.lens_i64, u);
+  const int64_t length = a.firsts ? w.keys : load_index(a.lens, a.lens_i64, u);
   const uint64_t at0 = look_up(t);
   if (mine) x.load_q(u, h, row0);
   const int keys = __builtin_amdgcn_readfirstlane(cross_keys(a, length)), n_tiles = (keys + TILE - 1) / TILE;
-  const int parts = cross_parts(a, keys), step = parts;
+  const int parts = __builtin_amdgcn_readfirstlane(a.firsts ? w.parts : cross_parts(a, keys)), step = parts;
   if (part >= parts) return;
   if (keys == 0) {  // nothing to attend
+    cross_note(a, w, rb);
 #pragma unroll 1
     for (int i = threadIdx.x; i < min(ROWS, rows - rb * ROWS) * CPR; i += 256) {
       const int m = rb * ROWS + i / CPR, token = m / a.g, head = m - token * a.g;
@@ -440,10 +520,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       if (t < n_tiles) process(1, kraw[1], vraw[1]);
     }
   }
+  cross_note(a, w, rb);
   const int m = row0 + x.n, token = m / a.g, head = m - token * a.g;
   if (m >= rows) return;
   if (parts > 1) {
-    float *const slot = a.slots + ((int64_t)(uh * a.row_blocks + rb) * a.parts + part) * cross_slot_floats<D, ROWS>();
+    float *const slot = a.slots + (a.firsts ? (int64_t)unit * a.row_blocks + rb : cross_slot(a, u, h, rb, 0) + part) * cross_slot_floats<D, ROWS>();
     const int row = m - rb * ROWS;
 #pragma unroll
     for (int db = 0; db < DBLK; ++db) {
@@ -466,27 +547,31 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 // thread's own (SLICES 1), where they are few.
 template <int D, int ROWS, int SLICES>
 __global__ __launch_bounds__(256) void cross_merge_kernel(CrossArgs a) {
-  constexpr int SLOT = cross_slot_floats<D, ROWS>(), PER = D / 4, BATCH = 4, THREADS = SLICES > 1 ? SLICES * PER : 256;
+  constexpr int SLOT = cross_slot_floats<D, ROWS>(), PER = D / 4, BATCH = SLICES > 1 ? 4 : 8, THREADS = SLICES > 1 ? SLICES * PER : 256;
   constexpr int AT_ONCE = THREADS / (PER * SLICES);  // rows of a workgroup
   const int slice = SLICES > 1 ? (int)threadIdx.x / PER : 0, f = threadIdx.x % PER;
   const int seg = blockIdx.x, m = blockIdx.y * AT_ONCE + (SLICES > 1 ? 0 : (int)threadIdx.x / PER), rb = m / ROWS, row = m - rb * ROWS;
   const int u = seg / a.hkv, h = seg - u * a.hkv, token = m / a.g, head = m - token * a.g;
   if (m >= a.g * a.s) return;
-  const int64_t length = load_index(a.lens, a.lens_i64, u);
   uint16_t *dst = a.out + u * a.o_bs + (int64_t)(h * a.g + head) * a.o_hs + token * a.o_ts + 4 * f;
-  const float *slot = a.slots + (int64_t)(seg * a.row_blocks + rb) * a.parts * SLOT;
+  const int64_t length = load_index(a.lens, a.lens_i64, u);
+  int first = 0, count = a.parts;
+  if (a.firsts) first = a.firsts[u].x, count = a.firsts[u].y;
+  const float *slot = a.slots + cross_slot(a, u, h, rb, first) * SLOT;
+  const int64_t behind = a.firsts ? (int64_t)a.hkv * a.row_blocks * SLOT : SLOT;
   float mv[BATCH], lv[BATCH];
   float4 v[BATCH];
   const auto fetch = [&](int p0) {
 #pragma unroll
     for (int j = 0; j < BATCH; ++j) {
-      const float *p = slot + (int64_t)min(p0 + j * SLICES, a.parts - 1) * SLOT;
+      if (p0 + j * SLICES >= count) continue;
+      const float *p = slot + (p0 + j * SLICES) * behind;
       v[j] = *reinterpret_cast<const float4 *>(p + row * D + 4 * f);
       mv[j] = p[ROWS * D + row], lv[j] = p[ROWS * (D + 1) + row];
     }
   };
-  fetch(slice);  // (beside the length; parts that the user does not have hold anything, and are not used)
-  const int count = cross_parts(a, cross_keys(a, length));
+  fetch(slice);  // (where they do not go by the plan, beside the length; parts that the user does not have hold anything, and are not used)
+  if (!a.firsts) count = cross_parts(a, cross_keys(a, length));
   if (count == 1) return;  // (the one workgroup has written the output)
   float mall = -INFINITY, num[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
   for (int p0 = slice; p0 < count; p0 += SLICES * BATCH) {
@@ -530,6 +615,12 @@ __global__ __launch_bounds__(256) void cross_merge_kernel(CrossArgs a) {
   *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_bf16x2(num[0] * inv, num[1] * inv), pack_bf16x2(num[2] * inv, num[3] * inv));
 }
 
+// TTPA_CROSS_FORM=rows|planned|stream, read on every call.
+bool form_is(const char *name) {
+  const char *e = getenv("TTPA_CROSS_FORM");
+  return e && !strcmp(e, name);
+}
+
 // How a call is cut: blocks of rows, and the groups of 16 that a wavefront has of one; parts of the keys and keys of a part.
 // Wavefronts share their tiles from 33 rows on, where blocks of 32 would read the keys more than once, and at head size 256, where 32 rows are too many for a wavefront
 // and tiles of its own leave room for one workgroup on a CU.  us per call, own tiles / shared, the best parts of each: 128, 8 users of 64 / 8 heads over 512 ... 5469 keys,
@@ -539,6 +630,8 @@ __global__ __launch_bounds__(256) void cross_merge_kernel(CrossArgs a) {
 struct CrossCut {
   bool shared;
   int groups, row_blocks, parts, share, tile;
+  int units;  // planned on the device: most of them; else 0
+  double step_us, two, merge_us;
   int rows() const { return (shared ? 64 : 16) * groups; }
 };
 
@@ -547,6 +640,10 @@ struct CrossCut {
 // the longest chain, or all of them.  The two are weighed 7 : 3; with tiles of their own, chains of more than eight count more while the launch does not fill the chip; a
 // split costs the merge.  Chosen / best of all: within 1 % over 28 shapes from 1 x 8 heads of 250 keys to 96 x 8 of 2033, 10 % at worst (8 x 8 of 512 ... 3597, 32
 // rows); shared, 3 % over 31 from 1 x 8 of 100 to 96 x 8 of 1500, 14 % at worst (one user of 1500, 56 rows).
+// Parts by the users' lengths: the host sees the longest alone, and a launch cut for tables as long as that leaves CUs to a few users' parts.  So where the estimate is 12 us or more, the
+// device plans (cross_work), which costs each workgroup a round trip, 0.5 ... 0.7 us a call.  us per call, by the longest / planned: 64 / 8 heads of 128, 5 tokens, 8 users over 512 ... 5469 keys
+// 26.5 / 22.0, seven over 200 and one over 6404 27.4 / 16.8, 32 over 256 ... 1983 35.1 / 31.0, 48 over 512 ... 6238 104 / 96, 8 over 1500 each (less than 12) 15.9 / 16.6; 32 / 8, 16
+// over 100 ... 6976 40.4 / 25.7, 32 over 256 ... 3911 35.2 / 33.9; of 64, 16 over 512 ... 5918, 5 tokens 24.0 / 19.9; of 256, 64 / 8, 8 over 512 ... 3597, 8 tokens 39.6 / 32.8.
 CrossCut cross_cut(int batch, int kv_heads, int64_t rows, int head_size, int64_t keys) {
   CrossCut c = {};
   c.shared = head_size == 256 || rows > 32;
@@ -571,10 +668,17 @@ CrossCut cross_cut(int batch, int kv_heads, int64_t rows, int head_size, int64_t
   }
   c.parts = std::max(c.parts, 1);
   c.share = std::max((tiles + c.parts - 1) / c.parts, chains) * c.tile;
+  if (c.parts > 1 && (best >= 12.0 || form_is("planned")) && batch > 1 && batch <= 1024 && (int64_t)batch * tiles < (1 << 30)) {
+    c.units = (int)(2 * cus / c.row_blocks) + 1 + batch * kv_heads;
+    c.step_us = tile_us, c.two = two, c.merge_us = (c.shared ? 1.75 * head_size / 128 : 1.0) * merged / (batch * kv_heads);
+  }
   return c;
 }
+int64_t firsts_bytes(int batch) { return ((int64_t)batch * 8 + 255) & ~int64_t(255); }
 int64_t cross_bytes(const CrossCut &c, int batch, int kv_heads, int head_size) {
-  return c.parts == 1 ? 256 : (int64_t)batch * kv_heads * c.row_blocks * c.parts * (c.rows() * (int64_t)(head_size + 2) * 4);
+  const int64_t slot = c.rows() * (int64_t)(head_size + 2) * 4;
+  if (c.units) return firsts_bytes(batch) + (int64_t)c.units * c.row_blocks * slot;
+  return c.parts == 1 ? 256 : (int64_t)batch * kv_heads * c.row_blocks * c.parts * slot;
 }
 
 template <int D, int RG, bool SHARED>
@@ -587,13 +691,13 @@ int launch_cross(const CrossArgs &a, hipStream_t st) {
   const size_t lds = SHARED ? 4 * shared_tile<D>() * D * 2 : 4 * cross_lds_bytes<D>();
   if (!ensure_dynamic_lds(reinterpret_cast<const void *>(kernel), lds, lds_ready))
     return fail(TTPA_ERR_LAUNCH, "cross attention: cannot reserve %d bytes of LDS", (int)lds);
-  const int64_t units = (int64_t)a.batch * a.hkv * a.parts;
+  const int64_t units = a.firsts ? a.units : (int64_t)a.batch * a.hkv * a.parts;
   launch_dominant(kernel, dim3((unsigned)((units + 7) / 8 * 8 * a.row_blocks)), dim3(256), lds, st, a);
   if (const int rc = check_launch("cross attention")) return rc;
   if (a.parts == 1) return TTPA_OK;
   // slices only for many parts: 2 / 3 / 4 parts of 64 rows, 8 users of 32 / 8 heads over 1500 keys 19.8 / 23.5 / 22.3 us with them, 17.0 / 20.5 / 19.5 without; 16 the same
   constexpr int ROWS = (SHARED ? 64 : 16) * RG, AT_ONCE = 1024 / D;
-  if (a.parts > 16)
+  if (a.firsts ? 2 * a.slots_of_cus > 16 * a.batch * a.hkv : a.parts > 16)
     cross_merge_kernel<D, ROWS, 1024 / D><<<dim3(a.batch * a.hkv, a.g * a.s), dim3(256), 0, st>>>(a);
   else
     cross_merge_kernel<D, ROWS, 1><<<dim3(a.batch * a.hkv, (a.g * a.s + AT_ONCE - 1) / AT_ONCE), dim3(256), 0, st>>>(a);
@@ -626,14 +730,15 @@ bool stream_args(const CrossArgs &c, int head_size, bool keys_known, int64_t key
 
 // Which form takes a call: the rows' where it reads the keys no more often than the streaming loop, which reads a key once for 128 rows, 32 tokens of four heads, whether
 // there are as many or not; and while its workgroups have no more than 28 shared tiles per CU to go through (14 at head size 128, 10 at 256).  us per call, rows / stream (row
-// blocks / groups of the loop per KV head, tiles per CU): 128, 32 / 8 heads, 8 users over 1500 keys, 16 tokens 17.6 / 22.8 (1 / 1), 32 (2 / 1, 12) 23.2 / 23.5, 48 (3 / 2, 18)
-// 31.7 / 29.5, 128 46.7 / 33.3; 32 over 800, 16 tokens 23.6 / 29.6, 24 (2 / 1, 26) 30.7 / 26.4; 64 / 8 heads, 8 over 512 ... 5469, 16 tokens (2 / 2, 43) 43.9 / 45.6, 32 (4 / 2) 77 / 45;
-// 64, 16 / 16 heads, 32 over 800, 64 tokens 22.7 / 26.1, 128 (2 / 1, 52) 37.3 / 27.1; 256, 16 / 8 heads, 2 over 6404, 32 tokens 30.2 / 37.5, 48 (2 / 1, 13) 40.6 / 39.5,
-// 96 51 / 43.  Of 525 such pairs the rule takes the slower one of 27, by 15 ... 18 % at worst (2 users over 256 keys, 2048 rows of a KV head; 64 over 300, 96 ... 128 rows).
-// TTPA_CROSS_FORM=rows|stream, read on every call, overrides.
+// blocks / groups of the loop per KV head, tiles per CU): 128, 32 / 8 heads, 8 users over 1500 keys, 16 tokens 18.4 / 22.8 (1 / 1), 32 (2 / 1, 12) 24.0 / 24.5, 48 (3 / 2, 18)
+// 32.0 / 29.5, 128 46.7 / 34.3; 32 over 800, 16 tokens 24.2 / 29.4, 24 (2 / 1, 26) 31.8 / 26.0; 64 / 8 heads, 8 over 512 ... 5469, 16 tokens (2 / 2, 43) 32.3 / 45.3, 32 (4 / 2) 49.6 / 45.3;
+// 64, 16 / 16 heads, 32 over 800, 64 tokens 23.0 / 27.9, 128 (2 / 1, 52) 37.0 / 31.1; 256, 16 / 8 heads, 2 over 6404, 32 tokens 29.6 / 37.2, 48 (2 / 1, 13) 42.5 / 39.5,
+// 96 57 / 44.  Of 525 such pairs the rule takes the slower one, by more than 3 %, of 47: by 13 ... 18 % at most where all users are as long as the longest, which is what the host
+// knows, and by 35 % where they are not and parts by their lengths would have paid (40 / 8 heads, 8 over 512 ... 5469, 48 tokens 49 / 66).
+// TTPA_CROSS_FORM overrides.
 bool streams(const CrossArgs &c, int head_size, int64_t keys) {
-  const char *e = getenv("TTPA_CROSS_FORM");
-  if (e && (!strcmp(e, "rows") || !strcmp(e, "stream"))) return !strcmp(e, "stream");
+  if (form_is("rows") || form_is("planned")) return false;
+  if (form_is("stream")) return true;
   const CrossCut cut = cross_cut(c.batch, c.hkv, (int64_t)c.g * c.s, head_size, keys);
   const int64_t tiles = (keys + cut.tile - 1) / cut.tile, row_blocks = (c.s + kRowsPerWave - 1) / kRowsPerWave;
   const int64_t groups = c.g % 4 == 0 ? c.g / 4 * row_blocks : (row_blocks * c.g + 3) / 4;  // workgroups of the streaming loop per KV head
@@ -711,12 +816,17 @@ extern "C" int ttpa_paged_cross_attention(void *out, int64_t out_batch_stride, i
   const decode::CrossCut c = decode::cross_cut(batch, kv_heads, (int64_t)a.g * q_len, head_size, keys);
   a.row_blocks = c.row_blocks, a.parts = c.parts, a.share = c.share;
   a.runs = (uint32_t)block_size / (c.tile / 4), a.runs_inv = 0xffffffffu / a.runs;
-  TTPA_REQUIRE(((int64_t)batch * kv_heads * c.parts + 8) * c.row_blocks < (1ll << 24) && (c.parts == 1 || (int64_t)a.g * q_len < 65536),
+  TTPA_REQUIRE(((int64_t)std::max(c.units, batch * kv_heads * c.parts) + 8) * c.row_blocks < (1ll << 24) && (c.parts == 1 || (int64_t)a.g * q_len < 65536),
                "cross attention: too many rows for one launch");
   const int64_t need = decode::cross_bytes(c, batch, kv_heads, head_size);
   if (a.parts > 1 && (!workspace || !aligned16(workspace) || workspace_bytes < need))
     return fail(TTPA_ERR_WORKSPACE, "cross attention: needs %lld bytes of workspace, 16-byte aligned", (long long)need);
   a.slots = static_cast<float *>(workspace);
+  if (c.units) {
+    a.firsts = static_cast<int2 *>(workspace), a.slots = reinterpret_cast<float *>(static_cast<char *>(workspace) + decode::firsts_bytes(batch));
+    a.units = c.units, a.slots_of_cus = (float)std::max(device_cus(), 1) / (float)c.row_blocks;
+    a.step_us = (float)c.step_us, a.two = (float)c.two, a.merge_us = (float)c.merge_us;
+  }
   switch (head_size) {
     case 64: return decode::launch_cross_d<64>(a, c, st);
     case 128: return decode::launch_cross_d<128>(a, c, st);
