@@ -723,6 +723,7 @@ int ttpa_qk_norm_rope_axes(void *q_out, int64_t q_out_token_stride, int64_t q_ou
  * limit); of a length of zero or less the result is zeros, a length beyond the page table's room counts as that.  What the cache holds behind the last
  * key is not used, whatever it is.  Ids outside [0, num_blocks) read block 0.  block_size a multiple of 32, head sizes 64, 128 and 256, scale > 0.
  * most_keys > 0: a bound of the lengths that the caller knows; the pass takes the page table as if it ended with the block of key most_keys - 1.
+ * workspace: 16-byte aligned, private to this call's stream; a call that needs none (0 bytes) takes null.
  */
 int64_t ttpa_paged_cross_attention_workspace_bytes(int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t q_len, int32_t head_size,
                                                    int32_t block_size, int32_t table_width, int64_t most_keys);

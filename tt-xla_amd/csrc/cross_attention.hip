@@ -656,11 +656,9 @@ CrossCut cross_cut(int batch, int kv_heads, int64_t rows, int head_size, int64_t
   const double two = c.shared ? 1.7 : 1.9, there = c.shared ? 0.4 : 0.3;
   const double merged = c.shared ? segments * std::min<int64_t>(rows, 64) * 0.2e-3 : segments * 6.25e-3;
   double best = 0;
-  for (int chain = (tiles + chains - 1) / chains; chain >= 1; --chain) {
-    const int parts = std::max(1, (tiles + chains * chain - 1) / (chains * chain));
-    if (parts == c.parts) continue;  // (as many parts of fewer tiles: the same)
-    if (parts > kMostCrossParts) break;
+  for (int parts = 1; parts <= kMostCrossParts && (parts == 1 || chains * (parts - 1) < tiles); ++parts) {
     const int longest = (tiles + chains * parts - 1) / (chains * parts);
+    if (parts > 1 && (tiles + chains * longest - 1) / (chains * longest) < parts) continue;  // (fewer parts are as short)
     const double all = segments * parts / cus, one = longest * tile_us, full = all <= 1 ? one : two * std::ceil(all / 2) * one;
     const double cost = 0.7 * full + 0.3 * std::max(one, there * all * one) + (!c.shared && segments < 2 * cus ? 0.2 * std::max(0, longest - 8) : 0.0) +
                         (parts > 1 ? 3.0 + parts * (merged + 0.02) : 0.0);
@@ -678,7 +676,7 @@ int64_t firsts_bytes(int batch) { return ((int64_t)batch * 8 + 255) & ~int64_t(2
 int64_t cross_bytes(const CrossCut &c, int batch, int kv_heads, int head_size) {
   const int64_t slot = c.rows() * (int64_t)(head_size + 2) * 4;
   if (c.units) return firsts_bytes(batch) + (int64_t)c.units * c.row_blocks * slot;
-  return c.parts == 1 ? 256 : (int64_t)batch * kv_heads * c.row_blocks * c.parts * slot;
+  return c.parts == 1 ? 0 : (int64_t)batch * kv_heads * c.row_blocks * c.parts * slot;
 }
 
 template <int D, int RG, bool SHARED>
@@ -736,10 +734,9 @@ bool stream_args(const CrossArgs &c, int head_size, bool keys_known, int64_t key
 // 96 57 / 44.  Of 525 such pairs the rule takes the slower one, by more than 3 %, of 47: by 13 ... 18 % at most where all users are as long as the longest, which is what the host
 // knows, and by 35 % where they are not and parts by their lengths would have paid (40 / 8 heads, 8 over 512 ... 5469, 48 tokens 49 / 66).
 // TTPA_CROSS_FORM overrides.
-bool streams(const CrossArgs &c, int head_size, int64_t keys) {
+bool streams(const CrossArgs &c, const CrossCut &cut, int head_size, int64_t keys) {
   if (form_is("rows") || form_is("planned")) return false;
   if (form_is("stream")) return true;
-  const CrossCut cut = cross_cut(c.batch, c.hkv, (int64_t)c.g * c.s, head_size, keys);
   const int64_t tiles = (keys + cut.tile - 1) / cut.tile, row_blocks = (c.s + kRowsPerWave - 1) / kRowsPerWave;
   const int64_t groups = c.g % 4 == 0 ? c.g / 4 * row_blocks : (row_blocks * c.g + 3) / 4;  // workgroups of the streaming loop per KV head
   if (cut.row_blocks <= groups) return false;
@@ -768,7 +765,7 @@ extern "C" int64_t ttpa_paged_cross_attention_workspace_bytes(int32_t batch, int
   decode::CrossArgs a = {};
   a.batch = batch, a.hkv = kv_heads, a.g = q_heads / kv_heads, a.s = q_len, a.bs = block_size, a.w = (int)((keys + block_size - 1) / block_size);
   PrefillArgs p;
-  if ((head_size == 64 || head_size == 128 || head_size == 256) && decode::stream_args(a, head_size, most_keys > 0, keys, p) && decode::streams(a, head_size, keys))
+  if ((head_size == 64 || head_size == 128 || head_size == 256) && decode::streams(a, c, head_size, keys) && decode::stream_args(a, head_size, most_keys > 0, keys, p))
     bytes = std::max(bytes, stream_ends_part_bytes(p, head_size));
   return bytes;
 }
@@ -808,12 +805,12 @@ extern "C" int ttpa_paged_cross_attention(void *out, int64_t out_batch_stride, i
   a.scale_log2e = scale * 1.4426950408889634f;
   hipStream_t st = static_cast<hipStream_t>(stream);
   PrefillArgs p;
-  if (decode::stream_args(a, head_size, most_keys > 0, keys, p) && decode::streams(a, head_size, keys)) {
+  const decode::CrossCut c = decode::cross_cut(batch, kv_heads, (int64_t)a.g * q_len, head_size, keys);
+  if (decode::streams(a, c, head_size, keys) && decode::stream_args(a, head_size, most_keys > 0, keys, p)) {
     TTPA_REQUIRE((int64_t)batch * q_heads * ((q_len + 31) / 32) < (1ll << 26), "cross attention: too many rows for one launch");
     if (workspace && aligned16(workspace)) p.part_acc = static_cast<float *>(workspace), p.part_bytes = workspace_bytes;
     return launch_stream_ends(p, head_size, st);
   }
-  const decode::CrossCut c = decode::cross_cut(batch, kv_heads, (int64_t)a.g * q_len, head_size, keys);
   a.row_blocks = c.row_blocks, a.parts = c.parts, a.share = c.share;
   a.runs = (uint32_t)block_size / (c.tile / 4), a.runs_inv = 0xffffffffu / a.runs;
   TTPA_REQUIRE(((int64_t)std::max(c.units, batch * kv_heads * c.parts) + 8) * c.row_blocks < (1ll << 24) && (c.parts == 1 || (int64_t)a.g * q_len < 65536),

@@ -618,12 +618,12 @@ void cross_into(const Call &c, const Tensor &out, const Tensor &query, const Ten
   if (users == 0 || s == 0) return;
   const Tensor q = rows(query), target = storable(out), k = aligned16(k_cache) ? k_cache : compact(k_cache), v = aligned16(v_cache) ? v_cache : compact(v_cache);
   const int64_t bytes = ttpa_paged_cross_attention_workspace_bytes(i32(users), i32(hq), i32(hkv), i32(s), i32(d), i32(bs), i32(pt.size(1)), most_keys);
-  const Tensor ws = c.scratch(bytes);
+  const Tensor ws = bytes ? c.scratch(bytes) : Tensor();
   ok("ttpa_paged_cross_attention",
      ttpa_paged_cross_attention(target.data_ptr(), step_of(target, 0), step_of(target, 1), step_of(target, 2), q.data_ptr(), step_of(q, 0), step_of(q, 1),
                                 step_of(q, 2), k.data_ptr(), v.data_ptr(), int_ptr(pt), step_of(pt, 0), lens.data_ptr(), is_i64(lens), i32(users),
-                                i32(hq), i32(hkv), i32(s), i32(d), i32(bs), i32(pt.size(1)), i32(nb), scale_of(scale, d), most_keys, ws.data_ptr(),
-                                bytes, c.stream()));
+                                i32(hq), i32(hkv), i32(s), i32(d), i32(bs), i32(pt.size(1)), i32(nb), scale_of(scale, d), most_keys,
+                                bytes ? ws.data_ptr() : nullptr, bytes, c.stream()));
   if (!target.is_same(out)) out.copy_(target);
 }
 
