@@ -42,6 +42,7 @@ class Call {
   void see(const Tensor &t, const char *what) const {
     TORCH_CHECK_NOT_IMPLEMENTED(t.is_cuda(), name_, ": ", what, " is not on a HIP device");
     TORCH_CHECK_VALUE(t.device() == device_, name_, ": ", what, " is on ", t.device(), ", not on ", device_);
+    if (!t.unsafeGetTensorImpl()->autograd_meta()) return;  // (a tensor that autograd has never seen)
     TORCH_CHECK_NOT_IMPLEMENTED(!(at::GradMode::is_enabled() && t.requires_grad()), name_, " has no backward pass, and ", what,
                                 " requires a gradient: call it under torch.no_grad()");
     TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), name_, " has no derivative, and ", what, " carries a tangent");
