@@ -1,6 +1,6 @@
 // Moves inside paged caches, for all layers in one call: copies of whole blocks (forks of sequences, moves of pages) and compaction of sequences
 // (chosen tokens move together).  Bytes are moved as they are, so any element type will do.  Both are bound by memory: read once, written once; a large copy by torch
-// reaches 5.3 TB/s both ways together on this card.  250 blocks of 64 x 8 heads x 128 bytes in 24 caches (786 MB) 157 us, 5.0 TB/s (164 with ordinary loads and stores);
+// reaches 5.3 TB/s both ways together on this card.  250 blocks of 64 x 8 heads x 128 bytes in 24 caches (786 MB) 151 us, 5.2 TB/s;
 // half of the last three quarters of 4 x 8192 tokens, K and V of 16 layers of 8 heads of 128 (1.6 GB) 328 us, 4.9; of 2048 ... 8192 tokens (867 MB), where the longest
 // user's chain of batches ends the launch, 178 us (203 with one batch on its way, 191 with streaming stores).  (Of one state again and again; of three in turn, which the
 // last cache holds less of, the first and the last take 10 % longer.)
@@ -16,7 +16,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr int kMostCaches = 192;        // of one launch: their addresses are arguments
 constexpr int kMostPairs = 4096;        // of one launch: a longer list takes several, one after the other
 constexpr int kMostMarks = 1 << 18;     // blocks of a cache that a workgroup can mark (32 KiB of LDS)
-constexpr int kThreads = 256, kChunks = 4, kAtOnce = 4;  // 16-byte chunks of a block per thread, pairs on their way at a time
+constexpr int kThreads = 256, kChunks = 4, kAtOnce = 2;  // 16-byte chunks of a block per thread, pairs on their way at a time
 
 struct CopyArgs {
   uint8_t *caches[kMostCaches];
@@ -258,8 +258,9 @@ int launch_copy(CopyArgs &a, int caches, hipStream_t st) {
   int64_t most = 0, all = 0;
   for (int i = 0; i < caches; ++i) most = std::max<int64_t>(most, a.block_units[i]), all += a.block_units[i];
   const int64_t slices = (most + kThreads * kChunks - 1) / (kThreads * kChunks), busy = (all + kThreads * kChunks - 1) / (kThreads * kChunks);
-  // workgroups for every CU a few times over, a run of pairs each at least
-  const int64_t runs = (a.pairs + kAtOnce - 1) / kAtOnce, want = (8ll * std::max(device_cus(), 1) + busy - 1) / busy;
+  // Workgroups for every CU many times over, a run of pairs each at least: 250 blocks of 64 KiB in 24 caches, three states in turn, 159 us with eight per CU and four pairs
+  // on their way, 154 with sixteen and two, 151 with sixty-four and one, which takes blocks of 8 KiB 14 % longer
+  const int64_t runs = (a.pairs + kAtOnce - 1) / kAtOnce, want = (16ll * std::max(device_cus(), 1) + busy - 1) / busy;
   a.parts = (int)std::max<int64_t>(1, std::min(runs, want));
   const size_t lds = a.pairs > 64 ? (size_t)(a.nb + 31) / 32 * 4 : 0;
   copy_blocks_kernel<T><<<dim3((unsigned)slices, (unsigned)caches, (unsigned)a.parts), dim3(kThreads), lds, st>>>(a);
