@@ -466,7 +466,7 @@ class TTAttentionBackendImpl(_ImplBase):
             raise ValueError("a cross attention pass has keys and values, or neither")
         ops = torch.ops.tt
         q = self._normalize_to_attention_format(query, "query", self.num_heads, self.head_size, users)
-        caches = list(kv_cache) if isinstance(kv_cache, (list, tuple)) else [kv_cache]
+        caches = list(kv_cache) if isinstance(kv_cache, (list, tuple)) else [] if kv_cache is None else [kv_cache]
         cached = len(caches) > 0 and caches[0].numel() > 0
         if cached:
             if len(caches) != 2 or caches[0].dtype != torch.bfloat16 or caches[0].dim() != 4 or caches[0].shape[2] % 32:
