@@ -733,6 +733,16 @@ int ttpa_paged_cross_attention(void *out, int64_t out_batch_stride, int64_t out_
                                int32_t q_heads, int32_t kv_heads, int32_t q_len, int32_t head_size, int32_t block_size, int32_t table_width,
                                int32_t num_blocks, float scale, int64_t most_keys, void *workspace, int64_t workspace_bytes, void *stream);
 
+/* The same over 8-bit caches (elements and scales as ttpa_paged_fp8_decode takes them). */
+int64_t ttpa_paged_fp8_cross_attention_workspace_bytes(int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t q_len, int32_t head_size,
+                                                       int32_t block_size, int32_t table_width, int64_t most_keys);
+int ttpa_paged_fp8_cross_attention(void *out, int64_t out_batch_stride, int64_t out_head_stride, int64_t out_token_stride, const void *q,
+                                   int64_t q_batch_stride, int64_t q_head_stride, int64_t q_token_stride, const void *k_cache, const void *v_cache,
+                                   const float *k_scales, const float *v_scales, const int32_t *page_table, int64_t page_table_row_stride,
+                                   const void *encoder_lens, int lens_is_i64, int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t q_len,
+                                   int32_t head_size, int32_t block_size, int32_t table_width, int32_t num_blocks, float scale, int64_t most_keys,
+                                   void *workspace, int64_t workspace_bytes, void *stream);
+
 /*
  * Copies blocks inside caches: of every cache, n_caches tensors [num_blocks][block_bytes[i]], block source_blocks[j] to target_blocks[j], as if j went from 0 on
  * (a block may be the target of one pair and the source of a later one).  Pairs with an id outside [0, num_blocks) are skipped.  caches_host is an array of

@@ -14,6 +14,8 @@ SCHEMAS = {
     "qk_norm_rope_axes_": f"tt::qk_norm_rope_axes_(Tensor(a!) query, Tensor(b!) key, {ROPE}) -> ()",
     "paged_cross_attention": f"tt::paged_cross_attention({CROSS}, float? scale=None, int most_keys=0) -> Tensor",
     "paged_cross_attention_out": f"tt::paged_cross_attention_out({CROSS}, Tensor(a!) out, float? scale=None, int most_keys=0) -> ()",
+    "paged_fp8_cross_attention": "tt::paged_fp8_cross_attention(Tensor query, Tensor k_cache, Tensor v_cache, Tensor k_scales, Tensor v_scales, Tensor page_table, "
+                                 "Tensor encoder_lens, float? scale=None, int most_keys=0) -> Tensor",
     "copy_cache_blocks_": "tt::copy_cache_blocks_(Tensor(a!)[] caches, Tensor source_blocks, Tensor target_blocks) -> ()",
     "keep_cache_tokens_": "tt::keep_cache_tokens_(Tensor(a!)[] caches, Tensor page_table, Tensor kept, Tensor kept_lens, Tensor? first=None) -> ()",
 }
@@ -68,6 +70,11 @@ def _cross(lib, q=16, lens=16, users=2, hq=8, hkv=2, s=3, d=128, bs=64, w=4, nb=
                                           scale, most, ws, ws_bytes, None)
 
 
+def _cross8(lib, q=16, scales=16, users=2, hq=8, hkv=2, s=3, d=128, bs=64, w=4, nb=8, scale=1.0, most=0, ws=256, ws_bytes=1 << 40):
+    return lib.ttpa_paged_fp8_cross_attention(16, 1 << 16, 128, 1024, q, 1 << 16, 128, 1024, 16, 16, scales, 16, 16, 4, 16, 0, users, hq, hkv, s, d, bs, w, nb,
+                                              scale, most, ws, ws_bytes, None)
+
+
 def _some(n=1, p=256):
     import ctypes
 
@@ -94,6 +101,9 @@ def _keep(lib, caches=256, n=1, pt=16, users=2, most=4, heads=2, row=128, bs=32,
     (_cross, dict(d=96), -2, b"head_size"), (_cross, dict(bs=48), -2, b"block_size"), (_cross, dict(bs=8192), -2, b"block_size"),
     (_cross, dict(scale=0.0), -1, b"scale"), (_cross, dict(scale=-1.0), -1, b"scale"), (_cross, dict(most=-1), -1, b"most_keys"), (_cross, dict(w=1 << 26), -1, b"too many keys"),
     (_cross, dict(q=24), -1, b"aligned"), (_cross, dict(stride=1028), -1, b"strides"), (_cross, dict(ws_bytes=0, users=1, w=400), -3, b"workspace"),
+    (_cross8, dict(q=None), -1, b"null"), (_cross8, dict(scales=None), -1, b"null"), (_cross8, dict(hq=9), -1, b"divisible"), (_cross8, dict(d=96), -2, b"head_size"),
+    (_cross8, dict(bs=16), -2, b"block_size"), (_cross8, dict(scale=0.0), -1, b"scale"), (_cross8, dict(ws_bytes=0, users=1, w=400), -3, b"workspace"),
+    (_cross8, dict(ws_bytes=0, users=8, s=600, w=100, nb=1000), -3, b"workspace"),
     (_copy, dict(caches=None), -1, b"null"), (_copy, dict(caches="none"), -1, b"null"), (_copy, dict(source=None), -1, b"null"), (_copy, dict(bytes_=0), -1, b"bytes"), (_copy, dict(bytes_=1 << 31), -1, b"bytes"), (_copy, dict(bytes_=None), -1, b"null"),
     (_copy, dict(pairs=-1), -1, b"dimension"), (_copy, dict(nb=0), -1, b"dimension"), (_copy, dict(n=-1), -1, b"null"),
     (_keep, dict(caches=None), -1, b"null"), (_keep, dict(pt=None), -1, b"null"), (_keep, dict(users=-1), -1, b"dimension"), (_keep, dict(row=24), -2, b"multiples of 16"),
@@ -130,7 +140,7 @@ def _layer(**kw):
 
 
 @pytest.mark.parametrize("wrong", [dict(sliding_window=64), dict(sinks=torch.zeros(8)), dict(sparse_kept_blocks=4), dict(functional_cache_ops=True),
-                                   dict(kv_cache_dtype="fp8_e4m3"), dict(head_size=96)])
+                                   dict(kv_cache_dtype="bfp_bf8"), dict(head_size=96)])
 def test_what_a_cross_attention_layer_is_not_built_with(lib, wrong):
     with pytest.raises(NotImplementedError, match="cross attention"):
         _layer(**wrong)

@@ -15,10 +15,13 @@
 //   S^T = K . Q^T                 16x16x32 bfloat16; the tile is four runs of TILE / 4 keys, one per quad of lanes: row 4 j + r of block b is
 //                                 key (TILE / 4) j + 4 b + r, so lane (row, quad) ends up with its quad's run in order, which is
 //   O^T += V^T . P^T              the order in which the second product wants its weights: no moves between the two
+// 8-bit caches: the same, an element becoming its bfloat16 value on its way into LDS; 32 users of 32 / 8 heads over 256 ... 4096 keys 22.4 us (34.0 with bfloat16), 96 of 64 / 8 over
+// 512 ... 2048 51 (75), 64 of 16 / 8 of 256 over 800 42.5 (71), 96 of 64 / 8, 5 tokens, over 1500 70 (111).
 // Statistics and accumulators are floats; weights are rounded once to bfloat16 for the matrix instruction, and the same rounded weights are summed.
 // Wavefronts' results of their own tiles meet in LDS, the parts' in memory, merged by a kernel of its own.  How many parts there are goes by an estimate of the time, the host's of the longest
 // user, or, where that is long enough to pay for it, the device's of all of them (cross_work).
 #include "decode_mfma16_kernel.h"
+#include "fp8.h"
 #include "prefill_common.h"
 
 #include <algorithm>
@@ -27,6 +30,12 @@
 #include <cstring>
 
 namespace ttpa {
+namespace fp8 {
+int expand_entries(const void *k_cache, const void *v_cache, const float *k_scales, const float *v_scales, void *k_copy, void *v_copy, int32_t *table,
+                   const int32_t *page_table, int64_t page_table_row_stride, const void *lens, int lens_i64, int batch, int width, int kv_heads,
+                   int block_size, int head_size, int num_blocks, hipStream_t st);
+}
+
 namespace decode {
 namespace {
 
@@ -36,7 +45,8 @@ struct CrossArgs {
   const uint16_t *q;
   uint16_t *out;
   int64_t q_bs, q_hs, q_ts, o_bs, o_hs, o_ts;
-  const uint16_t *k, *v;
+  const void *k, *v;
+  const float *k_scales, *v_scales;  // of 8-bit caches: [num_blocks][hkv]
   const int32_t *pt;
   int64_t pt_rs;
   const void *lens;
@@ -144,6 +154,23 @@ __device__ __forceinline__ int64_t cross_slot(const CrossArgs &a, int u, int h, 
   return a.firsts ? ((int64_t)first * a.hkv + h) * a.row_blocks + rb : ((int64_t)(u * a.hkv + h) * a.row_blocks + rb) * a.parts;
 }
 
+// Where a run of keys lies: its first byte, and its block and head.
+struct CrossSpot {
+  uint64_t at;
+  uint32_t slab;
+};
+// A 16-byte piece of a row -> LDS: eight bfloat16 values as they are, or sixteen elements of an 8-bit cache as bfloat16 values, exactly (their block's scale is a power
+// of two).  `key` swizzles the row's chunks.
+template <bool FP8>
+__device__ __forceinline__ void cross_put(uint8_t *row, int piece, int key, const u32x4 &x, float scale) {
+  if constexpr (FP8) {
+    *reinterpret_cast<u32x4 *>(row + ((2 * piece ^ key) << 4)) = __builtin_bit_cast(u32x4, fp8::decode8(x.x, x.y, scale));
+    *reinterpret_cast<u32x4 *>(row + (((2 * piece + 1) ^ key) << 4)) = __builtin_bit_cast(u32x4, fp8::decode8(x.z, x.w, scale));
+  } else {
+    *reinterpret_cast<u32x4 *>(row + ((piece ^ key) << 4)) = x;
+  }
+}
+
 // A wavefront's rows and what it has of the result; what it does with a tile of TILE keys that lies in LDS.
 template <int D, int RG, int KEYS>
 struct CrossRows {
@@ -182,12 +209,14 @@ struct CrossRows {
     }
   }
   // Where run x of the keys lies: a run is in one block.  (Ids out of range read block 0; tiles behind the table's room are not asked for.)
-  __device__ __forceinline__ uint64_t place(int u, int h, uint32_t x) const {
+  template <bool FP8>
+  __device__ __forceinline__ CrossSpot place(int u, int h, uint32_t x) const {
+    constexpr int BYTES = FP8 ? D : RB;
     uint32_t col = __umulhi(x, a.runs_inv), r = x - col * a.runs;  // one too few at most
     if (r >= a.runs) ++col, r -= a.runs;
     const int page = (int)col < a.w ? a.pt[(int64_t)u * a.pt_rs + (int)col] : 0;
-    const uint64_t slab = (uint64_t)((unsigned)page < (unsigned)a.nb ? page : 0) * (uint32_t)a.hkv + (uint32_t)h;
-    return slab * (uint64_t)(a.bs * RB) + r * (uint32_t)(RUN * RB);
+    const uint32_t slab = ((unsigned)page < (unsigned)a.nb ? (uint32_t)page : 0u) * (uint32_t)a.hkv + (uint32_t)h;  // (fewer than 2^32)
+    return {slab * (uint64_t)(a.bs * BYTES) + r * (uint32_t)(RUN * BYTES), slab};
   }
   // (non-temporal also where several blocks of rows read the same keys: 96 users of 64 / 8 heads of 128 over 2033 keys 91 -> 74 us, and three blocks of 8 users
   // over 1500 20.8 -> 19.5)
@@ -260,35 +289,42 @@ struct CrossRows {
 };
 
 // A wavefront with tiles of its own: on their way in registers, then in its share of LDS, K first and V over it.  A quad of lanes has a run of the keys.
-template <int D, int RG>
+template <int D, int RG, bool FP8>
 struct CrossTile : CrossRows<D, RG, cross_tile<D>()> {
   using Rows = CrossRows<D, RG, cross_tile<D>()>;
-  using Rows::TILE, Rows::RUN, Rows::RB, Rows::CPR, Rows::PSTEPS, Rows::a, Rows::n, Rows::quad, Rows::load;
-  static constexpr int NL = RUN * CPR / 16;  // loads of a tile and tensor
+  using Rows::TILE, Rows::RUN, Rows::RB, Rows::PSTEPS, Rows::a, Rows::n, Rows::quad, Rows::load;
+  static constexpr int PPR = (FP8 ? D : 2 * D) / 16, NL = RUN * PPR / 16;  // 16-byte pieces of a row, loads of a tile and tensor
   uint8_t *const tile;
   u32x4 kraw[NL], vraw[NL];
+  float k_scale, v_scale;  // of the tile on its way
 
-  __device__ __forceinline__ CrossTile(const CrossArgs &args, uint8_t *lds) : Rows(args), tile(lds) {}
-  __device__ __forceinline__ uint64_t look_up(int u, int h, int t) const { return this->place(u, h, (uint32_t)(t * 4 + quad)) + 16 * n; }
-  __device__ __forceinline__ void request_k(uint64_t at) {
-    const uint8_t *const kp = reinterpret_cast<const uint8_t *>(a.k) + at;
+  __device__ __forceinline__ CrossTile(const CrossArgs &args, uint8_t *lds) : Rows(args), tile(lds), k_scale(1.f), v_scale(1.f) {}
+  __device__ __forceinline__ CrossSpot look_up(int u, int h, int t) const {
+    CrossSpot s = this->template place<FP8>(u, h, (uint32_t)(t * 4 + quad));
+    s.at += 16 * n;
+    return s;
+  }
+  __device__ __forceinline__ void request_k(const CrossSpot &s) {
+    const uint8_t *const kp = static_cast<const uint8_t *>(a.k) + s.at;
 #pragma unroll
     for (int i = 0; i < NL; ++i) kraw[i] = load(kp + 256 * i);
+    if constexpr (FP8) k_scale = a.k_scales[s.slab];
   }
-  __device__ __forceinline__ void request_v(uint64_t at) {
-    const uint8_t *const vp = reinterpret_cast<const uint8_t *>(a.v) + at;
+  __device__ __forceinline__ void request_v(const CrossSpot &s) {
+    const uint8_t *const vp = static_cast<const uint8_t *>(a.v) + s.at;
 #pragma unroll
     for (int i = 0; i < NL; ++i) vraw[i] = load(vp + 256 * i);
+    if constexpr (FP8) v_scale = a.v_scales[s.slab];
   }
-  // Load i of a lane is chunk 16 i + n of its run.
-  __device__ __forceinline__ int run_row(int i) const { return (16 * i + n) / CPR; }
+  // Load i of a lane is piece 16 i + n of its run.
+  __device__ __forceinline__ int run_row(int i) const { return (16 * i + n) / PPR; }
   // Registers -> LDS (an LDS works through a wavefront's instructions in order: V overwrites K behind the last read of K); of the lane's run, `nvalid` keys
   // are attended.
   __device__ __forceinline__ void stage_k() {
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      const int row = RUN * quad + run_row(i), chunk = (16 * i + n) % CPR;
-      *reinterpret_cast<u32x4 *>(tile + row * RB + ((chunk ^ cross_kkey<D, TILE>(row)) << 4)) = kraw[i];
+      const int row = RUN * quad + run_row(i);
+      cross_put<FP8>(tile + row * RB, (16 * i + n) % PPR, cross_kkey<D, TILE>(row), kraw[i], k_scale);
     }
   }
   __device__ __forceinline__ void stage_v(int nvalid, bool partial) {
@@ -298,15 +334,16 @@ struct CrossTile : CrossRows<D, RG, cross_tile<D>()> {
         const uint32_t keep = run_row(i) < nvalid ? 0xffffffffu : 0u;
         vraw[i] = u32x4{vraw[i].x & keep, vraw[i].y & keep, vraw[i].z & keep, vraw[i].w & keep};
       }
+      v_scale = nvalid > 0 ? v_scale : 1.f;  // (of a block that holds nothing: anything)
     }
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      const int row = RUN * quad + run_row(i), chunk = (16 * i + n) % CPR;
-      *reinterpret_cast<u32x4 *>(tile + row * RB + ((chunk ^ cross_vkey<D, TILE>(row)) << 4)) = vraw[i];
+      const int row = RUN * quad + run_row(i);
+      cross_put<FP8>(tile + row * RB, (16 * i + n) % PPR, cross_vkey<D, TILE>(row), vraw[i], v_scale);
     }
   }
   template <bool MORE>
-  __device__ __forceinline__ void attend(int nvalid, bool partial, uint64_t next) {
+  __device__ __forceinline__ void attend(int nvalid, bool partial, const CrossSpot &next) {
     u32x4 pf[RG][PSTEPS];
     stage_k();
     if constexpr (MORE) request_k(next);
@@ -318,9 +355,9 @@ struct CrossTile : CrossRows<D, RG, cross_tile<D>()> {
 };
 
 // A workgroup per (user, KV head, block of rows): its wavefronts take the tiles in turn, and their results meet in LDS.
-template <int D, int RG>
+template <int D, int RG, bool FP8>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void cross_rows_kernel(CrossArgs a) {
-  using T = CrossTile<D, RG>;
+  using T = CrossTile<D, RG, FP8>;
   constexpr int TILE = T::TILE, ROWS = T::ROWS, DBLK = T::DBLK, CPR = T::CPR;
   extern __shared__ __attribute__((aligned(16))) uint8_t tiles[];
   __shared__ float2 s_ml[4][ROWS];
@@ -341,7 +378,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   T x(a, tiles + wib * cross_lds_bytes<D>());
   int t = part * 4 + wib;
   const int64_t length = a.firsts ? w.keys : load_index(a.lens, a.lens_i64, u);
-  const uint64_t at0 = x.look_up(u, h, t);
+  const CrossSpot at0 = x.look_up(u, h, t);
   x.load_q(u, h, row0);
   const int keys = __builtin_amdgcn_readfirstlane(cross_keys(a, length)), n_tiles = (keys + TILE - 1) / TILE;
   const int parts = __builtin_amdgcn_readfirstlane(a.firsts ? w.parts : cross_parts(a, keys)), step = 4 * parts;
@@ -356,12 +393,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
     return;
   }
-  uint64_t next = 0;
+  CrossSpot next = {0, 0};
   const auto process_tile = [&](auto more_tag) {
     constexpr bool more = decltype(more_tag)::value;
     const int nvalid = keys - (t * TILE + T::RUN * x.quad);
     const bool partial = (t + 1) * TILE > keys;
-    const uint64_t at = next;
+    const CrossSpot at = next;
     if constexpr (more) next = x.look_up(u, h, t + 2 * step);
     x.template attend<more>(nvalid, partial, at);
     t += step;
@@ -432,10 +469,11 @@ template <int D>
 constexpr int shared_tile() {
   return D == 256 ? 32 : 64;
 }
-template <int D>
+template <int D, bool FP8>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void cross_shared_kernel(CrossArgs a) {
   using T = CrossRows<D, 1, shared_tile<D>()>;
-  constexpr int TILE = T::TILE, RUN = T::RUN, RB = T::RB, CPR = T::CPR, ROWS = 64, DBLK = T::DBLK, NL = RUN * CPR / 64, BYTES = TILE * RB;
+  constexpr int TILE = T::TILE, RUN = T::RUN, RB = T::RB, CPR = T::CPR, ROWS = 64, DBLK = T::DBLK, BYTES = TILE * RB;
+  constexpr int PPR = FP8 ? CPR / 2 : CPR, NL = RUN * PPR / 64;  // 16-byte pieces of a row, loads of a tile, wavefront and tensor
   extern __shared__ __attribute__((aligned(16))) uint8_t tiles[];  // two of K and V
   const uint32_t span = 8u * a.row_blocks, set = blockIdx.x / span, in_set = blockIdx.x - set * span;
   const int rb = (int)(in_set >> 3), unit = (int)(set * 8 + (in_set & 7)), segments = a.batch * a.hkv;
@@ -452,9 +490,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const bool mine = row0 < rows;  // (a wavefront without rows loads its share of the keys)
   T x(a);
   int t = part;
-  const auto look_up = [&](int tile) { return x.place(u, h, (uint32_t)(tile * 4 + wib)) + 16 * lane; };
+  const auto look_up = [&](int tile) { return x.template place<FP8>(u, h, (uint32_t)(tile * 4 + wib)); };
   const int64_t length = a.firsts ? w.keys : load_index(a.lens, a.lens_i64, u);
-  const uint64_t at0 = look_up(t);
+  const CrossSpot at0 = look_up(t);
   if (mine) x.load_q(u, h, row0);
   const int keys = __builtin_amdgcn_readfirstlane(cross_keys(a, length)), n_tiles = (keys + TILE - 1) / TILE;
   const int parts = __builtin_amdgcn_readfirstlane(a.firsts ? w.parts : cross_parts(a, keys)), step = parts;
@@ -469,38 +507,44 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
     return;
   }
-  u32x4 kraw[2][NL], vraw[2][NL];
-  const auto request = [&](uint64_t at, u32x4 (&k)[NL], u32x4 (&v)[NL]) {
-    const uint8_t *const kp = reinterpret_cast<const uint8_t *>(a.k) + at, *const vp = reinterpret_cast<const uint8_t *>(a.v) + at;
-#pragma unroll
-    for (int i = 0; i < NL; ++i) k[i] = T::load(kp + 1024 * i);
-#pragma unroll
-    for (int i = 0; i < NL; ++i) v[i] = T::load(vp + 1024 * i);
+  struct Flight {  // a tile on its way
+    u32x4 k[NL], v[NL];
+    float k_scale, v_scale;
   };
-  uint64_t at2 = 0;  // of the tile two steps ahead
-  const auto process = [&](int buffer, u32x4 (&k)[NL], u32x4 (&v)[NL]) {
+  Flight flights[2];
+  const auto request = [&](const CrossSpot &s, Flight &f) {
+    const uint8_t *const kp = static_cast<const uint8_t *>(a.k) + s.at + 16 * lane, *const vp = static_cast<const uint8_t *>(a.v) + s.at + 16 * lane;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) f.k[i] = T::load(kp + 1024 * i);
+#pragma unroll
+    for (int i = 0; i < NL; ++i) f.v[i] = T::load(vp + 1024 * i);
+    f.k_scale = FP8 ? a.k_scales[s.slab] : 1.f, f.v_scale = FP8 ? a.v_scales[s.slab] : 1.f;
+  };
+  CrossSpot at2 = {0, 0};  // of the tile two steps ahead
+  const auto process = [&](int buffer, Flight &f) {
     uint8_t *const kt = tiles + buffer * 2 * BYTES, *const vt = kt + BYTES;
     const bool partial = (t + 1) * TILE > keys;
-    const uint64_t at = at2;
+    const CrossSpot at = at2;
     if (t + 3 * step < n_tiles) at2 = look_up(t + 3 * step);
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      const int c = 64 * i + lane, row = RUN * wib + c / CPR;
-      *reinterpret_cast<u32x4 *>(kt + row * RB + ((c % CPR ^ cross_kkey<D, TILE>(row)) << 4)) = k[i];
+      const int c = 64 * i + lane, row = RUN * wib + c / PPR;
+      cross_put<FP8>(kt + row * RB, c % PPR, cross_kkey<D, TILE>(row), f.k[i], f.k_scale);
     }
     if (partial) {
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
-        const uint32_t keep = t * TILE + RUN * wib + (64 * i + lane) / CPR < keys ? 0xffffffffu : 0u;
-        v[i] = u32x4{v[i].x & keep, v[i].y & keep, v[i].z & keep, v[i].w & keep};
+        const uint32_t keep = t * TILE + RUN * wib + (64 * i + lane) / PPR < keys ? 0xffffffffu : 0u;
+        f.v[i] = u32x4{f.v[i].x & keep, f.v[i].y & keep, f.v[i].z & keep, f.v[i].w & keep};
       }
+      f.v_scale = t * TILE + RUN * wib < keys ? f.v_scale : 1.f;  // (of a block that holds nothing: anything)
     }
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      const int c = 64 * i + lane, row = RUN * wib + c / CPR;
-      *reinterpret_cast<u32x4 *>(vt + row * RB + ((c % CPR ^ cross_vkey<D, TILE>(row)) << 4)) = v[i];
+      const int c = 64 * i + lane, row = RUN * wib + c / PPR;
+      cross_put<FP8>(vt + row * RB, c % PPR, cross_vkey<D, TILE>(row), f.v[i], f.v_scale);
     }
-    if (t + 2 * step < n_tiles) request(at, k, v);
+    if (t + 2 * step < n_tiles) request(at, f);
     __syncthreads();  // the tile is there; whoever is ahead writes the other buffer, whose tile everybody is done with
     if (mine) {
       u32x4 pf[1][T::PSTEPS];
@@ -510,14 +554,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     t += step;
   };
   if (t < n_tiles) {
-    uint64_t at1 = 0;
+    CrossSpot at1 = {0, 0};
     if (t + step < n_tiles) at1 = look_up(t + step);
     if (t + 2 * step < n_tiles) at2 = look_up(t + 2 * step);
-    request(at0, kraw[0], vraw[0]);
-    if (t + step < n_tiles) request(at1, kraw[1], vraw[1]);
+    request(at0, flights[0]);
+    if (t + step < n_tiles) request(at1, flights[1]);
     while (t < n_tiles) {
-      process(0, kraw[0], vraw[0]);
-      if (t < n_tiles) process(1, kraw[1], vraw[1]);
+      process(0, flights[0]);
+      if (t < n_tiles) process(1, flights[1]);
     }
   }
   cross_note(a, w, rb);
@@ -679,12 +723,12 @@ int64_t cross_bytes(const CrossCut &c, int batch, int kv_heads, int head_size) {
   return c.parts == 1 ? 0 : (int64_t)batch * kv_heads * c.row_blocks * c.parts * slot;
 }
 
-template <int D, int RG, bool SHARED>
+template <int D, int RG, bool SHARED, bool FP8>
 int launch_cross(const CrossArgs &a, hipStream_t st) {
   static std::atomic<uint64_t> lds_ready{0};
   constexpr auto kernel = [] {
-    if constexpr (SHARED) return &cross_shared_kernel<D>;
-    else return &cross_rows_kernel<D, RG>;
+    if constexpr (SHARED) return &cross_shared_kernel<D, FP8>;
+    else return &cross_rows_kernel<D, RG, FP8>;
   }();
   const size_t lds = SHARED ? 4 * shared_tile<D>() * D * 2 : 4 * cross_lds_bytes<D>();
   if (!ensure_dynamic_lds(reinterpret_cast<const void *>(kernel), lds, lds_ready))
@@ -702,11 +746,19 @@ int launch_cross(const CrossArgs &a, hipStream_t st) {
   return check_launch("cross attention (merge)");
 }
 
-template <int D>
+template <int D, bool FP8>
 int launch_cross_d(const CrossArgs &a, const CrossCut &c, hipStream_t st) {
   if constexpr (D < 256)
-    if (!c.shared) return c.groups == 2 ? launch_cross<D, 2, false>(a, st) : launch_cross<D, 1, false>(a, st);
-  return launch_cross<D, 1, true>(a, st);
+    if (!c.shared) return c.groups == 2 ? launch_cross<D, 2, false, FP8>(a, st) : launch_cross<D, 1, false, FP8>(a, st);
+  return launch_cross<D, 1, true, FP8>(a, st);
+}
+template <bool FP8>
+int launch_cross_any(const CrossArgs &a, int head_size, const CrossCut &c, hipStream_t st) {
+  switch (head_size) {
+    case 64: return launch_cross_d<64, FP8>(a, c, st);
+    case 128: return launch_cross_d<128, FP8>(a, c, st);
+    default: return launch_cross_d<256, FP8>(a, c, st);
+  }
 }
 
 // The streaming loop's arguments.  It steps through rows by unsigned 32-bit numbers of bytes and through blocks by a 32-bit inverse; what does not fit those is
@@ -718,7 +770,7 @@ bool stream_args(const CrossArgs &c, int head_size, bool keys_known, int64_t key
   a = {};
   a.out = c.out, a.out_bs = c.o_bs, a.out_hs = c.o_hs, a.out_ts = c.o_ts;
   a.q = c.q, a.q_bs = c.q_bs, a.q_hs = c.q_hs, a.q_ts = c.q_ts;
-  a.k = c.k, a.v = c.v, a.pt = c.pt, a.pt_rs = c.pt_rs, a.lens = c.lens, a.lens_i64 = c.lens_i64;
+  a.k = static_cast<const uint16_t *>(c.k), a.v = static_cast<const uint16_t *>(c.v), a.pt = c.pt, a.pt_rs = c.pt_rs, a.lens = c.lens, a.lens_i64 = c.lens_i64;
   a.batch = c.batch, a.hq = c.hkv * c.g, a.hkv = c.hkv, a.sq = c.s, a.skv = c.w * c.bs, a.bs = c.bs, a.w = c.w, a.nb = c.nb;
   a.bs_magic = (uint32_t)((1ull << 32) / (uint32_t)c.bs) + 1u;
   a.scale_log2e = c.scale_log2e, a.parts = 1, a.stream = 1;
@@ -733,13 +785,22 @@ bool stream_args(const CrossArgs &c, int head_size, bool keys_known, int64_t key
 // 64, 16 / 16 heads, 32 over 800, 64 tokens 23.0 / 27.9, 128 (2 / 1, 52) 37.0 / 31.1; 256, 16 / 8 heads, 2 over 6404, 32 tokens 29.6 / 37.2, 48 (2 / 1, 13) 42.5 / 39.5,
 // 96 57 / 44.  Of 525 such pairs the rule takes the slower one, by more than 3 %, of 47: by 13 ... 18 % at most where all users are as long as the longest, which is what the host
 // knows, and by 35 % where they are not and parts by their lengths would have paid (40 / 8 heads, 8 over 512 ... 5469, 48 tokens 49 / 66).
+// 8-bit caches become bfloat16 copies for the streaming loop, so there both are estimated, us: 0.47 / 0.85 / 0.8 per 256 shared tiles behind 10, and the loop's products at 0.55 / 1.0 /
+// 0.8 PFLOP/s, six bytes of copies per value at 6 TB/s and 17.  us per call, rows / copies (chosen so, but for *): 128, 32 / 8 heads, 8 users over 1500 keys, 48 tokens 32.7 / 50.3, 128
+// 44.8 / 51.8, 256 82 / 72; 32 over 800, 64 53 / 65, 128 96 / 92 (*); 2 over 6404, 128 52 / 59, 512 157 / 131; of 64, 16 / 16, 4 over 1500, 447 29.6 / 46.0; of 256, 16 / 8, 8 over 1500, 96
+// 63 / 73, 256 79 / 90; 2 over 1601 ... 4528, 2048 tokens 324 / 223.
 // TTPA_CROSS_FORM overrides.
-bool streams(const CrossArgs &c, const CrossCut &cut, int head_size, int64_t keys) {
+bool streams(const CrossArgs &c, const CrossCut &cut, int head_size, int64_t keys, bool fp8) {
   if (form_is("rows") || form_is("planned")) return false;
   if (form_is("stream")) return true;
   const int64_t tiles = (keys + cut.tile - 1) / cut.tile, row_blocks = (c.s + kRowsPerWave - 1) / kRowsPerWave;
   const int64_t groups = c.g % 4 == 0 ? c.g / 4 * row_blocks : (row_blocks * c.g + 3) / 4;  // workgroups of the streaming loop per KV head
   if (cut.row_blocks <= groups) return false;
+  if (fp8) {
+    const double segments = (double)c.batch * c.hkv, flops = 4.0 * segments * groups * 128 * keys * head_size;
+    const double rows_us = 10 + (head_size == 64 ? 0.47 : head_size == 128 ? 0.85 : 0.8) * segments * cut.row_blocks * tiles / std::max(device_cus(), 1);
+    return 17 + 6 * segments * keys * head_size / 6e6 + flops / (head_size == 64 ? 0.55e9 : head_size == 128 ? 1.0e9 : 0.8e9) < rows_us;
+  }
   return (int64_t)c.batch * c.hkv * cut.row_blocks * tiles > (head_size == 64 ? 28 : head_size == 128 ? 14 : 10) * (int64_t)std::max(device_cus(), 1);
 }
 
@@ -747,6 +808,87 @@ bool streams(const CrossArgs &c, const CrossCut &cut, int head_size, int64_t key
 int64_t room_of(int block_size, int table_width, int64_t most_keys) {
   const int64_t room = (int64_t)block_size * table_width;
   return most_keys > 0 ? std::min(room, most_keys) : room;
+}
+
+// An 8-bit cache in the streaming loop: bfloat16 copies of the keys (exact), their table and the parts, in the workspace.
+constexpr int64_t kMostCopies = int64_t(4) << 30;  // bytes of them: beyond, the rows' forms, which read the cache as it is
+struct CrossCopies {
+  int64_t copy, table;
+  CrossCopies(const CrossArgs &c, int head_size)
+      : copy(((int64_t)c.batch * c.w + 1) * c.hkv * c.bs * head_size * 2), table(((int64_t)c.batch * c.w * 4 + 255) & ~int64_t(255)) {}
+  bool fit(const CrossArgs &c) const { return 2 * copy <= kMostCopies && c.hkv < 32768; }
+  int64_t bytes() const { return 2 * copy + table; }
+};
+
+int64_t workspace_bytes(bool fp8, int batch, int q_heads, int kv_heads, int q_len, int head_size, int block_size, int table_width, int64_t most_keys) {
+  if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || q_len <= 0 || head_size <= 0 || block_size <= 0 || table_width <= 0 || q_heads % kv_heads) return 0;
+  const int64_t keys = room_of(block_size, table_width, most_keys);
+  const CrossCut c = cross_cut(batch, kv_heads, (int64_t)(q_heads / kv_heads) * q_len, head_size, keys);
+  int64_t bytes = cross_bytes(c, batch, kv_heads, head_size);
+  // (strides are not known here: what either form may want)
+  CrossArgs a = {};
+  a.batch = batch, a.hkv = kv_heads, a.g = q_heads / kv_heads, a.s = q_len, a.bs = block_size, a.w = (int)((keys + block_size - 1) / block_size);
+  PrefillArgs p;
+  const CrossCopies copies(a, head_size);
+  if ((head_size == 64 || head_size == 128 || head_size == 256) && streams(a, c, head_size, keys, fp8) && stream_args(a, head_size, most_keys > 0, keys, p) &&
+      (!fp8 || copies.fit(a)))
+    bytes = std::max(bytes, stream_ends_part_bytes(p, head_size) + (fp8 ? copies.bytes() : 0));
+  return bytes;
+}
+
+int attend(CrossArgs &a, bool fp8, int head_size, int64_t table_width, float scale, int64_t most_keys, void *workspace, int64_t workspace_bytes, hipStream_t st) {
+  const int batch = a.batch, kv_heads = a.hkv, block_size = a.bs;
+  TTPA_REQUIRE(a.out && a.q && a.k && a.v && a.pt && a.lens && (!fp8 || (a.k_scales && a.v_scales)), "cross attention: null pointer argument");
+  TTPA_REQUIRE(batch >= 0 && a.s >= 0 && a.g >= 0 && kv_heads > 0 && block_size > 0 && table_width > 0 && a.nb > 0, "cross attention: non-positive dimension");
+  if (head_size != 64 && head_size != 128 && head_size != 256)
+    return fail(TTPA_ERR_UNSUPPORTED, "cross attention: head_size %d; supported 64, 128, 256", head_size);
+  if (block_size % 32 || block_size > 4096)
+    return fail(TTPA_ERR_UNSUPPORTED, "cross attention: block_size %d must be a multiple of 32 up to 4096", block_size);
+  TTPA_REQUIRE(scale > 0.f, "cross attention: scale %g must be positive", (double)scale);
+  TTPA_REQUIRE(most_keys >= 0, "cross attention: most_keys must not be negative");
+  TTPA_REQUIRE(table_width * block_size < (1ll << 31) - 8192, "cross attention: a page-table row holds too many keys");
+  TTPA_REQUIRE((int64_t)a.g * a.s < (1ll << 30) && (int64_t)a.nb * kv_heads < (1ll << 32), "cross attention: too many rows or blocks");
+  TTPA_REQUIRE(aligned16(a.q) && aligned16(a.k) && aligned16(a.v) && aligned16(a.out), "cross attention: operands must be 16-byte aligned");
+  TTPA_REQUIRE(a.q_bs % 8 == 0 && a.q_hs % 8 == 0 && a.q_ts % 8 == 0 && a.o_bs % 4 == 0 && a.o_hs % 4 == 0 && a.o_ts % 4 == 0,
+               "cross attention: strides must be multiples of 8 elements (out: 4)");
+  if (batch == 0 || a.s == 0) return TTPA_OK;
+  // (what a caller's bound excludes is not there)
+  const int64_t keys = room_of(block_size, (int)table_width, most_keys);
+  a.w = (int)((keys + block_size - 1) / block_size);
+  a.scale_log2e = scale * 1.4426950408889634f;
+  PrefillArgs p;
+  const CrossCut c = cross_cut(batch, kv_heads, (int64_t)a.g * a.s, head_size, keys);
+  const CrossCopies copies(a, head_size);
+  if (streams(a, c, head_size, keys, fp8) && stream_args(a, head_size, most_keys > 0, keys, p) && (!fp8 || copies.fit(a))) {
+    TTPA_REQUIRE((int64_t)batch * kv_heads * a.g * ((a.s + 31) / 32) < (1ll << 26), "cross attention: too many rows for one launch");
+    char *ws = workspace && aligned16(workspace) ? static_cast<char *>(workspace) : nullptr;
+    if (fp8) {
+      if (!ws || workspace_bytes < copies.bytes())
+        return fail(TTPA_ERR_WORKSPACE, "cross attention: needs %lld bytes of workspace, 16-byte aligned", (long long)copies.bytes());
+      int32_t *const table = reinterpret_cast<int32_t *>(ws + 2 * copies.copy);
+      if (const int rc = fp8::expand_entries(a.k, a.v, a.k_scales, a.v_scales, ws, ws + copies.copy, table, a.pt, a.pt_rs, a.lens, a.lens_i64, batch, a.w,
+                                             kv_heads, block_size, head_size, a.nb, st))
+        return rc;
+      p.k = reinterpret_cast<uint16_t *>(ws), p.v = reinterpret_cast<uint16_t *>(ws + copies.copy), p.pt = table, p.pt_rs = a.w, p.nb = batch * a.w + 1;
+      ws += copies.bytes(), workspace_bytes -= copies.bytes();
+    }
+    if (ws) p.part_acc = reinterpret_cast<float *>(ws), p.part_bytes = workspace_bytes;
+    return launch_stream_ends(p, head_size, st);
+  }
+  a.row_blocks = c.row_blocks, a.parts = c.parts, a.share = c.share;
+  a.runs = (uint32_t)block_size / (c.tile / 4), a.runs_inv = 0xffffffffu / a.runs;
+  TTPA_REQUIRE(((int64_t)std::max(c.units, batch * kv_heads * c.parts) + 8) * c.row_blocks < (1ll << 24) && (c.parts == 1 || (int64_t)a.g * a.s < 65536),
+               "cross attention: too many rows for one launch");
+  const int64_t need = cross_bytes(c, batch, kv_heads, head_size);
+  if (a.parts > 1 && (!workspace || !aligned16(workspace) || workspace_bytes < need))
+    return fail(TTPA_ERR_WORKSPACE, "cross attention: needs %lld bytes of workspace, 16-byte aligned", (long long)need);
+  a.slots = static_cast<float *>(workspace);
+  if (c.units) {
+    a.firsts = static_cast<int2 *>(workspace), a.slots = reinterpret_cast<float *>(static_cast<char *>(workspace) + firsts_bytes(batch));
+    a.units = c.units, a.slots_of_cus = (float)std::max(device_cus(), 1) / (float)c.row_blocks;
+    a.step_us = (float)c.step_us, a.two = (float)c.two, a.merge_us = (float)c.merge_us;
+  }
+  return fp8 ? launch_cross_any<true>(a, head_size, c, st) : launch_cross_any<false>(a, head_size, c, st);
 }
 
 }  // namespace
@@ -757,18 +899,21 @@ using namespace ttpa;
 
 extern "C" int64_t ttpa_paged_cross_attention_workspace_bytes(int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t q_len, int32_t head_size,
                                                               int32_t block_size, int32_t table_width, int64_t most_keys) {
-  if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || q_len <= 0 || head_size <= 0 || block_size <= 0 || table_width <= 0 || q_heads % kv_heads) return 0;
-  const int64_t keys = decode::room_of(block_size, table_width, most_keys);
-  const decode::CrossCut c = decode::cross_cut(batch, kv_heads, (int64_t)(q_heads / kv_heads) * q_len, head_size, keys);
-  int64_t bytes = decode::cross_bytes(c, batch, kv_heads, head_size);
-  // (strides are not known here: what either form may want)
-  decode::CrossArgs a = {};
-  a.batch = batch, a.hkv = kv_heads, a.g = q_heads / kv_heads, a.s = q_len, a.bs = block_size, a.w = (int)((keys + block_size - 1) / block_size);
-  PrefillArgs p;
-  if ((head_size == 64 || head_size == 128 || head_size == 256) && decode::streams(a, c, head_size, keys) && decode::stream_args(a, head_size, most_keys > 0, keys, p))
-    bytes = std::max(bytes, stream_ends_part_bytes(p, head_size));
-  return bytes;
+  return decode::workspace_bytes(false, batch, q_heads, kv_heads, q_len, head_size, block_size, table_width, most_keys);
 }
+
+extern "C" int64_t ttpa_paged_fp8_cross_attention_workspace_bytes(int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t q_len, int32_t head_size,
+                                                                  int32_t block_size, int32_t table_width, int64_t most_keys) {
+  return decode::workspace_bytes(true, batch, q_heads, kv_heads, q_len, head_size, block_size, table_width, most_keys);
+}
+
+#define TTPA_CROSS_ARGS                                                                                                                                  \
+  TTPA_REQUIRE(q_heads > 0 && kv_heads > 0 && q_heads % kv_heads == 0, "cross attention: q_heads %d is not divisible by kv_heads %d", q_heads, kv_heads); \
+  decode::CrossArgs a = {};                                                                                                                              \
+  a.q = static_cast<const uint16_t *>(q), a.q_bs = q_batch_stride, a.q_hs = q_head_stride, a.q_ts = q_token_stride;                                      \
+  a.out = static_cast<uint16_t *>(out), a.o_bs = out_batch_stride, a.o_hs = out_head_stride, a.o_ts = out_token_stride;                                  \
+  a.k = k_cache, a.v = v_cache, a.pt = page_table, a.pt_rs = page_table_row_stride, a.lens = encoder_lens, a.lens_i64 = lens_is_i64;                     \
+  a.batch = batch, a.hkv = kv_heads, a.g = q_heads / kv_heads, a.s = q_len, a.bs = block_size, a.nb = num_blocks
 
 extern "C" int ttpa_paged_cross_attention(void *out, int64_t out_batch_stride, int64_t out_head_stride, int64_t out_token_stride, const void *q,
                                           int64_t q_batch_stride, int64_t q_head_stride, int64_t q_token_stride, const void *k_cache,
@@ -776,57 +921,18 @@ extern "C" int ttpa_paged_cross_attention(void *out, int64_t out_batch_stride, i
                                           int lens_is_i64, int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t q_len, int32_t head_size,
                                           int32_t block_size, int32_t table_width, int32_t num_blocks, float scale, int64_t most_keys,
                                           void *workspace, int64_t workspace_bytes, void *stream) {
-  TTPA_REQUIRE(out && q && k_cache && v_cache && page_table && encoder_lens, "cross attention: null pointer argument");
-  TTPA_REQUIRE(batch >= 0 && q_len >= 0 && q_heads > 0 && kv_heads > 0 && block_size > 0 && table_width > 0 && num_blocks > 0,
-               "cross attention: non-positive dimension");
-  TTPA_REQUIRE(q_heads % kv_heads == 0, "cross attention: q_heads %d is not divisible by kv_heads %d", q_heads, kv_heads);
-  if (head_size != 64 && head_size != 128 && head_size != 256)
-    return fail(TTPA_ERR_UNSUPPORTED, "cross attention: head_size %d; supported 64, 128, 256", head_size);
-  if (block_size % 32 || block_size > 4096)
-    return fail(TTPA_ERR_UNSUPPORTED, "cross attention: block_size %d must be a multiple of 32 up to 4096", block_size);
-  TTPA_REQUIRE(scale > 0.f, "cross attention: scale %g must be positive", (double)scale);
-  TTPA_REQUIRE(most_keys >= 0, "cross attention: most_keys must not be negative");
-  TTPA_REQUIRE((int64_t)table_width * block_size < (1ll << 31) - 8192, "cross attention: a page-table row holds too many keys");
-  TTPA_REQUIRE((int64_t)q_heads / kv_heads * q_len < (1ll << 30), "cross attention: too many rows");
-  TTPA_REQUIRE(aligned16(q) && aligned16(k_cache) && aligned16(v_cache) && aligned16(out), "cross attention: operands must be 16-byte aligned");
-  TTPA_REQUIRE(q_batch_stride % 8 == 0 && q_head_stride % 8 == 0 && q_token_stride % 8 == 0 && out_batch_stride % 4 == 0 && out_head_stride % 4 == 0 &&
-                   out_token_stride % 4 == 0,
-               "cross attention: strides must be multiples of 8 elements (out: 4)");
-  if (batch == 0 || q_len == 0) return TTPA_OK;
-  decode::CrossArgs a = {};
-  a.q = static_cast<const uint16_t *>(q), a.q_bs = q_batch_stride, a.q_hs = q_head_stride, a.q_ts = q_token_stride;
-  a.out = static_cast<uint16_t *>(out), a.o_bs = out_batch_stride, a.o_hs = out_head_stride, a.o_ts = out_token_stride;
-  a.k = static_cast<const uint16_t *>(k_cache), a.v = static_cast<const uint16_t *>(v_cache);
-  a.pt = page_table, a.pt_rs = page_table_row_stride, a.lens = encoder_lens, a.lens_i64 = lens_is_i64;
-  a.batch = batch, a.hkv = kv_heads, a.g = q_heads / kv_heads, a.s = q_len, a.bs = block_size, a.nb = num_blocks;
-  // (what a caller's bound excludes is not there)
-  const int64_t keys = decode::room_of(block_size, table_width, most_keys);
-  a.w = (int)((keys + block_size - 1) / block_size);
-  a.scale_log2e = scale * 1.4426950408889634f;
-  hipStream_t st = static_cast<hipStream_t>(stream);
-  PrefillArgs p;
-  const decode::CrossCut c = decode::cross_cut(batch, kv_heads, (int64_t)a.g * q_len, head_size, keys);
-  if (decode::streams(a, c, head_size, keys) && decode::stream_args(a, head_size, most_keys > 0, keys, p)) {
-    TTPA_REQUIRE((int64_t)batch * q_heads * ((q_len + 31) / 32) < (1ll << 26), "cross attention: too many rows for one launch");
-    if (workspace && aligned16(workspace)) p.part_acc = static_cast<float *>(workspace), p.part_bytes = workspace_bytes;
-    return launch_stream_ends(p, head_size, st);
-  }
-  a.row_blocks = c.row_blocks, a.parts = c.parts, a.share = c.share;
-  a.runs = (uint32_t)block_size / (c.tile / 4), a.runs_inv = 0xffffffffu / a.runs;
-  TTPA_REQUIRE(((int64_t)std::max(c.units, batch * kv_heads * c.parts) + 8) * c.row_blocks < (1ll << 24) && (c.parts == 1 || (int64_t)a.g * q_len < 65536),
-               "cross attention: too many rows for one launch");
-  const int64_t need = decode::cross_bytes(c, batch, kv_heads, head_size);
-  if (a.parts > 1 && (!workspace || !aligned16(workspace) || workspace_bytes < need))
-    return fail(TTPA_ERR_WORKSPACE, "cross attention: needs %lld bytes of workspace, 16-byte aligned", (long long)need);
-  a.slots = static_cast<float *>(workspace);
-  if (c.units) {
-    a.firsts = static_cast<int2 *>(workspace), a.slots = reinterpret_cast<float *>(static_cast<char *>(workspace) + decode::firsts_bytes(batch));
-    a.units = c.units, a.slots_of_cus = (float)std::max(device_cus(), 1) / (float)c.row_blocks;
-    a.step_us = (float)c.step_us, a.two = (float)c.two, a.merge_us = (float)c.merge_us;
-  }
-  switch (head_size) {
-    case 64: return decode::launch_cross_d<64>(a, c, st);
-    case 128: return decode::launch_cross_d<128>(a, c, st);
-    default: return decode::launch_cross_d<256>(a, c, st);
-  }
+  TTPA_CROSS_ARGS;
+  return decode::attend(a, false, head_size, table_width, scale, most_keys, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int ttpa_paged_fp8_cross_attention(void *out, int64_t out_batch_stride, int64_t out_head_stride, int64_t out_token_stride, const void *q,
+                                              int64_t q_batch_stride, int64_t q_head_stride, int64_t q_token_stride, const void *k_cache,
+                                              const void *v_cache, const float *k_scales, const float *v_scales, const int32_t *page_table,
+                                              int64_t page_table_row_stride, const void *encoder_lens, int lens_is_i64, int32_t batch, int32_t q_heads,
+                                              int32_t kv_heads, int32_t q_len, int32_t head_size, int32_t block_size, int32_t table_width,
+                                              int32_t num_blocks, float scale, int64_t most_keys, void *workspace, int64_t workspace_bytes,
+                                              void *stream) {
+  TTPA_CROSS_ARGS;
+  a.k_scales = k_scales, a.v_scales = v_scales;
+  return decode::attend(a, true, head_size, table_width, scale, most_keys, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
 }

@@ -58,6 +58,9 @@ struct ExpandArgs {
   int64_t pt_rs;
   const int32_t *chunk_start;
   int batch, w, hkv, bs, nb, q_len, d;
+  // cross attention: keys of each user, and nothing behind them is read
+  const void *lens;
+  int lens_i64;
 };
 
 constexpr int kExpandWorkgroups = 16384, kPieces = 4;
@@ -66,7 +69,7 @@ constexpr int kExpandWorkgroups = 16384, kPieces = 4;
 __global__ __launch_bounds__(256) void fp8_expand_kernel(ExpandArgs e) {
   // keys 0 .. chunk_start + q_len - 1 are read, in tiles of 64
   const int64_t end = (int64_t)(e.chunk_start ? max(*e.chunk_start, 0) : 0) + e.q_len;
-  const uint32_t cols = (uint32_t)min((int64_t)e.w, ((end + 63) / 64 * 64 + e.bs - 1) / e.bs);
+  const uint32_t cols = e.lens ? (uint32_t)e.w : (uint32_t)min((int64_t)e.w, ((end + 63) / 64 * 64 + e.bs - 1) / e.bs);
   const int slab = blockIdx.y;
   if (slab == 0)
     for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < (uint32_t)e.batch * e.w; i += gridDim.x * 256)
@@ -82,12 +85,14 @@ __global__ __launch_bounds__(256) void fp8_expand_kernel(ExpandArgs e) {
     // r = 0: the block of zeros; then the users' columns
     const uint32_t b = r ? (r - 1) / cols : 0, col = r ? r - 1 - b * cols : 0;
     const int64_t x = r ? (int64_t)b * e.w + col + 1 : 0;
+    const int64_t until = e.lens ? load_index(e.lens, e.lens_i64, b) : end;
+    if (r && until <= (int64_t)col * e.bs && e.lens) continue;
     int phys = e.pt[(int64_t)b * e.pt_rs + col];
     if ((unsigned)phys >= (unsigned)e.nb) phys = 0;
     const int64_t from = (int64_t)phys * e.hkv + h;
     const uint8_t *in = src + from * elements;
     uint16_t *out = copy + (x * e.hkv + h) * elements;
-    const int64_t left = r ? (end - (int64_t)col * e.bs) * e.d : 0;  // elements of the block in front of the chunk's end
+    const int64_t left = r ? min(until - (int64_t)col * e.bs, (int64_t)e.bs) * e.d : 0;  // elements of the block in front of the chunk's end
     const float scale = scales[from];
     for (int p = 0; p < pieces; p += kPieces) {
       u32x2 raw[kPieces];
@@ -117,7 +122,23 @@ ChunkLayout chunk_layout(int batch, int q_heads, int kv_heads, int q_len, int he
   return l;
 }
 
+dim3 expand_grid(const ExpandArgs &e) {
+  return dim3((unsigned)std::min<int64_t>((int64_t)e.batch * e.w + 1, std::max(1, kExpandWorkgroups / (2 * e.hkv))), 2 * e.hkv);
+}
+
 }  // namespace
+
+// Copies of users' first keys, a length each, in a table's first `width` columns, for cross attention: [1 + batch * width][kv_heads][block_size][head_size], and their table.
+int expand_entries(const void *k_cache, const void *v_cache, const float *k_scales, const float *v_scales, void *k_copy, void *v_copy, int32_t *table,
+                   const int32_t *page_table, int64_t page_table_row_stride, const void *lens, int lens_i64, int batch, int width, int kv_heads,
+                   int block_size, int head_size, int num_blocks, hipStream_t st) {
+  const ExpandArgs e = {static_cast<const uint8_t *>(k_cache), static_cast<const uint8_t *>(v_cache), k_scales, v_scales,
+                        static_cast<uint16_t *>(k_copy), static_cast<uint16_t *>(v_copy), table, page_table, page_table_row_stride, nullptr, batch, width,
+                        kv_heads, block_size, num_blocks, 0, head_size, lens, lens_i64};
+  fp8_expand_kernel<<<expand_grid(e), dim3(256), 0, st>>>(e);
+  return check_launch("fp8 cross attention (expansion)");
+}
+
 }  // namespace fp8
 }  // namespace ttpa
 
@@ -164,12 +185,12 @@ extern "C" int ttpa_chunked_fp8_attention(void *out, int64_t out_batch_stride, i
   uint8_t *ws = static_cast<uint8_t *>(workspace);
   fp8::ExpandArgs e = {static_cast<const uint8_t *>(k_cache), static_cast<const uint8_t *>(v_cache), k_scales, v_scales,
                        reinterpret_cast<uint16_t *>(ws), reinterpret_cast<uint16_t *>(ws + l.copy), reinterpret_cast<int32_t *>(ws + 2 * l.copy),
-                       page_table, page_table_row_stride, chunk_start, batch, l.width, kv_heads, block_size, num_blocks, q_len, head_size};
+                       page_table, page_table_row_stride, chunk_start, batch, l.width, kv_heads, block_size, num_blocks, q_len, head_size, nullptr, 0};
   hipStream_t st = static_cast<hipStream_t>(stream);
   // armed events: the pair brackets both launches
   hipEvent_t before, after;
   take_profile_events(before, after);
-  const dim3 grid((unsigned)std::min<int64_t>((int64_t)batch * l.width + 1, std::max(1, fp8::kExpandWorkgroups / (2 * kv_heads))), 2 * kv_heads);
+  const dim3 grid = fp8::expand_grid(e);
   if (before)
     hipExtLaunchKernelGGL(fp8::fp8_expand_kernel, grid, dim3(256), 0u, st, before, nullptr, 0u, e);
   else

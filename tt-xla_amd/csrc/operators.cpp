@@ -599,16 +599,34 @@ void chunked_fp8_attention_out(const Tensor &query, const Tensor &k_cache, const
 }
 
 // ---- cross attention --------------------------------------------------------------------------------
-void cross_into(const Call &c, const Tensor &out, const Tensor &query, const Tensor &k_cache, const Tensor &v_cache, const Tensor &page_table,
-                const Tensor &encoder_lens, const std::optional<double> &scale, int64_t most_keys) {
-  c.type(query, at::kBFloat16, "query");
-  for (const Tensor *t : {&k_cache, &v_cache}) {
-    c.type(*t, at::kBFloat16, "a cache");
-    TORCH_CHECK_VALUE(t->dim() == 4 && t->is_contiguous() && t->numel() > 0, c.name(),
-                      ": a cache must be a contiguous [num_blocks, kv_heads, block_size, head_size] tensor");
+// A layer's caches of an encoder's states, in bfloat16 or with a byte per element and their scales.
+struct CrossCache {
+  Tensor k, v;
+  const float *k_scales = nullptr, *v_scales = nullptr;
+  int64_t nb, hkv, bs, d;
+  CrossCache(const Call &c, const Tensor &k_cache, const Tensor &v_cache) : k(k_cache), v(v_cache) {
+    for (const Tensor *t : {&k_cache, &v_cache}) {
+      c.type(*t, at::kBFloat16, "a cache");
+      TORCH_CHECK_VALUE(t->dim() == 4 && t->is_contiguous() && t->numel() > 0, c.name(),
+                        ": a cache must be a contiguous [num_blocks, kv_heads, block_size, head_size] tensor");
+    }
+    TORCH_CHECK_VALUE(k.sizes() == v.sizes(), c.name(), ": K and V caches must have the same shape");
+    sizes();
   }
-  TORCH_CHECK_VALUE(k_cache.sizes() == v_cache.sizes(), c.name(), ": K and V caches must have the same shape");
-  const int64_t nb = k_cache.size(0), hkv = k_cache.size(1), bs = k_cache.size(2), d = k_cache.size(3);
+  CrossCache(const Call &c, const Cache &bytes) : k(bytes.k), v(bytes.v), k_scales(bytes.k_scales()), v_scales(bytes.v_scales()) { sizes(); }
+
+ private:
+  void sizes() {
+    nb = k.size(0), hkv = k.size(1), bs = k.size(2), d = k.size(3);
+    if (!aligned16(k)) k = compact(k);
+    if (!aligned16(v)) v = compact(v);
+  }
+};
+
+void cross_into(const Call &c, const Tensor &out, const Tensor &query, const CrossCache &cache, const Tensor &page_table, const Tensor &encoder_lens,
+                const std::optional<double> &scale, int64_t most_keys) {
+  c.type(query, at::kBFloat16, "query");
+  const int64_t nb = cache.nb, hkv = cache.hkv, bs = cache.bs, d = cache.d;
   TORCH_CHECK_VALUE(query.dim() == 4 && query.size(3) == d && query.size(1) > 0 && query.size(1) % hkv == 0, c.name(), ": query ", query.sizes(),
                     " must be [users, heads, tokens, head_size] and match the caches' kv_heads=", hkv, ", head_size=", d);
   const Tensor pt = table(c, page_table), lens = indices(c, encoder_lens, "encoder_lens");
@@ -617,30 +635,60 @@ void cross_into(const Call &c, const Tensor &out, const Tensor &query, const Ten
   TORCH_CHECK_VALUE(!scale || *scale > 0, c.name(), ": scale must be positive");
   TORCH_CHECK_VALUE(most_keys >= 0, c.name(), ": most_keys must not be negative");
   if (users == 0 || s == 0) return;
-  const Tensor q = rows(query), target = storable(out), k = aligned16(k_cache) ? k_cache : compact(k_cache), v = aligned16(v_cache) ? v_cache : compact(v_cache);
-  const int64_t bytes = ttpa_paged_cross_attention_workspace_bytes(i32(users), i32(hq), i32(hkv), i32(s), i32(d), i32(bs), i32(pt.size(1)), most_keys);
+  const Tensor q = rows(query), target = storable(out);
+  const auto bytes_of = cache.k_scales ? ttpa_paged_fp8_cross_attention_workspace_bytes : ttpa_paged_cross_attention_workspace_bytes;
+  const int64_t bytes = bytes_of(i32(users), i32(hq), i32(hkv), i32(s), i32(d), i32(bs), i32(pt.size(1)), most_keys);
   const Tensor ws = bytes ? c.scratch(bytes) : Tensor();
-  ok("ttpa_paged_cross_attention",
-     ttpa_paged_cross_attention(target.data_ptr(), step_of(target, 0), step_of(target, 1), step_of(target, 2), q.data_ptr(), step_of(q, 0), step_of(q, 1),
-                                step_of(q, 2), k.data_ptr(), v.data_ptr(), int_ptr(pt), step_of(pt, 0), lens.data_ptr(), is_i64(lens), i32(users),
-                                i32(hq), i32(hkv), i32(s), i32(d), i32(bs), i32(pt.size(1)), i32(nb), scale_of(scale, d), most_keys,
-                                bytes ? ws.data_ptr() : nullptr, bytes, c.stream()));
+  void *const room = bytes ? ws.data_ptr() : nullptr;
+  if (cache.k_scales)
+    ok("ttpa_paged_fp8_cross_attention",
+       ttpa_paged_fp8_cross_attention(target.data_ptr(), step_of(target, 0), step_of(target, 1), step_of(target, 2), q.data_ptr(), step_of(q, 0),
+                                      step_of(q, 1), step_of(q, 2), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scales, cache.v_scales, int_ptr(pt),
+                                      step_of(pt, 0), lens.data_ptr(), is_i64(lens), i32(users), i32(hq), i32(hkv), i32(s), i32(d), i32(bs),
+                                      i32(pt.size(1)), i32(nb), scale_of(scale, d), most_keys, room, bytes, c.stream()));
+  else
+    ok("ttpa_paged_cross_attention",
+       ttpa_paged_cross_attention(target.data_ptr(), step_of(target, 0), step_of(target, 1), step_of(target, 2), q.data_ptr(), step_of(q, 0), step_of(q, 1),
+                                  step_of(q, 2), cache.k.data_ptr(), cache.v.data_ptr(), int_ptr(pt), step_of(pt, 0), lens.data_ptr(), is_i64(lens),
+                                  i32(users), i32(hq), i32(hkv), i32(s), i32(d), i32(bs), i32(pt.size(1)), i32(nb), scale_of(scale, d), most_keys, room,
+                                  bytes, c.stream()));
   if (!target.is_same(out)) out.copy_(target);
 }
 
 Tensor paged_cross_attention(const Tensor &query, const Tensor &key, const Tensor &value, const Tensor &page_table, const Tensor &encoder_lens,
                              std::optional<double> scale, int64_t most_keys) {
   const Call c("tt::paged_cross_attention", query);
+  const CrossCache cache(c, key, value);
   const Tensor out = at::empty_like(query);  // keeps the query's (possibly token-major) strides
-  cross_into(c, out, query, key, value, page_table, encoder_lens, scale, most_keys);
+  cross_into(c, out, query, cache, page_table, encoder_lens, scale, most_keys);
   return out;
 }
 
 void paged_cross_attention_out(const Tensor &query, const Tensor &key, const Tensor &value, const Tensor &page_table, const Tensor &encoder_lens,
                                const Tensor &out, std::optional<double> scale, int64_t most_keys) {
   const Call c("tt::paged_cross_attention_out", query);
+  const CrossCache cache(c, key, value);
   check_out(c, out, query);
-  cross_into(c, out, query, key, value, page_table, encoder_lens, scale, most_keys);
+  cross_into(c, out, query, cache, page_table, encoder_lens, scale, most_keys);
+  written(out);
+}
+
+Tensor paged_fp8_cross_attention(const Tensor &query, const Tensor &k_cache, const Tensor &v_cache, const Tensor &k_scales, const Tensor &v_scales,
+                                 const Tensor &page_table, const Tensor &encoder_lens, std::optional<double> scale, int64_t most_keys) {
+  const Call c("tt::paged_fp8_cross_attention", query);
+  const CrossCache cache(c, Cache(c, k_cache, v_cache, k_scales, v_scales));
+  const Tensor out = at::empty_like(query);
+  cross_into(c, out, query, cache, page_table, encoder_lens, scale, most_keys);
+  return out;
+}
+
+void paged_fp8_cross_attention_out(const Tensor &query, const Tensor &k_cache, const Tensor &v_cache, const Tensor &k_scales, const Tensor &v_scales,
+                                   const Tensor &page_table, const Tensor &encoder_lens, const Tensor &out, std::optional<double> scale,
+                                   int64_t most_keys) {
+  const Call c("tt::paged_fp8_cross_attention_out", query);
+  const CrossCache cache(c, Cache(c, k_cache, v_cache, k_scales, v_scales));
+  check_out(c, out, query);
+  cross_into(c, out, query, cache, page_table, encoder_lens, scale, most_keys);
   written(out);
 }
 
@@ -731,6 +779,10 @@ TORCH_LIBRARY_FRAGMENT(tt, m) {
         "int most_keys=0) -> Tensor");
   m.def("paged_cross_attention_out(Tensor query, Tensor key, Tensor value, Tensor page_table, Tensor encoder_lens, Tensor(a!) out, "
         "float? scale=None, int most_keys=0) -> ()");
+  m.def("paged_fp8_cross_attention(Tensor query, " TT_CACHE ", Tensor page_table, Tensor encoder_lens, float? scale=None, "
+        "int most_keys=0) -> Tensor");
+  m.def("paged_fp8_cross_attention_out(Tensor query, " TT_CACHE ", Tensor page_table, Tensor encoder_lens, Tensor(a!) out, "
+        "float? scale=None, int most_keys=0) -> ()");
   m.def("copy_cache_blocks_(Tensor(a!)[] caches, Tensor source_blocks, Tensor target_blocks) -> ()");
   m.def("keep_cache_tokens_(Tensor(a!)[] caches, Tensor page_table, Tensor kept, Tensor kept_lens, Tensor? first=None) -> ()");
   m.def("qk_norm_rope_update_fp8_(Tensor query, Tensor key, Tensor value, " TT_ROPE ", " TT_CACHE_W ", Tensor page_table, "
@@ -760,6 +812,8 @@ TORCH_LIBRARY_IMPL(tt, CUDA, m) {
   m.impl("qk_norm_rope_axes_", &qk_norm_rope_axes_);
   m.impl("paged_cross_attention", &paged_cross_attention);
   m.impl("paged_cross_attention_out", &paged_cross_attention_out);
+  m.impl("paged_fp8_cross_attention", &paged_fp8_cross_attention);
+  m.impl("paged_fp8_cross_attention_out", &paged_fp8_cross_attention_out);
   m.impl("copy_cache_blocks_", &copy_cache_blocks_);
   m.impl("keep_cache_tokens_", &keep_cache_tokens_);
   m.impl("qk_norm_rope_update_fp8_", &qk_norm_rope_update_fp8_);

@@ -196,6 +196,12 @@ SIGNATURES = {
         [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _p, _i64, _p, _int, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32,
          _i64, _p, _i64, _p],
     ),
+    "ttpa_paged_fp8_cross_attention_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i64]),
+    "ttpa_paged_fp8_cross_attention": (
+        _int,
+        [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _p, _p, _p, _i64, _p, _int, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32,
+         _i64, _p, _i64, _p],
+    ),
     "ttpa_copy_cache_blocks": (_int, [_p, _p, _i32, _p, _p, _i32, _i32, _p]),
     "ttpa_keep_cache_tokens": (
         _int, [_p, _i32, _p, _i64, _p, _i64, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _p],

@@ -266,8 +266,10 @@ class TTAttentionBackendImpl(_ImplBase):
             )
         self.cross = attn_type == _ENCODER_DECODER
         if self.cross:
-            if sliding_window is not None or sinks is not None or sparse_kept_blocks is not None or functional_cache_ops or kv_cache_dtype not in ("auto", "bfloat16"):
-                raise NotImplementedError("cross attention is built for bfloat16 caches that are updated in place, without sliding windows, sinks and sparse decode")
+            if sliding_window is not None or sinks is not None or sparse_kept_blocks is not None or functional_cache_ops:
+                raise NotImplementedError("cross attention is built for caches that are updated in place, without sliding windows, sinks and sparse decode")
+            if kv_cache_dtype not in ("auto", "bfloat16", "fp8", "fp8_e4m3"):
+                raise NotImplementedError(f"cross attention is built for bfloat16 and fp8_e4m3 caches, not for {kv_cache_dtype}")
             if head_size not in (64, 128, 256):
                 raise NotImplementedError(f"cross attention is built for head sizes of 64, 128 and 256, not {head_size}")
         self.kv_cache_stored = None
@@ -468,10 +470,11 @@ class TTAttentionBackendImpl(_ImplBase):
         q = self._normalize_to_attention_format(query, "query", self.num_heads, self.head_size, users)
         caches = list(kv_cache) if isinstance(kv_cache, (list, tuple)) else [] if kv_cache is None else [kv_cache]
         cached = len(caches) > 0 and caches[0].numel() > 0
+        eight_bits = cached and caches[0].dtype == torch.float8_e4m3fn
         if cached:
-            if len(caches) != 2 or caches[0].dtype != torch.bfloat16 or caches[0].dim() != 4 or caches[0].shape[2] % 32:
-                raise NotImplementedError("cross attention is built for bfloat16 caches [k, v] of blocks of a multiple of 32 tokens, not for "
-                                          f"{[(tuple(t.shape), t.dtype) for t in caches]}")
+            if not (eight_bits and len(caches) in (4, 5) or caches[0].dtype == torch.bfloat16 and len(caches) == 2) or caches[0].dim() != 4 or caches[0].shape[2] % 32:
+                raise NotImplementedError("cross attention is built for bfloat16 caches [k, v] and 8-bit ones [k, v, k_scales, v_scales], or with key bounds behind them, of "
+                                          f"blocks of a multiple of 32 tokens, not for {[(tuple(t.shape), t.dtype) for t in caches]}")
             if attn_metadata.encoder_lens is None:
                 raise ValueError("cross attention needs encoder_lens in attn_metadata")
         elif key is None:
@@ -485,11 +488,15 @@ class TTAttentionBackendImpl(_ImplBase):
                 rows = attn_metadata.batch_idx
                 assert rows is not None, "batch_idx must be provided for an encoder's states."
                 k, v = (self._normalize_to_attention_format(x, n, self.num_kv_heads, self.head_size, rows.numel()) for x, n in ((key, "key"), (value, "value")))
-                ops.paged_fill_kv_cache_(caches[0], caches[1], k.transpose(1, 2), v.transpose(1, 2), attn_metadata.fill_page_table, batch_idx=rows)
+                if eight_bits:
+                    ops.paged_fill_fp8_cache_(*caches[:4], k.transpose(1, 2), v.transpose(1, 2), attn_metadata.fill_page_table, rows, *caches[4:])
+                else:
+                    ops.paged_fill_kv_cache_(caches[0], caches[1], k.transpose(1, 2), v.transpose(1, 2), attn_metadata.fill_page_table, batch_idx=rows)
             # (what a graph captures is replayed for other lengths: it has to have room for all that the table holds)
             most = 0 if torch.cuda.is_current_stream_capturing() else attn_metadata.most_encoder_len or 0
-            ops.paged_cross_attention_out(q.transpose(1, 2), caches[0], caches[1], attn_metadata.page_table, attn_metadata.encoder_lens,
-                                          into.transpose(1, 2), scale=self.scale, most_keys=most)
+            attend = ops.paged_fp8_cross_attention_out if eight_bits else ops.paged_cross_attention_out
+            attend(q.transpose(1, 2), *caches[: 4 if eight_bits else 2], attn_metadata.page_table, attn_metadata.encoder_lens, into.transpose(1, 2),
+                   scale=self.scale, most_keys=most)
         else:
             k, v = (self._normalize_to_attention_format(x, n, self.num_kv_heads, self.head_size, users) for x, n in ((key, "key"), (value, "value")))
             tokens = q.shape[1]  # (that operator takes whole blocks of 32 rows)

@@ -4,8 +4,8 @@ The operators are registered by the native host module (``csrc/operators.cpp``);
 
 ``tt::qk_norm_rope_axes``, ``tt::qk_norm_rope_axes_``
     norm and rotation as ``tt::qk_norm_rope``, every pair of features by the position on its axis (time, height, width).
-``tt::paged_cross_attention``, ``tt::paged_cross_attention_out``
-    attention to an encoder's states in a paged cache, a length per user and no causal limit.
+``tt::paged_cross_attention``, ``tt::paged_cross_attention_out``, ``tt::paged_fp8_cross_attention``, ``tt::paged_fp8_cross_attention_out``
+    attention to an encoder's states in a paged cache of bfloat16 values or of one byte per element, a length per user and no causal limit.
 ``tt::copy_cache_blocks_``, ``tt::keep_cache_tokens_``
     copies of whole blocks, and compaction of sequences, in the caches of all layers at once (``kv_blocks.CachePages`` plans them).
 
@@ -69,6 +69,14 @@ def register() -> None:
 
     @torch.library.register_fake("tt::paged_cross_attention_out")
     def _(query, key, value, page_table, encoder_lens, out, scale=None, most_keys=0):
+        return None
+
+    @torch.library.register_fake("tt::paged_fp8_cross_attention")
+    def _(query, k_cache, v_cache, k_scales, v_scales, page_table, encoder_lens, scale=None, most_keys=0):
+        return torch.empty_like(query)
+
+    @torch.library.register_fake("tt::paged_fp8_cross_attention_out")
+    def _(query, k_cache, v_cache, k_scales, v_scales, page_table, encoder_lens, out, scale=None, most_keys=0):
         return None
 
     @torch.library.register_fake("tt::copy_cache_blocks_")
