@@ -1,4 +1,4 @@
-// Attention of tokens to an encoder's states in a paged bfloat16 cache: a length per user, no causal limit.
+// Attention of tokens to an encoder's states in a paged cache, of bfloat16 values or of one byte per element: a length per user, no causal limit.
 //
 //   out[u, h, t] = sum_j softmax_j(scale q[u, h, t] . k[u, j]) v[u, j],   j < len[u];   zeros where len[u] is 0
 //
