@@ -5,10 +5,10 @@
 // This file holds the forms for few rows (a token per user, drafted ones, short texts) and the choice; many rows are the streaming prefill loop's
 // (prefill_stream_kernel.h, kEnds).  All tokens of a user see the same keys, so the rows of a KV head are its G query heads times the tokens.  Up to 32 rows, a workgroup's four
 // wavefronts have tiles of their own of a part of the keys and all of the rows; else, and at head size 256, they share the tiles and have 16 rows each.
-// Bound by memory: K and V are read once for each block of rows.  32 users of 32 / 8 heads of 128 over 256 ... 4096 keys (170 MB) 35 us, of which the merge is four:
+// Bound by memory: K and V are read once for each block of rows.  32 users of 32 / 8 heads of 128 over 256 ... 4096 keys (170 MB) 34 us, of which the merge is four:
 // 5.7 TB/s in the kernel; 64 users of 8 / 8 of 64 over 1500 (197 MB) 33.4, 5.9 TB/s; 96 of 64 / 8 of 128 over 512 ... 2048 (436 MB) 74, 5.9; shared, 96 of 64 / 8, 5 tokens, over
-// 1500 (590 MB) 115, 5.1; 64 of 16 / 8 of 256 over 800 (419 MB) 71, 5.9.  Between, the chains of tiles do, 1.1 us a tile of 32 keys, or of 64 that are shared:
-// 8 users of 32 / 8 over 1500 (49 MB) 13.4, 5 tokens of 64 / 8 16.0.  Tiles of TILE keys (64 at head size 64, else 32; shared 64, 32 at head size 256):
+// 1500 (590 MB) 102, 5.8; 64 of 16 / 8 of 256 over 800 (419 MB) 68, 6.1.  Between, the chains of tiles do, 1.1 us a tile of 32 keys, or of 64 that are shared:
+// 8 users of 32 / 8 over 1500 (49 MB) 13.2, 5 tokens of 64 / 8 16.0.  Tiles of TILE keys (64 at head size 64, else 32; shared 64, 32 at head size 256):
 //   memory -> registers -> LDS    whole lines, a tile ahead of its use (shared: two); what lies behind the last key becomes zeros on the way (V) or is masked (K).  One
 //                                 buffer takes K, then V: two workgroups share a CU.  (Three, with fewer registers, came to 5.0 TB/s: four wavefronts per SIMD ask for
 //                                 more than the memory takes well.)
@@ -16,7 +16,7 @@
 //                                 key (TILE / 4) j + 4 b + r, so lane (row, quad) ends up with its quad's run in order, which is
 //   O^T += V^T . P^T              the order in which the second product wants its weights: no moves between the two
 // 8-bit caches: the same, an element becoming its bfloat16 value on its way into LDS; 32 users of 32 / 8 heads over 256 ... 4096 keys 22.4 us (34.0 with bfloat16), 96 of 64 / 8 over
-// 512 ... 2048 51 (75), 64 of 16 / 8 of 256 over 800 42.5 (71), 96 of 64 / 8, 5 tokens, over 1500 70 (111).
+// 512 ... 2048 51 (75), 64 of 16 / 8 of 256 over 800 42.5 (68), 96 of 64 / 8, 5 tokens, over 1500 70 (102).
 // Statistics and accumulators are floats; weights are rounded once to bfloat16 for the matrix instruction, and the same rounded weights are summed.
 // Wavefronts' results of their own tiles meet in LDS, the parts' in memory, merged by a kernel of its own.  How many parts there are goes by an estimate of the time, the host's of the longest
 // user, or, where that is long enough to pay for it, the device's of all of them (cross_work).
