@@ -666,6 +666,18 @@ int ttpa_paged_fill_fp8_cache(void *k_cache, void *v_cache, float *k_scales, flo
                               int32_t seq_len, int32_t block_size, int32_t head_size, int32_t table_width, int32_t num_blocks, void *stream);
 
 /*
+ * The same for prompts and encoder states padded to one length: of a fill row the first lens[batch_idx[i]] tokens count (lens [table_rows], by the page table's
+ * rows; all of them where it is larger, none where it is zero or less).  What lies behind, whatever it is, has no part in a scale or in bounds, and its rows
+ * of the cache keep their bytes; blocks without a token that counts keep theirs, their scale and their bounds.  lens may be NULL: all tokens count.
+ */
+int ttpa_paged_fill_fp8_cache_lens(void *k_cache, void *v_cache, float *k_scales, float *v_scales, void *key_bounds, const void *k_fill,
+                                   int64_t k_user_stride, int64_t k_head_stride, int64_t k_token_stride, const void *v_fill, int64_t v_user_stride,
+                                   int64_t v_head_stride, int64_t v_token_stride, const int32_t *page_table, int64_t page_table_row_stride,
+                                   const void *batch_idx, int batch_idx_is_i64, const void *lens, int lens_is_i64, int32_t fill_users,
+                                   int32_t table_rows, int32_t kv_heads, int32_t seq_len, int32_t block_size, int32_t head_size, int32_t table_width,
+                                   int32_t num_blocks, void *stream);
+
+/*
  * ttpa_paged_sdpa_decode_windowed over the 8-bit cache, up to 16 query heads per KV head and 2048 users.  The workspace is
  * ttpa_paged_decode_workspace_bytes(users, q_heads, kv_heads, head_size) bytes.
  */

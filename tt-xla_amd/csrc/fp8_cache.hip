@@ -26,7 +26,14 @@ struct FillArgs {
   const void *bidx;
   int bidx_i64;
   int table_rows, s, blocks;  // blocks of a prompt
+  const void *lens;  // [table_rows] rows that count of those that go to a table row's blocks, or null: all
+  int lens_i64;
 };
+
+// Of `rows` rows of a block, from row `first` of a prompt on: how many count.
+__device__ __forceinline__ int counted_rows(const FillArgs &a, int64_t table_row, int first, int rows) {
+  return a.lens ? (int)max(min(max(load_index(a.lens, a.lens_i64, table_row), (int64_t)0) - first, (int64_t)rows), (int64_t)0) : rows;
+}
 
 // Whether a later fill row has the same index: of fill rows with one index the last one counts, so that blocks are written whole, and never with
 // another row's scale.  The same in every wavefront.
@@ -88,13 +95,17 @@ __global__ __launch_bounds__(256) void fill_kernel(FillArgs a) {
   // (uniform in the workgroup, like the next)
   const int64_t table_row = a.bidx ? load_index(a.bidx, a.bidx_i64, user) : 0;
   if (table_row < 0 || table_row >= a.table_rows || replaced(a, user, users, table_row)) return;
-  const int phys = a.c.pt[table_row * a.c.pt_rs + col];
-  if ((unsigned)phys >= (unsigned)a.c.nb) return;
+  const int phys = a.c.pt[table_row * a.c.pt_rs + col], counted = counted_rows(a, table_row, first, rows) * CPR;
+  if ((unsigned)phys >= (unsigned)a.c.nb || counted == 0) return;
   if constexpr (PIECES > 0) {
+    if (counted < pieces) {  // (the last ones that count again, in place of those behind)
+#pragma unroll
+      for (int j = 0; j < PIECES; ++j) x[j] = load(min(tid + 256 * j, counted - 1));
+    }
 #pragma unroll
     for (int j = 0; j < PIECES; ++j) look(x[j]);  // (a piece again changes nothing)
   } else {
-    for (int p = tid; p < pieces; p += 256) look(load(p));
+    for (int p = tid; p < counted; p += 256) look(load(p));
   }
   // over the wavefront, then over the workgroup
   for (int m = 1; m < 64; m <<= 1) most = max(most, (uint32_t)__shfl_xor((int)most, m));
@@ -117,9 +128,9 @@ __global__ __launch_bounds__(256) void fill_kernel(FillArgs a) {
   if constexpr (PIECES > 0) {
 #pragma unroll
     for (int j = 0; j < PIECES; ++j)
-      if (tid + 256 * j < pieces) __builtin_nontemporal_store(encode8(x[j], inv), reinterpret_cast<u32x2 *>(dst + 8 * (tid + 256 * j)));
+      if (tid + 256 * j < counted) __builtin_nontemporal_store(encode8(x[j], inv), reinterpret_cast<u32x2 *>(dst + 8 * (tid + 256 * j)));
   } else {
-    for (int p = tid; p < pieces; p += 256) *reinterpret_cast<u32x2 *>(dst + 8 * p) = encode8(load(p), inv);
+    for (int p = tid; p < counted; p += 256) *reinterpret_cast<u32x2 *>(dst + 8 * p) = encode8(load(p), inv);
   }
   if (tid == 0) (is_v ? a.c.v_scales : a.c.k_scales)[slab] = scale;
   if (bounded)
@@ -145,15 +156,18 @@ __global__ __launch_bounds__(256) void fill_small_kernel(FillArgs a) {
   const int64_t ts = is_v ? a.v_ts : a.k_ts;
   const int f = 8 * (lane % CPR);
   const uint16_t *src = (is_v ? a.v + user * a.v_us + h * a.v_hs : a.k + user * a.k_us + h * a.k_hs) + first * ts + f;
-  const int pieces = rows * CPR;
+  const auto load = [&](int row, int end) { return __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(src + min(row, end - 1) * ts)); };
   u32x4 x[PIECES];
 #pragma unroll
-  for (int j = 0; j < PIECES; ++j)
-    x[j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(src + min((lane + 64 * j) / CPR, rows - 1) * ts));
+  for (int j = 0; j < PIECES; ++j) x[j] = load((lane + 64 * j) / CPR, rows);
   const int64_t table_row = a.bidx ? load_index(a.bidx, a.bidx_i64, user) : 0;
   if (table_row < 0 || table_row >= a.table_rows || replaced(a, user, users, table_row)) return;
-  const int phys = a.c.pt[table_row * a.c.pt_rs + col];
-  if ((unsigned)phys >= (unsigned)a.c.nb) return;
+  const int phys = a.c.pt[table_row * a.c.pt_rs + col], counted = counted_rows(a, table_row, first, rows) * CPR;
+  if ((unsigned)phys >= (unsigned)a.c.nb || counted == 0) return;
+  if (counted < rows * CPR) {  // (the last row that counts again, in place of those behind)
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j) x[j] = load((lane + 64 * j) / CPR, counted / CPR);
+  }
   uint32_t most = 0;
 #pragma unroll
   for (int j = 0; j < PIECES; ++j)
@@ -166,7 +180,7 @@ __global__ __launch_bounds__(256) void fill_small_kernel(FillArgs a) {
   uint8_t *dst = (is_v ? a.c.v : a.c.k) + slab * a.c.bs * D;
 #pragma unroll
   for (int j = 0; j < PIECES; ++j)
-    if (lane + 64 * j < pieces) __builtin_nontemporal_store(encode8(x[j], inv), reinterpret_cast<u32x2 *>(dst + 8 * (lane + 64 * j)));
+    if (lane + 64 * j < counted) __builtin_nontemporal_store(encode8(x[j], inv), reinterpret_cast<u32x2 *>(dst + 8 * (lane + 64 * j)));
   if (lane == 0) (is_v ? a.c.v_scales : a.c.k_scales)[slab] = scale;
   if (!is_v && a.c.bounds) {
     float low[8], high[8];
@@ -207,12 +221,12 @@ int launch_fill(const FillArgs &a, int users, hipStream_t st) {
 
 using namespace ttpa;
 
-extern "C" int ttpa_paged_fill_fp8_cache(void *k_cache, void *v_cache, float *k_scales, float *v_scales, void *key_bounds, const void *k_fill,
-                                         int64_t k_user_stride, int64_t k_head_stride, int64_t k_token_stride, const void *v_fill,
-                                         int64_t v_user_stride, int64_t v_head_stride, int64_t v_token_stride, const int32_t *page_table,
-                                         int64_t page_table_row_stride, const void *batch_idx, int batch_idx_is_i64, int32_t fill_users,
-                                         int32_t table_rows, int32_t kv_heads, int32_t seq_len, int32_t block_size, int32_t head_size,
-                                         int32_t table_width, int32_t num_blocks, void *stream) {
+extern "C" int ttpa_paged_fill_fp8_cache_lens(void *k_cache, void *v_cache, float *k_scales, float *v_scales, void *key_bounds, const void *k_fill,
+                                              int64_t k_user_stride, int64_t k_head_stride, int64_t k_token_stride, const void *v_fill,
+                                              int64_t v_user_stride, int64_t v_head_stride, int64_t v_token_stride, const int32_t *page_table,
+                                              int64_t page_table_row_stride, const void *batch_idx, int batch_idx_is_i64, const void *lens,
+                                              int lens_is_i64, int32_t fill_users, int32_t table_rows, int32_t kv_heads, int32_t seq_len,
+                                              int32_t block_size, int32_t head_size, int32_t table_width, int32_t num_blocks, void *stream) {
   if (int rc = fp8::check_cache(k_cache, v_cache, k_scales, v_scales, page_table, kv_heads, head_size, block_size, table_width, num_blocks)) return rc;
   TTPA_REQUIRE(k_fill && v_fill, "fp8 fill: null pointer argument");
   TTPA_REQUIRE(fill_users >= 0 && seq_len >= 0 && table_rows > 0, "fp8 fill: non-positive dimension");
@@ -229,11 +243,22 @@ extern "C" int ttpa_paged_fill_fp8_cache(void *k_cache, void *v_cache, float *k_
                       page_table, page_table_row_stride, kv_heads, block_size, table_width, num_blocks, fp8::block_inverse(block_size)},
                      static_cast<const uint16_t *>(k_fill), static_cast<const uint16_t *>(v_fill), k_user_stride, k_head_stride, k_token_stride,
                      v_user_stride, v_head_stride, v_token_stride, batch_idx, batch_idx_is_i64, table_rows, seq_len,
-                     (seq_len + block_size - 1) / block_size};
+                     (seq_len + block_size - 1) / block_size, lens, lens_is_i64};
   hipStream_t st = static_cast<hipStream_t>(stream);
   switch (head_size) {
     case 64: return fp8::launch_fill<64>(a, fill_users, st);
     case 128: return fp8::launch_fill<128>(a, fill_users, st);
     default: return fp8::launch_fill<256>(a, fill_users, st);
   }
+}
+
+extern "C" int ttpa_paged_fill_fp8_cache(void *k_cache, void *v_cache, float *k_scales, float *v_scales, void *key_bounds, const void *k_fill,
+                                         int64_t k_user_stride, int64_t k_head_stride, int64_t k_token_stride, const void *v_fill,
+                                         int64_t v_user_stride, int64_t v_head_stride, int64_t v_token_stride, const int32_t *page_table,
+                                         int64_t page_table_row_stride, const void *batch_idx, int batch_idx_is_i64, int32_t fill_users,
+                                         int32_t table_rows, int32_t kv_heads, int32_t seq_len, int32_t block_size, int32_t head_size,
+                                         int32_t table_width, int32_t num_blocks, void *stream) {
+  return ttpa_paged_fill_fp8_cache_lens(k_cache, v_cache, k_scales, v_scales, key_bounds, k_fill, k_user_stride, k_head_stride, k_token_stride, v_fill,
+                                        v_user_stride, v_head_stride, v_token_stride, page_table, page_table_row_stride, batch_idx, batch_idx_is_i64,
+                                        nullptr, 0, fill_users, table_rows, kv_heads, seq_len, block_size, head_size, table_width, num_blocks, stream);
 }

@@ -372,8 +372,8 @@ void paged_update_fp8_cache_(const Tensor &k_cache, const Tensor &v_cache, const
   cache.changed(key_bounds);
 }
 
-void paged_fill_fp8_cache_(const Tensor &k_cache, const Tensor &v_cache, const Tensor &k_scales, const Tensor &v_scales, const Tensor &k_fill,
-                           const Tensor &v_fill, const Tensor &page_table, const OptTensor &batch_idx, const OptTensor &key_bounds) {
+void fill_fp8(const Tensor &k_cache, const Tensor &v_cache, const Tensor &k_scales, const Tensor &v_scales, const Tensor &k_fill, const Tensor &v_fill,
+              const Tensor &page_table, const OptTensor &batch_idx, const OptTensor &key_bounds, const OptTensor &row_lens) {
   const Call c("tt::paged_fill_fp8_cache_", k_cache);
   const Cache cache(c, k_cache, v_cache, k_scales, v_scales);
   cache.writable(c);
@@ -392,14 +392,30 @@ void paged_fill_fp8_cache_(const Tensor &k_cache, const Tensor &v_cache, const T
     TORCH_CHECK_VALUE(users <= 1, c.name(), ": batch_idx is required when the fill holds more than one user");
   }
   TORCH_CHECK_VALUE(s <= pt.size(1) * cache.bs, c.name(), ": ", s, " tokens do not fit ", pt.size(1), " page-table columns of ", cache.bs, " tokens");
+  Tensor lens;
+  if (row_lens) {
+    lens = indices(c, *row_lens, "lens");
+    TORCH_CHECK_VALUE(lens.dim() == 1 && lens.size(0) == pt.size(0), c.name(), ": lens must have one number per row of page_table");
+  }
   if (users == 0 || s == 0) return;
   const Tensor k = rows(k_fill), v = rows(v_fill);
   ok("ttpa_paged_fill_fp8_cache",
-     ttpa_paged_fill_fp8_cache(k_cache.data_ptr(), v_cache.data_ptr(), cache.k_scales(), cache.v_scales(), bounds, k.data_ptr(), step_of(k, 0),
-                               step_of(k, 1), step_of(k, 2), v.data_ptr(), step_of(v, 0), step_of(v, 1), step_of(v, 2), int_ptr(pt), step_of(pt, 0),
-                               bidx.defined() ? bidx.data_ptr() : nullptr, bidx.defined() && is_i64(bidx), i32(users), i32(pt.size(0)),
-                               i32(cache.hkv), i32(s), i32(cache.bs), i32(cache.d), i32(pt.size(1)), i32(cache.nb), c.stream()));
+     ttpa_paged_fill_fp8_cache_lens(k_cache.data_ptr(), v_cache.data_ptr(), cache.k_scales(), cache.v_scales(), bounds, k.data_ptr(), step_of(k, 0),
+                                    step_of(k, 1), step_of(k, 2), v.data_ptr(), step_of(v, 0), step_of(v, 1), step_of(v, 2), int_ptr(pt), step_of(pt, 0),
+                                    bidx.defined() ? bidx.data_ptr() : nullptr, bidx.defined() && is_i64(bidx), lens.defined() ? lens.data_ptr() : nullptr,
+                                    lens.defined() && is_i64(lens), i32(users), i32(pt.size(0)), i32(cache.hkv), i32(s), i32(cache.bs), i32(cache.d),
+                                    i32(pt.size(1)), i32(cache.nb), c.stream()));
   cache.changed(key_bounds);
+}
+void paged_fill_fp8_cache_(const Tensor &k_cache, const Tensor &v_cache, const Tensor &k_scales, const Tensor &v_scales, const Tensor &k_fill,
+                           const Tensor &v_fill, const Tensor &page_table, const OptTensor &batch_idx, const OptTensor &key_bounds) {
+  fill_fp8(k_cache, v_cache, k_scales, v_scales, k_fill, v_fill, page_table, batch_idx, key_bounds, std::nullopt);
+}
+// (a length for each of the page table's rows: what lies behind it is padding)
+void paged_fill_fp8_cache_lens_(const Tensor &k_cache, const Tensor &v_cache, const Tensor &k_scales, const Tensor &v_scales, const Tensor &k_fill,
+                                const Tensor &v_fill, const Tensor &page_table, const OptTensor &batch_idx, const OptTensor &key_bounds,
+                                const Tensor &lens) {
+  fill_fp8(k_cache, v_cache, k_scales, v_scales, k_fill, v_fill, page_table, batch_idx, key_bounds, lens);
 }
 
 // ---- attention --------------------------------------------------------------------------------------
@@ -791,6 +807,8 @@ TORCH_LIBRARY_FRAGMENT(tt, m) {
         "Tensor(e!)? key_bounds=None) -> ()");
   m.def("paged_fill_fp8_cache_(" TT_CACHE_W ", Tensor k_fill, Tensor v_fill, Tensor page_table, Tensor? batch_idx=None, "
         "Tensor(e!)? key_bounds=None) -> ()");
+  m.def("paged_fill_fp8_cache_.lens(" TT_CACHE_W ", Tensor k_fill, Tensor v_fill, Tensor page_table, Tensor? batch_idx, "
+        "Tensor(e!)? key_bounds, *, Tensor lens) -> ()");
   m.def("paged_fp8_attention_decode(Tensor query, " TT_CACHE ", Tensor page_table, Tensor cur_pos_tensor, Tensor? attention_sink=None, "
         "float? scale=None, int? sliding_window_size=None) -> Tensor");
   m.def("paged_fp8_attention_decode_out(Tensor query, " TT_CACHE ", Tensor page_table, Tensor cur_pos_tensor, Tensor(a!) out, "
@@ -819,6 +837,7 @@ TORCH_LIBRARY_IMPL(tt, CUDA, m) {
   m.impl("qk_norm_rope_update_fp8_", &qk_norm_rope_update_fp8_);
   m.impl("paged_update_fp8_cache_", &paged_update_fp8_cache_);
   m.impl("paged_fill_fp8_cache_", &paged_fill_fp8_cache_);
+  m.impl("paged_fill_fp8_cache_.lens", &paged_fill_fp8_cache_lens_);
   m.impl("paged_fp8_attention_decode", &paged_fp8_attention_decode);
   m.impl("paged_fp8_attention_decode_out", &paged_fp8_attention_decode_out);
   m.impl("paged_fp8_sparse_attention_decode", &paged_fp8_sparse_attention_decode);

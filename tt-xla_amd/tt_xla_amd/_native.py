@@ -168,6 +168,11 @@ SIGNATURES = {
         [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _p, _int, _i32, _i32, _i32, _i32, _i32,
          _i32, _i32, _i32, _p],
     ),
+    "ttpa_paged_fill_fp8_cache_lens": (
+        _int,
+        [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _p, _int, _p, _int, _i32, _i32, _i32, _i32, _i32,
+         _i32, _i32, _i32, _p],
+    ),
     "ttpa_paged_fp8_decode": (
         _int,
         [_p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _p, _p, _i64, _p, _int, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32,

@@ -489,7 +489,12 @@ class TTAttentionBackendImpl(_ImplBase):
                 assert rows is not None, "batch_idx must be provided for an encoder's states."
                 k, v = (self._normalize_to_attention_format(x, n, self.num_kv_heads, self.head_size, rows.numel()) for x, n in ((key, "key"), (value, "value")))
                 if eight_bits:
-                    ops.paged_fill_fp8_cache_(*caches[:4], k.transpose(1, 2), v.transpose(1, 2), attn_metadata.fill_page_table, rows, *caches[4:])
+                    fill = (*caches[:4], k.transpose(1, 2), v.transpose(1, 2), attn_metadata.fill_page_table, rows, caches[4] if len(caches) == 5 else None)
+                    # (a block's scale and bounds are those of its user's own states, whatever pads them; another table for the fill is not that of the lengths)
+                    if attn_metadata.fill_page_table is attn_metadata.page_table:
+                        ops.paged_fill_fp8_cache_.lens(*fill, lens=attn_metadata.encoder_lens)
+                    else:
+                        ops.paged_fill_fp8_cache_(*fill)
                 else:
                     ops.paged_fill_kv_cache_(caches[0], caches[1], k.transpose(1, 2), v.transpose(1, 2), attn_metadata.fill_page_table, batch_idx=rows)
             # (what a graph captures is replayed for other lengths: it has to have room for all that the table holds)

@@ -87,6 +87,10 @@ def register() -> None:
     def _(k_cache, v_cache, k_scales, v_scales, k_fill, v_fill, page_table, batch_idx=None, key_bounds=None):
         return None
 
+    @torch.library.register_fake("tt::paged_fill_fp8_cache_.lens")
+    def _(k_cache, v_cache, k_scales, v_scales, k_fill, v_fill, page_table, batch_idx, key_bounds, *, lens):
+        return None
+
     @torch.library.register_fake("tt::paged_fp8_attention_decode")
     def _(query, k_cache, v_cache, k_scales, v_scales, page_table, cur_pos_tensor, attention_sink=None, scale=None,
           sliding_window_size=None):

@@ -364,7 +364,7 @@ class CrossMetadataBuilder:
             raise ValueError(f"encoder lengths {encoder_lens.tolist()} do not fit {min(self.width, block_table.shape[1])} blocks of {self.block_size}")
         if any(not 0 <= r < reqs for r in new_rows):
             raise ValueError(f"new_rows {list(new_rows)} are not among {reqs} requests")
-        # (-1 behind a request's own blocks: padding of shorter outputs in a pass is written nowhere)
+        # (-1 behind a request's own blocks: whole blocks of a shorter output's padding are written nowhere; what pads a request's last block is not attended)
         table = torch.full((rows, self.width), -1, dtype=torch.int32)
         lens = torch.zeros(rows, dtype=torch.int32)
         for i, n in enumerate(blocks):
