@@ -710,7 +710,8 @@ CrossCut cross_cut(int batch, int kv_heads, int64_t rows, int head_size, int64_t
   }
   c.parts = std::max(c.parts, 1);
   c.share = std::max((tiles + c.parts - 1) / c.parts, chains) * c.tile;
-  if (c.parts > 1 && (best >= 12.0 || form_is("planned")) && batch > 1 && batch <= 1024 && (int64_t)batch * tiles < (1 << 30)) {
+  // (the plan counts a user's steps in floats: up to 2^24 they are exact, and the room for units holds)
+  if (c.parts > 1 && (best >= 12.0 || form_is("planned")) && batch > 1 && batch <= 1024 && tiles < (1 << 24) && (int64_t)batch * tiles < (1 << 30)) {
     c.units = (int)(2 * cus / c.row_blocks) + 1 + batch * kv_heads;
     c.step_us = tile_us, c.two = two, c.merge_us = (c.shared ? 1.75 * head_size / 128 : 1.0) * merged / (batch * kv_heads);
   }
