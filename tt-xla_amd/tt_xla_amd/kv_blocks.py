@@ -15,6 +15,7 @@ compaction want.
 
 from __future__ import annotations
 
+import heapq
 from typing import Dict, Hashable, Iterable, List, Literal, Sequence, Tuple, Union
 
 import torch
@@ -102,7 +103,7 @@ class CachePages:
         if num_blocks <= 0 or block_size <= 0 or not 0 <= reserved <= num_blocks:
             raise ValueError(f"{num_blocks} blocks of {block_size} with {reserved} reserved")
         self.num_blocks, self.block_size, self.reserved = num_blocks, block_size, reserved
-        self._free = list(range(num_blocks - 1, reserved - 1, -1))  # the lowest is taken next
+        self._free = list(range(reserved, num_blocks))  # a heap: the lowest is taken next
         self._holders = [0] * num_blocks
         self._pages: Dict[Hashable, List[int]] = {}
         self._length: Dict[Hashable, int] = {}
@@ -132,19 +133,16 @@ class CachePages:
     def _take(self, n: int) -> List[int]:
         if n > len(self._free):
             raise RuntimeError(f"{n} pages wanted, {len(self._free)} free")
-        pages = [self._free.pop() for _ in range(n)]
+        pages = [heapq.heappop(self._free) for _ in range(n)]
         for p in pages:
             self._holders[p] = 1
         return pages
 
     def _release(self, pages: Iterable[int]) -> None:
-        back = []
         for p in pages:
             self._holders[p] -= 1
             if self._holders[p] == 0:
-                back.append(p)
-        if back:
-            self._free = sorted(self._free + back, reverse=True)
+                heapq.heappush(self._free, p)
 
     def _own(self, sequence: Hashable, first: int, end: int, grow_to: int) -> List[Tuple[int, int]]:
         """Makes pages of positions [first, end) the sequence's own and appends pages up to ``grow_to``; all or nothing."""
@@ -215,5 +213,5 @@ class CachePages:
             self._holders[new], self._holders[old] = self._holders[old], 0
         for pages in self._pages.values():
             pages[:] = [moved.get(p, p) for p in pages]
-        self._free = list(range(self.num_blocks - 1, end - 1, -1))
+        self._free = list(range(end, self.num_blocks))
         return list(moved.items())
