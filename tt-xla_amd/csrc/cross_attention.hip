@@ -15,8 +15,9 @@
 //   S^T = K . Q^T                 16x16x32 bfloat16; the tile is four runs of TILE / 4 keys, one per quad of lanes: row 4 j + r of block b is
 //                                 key (TILE / 4) j + 4 b + r, so lane (row, quad) ends up with its quad's run in order, which is
 //   O^T += V^T . P^T              the order in which the second product wants its weights: no moves between the two
-// 8-bit caches: the same, an element becoming its bfloat16 value on its way into LDS; 32 users of 32 / 8 heads over 256 ... 4096 keys 22.4 us (34.0 with bfloat16), 96 of 64 / 8 over
-// 512 ... 2048 51 (75), 64 of 16 / 8 of 256 over 800 42.5 (68), 96 of 64 / 8, 5 tokens, over 1500 70 (102).
+// 8-bit caches: the same, an element becoming its bfloat16 value on its way into LDS; 32 users of 32 / 8 heads over 256 ... 4096 keys 23 us (34 with bfloat16), 96 of 64 / 8 over
+// 512 ... 2048 51 (75), 64 of 16 / 8 of 256 over 800 42 (67), 96 of 64 / 8, 5 tokens, over 1500 70 (102), 8, 5 tokens, over 512 ... 5469 21 (23).  A piece of 16 elements goes to two chunks of LDS: banks
+// that wait for each other are 25 ... 37 % of LDS's cycles, 0 with bfloat16.
 // Statistics and accumulators are floats; weights are rounded once to bfloat16 for the matrix instruction, and the same rounded weights are summed.
 // Wavefronts' results of their own tiles meet in LDS, the parts' in memory, merged by a kernel of its own.  How many parts there are goes by an estimate of the time, the host's of the longest
 // user, or, where that is long enough to pay for it, the device's of all of them (cross_work).
@@ -587,8 +588,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   }
 }
 
-// The parts of a segment's rows, four features per thread: a workgroup per row, eight slices of the parts that meet in LDS, or several rows and all of a row's parts a
-// thread's own (SLICES 1), where they are few.
+// The parts of a segment's rows, four features per thread: a workgroup per row, 1024 / D slices of the parts (16, 8 and 4 at head sizes 64, 128 and 256) that meet in
+// LDS, or several rows and all of a row's parts a thread's own (SLICES 1), where they are few.
 template <int D, int ROWS, int SLICES>
 __global__ __launch_bounds__(256) void cross_merge_kernel(CrossArgs a) {
   constexpr int SLOT = cross_slot_floats<D, ROWS>(), PER = D / 4, BATCH = SLICES > 1 ? 4 : 8, THREADS = SLICES > 1 ? SLICES * PER : 256;

@@ -8,6 +8,8 @@
 // ones: eight prompts of 4096 tokens of 8 heads of 128 (203 MB) take 41 us, 4.9 TB/s and the rate of a large copy, in blocks of 16 ... 128 tokens (64: 50
 // with ordinary loads and stores; 16 and 32: 65 and 46 with a workgroup each; 128: 65 with twice the registers it needs); at head size 64 22.
 // A grid with the heads of a block side by side is no faster for the workgroups' form (42).
+// With a length per row of the page table the block in which a length ends asks for its rows a second time, the last that counts in place of those behind it: the other
+// blocks take as long as without lengths (43, 41, 40 in blocks of 64, 16, 128; as predicates on every piece 44 in blocks of 16, and 25 for 21 at head size 64).
 #include "fp8.h"
 
 #include <algorithm>

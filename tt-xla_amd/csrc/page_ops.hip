@@ -1,9 +1,9 @@
 // Moves inside paged caches, for all layers in one call: copies of whole blocks (forks of sequences, moves of pages) and compaction of sequences
 // (chosen tokens move together).  Bytes are moved as they are, so any element type will do.  Both are bound by memory: read once, written once; a large copy by torch
-// reaches 5.3 TB/s both ways together on this card.  250 blocks of 64 x 8 heads x 128 bytes in 24 caches (786 MB) 151 us, 5.2 TB/s;
-// half of the last three quarters of 4 x 8192 tokens, K and V of 16 layers of 8 heads of 128 (1.6 GB) 328 us, 4.9; of 2048 ... 8192 tokens (867 MB), where the longest
-// user's chain of batches ends the launch, 178 us (203 with one batch on its way, 191 with streaming stores).  (Of one state again and again; of three in turn, which the
-// last cache holds less of, the first and the last take 10 % longer.)
+// reaches 5.3 TB/s both ways together on this card.  Three states in turn: 250 blocks of 64 x 8 heads x 128 bytes in 24 caches (786 MB) 153 us, 5.1 TB/s; half of the
+// last three quarters of 4 x 8192 tokens, K and V of 16 layers of 8 heads of 128 (1.6 GB), 326 us, 4.9; of 2048 ... 8192 tokens (867 MB), where the longest user's
+// chain of batches ends the launch, 200 us, 4.3.  (Of one state again and again, of which the last cache holds a part, the last takes 175 us; 203 with one batch on its way and
+// 191 with streaming stores, where these took 178.)
 #include "common.h"
 
 #include <algorithm>
