@@ -81,8 +81,9 @@ class TTMetadata:
     chunk_end       position behind the last row of a continuation chunk, where the host knows it: eager passes are
                     laid out for that many keys and not for all that the page table has room for.  Never what is
                     attended: chunk_start_idx says that.
-    encoder_lens    [users] int32, cross attention layers: states of each user's encoder that are in the cache, which all of its
-                    tokens attend; 0 where a user has none (its rows are zeros).
+    encoder_lens    [users] int32, cross attention layers: states of each user's encoder that are in the cache, those that come with
+                    the pass among them, which all of its tokens attend; 0 where a user has none (its rows are zeros).  What
+                    comes behind them is padding, which an 8-bit cache is not given.
     most_encoder_len  the largest of them, where the host knows it, as chunk_end: a bound, never what is attended.
     """
 
